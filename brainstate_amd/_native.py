@@ -159,6 +159,11 @@ SIGNATURES = {
                                              c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
     'bs_net_grid_blocks': (ctypes.c_int, [ctypes.POINTER(Net)]),
     'bs_net_error': (ctypes.c_int, [c_vp, c_vp]),
+    'bs_gated_delta_step': (ctypes.c_int, [c_vp, c_i32, c_i32, c_vp, ctypes.c_int64, c_vp, c_vp,
+                                           c_vp]),
+    'bs_gated_delta_workspace_size': (c_size, [c_vp, c_i32, c_i32, c_i32]),
+    'bs_gated_delta_rule': (ctypes.c_int, [c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                           c_vp, c_vp, c_size, c_vp]),
     'bs_net_seed_spikes': (ctypes.c_int, [c_vp, c_vp, ctypes.c_int64, c_vp, c_vp]),
 }
 

@@ -1,0 +1,158 @@
+"""Operators of sequence layers over the C ABI (torch device tensors in, device tensors out): the
+gated delta rule, the norms around a block, the 8-bit integer product.  They have no counterpart
+in brainstate; :mod:`brainstate_amd.ops` exports them.
+"""
+import struct
+
+import torch
+
+from . import _native as N
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # enum bs_dtype
+_CHUNK = 64
+_DELTA_IN = struct.Struct('5P15q7if')      # bs_delta_in
+
+
+def _floating(name, t, dtype=None):
+    if not torch.is_tensor(t):
+        raise TypeError(f'{name} must be a tensor, not {type(t).__name__}')
+    if t.dtype not in _DTYPES:
+        raise TypeError(f'{name}: dtype {t.dtype} not supported (float32, bfloat16, float16)')
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f'{name} is {t.dtype}, expected {dtype}')
+    if not t.is_cuda:
+        raise ValueError(f'{name} must be on the GPU')
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+# ------------------------------------------------------------------------- gated delta rule
+def _delta_operands(q, k, v, g, beta, scale):
+    """Checked operands as (views, bytes of bs_delta_in, sizes).  A head's values have to lie
+    side by side; any other strides are taken as they are."""
+    _floating('q', q)
+    for name, t in (('k', k), ('v', v)):
+        _floating(name, t, q.dtype)
+    for name, t in (('g', g), ('beta', beta)):
+        _floating(name, t)
+    if q.dim() != 4 or q.shape != k.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2]:
+        raise ValueError(f'q, k [batch, tokens, key heads, dk] and v [batch, tokens, heads, dv]: '
+                         f'got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
+    b, t, hk, dk = q.shape
+    hv, dv = v.shape[2:]
+    if hk < 1 or hv < 1 or hv % hk:
+        raise ValueError(f'{hv} value heads for {hk} key heads')
+    if not 1 <= dk <= 128 or not 1 <= dv <= 128:
+        raise ValueError(f'head sizes {dk}, {dv} outside 1..128')
+    if g.shape != v.shape[:3] or beta.shape != v.shape[:3]:
+        raise ValueError(f'g and beta must be {tuple(v.shape[:3])}: got {tuple(g.shape)}, '
+                         f'{tuple(beta.shape)}')
+    dev = q.device
+    if any(x.device != dev for x in (k, v, g, beta)):
+        raise ValueError('q, k, v, g and beta must be on one device')
+    q, k, v = (x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous() for x in (q, k, v))
+    scale = dk ** -0.5 if scale is None else float(scale)
+    packed = _DELTA_IN.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride(),
+        _DTYPES[q.dtype], _DTYPES[g.dtype], _DTYPES[beta.dtype], hk, hv, dk, dv, scale)
+    return (q, k, v, g, beta), packed, (b, t, hk, hv, dk, dv)
+
+
+def _states(name, s, n, hv, dk, dv, device):
+    if not torch.is_tensor(s) or s.dtype != torch.float32:
+        raise TypeError(f'{name} must be a float32 tensor')
+    if s.dim() != 4 or tuple(s.shape[1:]) != (hv, dk, dv) or n is not None and s.shape[0] != n:
+        raise ValueError(f'{name} must be [{"n" if n is None else n}, {hv}, {dk}, {dv}]: got '
+                         f'{tuple(s.shape)}')
+    if s.device != device:
+        raise ValueError(f'{name} must be on {device}')
+
+
+def gated_delta_step(q, k, v, g, beta, state, slots=None, scale=None):
+    """Tokens of running sequences through the gated delta rule, ``state`` updated in place.
+
+    Per head ``S' = exp(g) S``, ``u = beta (v - S'^T k)``, ``S = S' + k u^T``,
+    ``o = scale S^T q`` (``scale`` None: dk^-0.5), in 32 bits.
+
+    ``q``, ``k`` [batch, key heads, dk], ``v`` [batch, heads, dv], ``g`` (log decay) and ``beta``
+    [batch, heads]; each may have a dimension of tokens after the batch, which are taken in
+    order.  ``state`` [n, heads, dk, dv] float32, contiguous.  ``slots`` [batch] int32 names each
+    row's state; a negative one (or one from n on) marks an idle row, whose output is 0.  Without
+    it row b has state b.  Not differentiable."""
+    N.require_gpu()
+    if _wants_grad(q, k, v, g, beta, state):
+        raise ValueError('gated_delta_step updates its state in place and has no gradient: use '
+                         'gated_delta_rule, or torch.no_grad()')
+    one = torch.is_tensor(q) and q.dim() == 3
+    if one:
+        if v.dim() != 3 or k.dim() != 3 or g.dim() != 2 or beta.dim() != 2:
+            raise ValueError('q, k, v, g and beta must all have a dimension of tokens, or none')
+        q, k, v, g, beta = (x.unsqueeze(1) for x in (q, k, v, g, beta))
+    keep, packed, (b, t, _, hv, dk, dv) = _delta_operands(q, k, v, g, beta, scale)
+    _states('state', state, None, hv, dk, dv, q.device)
+    if not state.is_contiguous():
+        raise ValueError('state must be contiguous (it is updated in place)')
+    if slots is None:
+        if state.shape[0] != b:
+            raise ValueError(f'{state.shape[0]} states for {b} rows without slots')
+    elif slots.dtype != torch.int32 or slots.shape != (b,) or slots.device != q.device:
+        raise ValueError(f'slots must be int32 [{b}] on {q.device}')
+    else:
+        slots = slots.contiguous()
+    o = torch.empty((b, t, hv, dv), dtype=q.dtype, device=q.device)
+    N.check(N.lib().bs_gated_delta_step(packed, b, t, state.data_ptr(), state.shape[0],
+                                        N.ptr(slots), o.data_ptr(), N.raw_stream(q.device)),
+            'bs_gated_delta_step')
+    return o.squeeze(1) if one else o
+
+
+def _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, keep):
+    """(o, final state, what the backward pass needs of it or None)."""
+    held, packed, (b, t, hk, hv, dk, dv) = _delta_operands(q, k, v, g, beta, scale)
+    dev = q.device
+    n = b
+    if seq_offsets is not None:
+        if b != 1:
+            raise ValueError(f'packed sequences lie in one batch row, not {b}')
+        if seq_offsets.dtype != torch.int32 or seq_offsets.dim() != 1 or \
+                seq_offsets.numel() < 1 or seq_offsets.device != dev:
+            raise ValueError(f'seq_offsets must be int32 [sequences + 1] on {dev}')
+        seq_offsets = seq_offsets.contiguous()
+        n = seq_offsets.numel() - 1
+    if initial_state is not None:
+        _states('initial_state', initial_state, n, hv, dk, dv, dev)
+        initial_state = initial_state.contiguous()
+    o = torch.empty((b, t, hv, dv), dtype=q.dtype, device=dev)
+    final = torch.empty((n, hv, dk, dv), dtype=torch.float32, device=dev)
+    kept = (None, None)
+    if keep:
+        slots = t // _CHUNK + n if seq_offsets is not None else n * -(-t // _CHUNK)
+        dvp = -(-dv // 32) * 32
+        kept = (torch.empty((slots, hv, 64 if dk <= 64 else 128, dvp), dtype=torch.float32,
+                            device=dev),
+                torch.empty((slots, hv, _CHUNK, dvp), dtype=torch.float32, device=dev))
+    lib = N.lib()
+    nbytes = lib.bs_gated_delta_workspace_size(packed, n, t, seq_offsets is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    N.check(lib.bs_gated_delta_rule(
+        packed, n, t, N.ptr(seq_offsets), N.ptr(initial_state), final.data_ptr(), o.data_ptr(),
+        N.ptr(kept[0]), N.ptr(kept[1]), ws.data_ptr(), nbytes, N.raw_stream(dev)),
+        'bs_gated_delta_rule')
+    return o, final, kept
+
+
+def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, seq_offsets=None):
+    """Whole sequences through the gated delta rule (see :func:`gated_delta_step`), in chunks of
+    64 tokens -> (o [batch, tokens, heads, dv], final states [sequences, heads, dk, dv] float32).
+
+    ``q``, ``k`` [batch, tokens, key heads, dk], ``v`` [batch, tokens, heads, dv], ``g`` and
+    ``beta`` [batch, tokens, heads]; ``initial_state`` float32, None for zeros.  With
+    ``seq_offsets`` (int32 [sequences + 1], ascending) the sequences are packed end to end into
+    one batch row; tokens outside all of them give 0.  Differentiable in everything but
+    ``seq_offsets``."""
+    N.require_gpu()
+    o, final, _ = _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, False)
+    return o, final

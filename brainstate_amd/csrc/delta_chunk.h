@@ -1,0 +1,144 @@
+// Plan and workspace of the chunked gated delta rule (delta_chunk.hip, delta_grad.hip).
+#pragma once
+
+#include "delta.h"
+
+constexpr int kChunk = 64;   // tokens of a chunk
+
+// A sequence's chunks lie side by side in the workspace.  Where sequences are packed end to end
+// their lengths are known on the device only; sequence n then starts at slot offsets[n] / 64 + n,
+// which leaves room for every chunk of the sequences before it.
+struct DeltaPlan {
+  int seqs, tokens;           // tokens of each sequence, or of all of them when packed
+  const int32_t* offsets;     // [seqs + 1] or NULL
+  int slots;
+};
+
+struct DeltaSpan { int seq, chunks, slot; int64_t batch, first; int len; };
+
+__device__ __forceinline__ int delta_offset(const DeltaPlan& p, int n) {
+  return min(max(p.offsets[n], 0), p.tokens);
+}
+
+// Sequence n: its first slot, batch row, first token and length.
+__device__ __forceinline__ DeltaSpan delta_span(const DeltaPlan& p, int n) {
+  DeltaSpan s;
+  s.seq = n;
+  if (p.offsets) {
+    const int a = delta_offset(p, n);
+    s.batch = 0, s.first = a, s.len = max(delta_offset(p, n + 1) - a, 0);
+    s.slot = a / kChunk + n;
+    s.chunks = (s.len + kChunk - 1) / kChunk;
+  } else {
+    s.batch = n, s.first = 0, s.len = p.tokens;
+    s.chunks = (s.len + kChunk - 1) / kChunk;
+    s.slot = n * s.chunks;
+  }
+  return s;
+}
+
+// The sequence that owns a slot: the last one whose first slot is not past it.
+__device__ __forceinline__ int delta_owner(const DeltaPlan& p, int slot) {
+  if (!p.offsets) return slot / ((p.tokens + kChunk - 1) / kChunk);
+  int lo = 0, hi = p.seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (delta_offset(p, mid) / kChunk + mid <= slot) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Token of row m of row tile t of a chunk (or row of the state): the matrix cores leave rows
+// 4g..4g+3 of a 16-row tile in lane group g and take 8 values of the contracted index from it,
+// so tiles 2s and 2s+1 hold the 32 tokens of step s as 8 tokens a group, 4 from each tile:
+// what one product leaves in a lane is what the next one takes from it.
+__device__ __forceinline__ int delta_row(int t, int m) {
+  return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3);
+}
+
+// Device arrays of a call, per slot and head.
+struct DeltaWork {
+  uint16_t *kp, *qp;          // [slot][hk][parts][64][dkp]: k and q as bf16 parts, 0 past the end
+  uint16_t *kt, *qt;          // [slot][hk][parts][dkp][64]: the same, transposed
+  float *inv, *att;           // [slot][hv][64][64]: (1 + L)^-1, and the masked q k^T; in the
+                              // backward pass both transposed
+  float *coef;                // [slot][hv][4][64]: exp(run), exp(total - run), beta, exp(total)
+};
+
+struct DeltaSizes {
+  int64_t keys, square, coef, bytes;
+  int parts, dkp, dvp, ks;
+};
+
+static inline DeltaSizes delta_sizes(const bs_delta_in& in, int slots, int backward) {
+  DeltaSizes s;
+  s.parts = in.dtype == BS_BF16 ? 1 : in.dtype == BS_F16 ? 2 : 3;
+  s.ks = in.dk <= 64 ? 2 : 4;
+  s.dkp = 32 * s.ks;
+  s.dvp = (in.dv + 31) / 32 * 32;
+  s.keys = (int64_t)slots * in.hk * s.parts * kChunk * s.dkp;
+  s.square = (int64_t)slots * in.hv * kChunk * kChunk;
+  s.coef = (int64_t)slots * in.hv * 4 * kChunk;
+  s.bytes = s.keys * 2 * (backward ? 4 : 3) + s.square * 8 + s.coef * 4;
+  return s;
+}
+
+static inline DeltaWork delta_work(void* ws, const DeltaSizes& s, int backward) {
+  DeltaWork w;
+  char* p = (char*)ws;
+  auto take = [&](int64_t bytes) {
+    char* r = p;
+    p += bytes;
+    return r;
+  };
+  w.inv = (float*)take(s.square * 4);
+  w.att = (float*)take(s.square * 4);
+  w.coef = (float*)take(s.coef * 4);
+  w.kp = (uint16_t*)take(s.keys * 2);
+  w.qp = (uint16_t*)take(s.keys * 2);
+  w.kt = (uint16_t*)take(s.keys * 2);
+  w.qt = backward ? (uint16_t*)take(s.keys * 2) : nullptr;
+  return w;
+}
+
+static inline DeltaPlan delta_plan(int seqs, int tokens, const int32_t* offsets) {
+  DeltaPlan p;
+  p.seqs = seqs, p.tokens = tokens, p.offsets = offsets;
+  p.slots = offsets ? tokens / kChunk + seqs : seqs * ((tokens + kChunk - 1) / kChunk);
+  return p;
+}
+
+int delta_check_chunked(const bs_delta_in* in, int seqs, int tokens, const int32_t* offsets,
+                        const char* who);
+int delta_prepare(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork& w,
+                  const DeltaSizes& z, int backward, hipStream_t st);
+
+__device__ __forceinline__ bs_bf16x8 delta_frag(const uint16_t* p) { return *(const bs_bf16x8*)p; }
+
+// Parts of the 8 values at `p` + step * part.
+template <int PI>
+__device__ __forceinline__ bs_parts<PI> delta_frags(const uint16_t* p, int64_t step) {
+  bs_parts<PI> r;
+#pragma unroll
+  for (int i = 0; i < PI; ++i) r.p[i] = delta_frag(p + i * step);
+  return r;
+}
+
+// Parts of 8 values of one lane's place in LDS, [part][..][64 lanes][2] words of 4 values.
+template <int P>
+__device__ __forceinline__ bs_parts<P> delta_lds(const uint2* p, int step) {
+  bs_parts<P> r;
+#pragma unroll
+  for (int i = 0; i < P; ++i) r.p[i] = __builtin_bit_cast(bs_bf16x8, *(const uint4*)(p + i * step));
+  return r;
+}
+
+template <int P>
+__device__ __forceinline__ void delta_put(uint2* p, int step, const bs_f32x4& x) {
+  const float v[4] = {x[0], x[1], x[2], x[3]};
+  uint2 o[P];
+  bs_split4<P>(v, o);
+#pragma unroll
+  for (int i = 0; i < P; ++i) p[i * step] = o[i];
+}

@@ -797,3 +797,6 @@ def coba_hh_step(V, m, h, n, ge, gi, in_e, in_i, params, spk_out=None, I_ext=Non
 def ctypes_ref(s):
     import ctypes
     return ctypes.byref(s)
+
+
+from ._sequence import gated_delta_rule, gated_delta_step  # noqa: E402,F401  (operators of ops)

@@ -42,6 +42,9 @@ enum bs_status {
  * (brainevent.EventArray semantics, brainstate/nn/_event_fixedprob.py:249-252). */
 enum bs_spike_dtype { BS_SPK_U8 = 0, BS_SPK_F32 = 1 };
 
+/* Element types of the sequence-layer operators. */
+enum bs_dtype { BS_F32 = 0, BS_BF16 = 1, BS_F16 = 2 };
+
 BS_API const char* bs_last_error(void);
 BS_API int bs_version(void);
 
@@ -535,6 +538,42 @@ BS_API int bs_delay_gather(const void* hist, int32_t length, int64_t slot_elems,
 BS_API int bs_delay_taps_f32(const float* hist, int32_t length, int64_t slot_elems, int32_t taps,
                              const int32_t* slots, const float* weights, const int64_t* cols,
                              int64_t n_out, float* out, bs_stream_t stream);
+
+/* ---------------------------------------------------------------- gated delta rule
+ * Fast weights S [dk, dv] of one head, token by token (no counterpart in the reference):
+ *   S' = exp(g) S,  u = beta (v - S'^T k),  S = S' + k u^T,  o = scale S^T q.
+ * q, k [.., hk, dk] serve hv / hk value heads each, v [.., hv, dv]; g and beta [.., hv].
+ * Strides are those of (batch, token, head) in elements; a head's values lie side by side.
+ * dk, dv in 1..128.  g is a log decay (g = -inf empties the state). */
+typedef struct bs_delta_in {
+  const void *q, *k, *v, *g, *beta;
+  int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3], beta_stride[3];
+  int32_t dtype;                 /* of q, k, v and the outputs */
+  int32_t g_dtype, beta_dtype;
+  int32_t hk, hv, dk, dv;
+  float scale;
+} bs_delta_in;
+
+/* `tokens` tokens of `batch` sequences, o [batch, tokens, hv, dv].  Row b advances
+ * state[slots ? slots[b] : b] ([n_states, hv, dk, dv]) in place; a slot outside
+ * [0, n_states) marks an idle row (zero output).  Slots of live rows are distinct. */
+BS_API int bs_gated_delta_step(const bs_delta_in* in, int32_t batch, int32_t tokens,
+                               float* state, int64_t n_states, const int32_t* slots, void* o,
+                               bs_stream_t stream);
+
+/* Whole sequences, over chunks of 64 tokens: o [seqs, tokens, hv, dv].  With seq_offsets
+ * [seqs + 1] (device, ascending) the sequences are packed end to end into one batch row of
+ * `tokens` tokens (batch strides unused); rows outside all of them give 0.  States are
+ * [seqs, hv, dk, dv], NULL where not given or not wanted.  kept_states [slots, hv, dkp, dvp] and
+ * kept_u [slots, hv, 64, dvp] (both or neither) are written for the backward pass, with
+ * slots = seqs ceil(tokens / 64), or tokens / 64 + seqs when packed, dkp = 64 or 128 and
+ * dvp = dv rounded up to 32. */
+BS_API size_t bs_gated_delta_workspace_size(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                                            int32_t packed);
+BS_API int bs_gated_delta_rule(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                               const int32_t* seq_offsets, const float* initial_state,
+                               float* final_state, void* o, float* kept_states, float* kept_u,
+                               void* workspace, size_t workspace_bytes, bs_stream_t stream);
 
 #ifdef __cplusplus
 }
