@@ -164,6 +164,9 @@ SIGNATURES = {
     'bs_gated_delta_workspace_size': (c_size, [c_vp, c_i32, c_i32, c_i32]),
     'bs_gated_delta_rule': (ctypes.c_int, [c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
                                            c_vp, c_vp, c_size, c_vp]),
+    'bs_gated_delta_grad_workspace_size': (c_size, [c_vp, c_i32, c_i32, c_i32]),
+    'bs_gated_delta_rule_grad': (ctypes.c_int, [c_vp, c_i32, c_i32] + [c_vp] * 12 + [c_size,
+                                                                                   c_vp]),
     'bs_net_seed_spikes': (ctypes.c_int, [c_vp, c_vp, ctypes.c_int64, c_vp, c_vp]),
 }
 

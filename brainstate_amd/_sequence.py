@@ -144,6 +144,43 @@ def _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, keep):
     return o, final, kept
 
 
+class _DeltaRule(torch.autograd.Function):
+    """gated_delta_rule with its gradients; the states before every chunk and the values written
+    are kept for them."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, initial_state, scale, seq_offsets):
+        o, final, kept = _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, True)
+        ctx.save_for_backward(q, k, v, g, beta, seq_offsets, *kept)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return o, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go, gstate):
+        *x, seq_offsets, kept_s, kept_u = ctx.saved_tensors
+        held, packed, (b, t, hk, hv, dk, dv) = _delta_operands(*x, ctx.scale)
+        dev = x[0].device
+        n = b
+        if seq_offsets is not None:
+            seq_offsets, n = seq_offsets.contiguous(), seq_offsets.numel() - 1
+        go = torch.zeros(x[2].shape, dtype=x[2].dtype, device=dev) if go is None else \
+            go.contiguous()
+        gstate = None if gstate is None else gstate.contiguous()
+        grads = [torch.empty(y.shape, dtype=y.dtype, device=dev) for y in x]
+        ds = torch.empty((n, hv, dk, dv), dtype=torch.float32, device=dev) \
+            if ctx.needs_input_grad[5] else None
+        lib = N.lib()
+        nbytes = lib.bs_gated_delta_grad_workspace_size(packed, n, t, seq_offsets is not None)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        N.check(lib.bs_gated_delta_rule_grad(
+            packed, n, t, N.ptr(seq_offsets), go.data_ptr(), N.ptr(gstate), kept_s.data_ptr(),
+            kept_u.data_ptr(), *(y.data_ptr() for y in grads), N.ptr(ds), ws.data_ptr(), nbytes,
+            N.raw_stream(dev)), 'bs_gated_delta_rule_grad')
+        return (*grads, ds, None, None)
+
+
 def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, seq_offsets=None):
     """Whole sequences through the gated delta rule (see :func:`gated_delta_step`), in chunks of
     64 tokens -> (o [batch, tokens, heads, dv], final states [sequences, heads, dk, dv] float32).
@@ -154,5 +191,7 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, seq_offse
     one batch row; tokens outside all of them give 0.  Differentiable in everything but
     ``seq_offsets``."""
     N.require_gpu()
+    if _wants_grad(q, k, v, g, beta, initial_state):
+        return _DeltaRule.apply(q, k, v, g, beta, initial_state, scale, seq_offsets)
     o, final, _ = _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, False)
     return o, final

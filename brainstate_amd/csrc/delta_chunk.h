@@ -4,6 +4,7 @@
 #include "delta.h"
 
 constexpr int kChunk = 64;   // tokens of a chunk
+constexpr int kCoef = 6 * kChunk;
 
 // A sequence's chunks lie side by side in the workspace.  Where sequences are packed end to end
 // their lengths are known on the device only; sequence n then starts at slot offsets[n] / 64 + n,
@@ -63,11 +64,14 @@ struct DeltaWork {
   uint16_t *kt, *qt;          // [slot][hk][parts][dkp][64]: the same, transposed
   float *inv, *att;           // [slot][hv][64][64]: (1 + L)^-1, and the masked q k^T; in the
                               // backward pass both transposed
-  float *coef;                // [slot][hv][4][64]: exp(run), exp(total - run), beta, exp(total)
+  float *coef;                // [slot][hv][kCoef]: 64 each of exp(run), exp(total - run), beta
+                              // and exp(total), then 64 run in 64 bits
+  float *ds, *dr;             // backward: [slot][hv][dkp][dvp], the gradient of the state after
+                              // the chunk, and [slot][hv][64][dvp], that of R
 };
 
 struct DeltaSizes {
-  int64_t keys, square, coef, bytes;
+  int64_t keys, square, coef, state, rows, bytes;
   int parts, dkp, dvp, ks;
 };
 
@@ -79,8 +83,10 @@ static inline DeltaSizes delta_sizes(const bs_delta_in& in, int slots, int backw
   s.dvp = (in.dv + 31) / 32 * 32;
   s.keys = (int64_t)slots * in.hk * s.parts * kChunk * s.dkp;
   s.square = (int64_t)slots * in.hv * kChunk * kChunk;
-  s.coef = (int64_t)slots * in.hv * 4 * kChunk;
-  s.bytes = s.keys * 2 * (backward ? 4 : 3) + s.square * 8 + s.coef * 4;
+  s.coef = (int64_t)slots * in.hv * kCoef;
+  s.state = backward ? (int64_t)slots * in.hv * s.dkp * s.dvp : 0;
+  s.rows = backward ? (int64_t)slots * in.hv * kChunk * s.dvp : 0;
+  s.bytes = s.keys * 2 * (backward ? 4 : 3) + s.square * 8 + (s.coef + s.state + s.rows) * 4;
   return s;
 }
 
@@ -99,6 +105,8 @@ static inline DeltaWork delta_work(void* ws, const DeltaSizes& s, int backward) 
   w.qp = (uint16_t*)take(s.keys * 2);
   w.kt = (uint16_t*)take(s.keys * 2);
   w.qt = backward ? (uint16_t*)take(s.keys * 2) : nullptr;
+  w.ds = backward ? (float*)take(s.state * 4) : nullptr;
+  w.dr = backward ? (float*)take(s.rows * 4) : nullptr;
   return w;
 }
 
@@ -113,6 +121,57 @@ int delta_check_chunked(const bs_delta_in* in, int seqs, int tokens, const int32
                         const char* who);
 int delta_prepare(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork& w,
                   const DeltaSizes& z, int backward, hipStream_t st);
+
+__device__ __forceinline__ bs_f32x4 zero4() { return bs_f32x4{0.f, 0.f, 0.f, 0.f}; }
+
+// Parts of 8 floats in two vectors.
+__device__ __forceinline__ bs_parts<3> row_parts(const float4& a, const float4& b) {
+  const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  return bs_split8<3>(x);
+}
+__device__ __forceinline__ bs_parts<3> row_parts(const float* p) {
+  return row_parts(*(const float4*)p, *(const float4*)(p + 4));
+}
+
+// 8 values of a row as parts, 0 past `left`.
+template <int PI, typename T>
+__device__ __forceinline__ bs_parts<PI> load_parts(const T* p, int left, bool vec) {
+  if constexpr (PI == 1) {
+    bs_u16x8 r = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (vec && left >= 8) {
+      r = *(const bs_u16x8*)p;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) r[j] = p[j].u;
+    }
+    bs_parts<1> o;
+    o.p[0] = __builtin_bit_cast(bs_bf16x8, r);
+    return o;
+  } else {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < left ? bs_to_f32(p[j]) : 0.f;
+    return bs_split8<PI>(x);
+  }
+}
+
+// Rows of a packed batch before the first sequence and after the last one are no sequence's:
+// their values (row t of `o`, `heads` of `d` elements a row) are 0.
+template <typename T>
+__device__ void zero_outside(const DeltaPlan& plan, T* o, int heads, int d, int h, int c0,
+                             int cols) {
+  const int a = delta_offset(plan, 0), b = max(delta_offset(plan, plan.seqs), a);
+  const int c = c0 + threadIdx.x % cols, step = blockDim.x / cols;
+  if (c >= d) return;
+  for (int t = threadIdx.x / cols; t < plan.tokens; t += step) {
+    if (t >= a && t < b) {
+      t += (b - t - 1) / step * step;
+      continue;
+    }
+    o[((int64_t)t * heads + h) * d + c] = bs_from_f32<T>(0.f);
+  }
+}
 
 __device__ __forceinline__ bs_bf16x8 delta_frag(const uint16_t* p) { return *(const bs_bf16x8*)p; }
 

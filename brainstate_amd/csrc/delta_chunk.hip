@@ -19,29 +19,6 @@
 
 namespace {
 
-// 8 values of a row of q or k as parts, 0 past `left`.
-template <int PI, typename T>
-__device__ __forceinline__ bs_parts<PI> load_parts(const T* p, int left, bool vec) {
-  if constexpr (PI == 1) {
-    bs_u16x8 r = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (vec && left >= 8) {
-      r = *(const bs_u16x8*)p;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < left) r[j] = p[j].u;
-    }
-    bs_parts<1> o;
-    o.p[0] = __builtin_bit_cast(bs_bf16x8, r);
-    return o;
-  } else {
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < left ? bs_to_f32(p[j]) : 0.f;
-    return bs_split8<PI>(x);
-  }
-}
-
 // One chunk and value head: 4 waves, wave w has rows 16w..16w+15.
 // The inverse is formed by blocks of 16: the four on the diagonal by substitution, one column a
 // lane, the ones below by X_ij = -X_ii sum_k L_ik X_kj in 32-bit matrix instructions.
@@ -74,11 +51,12 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
     const float b = lane < len ? bs_delta_beta(in, sp.batch, t0 + lane, h) : 0.f;
     run[lane] = x, bt[lane] = b;
     const double total = __shfl(x, 63);
-    float* co = w.coef + ((int64_t)slot * in.hv + h) * 4 * kChunk;
+    float* co = w.coef + ((int64_t)slot * in.hv + h) * kCoef;
     co[lane] = expf((float)x);
     co[kChunk + lane] = expf((float)(total - x));
     co[2 * kChunk + lane] = b;
     co[3 * kChunk + lane] = expf((float)total);
+    ((double*)(co + 4 * kChunk))[lane] = x;
   }
   const int row = 16 * wave + m;
   bs_parts<PI> qf[KS], kf[KS];
@@ -212,31 +190,6 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
   }
 }
 
-__device__ __forceinline__ bs_f32x4 zero4() { return bs_f32x4{0.f, 0.f, 0.f, 0.f}; }
-
-// Rows of a packed batch before the first sequence and after the last one are no sequence's:
-// their outputs are 0.
-template <typename T>
-__device__ void zero_outside(const DeltaPlan& plan, T* o, int hv, int dv, int h, int slice,
-                             int cols) {
-  const int a = delta_offset(plan, 0), b = max(delta_offset(plan, plan.seqs), a);
-  const int c = slice * cols + threadIdx.x % cols;
-  if (c >= dv) return;
-  for (int t = threadIdx.x / cols; t < plan.tokens; t += 256 / cols) {
-    if (t >= a && t < b) {
-      t += (b - t - 1) / (256 / cols) * (256 / cols);
-      continue;
-    }
-    o[((int64_t)t * hv + h) * dv + c] = bs_from_f32<T>(0.f);
-  }
-}
-
-// Parts of a row of 8 floats.
-__device__ __forceinline__ bs_parts<3> row_parts(const float4& a, const float4& b) {
-  const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  return bs_split8<3>(x);
-}
-
 // Forward over the chunks of one sequence (z), value head (y) and slice of 16 NT value columns
 // (x).  Each of 4 waves has 16 tokens of a chunk and a quarter of the state's rows; what the
 // others need goes through LDS, as parts and in the lane that takes it.
@@ -252,7 +205,7 @@ __global__ __launch_bounds__(256) void chain_kernel(bs_delta_in in, DeltaPlan pl
   __shared__ __attribute__((aligned(16))) uint2 lv[PO * kR];
   const int h = blockIdx.y, n = blockIdx.z, hk = h / (in.hv / in.hk);
   if (n >= plan.seqs) {
-    zero_outside(plan, o, in.hv, in.dv, h, blockIdx.x, 16 * NT);
+    zero_outside(plan, o, in.hv, in.dv, h, blockIdx.x * 16 * NT, 16 * NT);
     return;
   }
   const DeltaSpan sp = delta_span(plan, n);
@@ -282,7 +235,7 @@ __global__ __launch_bounds__(256) void chain_kernel(bs_delta_in in, DeltaPlan pl
     const int slot = sp.slot + c;
     const int64_t sh = (int64_t)slot * in.hv + h;
     const int64_t kb = ((int64_t)slot * in.hk + hk) * PI * kChunk * DK;
-    const float* co = w.coef + sh * 4 * kChunk;
+    const float* co = w.coef + sh * kCoef;
     const float4 grow = *(const float4*)(co + out0), left = *(const float4*)(co + kChunk + out0),
                  beta = *(const float4*)(co + 2 * kChunk + out0);
     const float total = co[3 * kChunk];
@@ -336,8 +289,7 @@ __global__ __launch_bounds__(256) void chain_kernel(bs_delta_in in, DeltaPlan pl
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       if (st > blk) break;
-      const bs_parts<3> a = row_parts(*(const float4*)(ip + 32 * st),
-                                      *(const float4*)(ip + 32 * st + 4));
+      const bs_parts<3> a = row_parts(ip + 32 * st);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
         u[nt] = bs_mma<2>(a, delta_lds<3>(lr + ((st * NT + nt) * 64 + lane) * 2, kR), u[nt]);
@@ -381,8 +333,7 @@ __global__ __launch_bounds__(256) void chain_kernel(bs_delta_in in, DeltaPlan pl
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       if (st > blk) break;
-      const bs_parts<3> a = row_parts(*(const float4*)(ap + 32 * st),
-                                      *(const float4*)(ap + 32 * st + 4));
+      const bs_parts<3> a = row_parts(ap + 32 * st);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
         qs[nt] = bs_mma<PO - 1>(a, delta_lds<PO>(lv + ((st * NT + nt) * 64 + lane) * 2, kR),

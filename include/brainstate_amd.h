@@ -575,6 +575,19 @@ BS_API int bs_gated_delta_rule(const bs_delta_in* in, int32_t seqs, int32_t toke
                                float* final_state, void* o, float* kept_states, float* kept_u,
                                void* workspace, size_t workspace_bytes, bs_stream_t stream);
 
+/* Gradients of bs_gated_delta_rule given those of o (grad_o [seqs, tokens, hv, dv]) and of the
+ * final states (grad_state, NULL for none): dq, dk [seqs, tokens, hk, ..], dv [seqs, tokens, hv, ..]
+ * of `dtype`, dg and dbeta [seqs, tokens, hv] of the types of g and beta, dstate that of the
+ * initial states (NULL if not wanted).  kept_states and kept_u are the forward call's. */
+BS_API size_t bs_gated_delta_grad_workspace_size(const bs_delta_in* in, int32_t seqs,
+                                                 int32_t tokens, int32_t packed);
+BS_API int bs_gated_delta_rule_grad(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                                    const int32_t* seq_offsets, const void* grad_o,
+                                    const float* grad_state, const float* kept_states,
+                                    const float* kept_u, void* dq, void* dk, void* dv, void* dg,
+                                    void* dbeta, float* dstate, void* workspace,
+                                    size_t workspace_bytes, bs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

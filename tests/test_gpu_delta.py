@@ -173,6 +173,104 @@ def test_step_continues_the_chunked_form():
     _near(state, _np(s)[0], F32)
 
 
+GRADS = ('dq', 'dk', 'dv', 'dg', 'dbeta', 'dstate')
+
+
+def _grads(x, s0, do, dstate=None, **kw):
+    x = [y.detach().requires_grad_() for y in x]
+    s0 = None if s0 is None else s0.detach().requires_grad_()
+    o, s1 = ops.gated_delta_rule(*x, initial_state=s0, **kw)
+    outs, ups = ([o, s1], [do, dstate]) if dstate is not None else ([o], [do])
+    return torch.autograd.grad(outs, x + ([s0] if s0 is not None else []), ups)
+
+
+# Gradients are sums of the same kind as the outputs; dg is what is left of sums up to its
+# count of tokens times larger, so it gets that factor's root (8 for a chunk of 64).
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('size', SIZES)
+def test_gradients(size, dtype):
+    b, t, hk, h, dk, dv = size
+    x = _operands((b, t), hk, h, dk, dv, dtype, seed=t + 1)
+    gen = torch.Generator().manual_seed(t)
+    s0 = torch.randn(b, h, dk, dv, generator=gen).cuda()
+    do = torch.randn(b, t, h, dv, generator=gen).to(dtype).cuda()
+    dstate = torch.randn(b, h, dk, dv, generator=gen).cuda()
+    got = _grads(x, s0, do, dstate)
+    a = _np(*x, s0, do, dstate)
+    want = [sequence.gated_delta(*(y[i] for y in a[:5]), state=a[5][i], grad_o=a[6][i],
+                                 grad_state=a[7][i])[1] for i in range(b)]
+    for i, name in enumerate(GRADS):
+        print(name, flush=True)
+        tol = F32 if name == 'dstate' else 8 * F32 if name == 'dg' else TOL[dtype]
+        assert got[i].dtype == (torch.float32 if name in ('dg', 'dstate') else dtype)
+        _near(got[i], np.stack([w[i] for w in want]), tol)
+
+
+def test_gradients_against_differences():
+    """Of the operator itself, along random directions: central differences of a loss whose
+    terms are 32-bit, so the step is large (1e-2) and the agreement 1e-3."""
+    x = _operands((1, 90), 1, 2, 16, 16, torch.float32, seed=12)
+    s0 = torch.randn(1, 2, 16, 16, generator=torch.Generator().manual_seed(0)).cuda()
+    do = torch.randn(1, 90, 2, 16, generator=torch.Generator().manual_seed(1)).cuda()
+    got = _grads(x, s0, do)
+    args = x + [s0]
+    for i, gr in enumerate(got):
+        d = torch.randn(gr.shape, generator=torch.Generator().manual_seed(2 + i)).cuda()
+        d = d * args[i].norm() / d.norm()
+
+        def loss(e):
+            y = list(args)
+            y[i] = y[i] + e * d
+            return (ops.gated_delta_rule(*y[:5], initial_state=y[5])[0].double() * do).sum()
+
+        num = (8 * (loss(5e-3) - loss(-5e-3)) - (loss(1e-2) - loss(-1e-2))) / 6e-2
+        want = (gr.double() * d).sum()
+        assert abs(num - want) < 1e-3 * max(abs(want), gr.double().norm()), GRADS[i]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_packed_gradients(dtype):
+    offsets = [2, 2, 3, 70, 70, 134, 300, 301]
+    n, total = len(offsets) - 1, 305
+    x = _operands((1, total), 2, 4, 40, 48, dtype, seed=4, g_dtype=dtype)
+    do = torch.randn(1, total, 4, 48, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    off = torch.tensor(offsets, dtype=torch.int32).cuda()
+    got = _grads(x, None, do, seq_offsets=off)
+    a = _np(*x, do)
+    want = [np.zeros(y.shape) for y in a[:5]]
+    for p, e in zip(offsets, offsets[1:]):
+        r = sequence.gated_delta(*(y[0, p:e] for y in a[:5]), grad_o=a[5][0, p:e])[1]
+        for w, gr in zip(want, r):
+            w[0, p:e] = gr
+    for i in range(5):
+        _near(got[i], want[i], 8 * F32 + TOL[dtype])
+        assert (got[i][0, :2] == 0).all() and (got[i][0, 301:] == 0).all()
+
+
+def test_gradients_with_decays_that_empty_the_state():
+    x = _operands((1, 140), 1, 2, 32, 32, torch.float32, seed=5)
+    x[3][:, 10], x[3][:, 64], x[3][:, 100:103] = float('-inf'), float('-inf'), -1e30
+    do = torch.randn(1, 140, 2, 32, generator=torch.Generator().manual_seed(1)).cuda()
+    got = _grads(x, None, do)
+    a = _np(*x, do)
+    want = sequence.gated_delta(*(y[0] for y in a[:5]), grad_o=a[5][0])[1]
+    for i in range(5):
+        _near(got[i], want[i][None], 8 * F32)
+
+
+def test_zero_write_strengths():
+    """beta = 0 writes nothing, but its own gradient is there."""
+    x = _operands((1, 70), 1, 1, 16, 16, torch.float32, seed=7)
+    x[4][:] = 0
+    s0 = torch.randn(1, 1, 16, 16, generator=torch.Generator().manual_seed(3)).cuda()
+    do = torch.randn(1, 70, 1, 16, generator=torch.Generator().manual_seed(1)).cuda()
+    got = _grads(x, s0, do)
+    a = _np(*x, s0, do)
+    want = sequence.gated_delta(*(y[0] for y in a[:5]), state=a[5][0], grad_o=a[6][0])[1]
+    for i in range(6):
+        _near(got[i], want[i][None], 8 * F32)
+
+
 def test_on_another_stream():
     x = _operands((1, 130), 2, 2, 64, 64, torch.bfloat16, seed=8)
     o, s = ops.gated_delta_rule(*x)
