@@ -11,6 +11,7 @@ from . import _native as N
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # enum bs_dtype
 _CHUNK = 64
 _DELTA_IN = struct.Struct('5P15q7if')      # bs_delta_in
+_NORM_IN = struct.Struct('6P4q5i2f')       # bs_norm_in
 
 
 def _floating(name, t, dtype=None):
@@ -195,3 +196,104 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, seq_offse
         return _DeltaRule.apply(q, k, v, g, beta, initial_state, scale, seq_offsets)
     o, final, _ = _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, False)
     return o, final
+
+
+# ------------------------------------------------------------------------- norms around a block
+def _rows(t, dim):
+    """``t`` [.., dim] as rows with their values side by side."""
+    t = t.reshape(-1, dim)
+    return t if t.stride(1) == 1 or dim == 1 else t.contiguous()
+
+
+def _norm_operands(y, post, gate, scale, residual, pre, eps):
+    """Checked operands as (row views, bytes of bs_norm_in, rows, dim)."""
+    _floating('y', y)
+    if y.dim() < 1 or not 1 <= y.shape[-1] <= 16384:
+        raise ValueError(f'y [.., dim] with dim in 1..16384: got {tuple(y.shape)}')
+    dim, dev = y.shape[-1], y.device
+    for name, t in (('gate', gate), ('residual', residual)):
+        if t is not None:
+            _floating(name, t, y.dtype)
+            if t.shape != y.shape or t.device != dev:
+                raise ValueError(f'{name} must be {tuple(y.shape)} on {dev}: got '
+                                 f'{tuple(t.shape)} on {t.device}')
+    value = 1.0
+    if scale is not None and not torch.is_tensor(scale):
+        scale, value = None, float(scale)
+    weights = []
+    for name, t in (('post_weight', post), ('scale', scale), ('pre_weight', pre)):
+        if t is not None:
+            _floating(name, t)
+            if t.shape != (dim,) or t.device != dev:
+                raise ValueError(f'{name} must be [{dim}] on {dev}: got {tuple(t.shape)} on '
+                                 f'{t.device}')
+            t = t.contiguous()
+        weights.append(t)
+    acts = [t if t is None else _rows(t, dim) for t in (y, gate, residual)]
+    rows = acts[0].shape[0]
+    at = [0 if t is None else t.data_ptr() for t in acts + weights]
+    packed = _NORM_IN.pack(
+        at[0], at[3], at[1], at[4], at[2], at[5],
+        *(0 if t is None else t.stride(0) for t in acts), rows, dim, _DTYPES[y.dtype],
+        *(0 if t is None else _DTYPES[t.dtype] for t in weights), eps, value)
+    return (acts, weights), packed, rows, dim
+
+
+def _norm_forward(y, post, gate, scale, residual, pre, eps):
+    held, packed, _, _ = _norm_operands(y, post, gate, scale, residual, pre, eps)
+    stream = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    normed = torch.empty_like(stream) if pre is not None else None
+    N.check(N.lib().bs_norm_gate_residual(packed, stream.data_ptr(), N.ptr(normed),
+                                          N.raw_stream(y.device)), 'bs_norm_gate_residual')
+    return stream, normed
+
+
+class _NormGateResidual(torch.autograd.Function):
+    """norm_gate_residual with its gradients, formed from the operands alone."""
+
+    @staticmethod
+    def forward(ctx, y, post, gate, scale, residual, pre, eps):
+        ctx.eps = eps
+        ctx.value = None if torch.is_tensor(scale) else scale
+        ctx.save_for_backward(y, post, gate, scale if ctx.value is None else None, residual, pre)
+        ctx.set_materialize_grads(False)
+        return _norm_forward(y, post, gate, scale, residual, pre, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gs, gn):
+        y, post, gate, scale, residual, pre = x = ctx.saved_tensors
+        held, packed, rows, dim = _norm_operands(
+            y, post, gate, scale if ctx.value is None else ctx.value, residual, pre, ctx.eps)
+        dev = y.device
+        gs, gn = (None if t is None else t.contiguous() for t in (gs, gn))
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
+                 for t, need in zip(x, ctx.needs_input_grad)]
+        lib = N.lib()
+        nbytes, ws = 0, None
+        if any(grads[i] is not None for i in (1, 3, 5)):
+            nbytes = lib.bs_norm_grad_workspace_size(rows, dim)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        N.check(lib.bs_norm_gate_residual_grad(
+            packed, N.ptr(gs), N.ptr(gn), *(N.ptr(t) for t in grads), N.ptr(ws), nbytes,
+            N.raw_stream(dev)), 'bs_norm_gate_residual_grad')
+        return (*grads, None)
+
+
+def norm_gate_residual(y, post_weight=None, gate=None, scale=None, residual=None,
+                       pre_weight=None, eps=1e-6):
+    """What stands between a block's output and the next block, in one pass over rows [.., dim]:
+
+    ``stream = residual + scale * silu(gate) * (r(y) * post_weight)`` and
+    ``normed = r(stream) * pre_weight`` with ``r(x) = x / sqrt(mean(x^2) + eps)``
+    -> (stream, normed), (stream, None) without ``pre_weight``.
+
+    ``y``, ``gate`` and ``residual`` have one shape and type; ``post_weight``, ``scale`` and
+    ``pre_weight`` are [dim] of any floating type, ``scale`` may be a number.  Any of them may be
+    left out, with its norm or factor.  Sums are in 32 bits; ``normed`` is formed before
+    ``stream`` is rounded.  Differentiable in every tensor."""
+    N.require_gpu()
+    if _wants_grad(y, post_weight, gate, scale if torch.is_tensor(scale) else None, residual,
+                   pre_weight):
+        return _NormGateResidual.apply(y, post_weight, gate, scale, residual, pre_weight, eps)
+    return _norm_forward(y, post_weight, gate, scale, residual, pre_weight, eps)

@@ -799,4 +799,5 @@ def ctypes_ref(s):
     return ctypes.byref(s)
 
 
-from ._sequence import gated_delta_rule, gated_delta_step  # noqa: E402,F401  (operators of ops)
+from ._sequence import (gated_delta_rule, gated_delta_step,  # noqa: E402,F401
+                        norm_gate_residual)

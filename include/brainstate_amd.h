@@ -588,6 +588,30 @@ BS_API int bs_gated_delta_rule_grad(const bs_delta_in* in, int32_t seqs, int32_t
                                     void* dbeta, float* dstate, void* workspace,
                                     size_t workspace_bytes, bs_stream_t stream);
 
+/* ---------------------------------------------------------------- norms around a block
+ * Over rows of `dim` values (1..16384), with r(x) = (mean x^2 + eps)^-1/2 (no counterpart in
+ * the reference):
+ *   stream = residual + scale silu(gate) (y r(y) post),   normed = stream r(stream) pre.
+ * Weights are [dim]; a NULL one leaves its norm out (post, pre), or its factor (gate), or gives
+ * way to scale_value (scale); a NULL residual is 0.  y, gate and residual are of `dtype`, their
+ * rows *_stride elements apart; outputs are [rows, dim]. */
+typedef struct bs_norm_in {
+  const void *y, *post, *gate, *scale, *residual, *pre;
+  int64_t y_stride, gate_stride, residual_stride, rows;
+  int32_t dim, dtype, post_dtype, scale_dtype, pre_dtype;
+  float eps, scale_value;
+} bs_norm_in;
+
+BS_API int bs_norm_gate_residual(const bs_norm_in* in, void* stream_out, void* normed_out,
+                                 bs_stream_t stream);
+/* Gradients, given those of stream and normed ([rows, dim], NULL: none); a NULL output is not
+ * wanted.  Weights' gradients are of their weights' types and need the workspace. */
+BS_API size_t bs_norm_grad_workspace_size(int64_t rows, int32_t dim);
+BS_API int bs_norm_gate_residual_grad(const bs_norm_in* in, const void* grad_stream,
+                                      const void* grad_normed, void* dy, void* dpost, void* dgate,
+                                      void* dscale, void* dresidual, void* dpre, void* workspace,
+                                      size_t workspace_bytes, bs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
