@@ -170,6 +170,12 @@ SIGNATURES = {
     'bs_norm_gate_residual': (ctypes.c_int, [c_vp] * 4),
     'bs_norm_grad_workspace_size': (c_size, [ctypes.c_int64, c_i32]),
     'bs_norm_gate_residual_grad': (ctypes.c_int, [c_vp] * 10 + [c_size, c_vp]),
+    'bs_int8_quantize': (ctypes.c_int, [c_vp, c_i32, ctypes.c_int64, c_i32, ctypes.c_int64, c_vp,
+                                        c_vp, c_vp]),
+    'bs_int8_workspace_size': (c_size, [ctypes.c_int64, c_i32]),
+    'bs_int8_linear': (ctypes.c_int, [c_vp, c_i32, ctypes.c_int64, c_vp, ctypes.c_int64, c_i32,
+                                      c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_i32, c_vp, c_size,
+                                      c_vp]),
     'bs_net_seed_spikes': (ctypes.c_int, [c_vp, c_vp, ctypes.c_int64, c_vp, c_vp]),
 }
 

@@ -297,3 +297,90 @@ def norm_gate_residual(y, post_weight=None, gate=None, scale=None, residual=None
                    pre_weight):
         return _NormGateResidual.apply(y, post_weight, gate, scale, residual, pre_weight, eps)
     return _norm_forward(y, post_weight, gate, scale, residual, pre_weight, eps)
+
+
+# ------------------------------------------------------------------------- 8-bit integer product
+def _no_grad(who, *ts):
+    if _wants_grad(*ts):
+        raise ValueError(f'{who} has no gradient: detach its operands or use torch.no_grad()')
+
+
+def _channels(name, t, n, dev):
+    if not torch.is_tensor(t) or t.dtype != torch.float32 or t.shape != (n,) or t.device != dev:
+        raise ValueError(f'{name} must be float32 [{n}] on {dev}')
+    return t.contiguous()
+
+
+def int8_quantize(x):
+    """Rows of ``x`` [.., k] in 8 bits -> (int8 [.., k], float32 scales [..]): scale
+    ``max|x| / 127``, integers ``127 x / max|x|`` rounded to nearest (ties to even).  A row of zeros
+    has scale 0.  Not differentiable."""
+    N.require_gpu()
+    _floating('x', x)
+    _no_grad('int8_quantize', x)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 65536:
+        raise ValueError(f'x [.., k] with k in 1..65536: got {tuple(x.shape)}')
+    k = x.shape[-1]
+    rows = _rows(x, k)
+    x8 = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    N.check(N.lib().bs_int8_quantize(rows.data_ptr(), _DTYPES[x.dtype], rows.shape[0], k,
+                                     rows.stride(0), x8.data_ptr(), scale.data_ptr(),
+                                     N.raw_stream(x.device)), 'bs_int8_quantize')
+    return x8, scale
+
+
+def _int8_product(x, x_scale, w8, w_scale, bias, out_dtype):
+    dev = x.device
+    if not torch.is_tensor(w8) or w8.dtype != torch.int8 or w8.dim() != 2 or w8.device != dev:
+        raise ValueError(f'w8 must be int8 [channels, k] on {dev}')
+    n, k = w8.shape
+    if x.dim() < 1 or x.shape[-1] != k or not 1 <= k <= 65536:
+        raise ValueError(f'tokens [.., {k}] with k in 1..65536 expected: got {tuple(x.shape)}')
+    w8 = w8.contiguous()
+    w_scale = _channels('w_scale', w_scale, n, dev)
+    if bias is not None:
+        _floating('bias', bias)
+        if bias.shape != (n,) or bias.device != dev:
+            raise ValueError(f'bias must be [{n}] on {dev}: got {tuple(bias.shape)}')
+        bias = bias.contiguous()
+    if x_scale is None:
+        rows = _rows(x, k)
+    else:
+        if x_scale.dtype != torch.float32 or x_scale.shape != x.shape[:-1] or \
+                x_scale.device != dev:
+            raise ValueError(f'x_scale must be float32 {tuple(x.shape[:-1])} on {dev}')
+        rows, x_scale = x.reshape(-1, k).contiguous(), x_scale.contiguous()
+    m = rows.shape[0]
+    y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=dev)
+    nbytes = m * (-(-k // 128) * 128 + 4)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    N.check(N.lib().bs_int8_linear(
+        rows.data_ptr(), _DTYPES.get(x.dtype, 0), rows.stride(0), N.ptr(x_scale), m, k, n,
+        w8.data_ptr(), w_scale.data_ptr(), N.ptr(bias),
+        0 if bias is None else _DTYPES[bias.dtype], y.data_ptr(), _DTYPES[out_dtype],
+        ws.data_ptr(), nbytes, N.raw_stream(dev)), 'bs_int8_linear')
+    return y
+
+
+def int8_matmul(x8, x_scale, w8, w_scale, bias=None, out_dtype=torch.float32):
+    """``x_scale[m] * w_scale[n] * sum_k x8[m, k] * w8[n, k] + bias[n]`` with exact sums: tokens
+    ``x8`` int8 [.., k] with a scale each (:func:`int8_quantize`), weights ``w8`` int8 [n, k] with
+    a scale for each channel.  Not differentiable."""
+    N.require_gpu()
+    if not torch.is_tensor(x8) or x8.dtype != torch.int8 or not x8.is_cuda:
+        raise TypeError('x8 must be an int8 tensor on the GPU')
+    if out_dtype not in _DTYPES:
+        raise TypeError(f'out_dtype {out_dtype} not supported (float32, bfloat16, float16)')
+    _no_grad('int8_matmul', x_scale, w_scale, bias)
+    return _int8_product(x8, x_scale, w8, w_scale, bias, out_dtype)
+
+
+def int8_linear(x, w8, w_scale, bias=None):
+    """``x`` [.., k] times 8-bit weights ``w8`` [n, k] with a scale for each channel -> [.., n] of
+    the type of ``x``: its rows are quantized on the way (:func:`int8_quantize`), the sums are
+    exact, ``bias`` [n] is added in 32 bits.  Not differentiable."""
+    N.require_gpu()
+    _floating('x', x)
+    _no_grad('int8_linear', x, w_scale, bias)
+    return _int8_product(x, None, w8, w_scale, bias, x.dtype)

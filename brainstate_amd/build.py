@@ -21,7 +21,7 @@ LIBDIR = os.path.join(HERE, '_lib')
 LIB = os.path.join(LIBDIR, 'libbsamd.so')
 SOURCES = ['runtime.hip', 'compact.hip', 'event_sparse.hip', 'event_bucket.hip', 'event_dense.hip',
            'event_dense_packed.hip', 'neuron.hip', 'network.hip', 'delay.hip', 'conn.hip',
-           'delta_step.hip', 'delta_chunk.hip', 'delta_grad.hip', 'norm.hip']
+           'delta_step.hip', 'delta_chunk.hip', 'delta_grad.hip', 'norm.hip', 'int8.hip']
 ARCH = 'gfx950'
 
 

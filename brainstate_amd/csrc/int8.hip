@@ -1,0 +1,331 @@
+// Products of 8-bit integers with a scale for each token and each output channel:
+//
+//   a_m = max_k |x_mk| / 127,  x8 = round(127 x / max_k |x_mk|),  y_mn = a_m w_scale_n sum_k x8_mk w8_nk + bias_n
+//
+// Sums are exact (32-bit integers on the matrix cores), so no order of them changes a bit.
+// quant_kernel writes the tokens' integers in rows padded with zeros to whole 128-byte steps: the
+// products then need no test of k on that side, and what the weights' side reads past a row's end
+// is multiplied by 0.
+//
+// Few tokens (skinny_kernel): bound by the weights' bytes.  Each workgroup has 16 channels and its
+// waves share k; weights go straight from memory to the matrix instruction, whose operand is 16
+// rows x 64 bytes.  Many tokens (tile_kernel): bound by the matrix cores; tiles of both operands
+// are staged in LDS by direct loads, two deep, 16-byte pieces in an order (piece ^ row) that
+// keeps the reads off each other's banks.
+#include "lane_types.h"
+
+namespace {
+
+using i32x4 = __attribute__((__vector_size__(4 * sizeof(int)))) int;
+using i32x16 = __attribute__((__vector_size__(16 * sizeof(int)))) int;
+
+constexpr int kStep = 128;    // bytes of k in one step of the kernels
+
+// ------------------------------------------------------------------ tokens to 8 bits
+template <typename T>
+__global__ __launch_bounds__(256) void quant_kernel(const T* x, int64_t stride, int k, int ld,
+                                                    int8_t* x8, float* scale) {
+  __shared__ uint32_t sh[4];
+  const int64_t row = blockIdx.x;
+  const T* p = x + row * stride;
+  uint32_t top = 0;     // of |x| as bits: ordered like the values, NaN above infinity
+  for (int c = threadIdx.x * 8; c < k; c += 2048) {
+    if (c + 8 <= k) {
+      T t[8];
+      __builtin_memcpy(t, p + c, sizeof(t));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        top = max(top, __float_as_uint(bs_to_f32(t[j])) & 0x7FFFFFFFu);
+    } else {
+      for (int j = c; j < k; ++j) top = max(top, __float_as_uint(bs_to_f32(p[j])) & 0x7FFFFFFFu);
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = max(max(sh[0], sh[1]), max(sh[2], sh[3]));
+  const float most = __uint_as_float(top), a = most / 127.f;
+  if (threadIdx.x == 0) scale[row] = a;
+  // 127 x is exact for 16-bit values, so quotients of exactly a half round to even there; both
+  // sides of the quotient are divided by 256 where 127 x could overflow
+  const float up = most > 1e36f ? 127.f / 256.f : 127.f;
+  const float den = most > 1e36f ? most / 256.f : most;
+  const bool ok = a > 0.f && a < INFINITY;    // a row of 0, or with NaN or infinity, is 0: its
+                                              // scale makes the result 0 or NaN
+  int8_t* q = x8 + row * ld;
+  for (int c = threadIdx.x * 8; c < ld; c += 2048) {
+    int8_t r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      r[j] = ok && c + j < k ? (int8_t)rintf(up * bs_to_f32(p[c + j]) / den) : (int8_t)0;
+    if (c + 8 <= ld) {
+      __builtin_memcpy(q + c, r, 8);
+    } else {
+      for (int j = 0; c + j < ld; ++j) q[c + j] = r[j];
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void pad_kernel(const int8_t* x, int k, int ld, int8_t* x8) {
+  const int64_t row = blockIdx.x;
+  for (int c = threadIdx.x; c < ld; c += 256) x8[row * ld + c] = c < k ? x[row * k + c] : 0;
+}
+
+struct Out {
+  void* y;
+  const float *a, *w;       // scales
+  const void* bias;
+  int y_dtype, bias_dtype, m, n;
+};
+
+__device__ __forceinline__ void put(const Out& o, int m, int n, int acc, float w, float b) {
+  bs_store_any(o.y, o.y_dtype, (int64_t)m * o.n + n, fmaf((float)acc, o.a[m] * w, b));
+}
+
+// 16 bytes of a row of weights at k, which may start anywhere; 0 past the row's end.
+__device__ __forceinline__ i32x4 load_w(const int8_t* row, int k, int k_len) {
+  i32x4 r = {0, 0, 0, 0};
+  if (k + 16 <= k_len) {
+    __builtin_memcpy(&r, row + k, 16);
+  } else {
+    int8_t t[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t[j] = k + j < k_len ? row[k + j] : (int8_t)0;
+    __builtin_memcpy(&r, t, 16);
+  }
+  return r;
+}
+
+// ------------------------------------------------------------------ few tokens
+// MT tiles of 16 tokens.  A lane group g takes bytes 32g..32g+31 of a step for two products, so
+// the four groups read a row's 128 bytes side by side; tokens are taken in the same order.
+template <int MT>
+__global__ __launch_bounds__(256) void skinny_kernel(const int8_t* x8, int ld, const int8_t* w8,
+                                                     int k_len, Out o) {
+  __shared__ i32x4 sh[4][MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+  const int8_t* wr = w8 + (int64_t)min(n0 + r, o.n - 1) * k_len;
+  const int8_t* xr[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) xr[t] = x8 + (int64_t)min(m0 + 16 * t + r, o.m - 1) * ld + 32 * g;
+  i32x4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = i32x4{0, 0, 0, 0};
+  for (int k = wave * kStep; k < ld; k += 4 * kStep) {
+    const i32x4 b0 = load_w(wr, k + 32 * g, k_len), b1 = load_w(wr, k + 32 * g + 16, k_len);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(xr[t] + k), b0, acc[t], 0, 0,
+                                                     0);
+      acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(xr[t] + k + 16), b1, acc[t],
+                                                     0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) sh[wave][t][lane] = acc[t];
+  __syncthreads();
+  for (int t = wave; t < MT; t += 4) {
+    i32x4 s = sh[0][t][lane];
+#pragma unroll
+    for (int v = 1; v < 4; ++v) s += sh[v][t][lane];
+    const int n = n0 + r;
+    if (n >= o.n) continue;
+    const float w = o.w[n], b = o.bias ? bs_load_any(o.bias, o.bias_dtype, n) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = m0 + 16 * t + 4 * g + i;
+      if (m < o.m) put(o, m, n, s[i], w, b);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ many tokens
+typedef const __attribute__((address_space(1))) void* GlobalPtr;
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// Tile of BM tokens x BN channels, WM x WN waves, products of 32 x 32 x 32.
+template <int BM, int BN, int WM, int WN, bool DIRECT>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const int8_t* x8, int ld,
+                                                            const int8_t* w8, int k_len, Out o,
+                                                            int tiles_m, int tiles_n) {
+  constexpr int W = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int LA = BM * kStep / 1024 / W, LB = BN * kStep / 1024 / W;   // 1 KB loads a wave
+  __shared__ __attribute__((aligned(16))) int8_t sa[2][BM * kStep];
+  __shared__ __attribute__((aligned(16))) int8_t sb[2][BN * kStep];
+  // workgroups go round the 8 XCDs: each gets a run of tiles, so that its L2 keeps their rows
+  const int tiles = tiles_m * tiles_n, per = (tiles + 7) / 8;
+  const int tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || tile >= tiles) return;
+  const int m0 = tile % tiles_m * BM, n0 = tile / tiles_m * BN;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / WN, wn = wave % WN, r = lane & 31, g = lane >> 5;
+
+  // Load i of a wave fills rows 8 (wave LA + i) .. + 7; lane: row lane / 8, place lane % 8, which
+  // holds piece (place ^ row % 8).
+  const int piece = (lane & 7) ^ (lane >> 3);
+  const int8_t* ga[LA];
+  const int8_t* gb[LB];
+#pragma unroll
+  for (int i = 0; i < LA; ++i)
+    ga[i] = x8 + (int64_t)min(m0 + 8 * (wave * LA + i) + (lane >> 3), o.m - 1) * ld + 16 * piece;
+#pragma unroll
+  for (int i = 0; i < LB; ++i)
+    gb[i] = w8 + (int64_t)min(n0 + 8 * (wave * LB + i) + (lane >> 3), o.n - 1) * k_len;
+  const int last = max(k_len - 16, 0);     // DIRECT: the last whole piece of a row
+
+  auto stage = [&](int k, int buf) {
+#pragma unroll
+    for (int i = 0; i < LA; ++i)
+      __builtin_amdgcn_global_load_lds((GlobalPtr)(ga[i] + k),
+                                       (LdsPtr)(sa[buf] + (wave * LA + i) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+      if constexpr (DIRECT) {
+        __builtin_amdgcn_global_load_lds((GlobalPtr)(gb[i] + min(k + 16 * piece, last)),
+                                         (LdsPtr)(sb[buf] + (wave * LB + i) * 1024), 16, 0, 0);
+      } else {
+        *(i32x4*)(sb[buf] + (wave * LB + i) * 1024 + lane * 16) =
+            load_w(gb[i], k + 16 * piece, k_len);
+      }
+    }
+  };
+  i32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+  stage(0, 0);
+  int buf = 0;
+  for (int k = 0; k < ld; k += kStep, buf ^= 1) {
+    __syncthreads();
+    if (k + kStep < ld) stage(k + kStep, buf ^ 1);
+#pragma unroll
+    for (int s = 0; s < kStep / 32; ++s) {
+      i32x4 a[TM], b[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int row = (wm * TM + i) * 32 + r;
+        a[i] = *(const i32x4*)(sa[buf] + row * kStep + 16 * ((2 * s + g) ^ (row & 7)));
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int row = (wn * TN + j) * 32 + r;
+        b[j] = *(const i32x4*)(sb[buf] + row * kStep + 16 * ((2 * s + g) ^ (row & 7)));
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + (wn * TN + j) * 32 + r;
+    if (n >= o.n) continue;
+    const float w = o.w[n], b = o.bias ? bs_load_any(o.bias, o.bias_dtype, n) : 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int m = m0 + (wm * TM + i) * 32 + 8 * (e >> 2) + 4 * g + (e & 3);
+        if (m < o.m) put(o, m, n, acc[i][j][e], w, b);
+      }
+  }
+}
+
+template <int BM, int BN, int WM, int WN>
+void launch_tile(const int8_t* x8, int ld, const int8_t* w8, int k, const Out& o,
+                 hipStream_t st) {
+  const int tm = (o.m + BM - 1) / BM, tn = (o.n + BN - 1) / BN;
+  const int grid = (tm * tn + 7) / 8 * 8;
+  if (k % 16 == 0 && (uintptr_t)w8 % 16 == 0)
+    tile_kernel<BM, BN, WM, WN, true><<<grid, 64 * WM * WN, 0, st>>>(x8, ld, w8, k, o, tm, tn);
+  else
+    tile_kernel<BM, BN, WM, WN, false><<<grid, 64 * WM * WN, 0, st>>>(x8, ld, w8, k, o, tm, tn);
+}
+
+void product(const int8_t* x8, int ld, const int8_t* w8, int k, const Out& o, hipStream_t st) {
+  const unsigned tn = (o.n + 15) / 16;
+  if (o.m <= 16) skinny_kernel<1><<<dim3(tn, 1), 256, 0, st>>>(x8, ld, w8, k, o);
+  else if (o.m <= 32) skinny_kernel<2><<<dim3(tn, 1), 256, 0, st>>>(x8, ld, w8, k, o);
+  else if (o.m <= 128) skinny_kernel<4><<<dim3(tn, (o.m + 63) / 64), 256, 0, st>>>(x8, ld, w8, k, o);
+  else if ((int64_t)((o.m + 255) / 256) * ((o.n + 255) / 256) >= bs_num_cus())
+    launch_tile<256, 256, 2, 4>(x8, ld, w8, k, o, st);
+  else if ((int64_t)((o.m + 127) / 128) * ((o.n + 127) / 128) >= bs_num_cus())
+    launch_tile<128, 128, 2, 2>(x8, ld, w8, k, o, st);
+  else
+    launch_tile<64, 64, 2, 2>(x8, ld, w8, k, o, st);
+}
+
+int padded(int k) { return (k + kStep - 1) / kStep * kStep; }
+
+int check(int64_t m, int32_t k, int32_t n, const char* who) {
+  BS_CHECK_ARG(m >= 0 && m <= 0x7FFFFF00 && k >= 1 && k <= 65536 && n >= 0 && n <= 0x7FFFFF00,
+               "%s: %lld tokens of %d values (1..65536), %d channels", who, (long long)m, k, n);
+  const int64_t tiles = ((m + 63) / 64) * (((int64_t)n + 63) / 64);
+  BS_CHECK_ARG(tiles < 0x7FFFFF00, "%s: %lld tokens x %d channels exceed one launch", who,
+               (long long)m, n);
+  return BS_OK;
+}
+
+int quantize(const void* x, int dtype, int64_t m, int k, int64_t stride, int ld, int8_t* x8,
+             float* scale, hipStream_t st) {
+  if (dtype == BS_F32)
+    quant_kernel<<<(unsigned)m, 256, 0, st>>>((const float*)x, stride, k, ld, x8, scale);
+  else if (dtype == BS_BF16)
+    quant_kernel<<<(unsigned)m, 256, 0, st>>>((const bs_bf16*)x, stride, k, ld, x8, scale);
+  else
+    quant_kernel<<<(unsigned)m, 256, 0, st>>>((const bs_f16*)x, stride, k, ld, x8, scale);
+  BS_CHECK_LAUNCH();
+  return BS_OK;
+}
+
+}  // namespace
+
+extern "C" int bs_int8_quantize(const void* x, int32_t dtype, int64_t m, int32_t k,
+                                int64_t stride, int8_t* x8, float* scale, bs_stream_t stream) {
+  if (int rc = check(m, k, 0, "bs_int8_quantize")) return rc;
+  BS_CHECK_ARG(bs_dtype_ok(dtype), "bs_int8_quantize: dtype %d unknown", dtype);
+  if (m == 0) return BS_OK;
+  BS_CHECK_ARG(x && x8 && scale, "bs_int8_quantize: NULL pointer");
+  return quantize(x, dtype, m, k, stride, k, x8, scale, bs_stream(stream));
+}
+
+extern "C" size_t bs_int8_workspace_size(int64_t m, int32_t k) {
+  if (m < 0 || k < 1 || k > 65536) return 0;
+  return (size_t)m * padded(k) + (size_t)m * sizeof(float);
+}
+
+extern "C" int bs_int8_linear(const void* x, int32_t x_dtype, int64_t stride, const float* x_scale,
+                              int64_t m, int32_t k, int32_t n, const int8_t* w8,
+                              const float* w_scale, const void* bias, int32_t bias_dtype, void* y,
+                              int32_t y_dtype, void* workspace, size_t workspace_bytes,
+                              bs_stream_t stream) {
+  if (int rc = check(m, k, n, "bs_int8_linear")) return rc;
+  BS_CHECK_ARG((x_scale || bs_dtype_ok(x_dtype)) && bs_dtype_ok(bias_dtype) &&
+                   bs_dtype_ok(y_dtype), "bs_int8_linear: dtype unknown");
+  if (m == 0 || n == 0) return BS_OK;
+  BS_CHECK_ARG(x && w8 && w_scale && y, "bs_int8_linear: NULL pointer");
+  const size_t need = bs_int8_workspace_size(m, k);
+  BS_CHECK_ARG(workspace && workspace_bytes >= need,
+               "bs_int8_linear: workspace of %zu bytes needed", need);
+  hipStream_t st = bs_stream(stream);
+  const int ld = padded(k);
+  int8_t* x8 = (int8_t*)workspace;
+  float* a = (float*)(x8 + (size_t)m * ld);
+  if (x_scale) {
+    pad_kernel<<<(unsigned)m, 256, 0, st>>>((const int8_t*)x, k, ld, x8);
+    BS_CHECK_LAUNCH();
+  } else if (int rc = quantize(x, x_dtype, m, k, stride, ld, x8, a, st)) {
+    return rc;
+  }
+  const Out o = {y, x_scale ? x_scale : a, w_scale, bias, y_dtype, bias_dtype, (int)m, n};
+  product(x8, ld, w8, k, o, st);
+  BS_CHECK_LAUNCH();
+  return BS_OK;
+}

@@ -800,4 +800,4 @@ def ctypes_ref(s):
 
 
 from ._sequence import (gated_delta_rule, gated_delta_step,  # noqa: E402,F401
-                        norm_gate_residual)
+                        int8_linear, int8_matmul, int8_quantize, norm_gate_residual)

@@ -612,6 +612,23 @@ BS_API int bs_norm_gate_residual_grad(const bs_norm_in* in, const void* grad_str
                                       void* dscale, void* dresidual, void* dpre, void* workspace,
                                       size_t workspace_bytes, bs_stream_t stream);
 
+/* ---------------------------------------------------------------- 8-bit integer products
+ * Tokens x [m, k] (rows `stride` elements apart) to 8 bits with a scale each (no counterpart in
+ * the reference): scale = max|x| / 127, x8 = 127 x / max|x| rounded to nearest, ties to even, in
+ * -127..127; a row of zeros gives zeros and scale 0, one with NaN or infinity gives zeros and
+ * that scale.  k in 1..65536. */
+BS_API int bs_int8_quantize(const void* x, int32_t dtype, int64_t m, int32_t k, int64_t stride,
+                            int8_t* x8, float* scale, bs_stream_t stream);
+/* y [m, n] = x_scale[m] w_scale[n] sum_k x8[m, k] w8[n, k] + bias[n], sums exact.  With
+ * x_scale, x holds the integers [m, k] (stride unused); without it x is of x_dtype and is
+ * quantized on the way.  bias may be NULL.  The workspace starts on 16 bytes. */
+BS_API size_t bs_int8_workspace_size(int64_t m, int32_t k);
+BS_API int bs_int8_linear(const void* x, int32_t x_dtype, int64_t stride, const float* x_scale,
+                          int64_t m, int32_t k, int32_t n, const int8_t* w8,
+                          const float* w_scale, const void* bias, int32_t bias_dtype, void* y,
+                          int32_t y_dtype, void* workspace, size_t workspace_bytes,
+                          bs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

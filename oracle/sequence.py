@@ -88,12 +88,12 @@ def norm_gate_residual(y, post=None, gate=None, scale=None, residual=None, pre=N
 
 
 def int8_quantize(x):
-    """Rows of x in 8 bits: a = max|x| / 127 and round-half-even of x / a (0 for a row of 0)."""
+    """Rows of x in 8 bits: a = max|x| / 127 and round-half-even of x / a = 127 x / max|x| (one
+    rounding, so halves of 16-bit values are met exactly); 0 for a row of 0."""
     x = np.asarray(x, np.float64)
-    a = np.abs(x).max(1) / 127 if x.shape[1] else np.zeros(x.shape[0])
-    with np.errstate(invalid='ignore', divide='ignore'):
-        x8 = np.where(a[:, None] > 0, np.rint(x / a[:, None]), 0.0)
-    return x8, a
+    top = np.abs(x).max(1, keepdims=True) if x.shape[1] else np.zeros((x.shape[0], 1))
+    x8 = np.where(top > 0, np.rint(127 * x / np.where(top > 0, top, 1)), 0.0)
+    return x8, top[:, 0] / 127
 
 
 def int8_linear(x, w8, w_scale, bias=None):
