@@ -50,43 +50,58 @@ __device__ __forceinline__ int delta_owner(const DeltaPlan& p, int slot) {
   return lo;
 }
 
-// Token of row m of row tile t of a chunk (or row of the state): the matrix cores leave rows
-// 4g..4g+3 of a 16-row tile in lane group g and take 8 values of the contracted index from it,
-// so tiles 2s and 2s+1 hold the 32 tokens of step s as 8 tokens a group, 4 from each tile:
-// what one product leaves in a lane is what the next one takes from it.
+// The products are of 16 x 16 tiles over 32 values.  A product leaves rows 4g..4g+3 of a tile in
+// lane group g and takes 8 values of the contracted index from it, so rows are dealt to tiles
+// such that tiles 2s and 2s+1 hold rows 32s..32s+31 with 8 rows in a group, 4 in each tile: what
+// one product leaves in a lane is what the next one takes from it.  delta_row is the token (or
+// row of the state) of row m of tile t.
 __device__ __forceinline__ int delta_row(int t, int m) {
   return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3);
 }
 
-// Device arrays of a call, per slot and head.
+// Device arrays of a call, per slot and head, of fragments: the 8 values of each of 64 lanes as a
+// product takes them, 1 KB side by side.  Fragment (t, s) of a matrix holds rows delta_row(t, .)
+// and columns 32s + 8g .. + 7.
 struct DeltaWork {
-  uint16_t *kp, *qp;          // [slot][hk][parts][64][dkp]: k and q as bf16 parts, 0 past the end
-  uint16_t *kt, *qt;          // [slot][hk][parts][dkp][64]: the same, transposed
-  float *inv, *att;           // [slot][hv][64][64]: (1 + L)^-1, and the masked q k^T; in the
-                              // backward pass both transposed
-  float *coef;                // [slot][hv][kCoef]: 64 each of exp(run), exp(total - run), beta
-                              // and exp(total), then 64 run in 64 bits
+  uint16_t *kp, *qp;          // [slot][hk][parts][4][dkp / 32]: k and q, 0 past the end
+  uint16_t *kt, *qt;          // [slot][hk][parts][dkp / 16][2]: their transposes
+  uint16_t *inv;              // [slot][hv][3][6]: (1 + L)^-1 without its 32 x 32 block of zeros
+  uint16_t *att;              // [slot][hv][att parts][6]: the masked q k^T; in the backward pass
+                              // the transposes of both
+  float *coef;                // [slot][hv][kCoef], see delta_coef
   float *ds, *dr;             // backward: [slot][hv][dkp][dvp], the gradient of the state after
                               // the chunk, and [slot][hv][64][dvp], that of R
 };
 
+// Rows of coef, 64 values each (the last in 64 bits).
+enum delta_coef { kGrow = 0, kLeft = 1, kBeta = 2, kTotal = 3, kRun = 4 };
+constexpr int kFrag = 512;                 // values of a fragment
+constexpr int kSquare = 6 * kFrag;
+
+// Fragment (t, s) of a lower triangular square, s <= t / 2; of an upper one, s >= t / 2.
+__device__ __forceinline__ int delta_lower(int t, int s) { return t < 2 ? t : 2 * t - 2 + s; }
+__device__ __forceinline__ int delta_upper(int t, int s) { return t < 2 ? 2 * t + s : t + 2; }
+
 struct DeltaSizes {
   int64_t keys, square, coef, state, rows, bytes;
-  int parts, dkp, dvp, ks;
+  int parts, att_parts, dkp, dvp, ks;
 };
 
 static inline DeltaSizes delta_sizes(const bs_delta_in& in, int slots, int backward) {
   DeltaSizes s;
   s.parts = in.dtype == BS_BF16 ? 1 : in.dtype == BS_F16 ? 2 : 3;
+  // outputs in 16 bits take two parts of the masked product, gradients three
+  s.att_parts = backward || in.dtype == BS_F32 ? 3 : 2;
   s.ks = in.dk <= 64 ? 2 : 4;
   s.dkp = 32 * s.ks;
   s.dvp = (in.dv + 31) / 32 * 32;
   s.keys = (int64_t)slots * in.hk * s.parts * kChunk * s.dkp;
-  s.square = (int64_t)slots * in.hv * kChunk * kChunk;
+  s.square = (int64_t)slots * in.hv * kSquare;
   s.coef = (int64_t)slots * in.hv * kCoef;
   s.state = backward ? (int64_t)slots * in.hv * s.dkp * s.dvp : 0;
   s.rows = backward ? (int64_t)slots * in.hv * kChunk * s.dvp : 0;
-  s.bytes = s.keys * 2 * (backward ? 4 : 3) + s.square * 8 + (s.coef + s.state + s.rows) * 4;
+  s.bytes = s.keys * 2 * (backward ? 4 : 3) + s.square * 2 * (3 + s.att_parts) +
+            (s.coef + s.state + s.rows) * 4;
   return s;
 }
 
@@ -98,8 +113,8 @@ static inline DeltaWork delta_work(void* ws, const DeltaSizes& s, int backward) 
     p += bytes;
     return r;
   };
-  w.inv = (float*)take(s.square * 4);
-  w.att = (float*)take(s.square * 4);
+  w.inv = (uint16_t*)take(s.square * 6);
+  w.att = (uint16_t*)take(s.square * 2 * s.att_parts);
   w.coef = (float*)take(s.coef * 4);
   w.kp = (uint16_t*)take(s.keys * 2);
   w.qp = (uint16_t*)take(s.keys * 2);
@@ -154,6 +169,17 @@ __device__ __forceinline__ bs_parts<PI> load_parts(const T* p, int left, bool ve
     for (int j = 0; j < 8; ++j) x[j] = j < left ? bs_to_f32(p[j]) : 0.f;
     return bs_split8<PI>(x);
   }
+}
+
+// Workgroup of a grid of units x slices: the slices of a unit (one sequence and head) read the
+// same chunks, so they are given to one of the 8 XCDs, whose L2 then reads each chunk once.
+struct DeltaPlace { int unit, slice; };
+__device__ __forceinline__ DeltaPlace delta_place(int slices) {
+  const int k = blockIdx.x >> 3;
+  return {k / slices * 8 + (int)(blockIdx.x & 7), k % slices};
+}
+static inline unsigned delta_grid(int64_t units, int slices) {
+  return (unsigned)((units + 7) / 8 * 8 * slices);
 }
 
 // Rows of a packed batch before the first sequence and after the last one are no sequence's:

@@ -19,10 +19,10 @@
 
 namespace {
 
-// One chunk and value head: 4 waves, wave w has rows 16w..16w+15.
-// The inverse is formed by blocks of 16: the four on the diagonal by substitution, one column a
-// lane, the ones below by X_ij = -X_ii sum_k L_ik X_kj in 32-bit matrix instructions.
-template <typename T, int PI, int KS, bool BWD>
+// One chunk and value head: 4 waves, wave w has tile w's rows.
+// The inverse is formed by blocks of 16 tokens: the four on the diagonal by substitution, one
+// column a lane, the ones below by X_ij = -X_ii sum_k L_ik X_kj in 32-bit matrix instructions.
+template <typename T, int PI, int KS, bool BWD, int PA>
 __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan plan, DeltaWork w,
                                                       int vec) {
   constexpr int DK = KS * 32, LD = DK + 8;
@@ -38,8 +38,11 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
   if (c >= sp.chunks) return;
   const int64_t t0 = sp.first + (int64_t)c * kChunk;
   const int len = min(sp.len - c * kChunk, kChunk);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool first = h % group == 0;
+  const int64_t sh = (int64_t)slot * in.hv + h;
+  const int64_t kb = ((int64_t)slot * in.hk + hk) * PI * kChunk * DK;
 
   if (wave == 0) {      // lane = token
     double x = lane < len ? (double)bs_delta_g(in, sp.batch, t0 + lane, h) : 0.0;
@@ -51,21 +54,20 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
     const float b = lane < len ? bs_delta_beta(in, sp.batch, t0 + lane, h) : 0.f;
     run[lane] = x, bt[lane] = b;
     const double total = __shfl(x, 63);
-    float* co = w.coef + ((int64_t)slot * in.hv + h) * kCoef;
-    co[lane] = expf((float)x);
-    co[kChunk + lane] = expf((float)(total - x));
-    co[2 * kChunk + lane] = b;
-    co[3 * kChunk + lane] = expf((float)total);
-    ((double*)(co + 4 * kChunk))[lane] = x;
+    float* co = w.coef + sh * kCoef;
+    co[kGrow * kChunk + lane] = expf((float)x);
+    co[kLeft * kChunk + lane] = expf((float)(total - x));
+    co[kBeta * kChunk + lane] = b;
+    co[kTotal * kChunk + lane] = expf((float)total);
+    ((double*)(co + kRun * kChunk))[lane] = x;
   }
-  const int row = 16 * wave + m;
+  const int row = delta_row(wave, m);
   bs_parts<PI> qf[KS], kf[KS];
   {
     const bool live = row < len;
     const int64_t t = live ? t0 + row : t0;
     const T* kp = (const T*)in.k + bs_delta_at(in.k_stride, sp.batch, t, hk);
     const T* qp = (const T*)in.q + bs_delta_at(in.q_stride, sp.batch, t, hk);
-    const int64_t base = ((int64_t)slot * in.hk + hk) * PI * kChunk * DK;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = 32 * s + 8 * g, left = live ? in.dk - d : 0;
@@ -75,23 +77,34 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
       for (int p = 0; p < PI; ++p) {
         *(bs_bf16x8*)&kl[p][row][d] = kf[s].p[p];
         if (first) {
-          *(bs_bf16x8*)(w.kp + base + ((int64_t)p * kChunk + row) * DK + d) = kf[s].p[p];
-          *(bs_bf16x8*)(w.qp + base + ((int64_t)p * kChunk + row) * DK + d) = qf[s].p[p];
+          const int64_t f = kb + (int64_t)((p * 4 + wave) * KS + s) * kFrag + lane * 8;
+          *(bs_bf16x8*)(w.kp + f) = kf[s].p[p];
+          *(bs_bf16x8*)(w.qp + f) = qf[s].p[p];
         }
       }
     }
   }
   __syncthreads();
-  float* att = w.att + ((int64_t)slot * in.hv + h) * kChunk * kChunk;
+  // the transposed copy of what kl holds, by fragments
+  auto transposed = [&](uint16_t* to) {
+#pragma unroll
+    for (int p = 0; p < PI; ++p)
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int f = wave * KS + i, d = delta_row(f >> 1, m), j0 = 32 * (f & 1) + 8 * g;
+        bs_u16x8 r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = kl[p][j0 + j][d];
+        *(bs_u16x8*)(to + kb + (int64_t)(p * 4 * KS + f) * kFrag + lane * 8) = r;
+      }
+  };
+  const int i0 = 32 * (wave >> 1) + 8 * g + 4 * (wave & 1);     // rows i0 .. i0 + 3 come back
+  float am[4][4];                 // the masked product, for LDS later
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt) {
-    if (jt > (wave | 1)) {       // past the 32-token block of the diagonal: never read
-      if (BWD) continue;
-      break;
-    }
-    const int j = 16 * jt + m;
-    bs_f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
-    if (jt <= wave) {
+    const int j = delta_row(jt, m);
+    bs_f32x4 kk = zero4(), qk = zero4();
+    if (jt <= (wave | 1)) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         bs_parts<PI> b;
@@ -101,30 +114,16 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
         qk = bs_mma<2>(qf[s], b, qk);
       }
     }
-    float4 row4;
-    float* r4 = (float*)&row4;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wave + 4 * g + r;
+      const int i = i0 + r;
       const float e = j <= i ? expf((float)(run[i] - run[j])) : 0.f;
-      if (jt <= wave) lm[i][j] = j < i ? bt[i] * e * kk[r] : 0.f;
-      else xm[i][j] = 0.f;
-      const float a = j <= i ? in.scale * e * qk[r] : 0.f;
-      r4[r] = a;
-      if (!BWD) att[i * kChunk + j] = a;
+      lm[i][j] = j < i ? bt[i] * e * kk[r] : 0.f;
+      if ((i >> 4) < (j >> 4)) xm[i][j] = 0.f;
+      am[jt][r] = j <= i ? in.scale * e * qk[r] : 0.f;
     }
-    if (BWD) *(float4*)(att + j * kChunk + 16 * wave + 4 * g) = row4;
   }
-  if (first) {                    // the transposed copies: 8 lanes write a row of 64 tokens
-    const int64_t base = ((int64_t)slot * in.hk + hk) * PI * kChunk * DK;
-    for (int p = 0; p < PI; ++p)
-      for (int d = tid >> 3; d < DK; d += 32) {
-        bs_u16x8 r;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = kl[p][8 * (tid & 7) + j][d];
-        *(bs_u16x8*)(w.kt + base + ((int64_t)p * DK + d) * kChunk + 8 * (tid & 7)) = r;
-      }
-  }
+  if (first) transposed(w.kt);
   __syncthreads();
   {
     float x[16];
@@ -147,20 +146,11 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
       for (int p = 0; p < PI; ++p) *(bs_bf16x8*)&kl[p][row][32 * s + 8 * g] = qf[s].p[p];
   }
   __syncthreads();
-  if (BWD && first) {
-    const int64_t base = ((int64_t)slot * in.hk + hk) * PI * kChunk * DK;
-    for (int p = 0; p < PI; ++p)
-      for (int d = tid >> 3; d < DK; d += 32) {
-        bs_u16x8 r;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = kl[p][8 * (tid & 7) + j][d];
-        *(bs_u16x8*)(w.qt + base + ((int64_t)p * DK + d) * kChunk + 8 * (tid & 7)) = r;
-      }
-  }
+  if (BWD && first) transposed(w.qt);
   for (int d = 1; d < 4; ++d) {
     const int j = wave, i = wave + d;
     if (i < 4) {
-      bs_f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+      bs_f32x4 a = zero4(), b = zero4();
       for (int k = j; k < i; ++k)
 #pragma unroll
         for (int s = 0; s < 4; ++s)
@@ -175,196 +165,237 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
     }
     __syncthreads();
   }
-  float* inv = w.inv + ((int64_t)slot * in.hv + h) * kChunk * kChunk;
-  for (int e = tid; e < kChunk * 16; e += 256) {
-    const int i = e >> 4, j = (e & 15) * 4;
-    if (BWD) {
-      if ((j | 31) < i) continue;     // row i of the transpose starts at its 32-token block
-      *(float4*)(inv + i * kChunk + j) =
-          make_float4(j < i ? 0.f : xm[j][i], j + 1 < i ? 0.f : xm[j + 1][i],
-                      j + 2 < i ? 0.f : xm[j + 2][i], j + 3 < i ? 0.f : xm[j + 3][i]);
-    } else {
-      if (j > (i | 31)) continue;
-      *(float4*)(inv + i * kChunk + j) = *(const float4*)&xm[i][j];
+#pragma unroll
+  for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lm[i0 + r][delta_row(jt, m)] = am[jt][r];
+  __syncthreads();
+  for (int f = wave; f < 6; f += 4) {
+    const int t = BWD ? (f < 4 ? f >> 1 : f - 2) : f < 2 ? f : (f + 2) >> 1;
+    const int s = BWD ? (f < 4 ? f & 1 : 1) : f < 2 ? 0 : f & 1;
+    const int i = delta_row(t, m), j = 32 * s + 8 * g;
+    float x[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = BWD ? xm[j + e][i] : xm[i][j + e];
+      y[e] = BWD ? lm[j + e][i] : lm[i][j + e];
     }
+    const bs_parts<3> xp = bs_split8<3>(x);
+    const bs_parts<PA> yp = bs_split8<PA>(y);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      *(bs_bf16x8*)(w.inv + (sh * 3 + p) * kSquare + f * kFrag + lane * 8) = xp.p[p];
+#pragma unroll
+    for (int p = 0; p < PA; ++p)
+      *(bs_bf16x8*)(w.att + (sh * PA + p) * kSquare + f * kFrag + lane * 8) = yp.p[p];
   }
 }
 
-// Forward over the chunks of one sequence (z), value head (y) and slice of 16 NT value columns
-// (x).  Each of 4 waves has 16 tokens of a chunk and a quarter of the state's rows; what the
-// others need goes through LDS, as parts and in the lane that takes it.
-template <typename T, int PI, int KS, int NT>
+// Forward over the chunks of one sequence, value head and slice of 16 value columns.  Each of 4
+// waves has 16 tokens of a chunk and a quarter of the state's rows; what the others need goes
+// through LDS, as parts and in the lane that takes it.  Operands that do not depend on the state
+// are loaded into registers a chunk ahead, each as soon as its last use is issued.  The output
+// is formed transposed (the operands of a product swapped), which leaves 4 neighbouring columns
+// of a token in a lane.
+template <typename T, int PI, int KS>
 __global__ __launch_bounds__(256) void chain_kernel(bs_delta_in in, DeltaPlan plan, DeltaWork w,
                                                     const float* state0, float* state1, T* o,
-                                                    float* keep_s, float* keep_u, int dvp) {
+                                                    float* keep_s, float* keep_u, int dvp,
+                                                    int units, int vec) {
   constexpr int DK = KS * 32, TW = KS / 2, PO = PI == 3 ? 3 : 2;
-  constexpr int kS = KS * NT * 128, kR = 2 * NT * 128;       // words of a part
+  constexpr int kS = KS * 128, kR = 2 * 128;       // words of a part
   __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];
   __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];
   __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];
   __shared__ __attribute__((aligned(16))) uint2 lv[PO * kR];
-  const int h = blockIdx.y, n = blockIdx.z, hk = h / (in.hv / in.hk);
+  __shared__ __attribute__((aligned(16))) float turn[4][16][20];
+  const DeltaPlace at = delta_place(dvp / 16);
+  if (at.unit >= units) return;
+  const int h = at.unit % in.hv, n = at.unit / in.hv, hk = h / (in.hv / in.hk);
   if (n >= plan.seqs) {
-    zero_outside(plan, o, in.hv, in.dv, h, blockIdx.x * 16 * NT, 16 * NT);
+    zero_outside(plan, o, in.hv, in.dv, h, at.slice * 16, 16);
     return;
   }
   const DeltaSpan sp = delta_span(plan, n);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int col0 = blockIdx.x * 16 * NT + m;
-  const int tok = delta_row(wave, m);                 // the row this lane feeds
-  const int out0 = 32 * (wave >> 1) + 8 * g + 4 * (wave & 1);   // the 4 rows it receives
-  const int blk = wave >> 1;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), blk = wave >> 1;
+  const int col = at.slice * 16 + m, ocol = at.slice * 16 + 4 * g;
+  const bool live = col < in.dv;
+  const int tok = delta_row(wave, m);                      // the row this lane feeds
+  const int out0 = 32 * blk + 8 * g + 4 * (wave & 1);      // the 4 rows it receives
+  const int own = (blk * 64 + lane) * 2 + (wave & 1);
 
-  bs_f32x4 s[TW][NT];
+  bs_f32x4 s[TW];
+  int d0[TW], sown[TW];
 #pragma unroll
   for (int i = 0; i < TW; ++i) {
-    const int t = TW * wave + i, d0 = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
+    const int t = TW * wave + i;
+    d0[i] = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
+    sown[i] = ((t >> 1) * 64 + lane) * 2 + (t & 1);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int r = 0; r < 4; ++r)
+      s[i][r] = state0 && d0[i] + r < in.dk && live
+          ? state0[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] : 0.f;
+    delta_put<3>(ls + sown[i], kS, s[i]);
+  }
+
+  const uint16_t* kp = w.kp + ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK + wave * KS * kFrag;
+  const uint16_t* qp = w.qp + ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK + wave * KS * kFrag;
+  const uint16_t* kt = w.kt + ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK +
+                       wave * TW * 2 * kFrag;
+  const uint16_t* ip = w.inv + ((int64_t)sp.slot * in.hv + h) * 3 * kSquare +
+                       delta_lower(wave, 0) * kFrag;
+  const uint16_t* ap = w.att + ((int64_t)sp.slot * in.hv + h) * PO * kSquare +
+                       delta_lower(wave, 0) * kFrag;
+  const float* cp = w.coef + ((int64_t)sp.slot * in.hv + h) * kCoef;
+  const T* vp = (const T*)in.v + bs_delta_at(in.v_stride, sp.batch, sp.first, h) +
+                min(col, in.dv - 1);
+  const int64_t keys = (int64_t)in.hk * PI * kChunk * DK;
+  bs_parts<PI> kf[KS], qf[KS], ktf[TW][2];
+  bs_parts<3> tf[2];
+  bs_parts<PO> af[2];
+  T vr[4];
+  float4 grow, left, beta;
+  float total, scale;
+  auto load_keys = [&](int c) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int c = col0 + 16 * nt;
-        s[i][nt][r] = state0 && d0 + r < in.dk && c < in.dv
-            ? state0[(((int64_t)n * in.hv + h) * in.dk + d0 + r) * in.dv + c] : 0.f;
-      }
-      delta_put<3>(ls + (((t >> 1) * NT + nt) * 64 + lane) * 2 + (t & 1), kS, s[i][nt]);
+    for (int st = 0; st < KS; ++st) {
+      kf[st] = delta_frags<PI>(kp + c * keys + st * kFrag + lane * 8, kChunk * DK);
+      qf[st] = delta_frags<PI>(qp + c * keys + st * kFrag + lane * 8, kChunk * DK);
     }
+  };
+  auto load_values = [&](int c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      vr[r] = vp[min(c * kChunk + out0 + r, sp.len - 1) * in.v_stride[1]];
+    const float* co = cp + (int64_t)c * in.hv * kCoef;
+    grow = *(const float4*)(co + kGrow * kChunk + out0);
+    left = *(const float4*)(co + kLeft * kChunk + out0);
+    beta = *(const float4*)(co + kBeta * kChunk + out0);
+    scale = in.scale * co[kGrow * kChunk + tok];
+    total = co[kTotal * kChunk];
+  };
+  auto load_inverse = [&](int c) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+      if (st <= blk)
+        tf[st] = delta_frags<3>(ip + (int64_t)c * in.hv * 3 * kSquare + st * kFrag + lane * 8,
+                                kSquare);
+  };
+  auto load_columns = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < 2 * TW; ++i)
+      ktf[i >> 1][i & 1] = delta_frags<PI>(kt + c * keys + i * kFrag + lane * 8, kChunk * DK);
+  };
+  auto load_masked = [&](int c) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+      if (st <= blk)
+        af[st] = delta_frags<PO>(ap + (int64_t)c * in.hv * PO * kSquare + st * kFrag + lane * 8,
+                                 kSquare);
+  };
+  // a 16 x 16 tile with its rows r0 + 0..15 (in delta_row order) to row-major memory
+  auto keep = [&](float* to, int t, const bs_f32x4& x) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) turn[wave][4 * g + r][m] = x[r];
+    __builtin_amdgcn_wave_barrier();     // one wave's LDS accesses are done in order
+    *(float4*)(to + (int64_t)delta_row(t, m) * dvp + ocol) = *(const float4*)&turn[wave][m][4 * g];
+  };
+  if (sp.chunks) {
+    load_keys(0);
+    load_values(0);
+    load_inverse(0);
+    load_columns(0);
+    load_masked(0);
   }
   __syncthreads();
   for (int c = 0; c < sp.chunks; ++c) {
-    const int slot = sp.slot + c;
-    const int64_t sh = (int64_t)slot * in.hv + h;
-    const int64_t kb = ((int64_t)slot * in.hk + hk) * PI * kChunk * DK;
-    const float* co = w.coef + sh * kCoef;
-    const float4 grow = *(const float4*)(co + out0), left = *(const float4*)(co + kChunk + out0),
-                 beta = *(const float4*)(co + 2 * kChunk + out0);
-    const float total = co[3 * kChunk];
-    const float* gr = (const float*)&grow;
-    const float* lf = (const float*)&left;
-    const float* be = (const float*)&beta;
+    const int next = min(c + 1, sp.chunks - 1);
+    const int64_t sh = (int64_t)(sp.slot + c) * in.hv + h;
+    bs_f32x4 ks = zero4(), qs = zero4(), u = zero4();
+    bs_parts<3> sf[KS];
+#pragma unroll
+    for (int st = 0; st < KS; ++st) sf[st] = delta_lds<3>(ls + (st * 64 + lane) * 2, kS);
+#pragma unroll
+    for (int st = 0; st < KS; ++st) ks = bs_mma<2>(kf[st], sf[st], ks);
+    {
+      bs_f32x4 x;
+      const float* gr = (const float*)&grow;
+      const float* be = (const float*)&beta;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = c * kChunk + out0 + r < sp.len && live ? bs_to_f32(vr[r]) : 0.f;
+        x[r] = be[r] * fmaf(-gr[r], ks[r], v);
+      }
+      delta_put<3>(lr + own, kR, x);
+    }
+    // the state's part of the output, while the others arrive
+#pragma unroll
+    for (int st = 0; st < KS; ++st) qs = bs_mma<PO - 1>(sf[st], qf[st], qs);
+    load_keys(next);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) qs[r] *= scale;
+    const float4 lf4 = left;
+    const float all = total;
+    load_values(next);
+    __syncthreads();
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+      if (st <= blk) u = bs_mma<2>(tf[st], delta_lds<3>(lr + (st * 64 + lane) * 2, kR), u);
+    {
+      bs_f32x4 x;
+      const float* lf = (const float*)&lf4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = lf[r] * u[r];
+      delta_put<3>(lu + own, kR, x);
+      delta_put<PO>(lv + own, kR, u);
+    }
+    load_inverse(next);
     if (keep_s) {
+      keep(keep_u + sh * kChunk * dvp, wave, u);
 #pragma unroll
-      for (int i = 0; i < TW; ++i) {
-        const int t = TW * wave + i, d0 = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            keep_s[(sh * DK + d0 + r) * dvp + col0 + 16 * nt] = s[i][nt][r];
-      }
-    }
-    bs_f32x4 ks[NT], qs[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) ks[nt] = qs[nt] = zero4();
-#pragma unroll
-    for (int st = 0; st < KS; ++st) {
-      const bs_parts<PI> kf = delta_frags<PI>(w.kp + kb + tok * DK + 32 * st + 8 * g, kChunk * DK);
-      const bs_parts<PI> qf = delta_frags<PI>(w.qp + kb + tok * DK + 32 * st + 8 * g, kChunk * DK);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const bs_parts<3> b = delta_lds<3>(ls + ((st * NT + nt) * 64 + lane) * 2, kS);
-        ks[nt] = bs_mma<2>(kf, b, ks[nt]);
-        qs[nt] = bs_mma<PO - 1>(qf, b, qs[nt]);
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int cc = col0 + 16 * nt;
-      bs_f32x4 x;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = c * kChunk + out0 + r;
-        const float v = t < sp.len && cc < in.dv
-            ? bs_to_f32(((const T*)in.v)[bs_delta_at(in.v_stride, sp.batch, sp.first + t, h) + cc])
-            : 0.f;
-        x[r] = be[r] * (v - gr[r] * ks[nt][r]);
-      }
-      delta_put<3>(lr + ((blk * NT + nt) * 64 + lane) * 2 + (wave & 1), kR, x);
-    }
-    __syncthreads();
-    bs_f32x4 u[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) u[nt] = zero4();
-    const float* ip = w.inv + sh * kChunk * kChunk + tok * kChunk + 8 * g;
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      if (st > blk) break;
-      const bs_parts<3> a = row_parts(ip + 32 * st);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        u[nt] = bs_mma<2>(a, delta_lds<3>(lr + ((st * NT + nt) * 64 + lane) * 2, kR), u[nt]);
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int at = ((blk * NT + nt) * 64 + lane) * 2 + (wave & 1);
-      delta_put<PO>(lv + at, kR, u[nt]);
-      bs_f32x4 x;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[r] = lf[r] * u[nt][r];
-        if (keep_u) keep_u[(sh * kChunk + out0 + r) * dvp + col0 + 16 * nt] = u[nt][r];
-      }
-      delta_put<3>(lu + at, kR, x);
+      for (int i = 0; i < TW; ++i) keep(keep_s + sh * DK * dvp, TW * wave + i, s[i]);
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < TW; ++i) {
-      const int t = TW * wave + i;
-      const uint16_t* kt = w.kt + kb + delta_row(t, m) * kChunk + 8 * g;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[i][nt] *= total;
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const bs_parts<PI> a = delta_frags<PI>(kt + 32 * st, DK * kChunk);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          s[i][nt] = bs_mma<2>(a, delta_lds<3>(lu + ((st * NT + nt) * 64 + lane) * 2, kR),
-                               s[i][nt]);
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        delta_put<3>(ls + (((t >> 1) * NT + nt) * 64 + lane) * 2 + (t & 1), kS, s[i][nt]);
-    }
-    const float* ap = w.att + sh * kChunk * kChunk + tok * kChunk + 8 * g;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) qs[nt][r] *= in.scale * gr[r];
+    for (int i = 0; i < TW; ++i) s[i] *= all;
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
-      if (st > blk) break;
-      const bs_parts<3> a = row_parts(ap + 32 * st);
+      const bs_parts<3> b = delta_lds<3>(lu + (st * 64 + lane) * 2, kR);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        qs[nt] = bs_mma<PO - 1>(a, delta_lds<PO>(lv + ((st * NT + nt) * 64 + lane) * 2, kR),
-                                qs[nt]);
+      for (int i = 0; i < TW; ++i) s[i] = bs_mma<2>(ktf[i][st], b, s[i]);
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int cc = col0 + 16 * nt;
+    for (int i = 0; i < TW; ++i) delta_put<3>(ls + sown[i], kS, s[i]);
+    load_columns(next);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = c * kChunk + out0 + r;
-        if (t < sp.len && cc < in.dv)
-          o[((sp.batch * plan.tokens + sp.first + t) * in.hv + h) * in.dv + cc] =
-              bs_from_f32<T>(qs[nt][r]);
+    for (int st = 0; st < 2; ++st)
+      if (st <= blk)
+        qs = bs_mma<PO - 1>(delta_lds<PO>(lv + (st * 64 + lane) * 2, kR), af[st], qs);
+    load_masked(next);
+    if (c * kChunk + tok < sp.len) {
+      T* op = o + ((sp.batch * plan.tokens + sp.first + c * kChunk + tok) * in.hv + h) * in.dv +
+              ocol;
+      T y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = bs_from_f32<T>(qs[r]);
+      if (vec) {
+        if (ocol < in.dv) __builtin_memcpy(__builtin_assume_aligned(op, 4 * sizeof(T)), y, sizeof(y));
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (ocol + r < in.dv) op[r] = y[r];
       }
     }
     __syncthreads();
   }
-  if (state1) {
+  if (state1 && live) {
 #pragma unroll
-    for (int i = 0; i < TW; ++i) {
-      const int t = TW * wave + i, d0 = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
+    for (int i = 0; i < TW; ++i)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int cc = col0 + 16 * nt;
-          if (d0 + r < in.dk && cc < in.dv)
-            state1[(((int64_t)n * in.hv + h) * in.dk + d0 + r) * in.dv + cc] = s[i][nt][r];
-        }
-    }
+      for (int r = 0; r < 4; ++r)
+        if (d0[i] + r < in.dk)
+          state1[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] = s[i][r];
   }
 }
 
@@ -374,18 +405,18 @@ void launch_prepare(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWor
   const dim3 grid(plan.slots, in.hv);
   int vec = (uintptr_t)in.q % 16 == 0 && (uintptr_t)in.k % 16 == 0;
   for (int i = 0; i < 3; ++i) vec = vec && in.q_stride[i] % 8 == 0 && in.k_stride[i] % 8 == 0;
-  if (backward) prepare_kernel<T, PI, KS, true><<<grid, 256, 0, st>>>(in, plan, w, vec);
-  else prepare_kernel<T, PI, KS, false><<<grid, 256, 0, st>>>(in, plan, w, vec);
+  if (backward) prepare_kernel<T, PI, KS, true, 3><<<grid, 256, 0, st>>>(in, plan, w, vec);
+  else prepare_kernel<T, PI, KS, false, PI == 3 ? 3 : 2><<<grid, 256, 0, st>>>(in, plan, w, vec);
 }
 
 template <typename T, int PI, int KS>
 void launch_chain(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork& w,
                   const DeltaSizes& z, const float* s0, float* s1, void* o, float* keep_s,
                   float* keep_u, hipStream_t st) {
-  const unsigned rows = plan.seqs + (plan.offsets ? 1 : 0);
-  // 16 columns a workgroup
-  chain_kernel<T, PI, KS, 1><<<dim3(z.dvp / 16, in.hv, rows), 256, 0, st>>>(
-      in, plan, w, s0, s1, (T*)o, keep_s, keep_u, z.dvp);
+  const int units = (plan.seqs + (plan.offsets ? 1 : 0)) * in.hv;
+  chain_kernel<T, PI, KS><<<delta_grid(units, z.dvp / 16), 256, 0, st>>>(
+      in, plan, w, s0, s1, (T*)o, keep_s, keep_u, z.dvp, units,
+      in.dv % 4 == 0 && (uintptr_t)o % (4 * sizeof(T)) == 0);
 }
 
 template <typename T, int PI>
@@ -421,7 +452,8 @@ int delta_check_chunked(const bs_delta_in* in, int seqs, int tokens, const int32
   BS_CHECK_ARG(seqs >= 0 && tokens >= 0, "%s: %d sequences, %d tokens", who, seqs, tokens);
   const int64_t slots = offsets ? (int64_t)tokens / kChunk + seqs
                                 : (int64_t)seqs * ((tokens + kChunk - 1) / kChunk);
-  BS_CHECK_ARG(slots <= 0x7FFFFFFF / kChunk && seqs < 65535 && in->hv <= 65535,
+  BS_CHECK_ARG(slots <= 0x7FFFFFFF / kChunk && in->hv <= 65535 &&
+                   ((int64_t)seqs + 1) * in->hv <= 0x7FFFFFFF / 64,
                "%s: %d sequences of %d tokens, %d heads exceed one launch", who, seqs, tokens,
                in->hv);
   return BS_OK;

@@ -24,11 +24,13 @@
 
 namespace {
 
+// Chunks of one sequence, value head and slice of 16 value columns, last to first; waves and
+// operands as in the forward pass.
 template <typename T, int PI, int KS>
 __global__ __launch_bounds__(256) void grad_chain_kernel(bs_delta_in in, DeltaPlan plan,
                                                          DeltaWork w, const T* go,
                                                          const float* gstate, T* dv,
-                                                         float* dstate, int dvp) {
+                                                         float* dstate, int dvp, int units) {
   constexpr int DK = KS * 32, TW = KS / 2;
   constexpr int kS = KS * 128, kR = 2 * 128;       // words of a part
   __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];
@@ -36,171 +38,227 @@ __global__ __launch_bounds__(256) void grad_chain_kernel(bs_delta_in in, DeltaPl
   __shared__ __attribute__((aligned(16))) uint2 lg[2][3 * kR];
   __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];
   __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];
-  const int h = blockIdx.y, n = blockIdx.z, hk = h / (in.hv / in.hk);
+  __shared__ __attribute__((aligned(16))) float turn[4][16][20];
+  const DeltaPlace at = delta_place(dvp / 16);
+  if (at.unit >= units) return;
+  const int h = at.unit % in.hv, n = at.unit / in.hv, hk = h / (in.hv / in.hk);
   if (n >= plan.seqs) {
-    zero_outside(plan, dv, in.hv, in.dv, h, blockIdx.x * 16, 16);
+    zero_outside(plan, dv, in.hv, in.dv, h, at.slice * 16, 16);
     return;
   }
   const DeltaSpan sp = delta_span(plan, n);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int col = blockIdx.x * 16 + m;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), blk = wave >> 1;
+  const int col = at.slice * 16 + m;
+  const bool live = col < in.dv;
   const int tok = delta_row(wave, m);
-  const int out0 = 32 * (wave >> 1) + 8 * g + 4 * (wave & 1);
-  const int blk = wave >> 1, own = (blk * 64 + lane) * 2 + (wave & 1);
+  const int out0 = 32 * blk + 8 * g + 4 * (wave & 1);
+  const int own = (blk * 64 + lane) * 2 + (wave & 1);
 
+  bs_f32x4 s[TW];
+  int d0[TW];
+#pragma unroll
+  for (int i = 0; i < TW; ++i) {
+    const int t = TW * wave + i;
+    d0[i] = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      s[i][r] = gstate && d0[i] + r < in.dk && live
+          ? gstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] : 0.f;
+    delta_put<3>(ls + ((t >> 1) * 64 + lane) * 2 + (t & 1), kS, s[i]);
+  }
+  const uint16_t* kp = w.kp + ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK + wave * KS * kFrag;
+  const int64_t tb = ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK + wave * TW * 2 * kFrag;
+  const int64_t sq = ((int64_t)sp.slot * in.hv + h) * 3 * kSquare;
+  const float* cp = w.coef + ((int64_t)sp.slot * in.hv + h) * kCoef;
+  const T* gp = go + ((sp.batch * plan.tokens + sp.first) * in.hv + h) * in.dv +
+                min(col, in.dv - 1);
+  const int64_t keys = (int64_t)in.hk * PI * kChunk * DK;
+  bs_parts<PI> kf[KS], ktf[TW][2], qtf[TW][2];
+  bs_parts<3> tf[2], af[2];
+  T gr[4];
+  float4 coef[3];
+  float total, token_beta;
+  auto load_keys = [&](int c) {
+#pragma unroll
+    for (int st = 0; st < KS; ++st)
+      kf[st] = delta_frags<PI>(kp + c * keys + st * kFrag + lane * 8, kChunk * DK);
+  };
+  auto load_grad = [&](int c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      gr[r] = gp[(int64_t)min(c * kChunk + out0 + r, sp.len - 1) * in.hv * in.dv];
+    const float* co = cp + (int64_t)c * in.hv * kCoef;
+    coef[0] = *(const float4*)(co + kGrow * kChunk + out0);
+    coef[1] = *(const float4*)(co + kLeft * kChunk + out0);
+    coef[2] = *(const float4*)(co + kBeta * kChunk + out0);
+    total = co[kTotal * kChunk];
+    token_beta = co[kBeta * kChunk + tok];
+  };
+  auto load_square = [&](const uint16_t* a, int c, bs_parts<3>* f) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+      if (st >= blk)
+        f[st] = delta_frags<3>(a + sq + (int64_t)c * in.hv * 3 * kSquare +
+                                   delta_upper(wave, st) * kFrag + lane * 8, kSquare);
+  };
+  auto load_columns = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < 2 * TW; ++i) {
+      const int64_t a = tb + c * keys + i * kFrag + lane * 8;
+      ktf[i >> 1][i & 1] = delta_frags<PI>(w.kt + a, kChunk * DK);
+      qtf[i >> 1][i & 1] = delta_frags<PI>(w.qt + a, kChunk * DK);
+    }
+  };
+  auto keep = [&](float* to, int t, const bs_f32x4& x) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) turn[wave][4 * g + r][m] = x[r];
+    __builtin_amdgcn_wave_barrier();     // one wave's LDS accesses are done in order
+    *(float4*)(to + (int64_t)delta_row(t, m) * dvp + at.slice * 16 + 4 * g) =
+        *(const float4*)&turn[wave][m][4 * g];
+  };
+  float grow[4], left[4], beta[4], all = 0.f, mine = 0.f;
   // dO of a chunk and scale G dO, into LDS
   auto stage = [&](int c) {
-    const float* co = w.coef + ((int64_t)(sp.slot + c) * in.hv + h) * kCoef;
-    const float4 grow = *(const float4*)(co + out0);
-    const float* gr = (const float*)&grow;
+    grow[0] = coef[0].x, grow[1] = coef[0].y, grow[2] = coef[0].z, grow[3] = coef[0].w;
+    left[0] = coef[1].x, left[1] = coef[1].y, left[2] = coef[1].z, left[3] = coef[1].w;
+    beta[0] = coef[2].x, beta[1] = coef[2].y, beta[2] = coef[2].z, beta[3] = coef[2].w;
+    all = total, mine = token_beta;
     bs_f32x4 x, y;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int t = c * kChunk + out0 + r;
-      x[r] = t < sp.len && col < in.dv
-          ? bs_to_f32(go[((sp.batch * plan.tokens + sp.first + t) * in.hv + h) * in.dv + col])
-          : 0.f;
-      y[r] = in.scale * gr[r] * x[r];
+      x[r] = c * kChunk + out0 + r < sp.len && live ? bs_to_f32(gr[r]) : 0.f;
+      y[r] = in.scale * grow[r] * x[r];
     }
     delta_put<PI>(lo + own, kR, x);
     delta_put<3>(lg[c & 1] + own, kR, y);
   };
-
-  bs_f32x4 s[TW];
-#pragma unroll
-  for (int i = 0; i < TW; ++i) {
-    const int t = TW * wave + i, d0 = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      s[i][r] = gstate && d0 + r < in.dk && col < in.dv
-          ? gstate[(((int64_t)n * in.hv + h) * in.dk + d0 + r) * in.dv + col] : 0.f;
-    delta_put<3>(ls + ((t >> 1) * 64 + lane) * 2 + (t & 1), kS, s[i]);
+  if (const int c = sp.chunks - 1; c >= 0) {
+    load_grad(c);
+    load_keys(c);
+    load_square(w.att, c, af);
+    load_square(w.inv, c, tf);
+    load_columns(c);
+    stage(c);
+    load_grad(max(c - 1, 0));
   }
-  if (sp.chunks) stage(sp.chunks - 1);
   __syncthreads();
   for (int c = sp.chunks - 1; c >= 0; --c) {
-    const int slot = sp.slot + c;
-    const int64_t sh = (int64_t)slot * in.hv + h;
-    const int64_t kb = ((int64_t)slot * in.hk + hk) * PI * kChunk * DK;
-    const float* co = w.coef + sh * kCoef;
-    const float4 grow = *(const float4*)(co + out0), left = *(const float4*)(co + kChunk + out0),
-                 beta = *(const float4*)(co + 2 * kChunk + out0);
-    const float total = co[3 * kChunk];
-    const float* gr = (const float*)&grow;
-    const float* lf = (const float*)&left;
-    const float* be = (const float*)&beta;
-    bs_f32x4 du = zero4();
+    const int next = max(c - 1, 0);
+    const int64_t sh = (int64_t)(sp.slot + c) * in.hv + h;
+    bs_f32x4 du = zero4(), dr = zero4(), x;
 #pragma unroll
     for (int st = 0; st < KS; ++st)
-      du = bs_mma<2>(delta_frags<PI>(w.kp + kb + tok * DK + 32 * st + 8 * g, kChunk * DK),
-                     delta_lds<3>(ls + (st * 64 + lane) * 2, kS), du);
+      du = bs_mma<2>(kf[st], delta_lds<3>(ls + (st * 64 + lane) * 2, kS), du);
+    load_keys(next);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) du[r] *= lf[r];
-    const float* ap = w.att + sh * kChunk * kChunk + tok * kChunk + 8 * g;
+    for (int r = 0; r < 4; ++r) du[r] *= left[r];
 #pragma unroll
     for (int st = 0; st < 2; ++st)
-      if (st >= blk)
-        du = bs_mma<2>(row_parts(ap + 32 * st), delta_lds<PI>(lo + (st * 64 + lane) * 2, kR), du);
+      if (st >= blk) du = bs_mma<2>(af[st], delta_lds<PI>(lo + (st * 64 + lane) * 2, kR), du);
+    load_square(w.att, next, af);
     delta_put<3>(lu + own, kR, du);
+#pragma unroll
+    for (int i = 0; i < TW; ++i) keep(w.ds + sh * DK * dvp, TW * wave + i, s[i]);
     __syncthreads();
-    bs_f32x4 dr = zero4();
-    const float* ip = w.inv + sh * kChunk * kChunk + tok * kChunk + 8 * g;
 #pragma unroll
     for (int st = 0; st < 2; ++st)
-      if (st >= blk)
-        dr = bs_mma<2>(row_parts(ip + 32 * st), delta_lds<3>(lu + (st * 64 + lane) * 2, kR), dr);
-    bs_f32x4 x;
+      if (st >= blk) dr = bs_mma<2>(tf[st], delta_lds<3>(lu + (st * 64 + lane) * 2, kR), dr);
+    load_square(w.inv, next, tf);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = c * kChunk + out0 + r;
-      const float b = be[r] * dr[r];
-      x[r] = -gr[r] * b;
-      w.dr[(sh * kChunk + out0 + r) * dvp + col] = dr[r];
-      if (t < sp.len && col < in.dv)
-        dv[((sp.batch * plan.tokens + sp.first + t) * in.hv + h) * in.dv + col] =
-            bs_from_f32<T>(b);
-    }
+    for (int r = 0; r < 4; ++r) x[r] = -grow[r] * (beta[r] * dr[r]);
     delta_put<3>(lr + own, kR, x);
+    keep(w.dr + sh * kChunk * dvp, wave, dr);
+    {                                // the tile is still in `turn`, by tokens
+      const int t = c * kChunk + delta_row(wave, m), oc = at.slice * 16 + 4 * g;
+      if (t < sp.len) {
+        const float4 d4 = *(const float4*)&turn[wave][m][4 * g];
+        const float* d = (const float*)&d4;
+        T* op = dv + ((sp.batch * plan.tokens + sp.first + t) * in.hv + h) * in.dv + oc;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (oc + r < in.dv) op[r] = bs_from_f32<T>(mine * d[r]);
+      }
+    }
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TW; ++i) s[i] *= all;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const bs_parts<3> a = delta_lds<3>(lg[c & 1] + (st * 64 + lane) * 2, kR);
+      const bs_parts<3> b = delta_lds<3>(lr + (st * 64 + lane) * 2, kR);
+#pragma unroll
+      for (int i = 0; i < TW; ++i) {
+        s[i] = bs_mma<2>(qtf[i][st], a, s[i]);
+        s[i] = bs_mma<2>(ktf[i][st], b, s[i]);
+      }
+    }
+    load_columns(next);
 #pragma unroll
     for (int i = 0; i < TW; ++i) {
-      const int t = TW * wave + i, d0 = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) w.ds[(sh * DK + d0 + r) * dvp + col] = s[i][r];
-      s[i] *= total;
-      const int64_t at = kb + delta_row(t, m) * kChunk + 8 * g;
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        s[i] = bs_mma<2>(delta_frags<PI>(w.qt + at + 32 * st, DK * kChunk),
-                         delta_lds<3>(lg[c & 1] + (st * 64 + lane) * 2, kR), s[i]);
-        s[i] = bs_mma<2>(delta_frags<PI>(w.kt + at + 32 * st, DK * kChunk),
-                         delta_lds<3>(lr + (st * 64 + lane) * 2, kR), s[i]);
-      }
+      const int t = TW * wave + i;
       delta_put<3>(ls + ((t >> 1) * 64 + lane) * 2 + (t & 1), kS, s[i]);
     }
-    if (c) stage(c - 1);
+    if (c) {
+      stage(next);
+      load_grad(max(c - 2, 0));
+    }
     __syncthreads();
   }
-  if (dstate) {
+  if (dstate && live) {
 #pragma unroll
-    for (int i = 0; i < TW; ++i) {
-      const int t = TW * wave + i, d0 = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
+    for (int i = 0; i < TW; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (d0 + r < in.dk && col < in.dv)
-          dstate[(((int64_t)n * in.hv + h) * in.dk + d0 + r) * in.dv + col] = s[i][r];
-    }
+        if (d0[i] + r < in.dk)
+          dstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] = s[i][r];
   }
 }
 
-__device__ __forceinline__ float sum16(float x) {     // over the 16 lanes of a group
-  x += __shfl_xor(x, 1);
-  x += __shfl_xor(x, 2);
-  x += __shfl_xor(x, 4);
-  return x + __shfl_xor(x, 8);
-}
 __device__ __forceinline__ float sum4(float x) {      // over the 4 lane groups
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
 }
 
-// Four tokens (4g..4g+3 of 16 at t0) of column d of a transposed copy, parts added up.
+// Value e (0..7) of a fragment, its parts added up.
 template <int PI>
-__device__ __forceinline__ bs_f32x4 column4(const uint16_t* p, int64_t step) {
-  bs_f32x4 r = zero4();
+__device__ __forceinline__ float frag_value(const bs_parts<PI>& f, int e) {
+  float x = 0.f;
 #pragma unroll
-  for (int i = 0; i < PI; ++i) {
-    const uint2 x = *(const uint2*)(p + i * step);
-    r[0] += __uint_as_float(x.x << 16), r[1] += __uint_as_float(x.x & 0xFFFF0000u);
-    r[2] += __uint_as_float(x.y << 16), r[3] += __uint_as_float(x.y & 0xFFFF0000u);
-  }
-  return r;
+  for (int p = PI - 1; p >= 0; --p)
+    x += __uint_as_float((uint32_t)__builtin_bit_cast(bs_u16x8, f.p[p])[e] << 16);
+  return x;
 }
 
-// One chunk (x) and key head (y): 4 waves, wave w has tokens 16w..16w+15; the value heads that
-// share the key head are taken in turn, their dq and dk summed in registers.
+// One chunk (x) and key head (y); the value heads that share the key head are taken in turn,
+// their dq and dk summed in registers.  8 waves: wave (t, half) has the tokens of tile t and half
+// of the dk rows, everything transposed (rows dk, columns tokens), so that factors of a token are
+// one value a lane and a token's dk lie side by side.  The exponents' gradients need no sums of
+// their own: run_i multiplies q_i in dq's terms and k_i in the terms of R and L's rows, and
+// divides k_i in the others, so
+//   drun_i = q_i.dq_i + k_i.dkA_i - k_i.dkB_i,   dk = dkA + dkB.
 template <typename T, int PI, int KS>
-__global__ __launch_bounds__(256) void grad_chunk_kernel(bs_delta_in in, DeltaPlan plan,
+__global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPlan plan,
                                                          DeltaWork w, const T* go,
                                                          const float* keep_s, const float* keep_u,
                                                          T* dq, T* dk, void* dg, void* dbeta,
                                                          int dvp, int vec) {
-  constexpr int DK = KS * 32, CT = KS * 2;
-  __shared__ float lp[kChunk][kChunk + 4];
-  __shared__ float lm[kChunk][kChunk + 4];
-  __shared__ float cols[4][kChunk], rows[kChunk], tot[4], bsum[kChunk];
-  __shared__ double run[kChunk];
+  constexpr int DK = KS * 32, CT = KS, HS = KS / 2;     // tiles and steps of dk of a wave
+  __shared__ __attribute__((aligned(16))) float lp[kChunk][kChunk + 4];
+  __shared__ __attribute__((aligned(16))) float lm[kChunk][kChunk + 4];
+  __shared__ float rows[2][kChunk], betas[2][kChunk], tot[8];
   const int slot = blockIdx.x, hk = blockIdx.y, group = in.hv / in.hk;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), t = wave & 3, half = wave >> 2;
   if (slot == plan.slots) {       // packed only: rows outside all sequences
     zero_outside(plan, dq, in.hk, in.dk, hk, 0, 128);
     zero_outside(plan, dk, in.hk, in.dk, hk, 0, 128);
     const int a = delta_offset(plan, 0), b = max(delta_offset(plan, plan.seqs), a);
-    for (int t = tid; t < plan.tokens; t += 256)
-      if (t < a || t >= b)
+    for (int r = tid; r < plan.tokens; r += 512)
+      if (r < a || r >= b)
         for (int h = hk * group; h < (hk + 1) * group; ++h) {
-          bs_store_any(dg, in.g_dtype, (int64_t)t * in.hv + h, 0.f);
-          bs_store_any(dbeta, in.beta_dtype, (int64_t)t * in.hv + h, 0.f);
+          bs_store_any(dg, in.g_dtype, (int64_t)r * in.hv + h, 0.f);
+          bs_store_any(dbeta, in.beta_dtype, (int64_t)r * in.hv + h, 0.f);
         }
     return;
   }
@@ -210,183 +268,205 @@ __global__ __launch_bounds__(256) void grad_chunk_kernel(bs_delta_in in, DeltaPl
   const int64_t t0 = sp.first + (int64_t)c * kChunk;
   const int len = min(sp.len - c * kChunk, kChunk);
   const int64_t kb = ((int64_t)slot * in.hk + hk) * PI * kChunk * DK;
-  const int row = 16 * wave + m, out0 = 16 * wave + 4 * g, blk = wave >> 1;
-  const bool live = row < len;
+  const int blk = t >> 1, tok = delta_row(t, m);
+  const bool live = tok < len;
+  // tiles of columns of the masked products of this wave: j0, and j0 + 1 in the second block
+  const int j0 = blk ? 2 * half : half, nj = blk ? 2 : 1;
 
-  bs_f32x4 qk[4], kk[4], aq[CT], ak[CT];
+  bs_f32x4 qk[2], kk[2], aq[CT], ak[CT];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) qk[j] = kk[j] = zero4();
+  for (int j = 0; j < 2; ++j) qk[j] = kk[j] = zero4();
 #pragma unroll
   for (int i = 0; i < CT; ++i) aq[i] = ak[i] = zero4();
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    const bs_parts<PI> qf = delta_frags<PI>(w.qp + kb + row * DK + 32 * s + 8 * g, kChunk * DK);
-    const bs_parts<PI> kf = delta_frags<PI>(w.kp + kb + row * DK + 32 * s + 8 * g, kChunk * DK);
+    const uint16_t* p = w.kp + kb + lane * 8 + s * kFrag;
+    const bs_parts<PI> qf = delta_frags<PI>(w.qp + kb + lane * 8 + (t * KS + s) * kFrag, kChunk * DK);
+    const bs_parts<PI> kf = delta_frags<PI>(p + t * KS * kFrag, kChunk * DK);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j <= wave) {
-        const bs_parts<PI> b =
-            delta_frags<PI>(w.kp + kb + (16 * j + m) * DK + 32 * s + 8 * g, kChunk * DK);
-        qk[j] = bs_mma<2>(qf, b, qk[j]);
-        kk[j] = bs_mma<2>(kf, b, kk[j]);
+    for (int j = 0; j < 2; ++j)
+      if (j < nj) {
+        const bs_parts<PI> a = delta_frags<PI>(p + (j0 + j) * KS * kFrag, kChunk * DK);
+        qk[j] = bs_mma<2>(a, qf, qk[j]);
+        kk[j] = bs_mma<2>(a, kf, kk[j]);
       }
   }
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
     const int64_t sh = (int64_t)slot * in.hv + h;
     const float* co = w.coef + sh * kCoef;
+    const double* run = (const double*)(co + kRun * kChunk);
     const float* us = keep_u + sh * kChunk * dvp;
     const float* dr = w.dr + sh * kChunk * dvp;
-    const float* s0 = keep_s + sh * DK * dvp;
-    const float* ds = w.ds + sh * DK * dvp;
-    const T* gp = go + ((sp.batch * plan.tokens + t0 + (live ? row : 0)) * in.hv + h) * in.dv;
-    const T* vp = (const T*)in.v + bs_delta_at(in.v_stride, sp.batch, t0 + (live ? row : 0), h);
-    if (tid < kChunk) run[tid] = ((const double*)(co + 4 * kChunk))[tid];
-    bs_f32x4 xq[CT], xs[CT], xr[CT], da[4], dl[4];
+    const float* s0 = keep_s + (sh * DK + half * (DK / 2)) * dvp;
+    const float* ds = w.ds + (sh * DK + half * (DK / 2)) * dvp;
+    const T* gp = go + ((sp.batch * plan.tokens + t0 + (live ? tok : 0)) * in.hv + h) * in.dv;
+    const T* vp = (const T*)in.v + bs_delta_at(in.v_stride, sp.batch, t0 + (live ? tok : 0), h);
+    bs_f32x4 xq[CT], xs[CT], xr[CT], da[2], dl[2];
     float dot_s = 0.f, dot_v = 0.f;
 #pragma unroll
     for (int i = 0; i < CT; ++i) xq[i] = xs[i] = xr[i] = zero4();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) da[j] = dl[j] = zero4();
+    for (int j = 0; j < 2; ++j) da[j] = dl[j] = zero4();
     for (int e = 0; e < dvp; e += 32) {
       const int d = e + 8 * g, left = live ? in.dv - d : 0;
       const bs_parts<PI> of = load_parts<PI>(gp + d, left, vec);
-      const float4 r0 = *(const float4*)(dr + row * dvp + d),
-                   r1 = *(const float4*)(dr + row * dvp + d + 4);
+      const float4 r0 = *(const float4*)(dr + tok * dvp + d),
+                   r1 = *(const float4*)(dr + tok * dvp + d + 4);
       const bs_parts<3> rf = row_parts(r0, r1);
-      const bs_parts<3> uf = row_parts(us + row * dvp + d);
-      const float rr[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+      const bs_parts<3> uf = row_parts(us + tok * dvp + d);
+      if (((e >> 5) & 1) == half) {
+        const float rr[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < left) dot_v = fmaf(rr[j], bs_to_f32(vp[d + j]), dot_v);
+        for (int j = 0; j < 8; ++j)
+          if (j < left) dot_v = fmaf(rr[j], bs_to_f32(vp[d + j]), dot_v);
+      }
 #pragma unroll
       for (int i = 0; i < CT; ++i) {
-        const int64_t at = (int64_t)(16 * i + m) * dvp + d;
+        const int64_t at = (int64_t)delta_row(i, m) * dvp + d;
         const float4 a0 = *(const float4*)(s0 + at), a1 = *(const float4*)(s0 + at + 4);
         const float4 b0 = *(const float4*)(ds + at), b1 = *(const float4*)(ds + at + 4);
-        if ((i & 3) == wave) {
+        if (i == t) {
           float x = a0.x * b0.x;
           x = fmaf(a0.y, b0.y, x), x = fmaf(a0.z, b0.z, x), x = fmaf(a0.w, b0.w, x);
           x = fmaf(a1.x, b1.x, x), x = fmaf(a1.y, b1.y, x), x = fmaf(a1.z, b1.z, x);
           dot_s += fmaf(a1.w, b1.w, x);
         }
         const bs_parts<3> sf = row_parts(a0, a1), df = row_parts(b0, b1);
-        xq[i] = bs_mma<2>(of, sf, xq[i]);
-        xr[i] = bs_mma<2>(rf, sf, xr[i]);
-        xs[i] = bs_mma<2>(uf, df, xs[i]);
+        xq[i] = bs_mma<2>(sf, of, xq[i]);
+        xr[i] = bs_mma<2>(sf, rf, xr[i]);
+        xs[i] = bs_mma<2>(df, uf, xs[i]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j <= wave) {
-          const bs_parts<3> b = row_parts(us + (16 * j + m) * dvp + d);
-          da[j] = bs_mma<2>(of, b, da[j]);
-          dl[j] = bs_mma<2>(rf, b, dl[j]);
+      for (int j = 0; j < 2; ++j)
+        if (j < nj) {
+          const bs_parts<3> a = row_parts(us + delta_row(j0 + j, m) * dvp + d);
+          da[j] = bs_mma<2>(a, of, da[j]);
+          dl[j] = bs_mma<2>(a, rf, dl[j]);
         }
     }
-    const float4 grow = *(const float4*)(co + out0), lft = *(const float4*)(co + kChunk + out0),
-                 beta = *(const float4*)(co + 2 * kChunk + out0);
-    const float* gr = (const float*)&grow;
-    const float* lf = (const float*)&lft;
-    const float* be = (const float*)&beta;
-    // terms of the state products, by rows out0 + r
-    float drun[4] = {0.f, 0.f, 0.f, 0.f}, db[4] = {0.f, 0.f, 0.f, 0.f}, dtot = 0.f;
+    // the masked products of this wave, to LDS by rows
+    const float grow = co[kGrow * kChunk + tok], beta = co[kBeta * kChunk + tok];
+    const double run_i = run[tok];
+    float db = 0.f;
 #pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      const int64_t at = kb + (int64_t)(16 * i + m) * kChunk + out0;
-      const bs_f32x4 k4 = column4<PI>(w.kt + at, DK * kChunk);
-      const bs_f32x4 q4 = column4<PI>(w.qt + at, DK * kChunk);
+    for (int j = 0; j < 2; ++j)
+      if (j < nj) {
+        const int jj = 32 * ((j0 + j) >> 1) + 8 * g + 4 * ((j0 + j) & 1);
+        float p[4], q[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float a = in.scale * gr[r] * xq[i][r], b = gr[r] * xr[i][r], s = lf[r] * xs[i][r];
-        aq[i][r] += a;
-        ak[i][r] += s - be[r] * b;
-        drun[r] += q4[r] * a - k4[r] * (be[r] * b + s);
-        db[r] -= k4[r] * b;
-        dtot = fmaf(k4[r], s, dtot);
-      }
-    }
-    dtot += co[3 * kChunk] * dot_s;
-    __syncthreads();                // run
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float cs = 0.f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = out0 + r, jj = 16 * j + m;
-        float p = 0.f, q = 0.f;
-        if (j <= wave && jj <= i) {
-          const float e = expf((float)(run[i] - run[jj]));
-          p = in.scale * e * da[j][r];
-          const float x = jj < i ? -dl[j][r] * e : 0.f;
-          q = be[r] * x;
-          const float both = p * qk[j][r] + q * kk[j][r];
-          db[r] = fmaf(x, kk[j][r], db[r]);
-          drun[r] += both;
-          cs += both;
+        for (int r = 0; r < 4; ++r) {
+          const float e = jj + r <= tok ? expf((float)(run_i - run[jj + r])) : 0.f;
+          const float x = jj + r < tok ? -dl[j][r] * e : 0.f;
+          p[r] = in.scale * e * da[j][r];
+          q[r] = beta * x;
+          db = fmaf(x, kk[j][r], db);
         }
-        lp[i][jj] = p, lm[i][jj] = q;
+        *(float4*)&lp[tok][jj] = make_float4(p[0], p[1], p[2], p[3]);
+        *(float4*)&lm[tok][jj] = make_float4(q[0], q[1], q[2], q[3]);
       }
-      cs = sum4(cs);
-      if (g == 0) cols[wave][16 * j + m] = cs;
+    // factors of the state products, and what they give beta and the chunk's total
+    const float fq = in.scale * grow, fr = -beta * grow, fs = co[kLeft * kChunk + tok];
+    float kx = 0.f, kt = 0.f;
+    bs_parts<PI> kf[HS], qf[HS];
+#pragma unroll
+    for (int s = 0; s < HS; ++s) {
+      const int64_t at = kb + lane * 8 + (t * KS + half * HS + s) * kFrag;
+      kf[s] = delta_frags<PI>(w.kp + at, kChunk * DK);
+      qf[s] = delta_frags<PI>(w.qp + at, kChunk * DK);
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      drun[r] = sum16(drun[r]);
-      db[r] = sum16(db[r]);
-      if (m == 0) rows[out0 + r] = drun[r], bsum[out0 + r] = db[r];
-    }
-    dtot = sum4(sum16(dtot));
-    if (lane == 0) tot[wave] = dtot;
-    dot_v = sum4(dot_v);
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float k = frag_value(kf[i >> 1], 4 * (i & 1) + r);
+        kx = fmaf(k, xr[i][r], kx);
+        xq[i][r] *= fq, xr[i][r] *= fr, xs[i][r] *= fs;
+        kt = fmaf(k, xs[i][r], kt);
+      }
+    db -= grow * kx;
     __syncthreads();
-    if (g == 0 && live)
-      bs_store_any(dbeta, in.beta_dtype, (sp.batch * plan.tokens + t0 + row) * in.hv + h,
-                   bsum[row] + dot_v);
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const int y = 32 * st + 8 * g;
+      if (st <= blk) {             // rows of the masked products: this tile's tokens as i
+        const bs_parts<3> pf = row_parts(&lp[tok][y]), mf = row_parts(&lm[tok][y]);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          const bs_parts<PI> a = delta_frags<PI>(
+              w.kt + kb + lane * 8 + ((half * CT + i) * 2 + st) * kFrag, kChunk * DK);
+          xq[i] = bs_mma<2>(a, pf, xq[i]);
+          xr[i] = bs_mma<2>(a, mf, xr[i]);
+        }
+      }
+      if (st >= blk) {             // columns: as j
+        float p[8], q[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) p[x] = lp[y + x][tok], q[x] = lm[y + x][tok];
+        const bs_parts<3> pf = bs_split8<3>(p), mf = bs_split8<3>(q);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          const int64_t at = kb + lane * 8 + ((half * CT + i) * 2 + st) * kFrag;
+          xs[i] = bs_mma<2>(delta_frags<PI>(w.qt + at, kChunk * DK), pf, xs[i]);
+          xs[i] = bs_mma<2>(delta_frags<PI>(w.kt + at, kChunk * DK), mf, xs[i]);
+        }
+      }
+    }
+    float drun = 0.f;
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int e = 4 * (i & 1) + r;
+        drun = fmaf(frag_value(qf[i >> 1], e), xq[i][r], drun);
+        drun = fmaf(frag_value(kf[i >> 1], e), xr[i][r] - xs[i][r], drun);
+        aq[i][r] += xq[i][r];
+        ak[i][r] += xr[i][r] + xs[i][r];
+      }
+    drun = sum4(drun);
+    db = sum4(db + dot_v);
+    if (g == 0) rows[half][tok] = drun, betas[half][tok] = db;
+    kt = fmaf(co[kTotal * kChunk], dot_s, kt);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) kt += __shfl_xor(kt, x);
+    if (lane == 0) tot[wave] = kt;
+    __syncthreads();
     if (wave == 0) {
-      double x = (double)rows[lane] - cols[0][lane] - cols[1][lane] - cols[2][lane] -
-                 cols[3][lane];
-      if (lane == 63) x += (double)tot[0] + tot[1] + tot[2] + tot[3];
+      double x = (double)rows[0][lane] + rows[1][lane];
+      if (lane == 63) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x += tot[i];
+      }
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const double y = __shfl_down(x, d);
         if (lane + d < 64) x += y;
       }
-      if (lane < len)
-        bs_store_any(dg, in.g_dtype, (sp.batch * plan.tokens + t0 + lane) * in.hv + h, (float)x);
-    }
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const int j0 = 32 * st + 8 * g;
-      float sym[8], pt[8];
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        sym[x] = lm[row][j0 + x] + lm[j0 + x][row];
-        pt[x] = lp[j0 + x][row];
-      }
-      const bs_parts<3> pf = row_parts(&lp[row][j0]);
-      const bs_parts<3> sf = bs_split8<3>(sym), tf = bs_split8<3>(pt);
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        const int64_t at = kb + (int64_t)(16 * i + m) * kChunk + j0;
-        const bs_parts<PI> kf = delta_frags<PI>(w.kt + at, DK * kChunk);
-        if (st <= blk) aq[i] = bs_mma<2>(pf, kf, aq[i]);
-        ak[i] = bs_mma<2>(sf, kf, ak[i]);
-        if (st >= blk)
-          ak[i] = bs_mma<2>(tf, delta_frags<PI>(w.qt + at, DK * kChunk), ak[i]);
+      if (lane < len) {
+        const int64_t at = (sp.batch * plan.tokens + t0 + lane) * in.hv + h;
+        bs_store_any(dg, in.g_dtype, at, (float)x);
+        bs_store_any(dbeta, in.beta_dtype, at, betas[0][lane] + betas[1][lane]);
       }
     }
-    __syncthreads();
   }
+  if (!live) return;
 #pragma unroll
-  for (int i = 0; i < CT; ++i) {
-    const int d = 16 * i + m;
-    if (d >= in.dk) continue;
+  for (int s = 0; s < HS; ++s) {
+    const int d = 32 * (half * HS + s) + 8 * g;
+    const int64_t at = ((sp.batch * plan.tokens + t0 + tok) * in.hk + hk) * in.dk + d;
+    T x[8], y[8];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (out0 + r < len) {
-        const int64_t at = ((sp.batch * plan.tokens + t0 + out0 + r) * in.hk + hk) * in.dk + d;
-        dq[at] = bs_from_f32<T>(aq[i][r]);
-        dk[at] = bs_from_f32<T>(ak[i][r]);
-      }
+    for (int e = 0; e < 8; ++e) {
+      x[e] = bs_from_f32<T>(aq[2 * s + (e >> 2)][e & 3]);
+      y[e] = bs_from_f32<T>(ak[2 * s + (e >> 2)][e & 3]);
+    }
+    if (d + 8 <= in.dk) {
+      __builtin_memcpy(dq + at, x, sizeof(x));
+      __builtin_memcpy(dk + at, y, sizeof(y));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (d + e < in.dk) dq[at + e] = x[e], dk[at + e] = y[e];
+    }
   }
 }
 
@@ -397,11 +477,12 @@ void launch_grad(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork& 
                  const DeltaSizes& z, const void* go, const float* gstate, const float* keep_s,
                  const float* keep_u, const GradOut& o, hipStream_t st) {
   const unsigned extra = plan.offsets ? 1 : 0;
-  grad_chain_kernel<T, PI, KS><<<dim3(z.dvp / 16, in.hv, plan.seqs + extra), 256, 0, st>>>(
-      in, plan, w, (const T*)go, gstate, (T*)o.dv, o.dstate, z.dvp);
+  const int units = (plan.seqs + (int)extra) * in.hv;
+  grad_chain_kernel<T, PI, KS><<<delta_grid(units, z.dvp / 16), 256, 0, st>>>(
+      in, plan, w, (const T*)go, gstate, (T*)o.dv, o.dstate, z.dvp, units);
   if (plan.slots + extra == 0) return;
   const int vec = in.dv % 8 == 0 && (uintptr_t)go % 16 == 0;
-  grad_chunk_kernel<T, PI, KS><<<dim3(plan.slots + extra, in.hk), 256, 0, st>>>(
+  grad_chunk_kernel<T, PI, KS><<<dim3(plan.slots + extra, in.hk), 512, 0, st>>>(
       in, plan, w, (const T*)go, keep_s, keep_u, (T*)o.dq, (T*)o.dk, o.dg, o.dbeta, z.dvp, vec);
 }
 
