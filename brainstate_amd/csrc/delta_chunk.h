@@ -137,6 +137,61 @@ int delta_check_chunked(const bs_delta_in* in, int seqs, int tokens, const int32
 int delta_prepare(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork& w,
                   const DeltaSizes& z, int backward, hipStream_t st);
 
+// Four rows of one column of a chunk, 0 past the last row and past the last column: buffer loads,
+// whose bounds the hardware checks, so that the loads of a chunk stay free of branches (at a
+// branch every load in flight is waited for).
+template <typename T>
+struct DeltaRows {
+  const char* base;        // the first chunk's first row
+  int64_t step;            // bytes of a chunk's rows
+  int bytes, row;          // of a row's columns; from row to row
+  uint32_t at[4];
+  __device__ __forceinline__ DeltaRows(const T* first, int64_t stride, int out0, int col, int dv) {
+    base = (const char*)first;
+    row = (int)(stride * sizeof(T));
+    step = (int64_t)kChunk * stride * sizeof(T);
+    bytes = dv * (int)sizeof(T);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      at[r] = col < dv ? (uint32_t)(out0 + r) * (uint32_t)row + col * (uint32_t)sizeof(T)
+                       : 0xFFFFFFF0u;
+  }
+  // of chunk c of a sequence of `len`, raw
+  __device__ __forceinline__ void load(int c, int len, float* x) const {
+    const int rows = min(len - c * kChunk, kChunk);
+    const uint32_t n = (uint32_t)(rows - 1) * (uint32_t)row + (uint32_t)bytes;
+    __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(base + c * step), 0, n, 0x00027000);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (sizeof(T) == 4)
+        x[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, at[r], 0, 0));
+      else
+        x[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b16(rs, at[r], 0, 0));
+    }
+  }
+  // what load gave, as numbers
+  static __device__ __forceinline__ float value(float x) {
+    if constexpr (sizeof(T) == 4) return x;
+    else return bs_to_f32(T{(uint16_t)__float_as_uint(x)});
+  }
+};
+
+// Kept matrices (states, U, dR: rows x dvp) are laid out as the backward pass's products over the
+// value columns take them: fragment (t, s) has rows delta_row(t, .) and columns 32s + 8g .. + 7,
+// in two halves of 4 columns, 1 KB each.  delta_kept is the place of the 4 columns 4g .. 4g + 3 of
+// a slice of 16, row delta_row(t, m).
+__device__ __forceinline__ int delta_kept(int t, int slice, int lane, int dvp) {
+  const int m = lane & 15, g = lane >> 4;
+  return (((t * (dvp >> 5) + (slice >> 1)) * 2 + (g & 1)) * 64 + 16 * (2 * (slice & 1) + (g >> 1)) +
+          m) * 4;
+}
+// The 8 values of lane's fragment (t, s).
+__device__ __forceinline__ const float* delta_kept_frag(const float* p, int t, int s, int lane,
+                                                        int dvp) {
+  return p + ((t * (dvp >> 5) + s) * 2 * 64 + lane) * 4;
+}
+
 __device__ __forceinline__ bs_f32x4 zero4() { return bs_f32x4{0.f, 0.f, 0.f, 0.f}; }
 
 // Parts of 8 floats in two vectors.
@@ -180,6 +235,21 @@ __device__ __forceinline__ DeltaPlace delta_place(int slices) {
 }
 static inline unsigned delta_grid(int64_t units, int slices) {
   return (unsigned)((units + 7) / 8 * 8 * slices);
+}
+
+// The 16 columns' rows of tile 2s + odd of an operand over 32 rows, transposed: its product with
+// 1, exact.  A lane receives 4 columns of row delta_row(.., m).
+__device__ __forceinline__ bs_f32x4 delta_turn(const bs_parts<3>& x, int odd, int lane) {
+  const int m = lane & 15, g = lane >> 4;
+  bs_u16x8 one;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) one[e] = g == m >> 2 && e == 4 * odd + (m & 3) ? 0x3F80 : 0;
+  const bs_bf16x8 b = __builtin_bit_cast(bs_bf16x8, one);
+  bs_f32x4 r = zero4();
+#pragma unroll
+  for (int p = 2; p >= 0; --p)
+    r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[p], b, r, 0, 0, 0);
+  return r;
 }
 
 // Rows of a packed batch before the first sequence and after the last one are no sequence's:

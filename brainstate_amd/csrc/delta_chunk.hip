@@ -191,24 +191,25 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
   }
 }
 
-// Forward over the chunks of one sequence, value head and slice of 16 value columns.  Each of 4
-// waves has 16 tokens of a chunk and a quarter of the state's rows; what the others need goes
-// through LDS, as parts and in the lane that takes it.  Operands that do not depend on the state
-// are loaded into registers a chunk ahead, each as soon as its last use is issued.  The output
-// is formed transposed (the operands of a product swapped), which leaves 4 neighbouring columns
-// of a token in a lane.
-template <typename T, int PI, int KS>
-__global__ __launch_bounds__(256) void chain_kernel(bs_delta_in in, DeltaPlan plan, DeltaWork w,
-                                                    const float* state0, float* state1, T* o,
-                                                    float* keep_s, float* keep_u, int dvp,
-                                                    int units, int vec) {
+// Forward over the chunks of one sequence, value head and slice of 16 value columns, by two sets
+// of 4 waves.  The first has the recurrence: each wave 16 tokens of a chunk and a quarter of the
+// state's rows; what the others need goes through LDS, as parts and in the lane that takes it.
+// The second forms from the same LDS what the recurrence does not wait for: the output and, for
+// the backward pass, U and the state before the chunk, transposed (the operands of a product
+// swapped; for the state, times 1), which leaves 4 neighbouring columns of a row in a lane.  So
+// no wave of the recurrence waits for a store, and a SIMD has two waves to issue from: the
+// recurrence's own arithmetic (products of 3 parts, splitting) leaves it idle half the time.
+// Operands that do not depend on the state are loaded into registers a chunk ahead.
+template <typename T, int PI, int KS, bool KEEP>
+__global__ __launch_bounds__(512, PI == 1 ? 4 : 2) void chain_kernel(
+    bs_delta_in in, DeltaPlan plan, DeltaWork w, const float* state0, float* state1, T* o,
+    float* keep_s, float* keep_u, int dvp, int units, int vec) {
   constexpr int DK = KS * 32, TW = KS / 2, PO = PI == 3 ? 3 : 2;
   constexpr int kS = KS * 128, kR = 2 * 128;       // words of a part
-  __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];
-  __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];
-  __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];
-  __shared__ __attribute__((aligned(16))) uint2 lv[PO * kR];
-  __shared__ __attribute__((aligned(16))) float turn[4][16][20];
+  __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];     // the state
+  __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];     // R
+  __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];     // exp(total - run) U
+  __shared__ __attribute__((aligned(16))) uint2 lv[PO * kR];    // U
   const DeltaPlace at = delta_place(dvp / 16);
   if (at.unit >= units) return;
   const int h = at.unit % in.hv, n = at.unit / in.hv, hk = h / (in.hv / in.hk);
@@ -217,185 +218,201 @@ __global__ __launch_bounds__(256) void chain_kernel(bs_delta_in in, DeltaPlan pl
     return;
   }
   const DeltaSpan sp = delta_span(plan, n);
-  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), blk = wave >> 1;
-  const int col = at.slice * 16 + m, ocol = at.slice * 16 + 4 * g;
-  const bool live = col < in.dv;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int role = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3), blk = wave >> 1;
   const int tok = delta_row(wave, m);                      // the row this lane feeds
-  const int out0 = 32 * blk + 8 * g + 4 * (wave & 1);      // the 4 rows it receives
-  const int own = (blk * 64 + lane) * 2 + (wave & 1);
+  const int64_t keys = (int64_t)in.hk * PI * kChunk * DK;  // from chunk to chunk
+  const int64_t kb = ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK;
+  const int64_t hb = (int64_t)sp.slot * in.hv + h;
+  const float* cp = w.coef + hb * kCoef;
+  const uint16_t* ip = w.inv + hb * 3 * kSquare + lane * 8;
 
-  bs_f32x4 s[TW];
-  int d0[TW], sown[TW];
+  if (role == 0) {
+    const int col = at.slice * 16 + m;
+    const bool live = col < in.dv;
+    const int out0 = 32 * blk + 8 * g + 4 * (wave & 1);    // the 4 rows it receives
+    const int own = (blk * 64 + lane) * 2 + (wave & 1);
+    bs_f32x4 s[TW];
+    int d0[TW], sown[TW];
 #pragma unroll
-  for (int i = 0; i < TW; ++i) {
-    const int t = TW * wave + i;
-    d0[i] = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
-    sown[i] = ((t >> 1) * 64 + lane) * 2 + (t & 1);
+    for (int i = 0; i < TW; ++i) {
+      const int t = TW * wave + i;
+      d0[i] = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
+      sown[i] = ((t >> 1) * 64 + lane) * 2 + (t & 1);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      s[i][r] = state0 && d0[i] + r < in.dk && live
-          ? state0[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] : 0.f;
-    delta_put<3>(ls + sown[i], kS, s[i]);
-  }
-
-  const uint16_t* kp = w.kp + ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK + wave * KS * kFrag;
-  const uint16_t* qp = w.qp + ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK + wave * KS * kFrag;
-  const uint16_t* kt = w.kt + ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK +
-                       wave * TW * 2 * kFrag;
-  const uint16_t* ip = w.inv + ((int64_t)sp.slot * in.hv + h) * 3 * kSquare +
-                       delta_lower(wave, 0) * kFrag;
-  const uint16_t* ap = w.att + ((int64_t)sp.slot * in.hv + h) * PO * kSquare +
-                       delta_lower(wave, 0) * kFrag;
-  const float* cp = w.coef + ((int64_t)sp.slot * in.hv + h) * kCoef;
-  const T* vp = (const T*)in.v + bs_delta_at(in.v_stride, sp.batch, sp.first, h) +
-                min(col, in.dv - 1);
-  const int64_t keys = (int64_t)in.hk * PI * kChunk * DK;
-  bs_parts<PI> kf[KS], qf[KS], ktf[TW][2];
-  bs_parts<3> tf[2];
-  bs_parts<PO> af[2];
-  T vr[4];
-  float4 grow, left, beta;
-  float total, scale;
-  auto load_keys = [&](int c) {
-#pragma unroll
-    for (int st = 0; st < KS; ++st) {
-      kf[st] = delta_frags<PI>(kp + c * keys + st * kFrag + lane * 8, kChunk * DK);
-      qf[st] = delta_frags<PI>(qp + c * keys + st * kFrag + lane * 8, kChunk * DK);
+      for (int r = 0; r < 4; ++r)
+        s[i][r] = state0 && d0[i] + r < in.dk && live
+            ? state0[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] : 0.f;
+      delta_put<3>(ls + sown[i], kS, s[i]);
     }
-  };
-  auto load_values = [&](int c) {
+    const uint16_t* kp = w.kp + kb + wave * KS * kFrag + lane * 8;
+    const uint16_t* kt = w.kt + kb + wave * TW * 2 * kFrag + lane * 8;
+    const DeltaRows<T> rows((const T*)in.v + bs_delta_at(in.v_stride, sp.batch, sp.first, h),
+                            in.v_stride[1], out0, col, in.dv);
+    bs_parts<PI> kf[KS], ktf[TW][2];
+    bs_parts<3> tf[2];
+    float vr[4], total;
+    float4 grow, left, beta;
+    auto load_keys = [&](int c) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      vr[r] = vp[min(c * kChunk + out0 + r, sp.len - 1) * in.v_stride[1]];
-    const float* co = cp + (int64_t)c * in.hv * kCoef;
-    grow = *(const float4*)(co + kGrow * kChunk + out0);
-    left = *(const float4*)(co + kLeft * kChunk + out0);
-    beta = *(const float4*)(co + kBeta * kChunk + out0);
-    scale = in.scale * co[kGrow * kChunk + tok];
-    total = co[kTotal * kChunk];
-  };
-  auto load_inverse = [&](int c) {
+      for (int st = 0; st < KS; ++st)
+        kf[st] = delta_frags<PI>(kp + c * keys + st * kFrag, kChunk * DK);
+    };
+    auto load_values = [&](int c) {
+      const float* co = cp + (int64_t)c * in.hv * kCoef;
+      rows.load(c, sp.len, vr);
+      grow = *(const float4*)(co + kGrow * kChunk + out0);
+      left = *(const float4*)(co + kLeft * kChunk + out0);
+      beta = *(const float4*)(co + kBeta * kChunk + out0);
+      total = co[kTotal * kChunk];
+    };
+    auto load_inverse = [&](int c) {
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
-      if (st <= blk)
-        tf[st] = delta_frags<3>(ip + (int64_t)c * in.hv * 3 * kSquare + st * kFrag + lane * 8,
-                                kSquare);
-  };
-  auto load_columns = [&](int c) {
+      for (int st = 0; st < 2; ++st)
+        tf[st] = delta_frags<3>(ip + (int64_t)c * in.hv * 3 * kSquare +
+                                    delta_lower(wave, min(st, blk)) * kFrag, kSquare);
+    };
+    auto load_columns = [&](int c) {
 #pragma unroll
-    for (int i = 0; i < 2 * TW; ++i)
-      ktf[i >> 1][i & 1] = delta_frags<PI>(kt + c * keys + i * kFrag + lane * 8, kChunk * DK);
-  };
-  auto load_masked = [&](int c) {
+      for (int i = 0; i < 2 * TW; ++i)
+        ktf[i >> 1][i & 1] = delta_frags<PI>(kt + c * keys + i * kFrag, kChunk * DK);
+    };
+    if (sp.chunks) {
+      load_keys(0);
+      load_values(0);
+      load_inverse(0);
+      load_columns(0);
+    }
+    __syncthreads();
+    for (int c = 0; c < sp.chunks; ++c) {
+      const int next = min(c + 1, sp.chunks - 1);
+      bs_f32x4 x = zero4(), u = zero4();
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
-      if (st <= blk)
-        af[st] = delta_frags<PO>(ap + (int64_t)c * in.hv * PO * kSquare + st * kFrag + lane * 8,
-                                 kSquare);
-  };
-  // a 16 x 16 tile with its rows r0 + 0..15 (in delta_row order) to row-major memory
-  auto keep = [&](float* to, int t, const bs_f32x4& x) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) turn[wave][4 * g + r][m] = x[r];
-    __builtin_amdgcn_wave_barrier();     // one wave's LDS accesses are done in order
-    *(float4*)(to + (int64_t)delta_row(t, m) * dvp + ocol) = *(const float4*)&turn[wave][m][4 * g];
-  };
-  if (sp.chunks) {
-    load_keys(0);
-    load_values(0);
-    load_inverse(0);
-    load_columns(0);
-    load_masked(0);
-  }
-  __syncthreads();
-  for (int c = 0; c < sp.chunks; ++c) {
-    const int next = min(c + 1, sp.chunks - 1);
-    const int64_t sh = (int64_t)(sp.slot + c) * in.hv + h;
-    bs_f32x4 ks = zero4(), qs = zero4(), u = zero4();
-    bs_parts<3> sf[KS];
-#pragma unroll
-    for (int st = 0; st < KS; ++st) sf[st] = delta_lds<3>(ls + (st * 64 + lane) * 2, kS);
-#pragma unroll
-    for (int st = 0; st < KS; ++st) ks = bs_mma<2>(kf[st], sf[st], ks);
-    {
-      bs_f32x4 x;
+      for (int st = 0; st < KS; ++st)
+        x = bs_mma<2>(kf[st], delta_lds<3>(ls + (st * 64 + lane) * 2, kS), x);
       const float* gr = (const float*)&grow;
       const float* be = (const float*)&beta;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float v = c * kChunk + out0 + r < sp.len && live ? bs_to_f32(vr[r]) : 0.f;
-        x[r] = be[r] * fmaf(-gr[r], ks[r], v);
-      }
+      for (int r = 0; r < 4; ++r) x[r] = be[r] * fmaf(-gr[r], x[r], rows.value(vr[r]));
       delta_put<3>(lr + own, kR, x);
-    }
-    // the state's part of the output, while the others arrive
+      __builtin_amdgcn_sched_barrier(0);   // loads after what the others wait for
+      const float4 lf4 = left;
+      const float all = total;
+      load_values(next);
+      load_keys(next);
+      __syncthreads();                     // R
 #pragma unroll
-    for (int st = 0; st < KS; ++st) qs = bs_mma<PO - 1>(sf[st], qf[st], qs);
-    load_keys(next);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) qs[r] *= scale;
-    const float4 lf4 = left;
-    const float all = total;
-    load_values(next);
-    __syncthreads();
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-      if (st <= blk) u = bs_mma<2>(tf[st], delta_lds<3>(lr + (st * 64 + lane) * 2, kR), u);
-    {
-      bs_f32x4 x;
+      for (int st = 0; st < 2; ++st)
+        if (st <= blk)
+          u = bs_mma<2>(tf[st], delta_lds<3>(lr + (st * 64 + lane) * 2, kR), u);
       const float* lf = (const float*)&lf4;
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = lf[r] * u[r];
       delta_put<3>(lu + own, kR, x);
       delta_put<PO>(lv + own, kR, u);
+      __builtin_amdgcn_sched_barrier(0);
+      load_inverse(next);
+      __syncthreads();                     // U; the state's last readers are through
+#pragma unroll
+      for (int i = 0; i < TW; ++i) s[i] *= all;
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const bs_parts<3> b = delta_lds<3>(lu + (st * 64 + lane) * 2, kR);
+#pragma unroll
+        for (int i = 0; i < TW; ++i) s[i] = bs_mma<2>(ktf[i][st], b, s[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < TW; ++i) delta_put<3>(ls + sown[i], kS, s[i]);
+      __builtin_amdgcn_sched_barrier(0);
+      load_columns(next);
+      __syncthreads();                     // the state
     }
-    load_inverse(next);
-    if (keep_s) {
-      keep(keep_u + sh * kChunk * dvp, wave, u);
+    if (state1 && live) {
 #pragma unroll
-      for (int i = 0; i < TW; ++i) keep(keep_s + sh * DK * dvp, TW * wave + i, s[i]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < TW; ++i) s[i] *= all;
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const bs_parts<3> b = delta_lds<3>(lu + (st * 64 + lane) * 2, kR);
-#pragma unroll
-      for (int i = 0; i < TW; ++i) s[i] = bs_mma<2>(ktf[i][st], b, s[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < TW; ++i) delta_put<3>(ls + sown[i], kS, s[i]);
-    load_columns(next);
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-      if (st <= blk)
-        qs = bs_mma<PO - 1>(delta_lds<PO>(lv + (st * 64 + lane) * 2, kR), af[st], qs);
-    load_masked(next);
-    if (c * kChunk + tok < sp.len) {
-      T* op = o + ((sp.batch * plan.tokens + sp.first + c * kChunk + tok) * in.hv + h) * in.dv +
-              ocol;
-      T y[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = bs_from_f32<T>(qs[r]);
-      if (vec) {
-        if (ocol < in.dv) __builtin_memcpy(__builtin_assume_aligned(op, 4 * sizeof(T)), y, sizeof(y));
-      } else {
+      for (int i = 0; i < TW; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (ocol + r < in.dv) op[r] = y[r];
-      }
+          if (d0[i] + r < in.dk)
+            state1[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] = s[i][r];
     }
+  } else {
+    const int ocol = at.slice * 16 + 4 * g;
+    const uint16_t* qp = w.qp + kb + wave * KS * kFrag + lane * 8;
+    const uint16_t* ap = w.att + hb * PO * kSquare + lane * 8;
+    bs_parts<PI> qf[KS];
+    bs_parts<PO> af[2];
+    bs_parts<3> tf[2];
+    float scale;
+    auto load_keys = [&](int c) {
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+        qf[st] = delta_frags<PI>(qp + c * keys + st * kFrag, kChunk * DK);
+      scale = in.scale * cp[(int64_t)c * in.hv * kCoef + kGrow * kChunk + tok];
+    };
+    auto load_squares = [&](int c) {
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const int f = delta_lower(wave, min(st, blk)) * kFrag;
+        af[st] = delta_frags<PO>(ap + (int64_t)c * in.hv * PO * kSquare + f, kSquare);
+        if (KEEP) tf[st] = delta_frags<3>(ip + (int64_t)c * in.hv * 3 * kSquare + f, kSquare);
+      }
+    };
+    if (sp.chunks) {
+      load_keys(0);
+      load_squares(0);
+    }
+    T* op = o + ((sp.batch * plan.tokens + sp.first + tok) * in.hv + h) * in.dv + ocol;
     __syncthreads();
-  }
-  if (state1 && live) {
+    for (int c = 0; c < sp.chunks; ++c) {
+      const int next = min(c + 1, sp.chunks - 1);
+      const int64_t sh = hb + (int64_t)c * in.hv;
+      bs_f32x4 y = zero4();
 #pragma unroll
-    for (int i = 0; i < TW; ++i)
+      for (int st = 0; st < KS; ++st)
+        y = bs_mma<PO - 1>(delta_lds<PO>(ls + (st * 64 + lane) * 2, kS), qf[st], y);
+      if (KEEP) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (d0[i] + r < in.dk)
-          state1[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] = s[i][r];
+        for (int i = 0; i < TW; ++i) {
+          const int t = TW * wave + i;
+          const bs_f32x4 x = delta_turn(delta_lds<3>(ls + ((t >> 1) * 64 + lane) * 2, kS), t & 1, lane);
+          *(bs_f32x4*)(keep_s + sh * DK * dvp + delta_kept(t, at.slice, lane, dvp)) = x;
+        }
+      }
+      const float f = scale;
+      load_keys(next);
+      __syncthreads();                     // R
+      if (KEEP) {
+        bs_f32x4 u = zero4();
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+          if (st <= blk)
+            u = bs_mma<2>(delta_lds<3>(lr + (st * 64 + lane) * 2, kR), tf[st], u);
+        *(bs_f32x4*)(keep_u + sh * kChunk * dvp + delta_kept(wave, at.slice, lane, dvp)) = u;
+      }
+      y *= f;
+      __syncthreads();                     // U
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+        if (st <= blk)
+          y = bs_mma<PO - 1>(delta_lds<PO>(lv + (st * 64 + lane) * 2, kR), af[st], y);
+      load_squares(next);
+      if (c * kChunk + tok < sp.len) {
+        T* p = op + (int64_t)c * kChunk * in.hv * in.dv;
+        T z[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[r] = bs_from_f32<T>(y[r]);
+        if (vec) {
+          if (ocol < in.dv)
+            __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(T)), z, sizeof(z));
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (ocol + r < in.dv) p[r] = z[r];
+        }
+      }
+      __syncthreads();                     // the state
+    }
   }
 }
 
@@ -414,9 +431,14 @@ void launch_chain(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork&
                   const DeltaSizes& z, const float* s0, float* s1, void* o, float* keep_s,
                   float* keep_u, hipStream_t st) {
   const int units = (plan.seqs + (plan.offsets ? 1 : 0)) * in.hv;
-  chain_kernel<T, PI, KS><<<delta_grid(units, z.dvp / 16), 256, 0, st>>>(
-      in, plan, w, s0, s1, (T*)o, keep_s, keep_u, z.dvp, units,
-      in.dv % 4 == 0 && (uintptr_t)o % (4 * sizeof(T)) == 0);
+  const int vec = in.dv % 4 == 0 && (uintptr_t)o % (4 * sizeof(T)) == 0;
+  const unsigned grid = delta_grid(units, z.dvp / 16);
+  if (keep_s)
+    chain_kernel<T, PI, KS, true><<<grid, 512, 0, st>>>(in, plan, w, s0, s1, (T*)o, keep_s,
+                                                        keep_u, z.dvp, units, vec);
+  else
+    chain_kernel<T, PI, KS, false><<<grid, 512, 0, st>>>(in, plan, w, s0, s1, (T*)o, keep_s,
+                                                         keep_u, z.dvp, units, vec);
 }
 
 template <typename T, int PI>
@@ -450,6 +472,9 @@ int delta_check_chunked(const bs_delta_in* in, int seqs, int tokens, const int32
                         const char* who) {
   if (int rc = bs_delta_check(in, who)) return rc;
   BS_CHECK_ARG(seqs >= 0 && tokens >= 0, "%s: %d sequences, %d tokens", who, seqs, tokens);
+  // a chunk's rows are addressed in 32 bits
+  BS_CHECK_ARG(in->v_stride[1] >= 0 && in->v_stride[1] < (1 << 23) && in->hv * in->dv < (1 << 23),
+               "%s: %lld elements from token to token", who, (long long)in->v_stride[1]);
   const int64_t slots = offsets ? (int64_t)tokens / kChunk + seqs
                                 : (int64_t)seqs * ((tokens + kChunk - 1) / kChunk);
   BS_CHECK_ARG(slots <= 0x7FFFFFFF / kChunk && in->hv <= 65535 &&

@@ -24,21 +24,20 @@
 
 namespace {
 
-// Chunks of one sequence, value head and slice of 16 value columns, last to first; waves and
-// operands as in the forward pass.
+// Chunks of one sequence, value head and slice of 16 value columns, last to first, by two sets of
+// 4 waves as in the forward pass: the first has the recurrence, the second forms dR again for the
+// gradient of v and the chunk's gradients, and keeps the gradient of the state.
 template <typename T, int PI, int KS>
-__global__ __launch_bounds__(256) void grad_chain_kernel(bs_delta_in in, DeltaPlan plan,
-                                                         DeltaWork w, const T* go,
-                                                         const float* gstate, T* dv,
-                                                         float* dstate, int dvp, int units) {
+__global__ __launch_bounds__(512, 2) void grad_chain_kernel(
+    bs_delta_in in, DeltaPlan plan, DeltaWork w, const T* go, const float* gstate, T* dv,
+    float* dstate, int dvp, int units, int vec) {
   constexpr int DK = KS * 32, TW = KS / 2;
   constexpr int kS = KS * 128, kR = 2 * 128;       // words of a part
-  __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];
-  __shared__ __attribute__((aligned(16))) uint2 lo[PI * kR];
-  __shared__ __attribute__((aligned(16))) uint2 lg[2][3 * kR];
-  __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];
-  __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];
-  __shared__ __attribute__((aligned(16))) float turn[4][16][20];
+  __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];        // dS
+  __shared__ __attribute__((aligned(16))) uint2 lo[PI * kR];       // dO
+  __shared__ __attribute__((aligned(16))) uint2 lg[2][3 * kR];     // scale G dO
+  __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];        // dU
+  __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];        // -beta G dR
   const DeltaPlace at = delta_place(dvp / 16);
   if (at.unit >= units) return;
   const int h = at.unit % in.hv, n = at.unit / in.hv, hk = h / (in.hv / in.hk);
@@ -47,171 +46,190 @@ __global__ __launch_bounds__(256) void grad_chain_kernel(bs_delta_in in, DeltaPl
     return;
   }
   const DeltaSpan sp = delta_span(plan, n);
-  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), blk = wave >> 1;
-  const int col = at.slice * 16 + m;
-  const bool live = col < in.dv;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int role = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3), blk = wave >> 1;
   const int tok = delta_row(wave, m);
-  const int out0 = 32 * blk + 8 * g + 4 * (wave & 1);
-  const int own = (blk * 64 + lane) * 2 + (wave & 1);
-
-  bs_f32x4 s[TW];
-  int d0[TW];
-#pragma unroll
-  for (int i = 0; i < TW; ++i) {
-    const int t = TW * wave + i;
-    d0[i] = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      s[i][r] = gstate && d0[i] + r < in.dk && live
-          ? gstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] : 0.f;
-    delta_put<3>(ls + ((t >> 1) * 64 + lane) * 2 + (t & 1), kS, s[i]);
-  }
-  const uint16_t* kp = w.kp + ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK + wave * KS * kFrag;
-  const int64_t tb = ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK + wave * TW * 2 * kFrag;
-  const int64_t sq = ((int64_t)sp.slot * in.hv + h) * 3 * kSquare;
-  const float* cp = w.coef + ((int64_t)sp.slot * in.hv + h) * kCoef;
-  const T* gp = go + ((sp.batch * plan.tokens + sp.first) * in.hv + h) * in.dv +
-                min(col, in.dv - 1);
   const int64_t keys = (int64_t)in.hk * PI * kChunk * DK;
-  bs_parts<PI> kf[KS], ktf[TW][2], qtf[TW][2];
-  bs_parts<3> tf[2], af[2];
-  T gr[4];
-  float4 coef[3];
-  float total, token_beta;
-  auto load_keys = [&](int c) {
-#pragma unroll
-    for (int st = 0; st < KS; ++st)
-      kf[st] = delta_frags<PI>(kp + c * keys + st * kFrag + lane * 8, kChunk * DK);
-  };
-  auto load_grad = [&](int c) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      gr[r] = gp[(int64_t)min(c * kChunk + out0 + r, sp.len - 1) * in.hv * in.dv];
-    const float* co = cp + (int64_t)c * in.hv * kCoef;
-    coef[0] = *(const float4*)(co + kGrow * kChunk + out0);
-    coef[1] = *(const float4*)(co + kLeft * kChunk + out0);
-    coef[2] = *(const float4*)(co + kBeta * kChunk + out0);
-    total = co[kTotal * kChunk];
-    token_beta = co[kBeta * kChunk + tok];
-  };
+  const int64_t kb = ((int64_t)sp.slot * in.hk + hk) * PI * kChunk * DK;
+  const int64_t hb = (int64_t)sp.slot * in.hv + h;
+  const float* cp = w.coef + hb * kCoef;
   auto load_square = [&](const uint16_t* a, int c, bs_parts<3>* f) {
 #pragma unroll
     for (int st = 0; st < 2; ++st)
-      if (st >= blk)
-        f[st] = delta_frags<3>(a + sq + (int64_t)c * in.hv * 3 * kSquare +
-                                   delta_upper(wave, st) * kFrag + lane * 8, kSquare);
+      f[st] = delta_frags<3>(a + (hb + (int64_t)c * in.hv) * 3 * kSquare +
+                                 delta_upper(wave, max(st, blk)) * kFrag + lane * 8, kSquare);
   };
-  auto load_columns = [&](int c) {
-#pragma unroll
-    for (int i = 0; i < 2 * TW; ++i) {
-      const int64_t a = tb + c * keys + i * kFrag + lane * 8;
-      ktf[i >> 1][i & 1] = delta_frags<PI>(w.kt + a, kChunk * DK);
-      qtf[i >> 1][i & 1] = delta_frags<PI>(w.qt + a, kChunk * DK);
-    }
-  };
-  auto keep = [&](float* to, int t, const bs_f32x4& x) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) turn[wave][4 * g + r][m] = x[r];
-    __builtin_amdgcn_wave_barrier();     // one wave's LDS accesses are done in order
-    *(float4*)(to + (int64_t)delta_row(t, m) * dvp + at.slice * 16 + 4 * g) =
-        *(const float4*)&turn[wave][m][4 * g];
-  };
-  float grow[4], left[4], beta[4], all = 0.f, mine = 0.f;
-  // dO of a chunk and scale G dO, into LDS
-  auto stage = [&](int c) {
-    grow[0] = coef[0].x, grow[1] = coef[0].y, grow[2] = coef[0].z, grow[3] = coef[0].w;
-    left[0] = coef[1].x, left[1] = coef[1].y, left[2] = coef[1].z, left[3] = coef[1].w;
-    beta[0] = coef[2].x, beta[1] = coef[2].y, beta[2] = coef[2].z, beta[3] = coef[2].w;
-    all = total, mine = token_beta;
-    bs_f32x4 x, y;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      x[r] = c * kChunk + out0 + r < sp.len && live ? bs_to_f32(gr[r]) : 0.f;
-      y[r] = in.scale * grow[r] * x[r];
-    }
-    delta_put<PI>(lo + own, kR, x);
-    delta_put<3>(lg[c & 1] + own, kR, y);
-  };
-  if (const int c = sp.chunks - 1; c >= 0) {
-    load_grad(c);
-    load_keys(c);
-    load_square(w.att, c, af);
-    load_square(w.inv, c, tf);
-    load_columns(c);
-    stage(c);
-    load_grad(max(c - 1, 0));
-  }
-  __syncthreads();
-  for (int c = sp.chunks - 1; c >= 0; --c) {
-    const int next = max(c - 1, 0);
-    const int64_t sh = (int64_t)(sp.slot + c) * in.hv + h;
-    bs_f32x4 du = zero4(), dr = zero4(), x;
-#pragma unroll
-    for (int st = 0; st < KS; ++st)
-      du = bs_mma<2>(kf[st], delta_lds<3>(ls + (st * 64 + lane) * 2, kS), du);
-    load_keys(next);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) du[r] *= left[r];
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-      if (st >= blk) du = bs_mma<2>(af[st], delta_lds<PI>(lo + (st * 64 + lane) * 2, kR), du);
-    load_square(w.att, next, af);
-    delta_put<3>(lu + own, kR, du);
-#pragma unroll
-    for (int i = 0; i < TW; ++i) keep(w.ds + sh * DK * dvp, TW * wave + i, s[i]);
-    __syncthreads();
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-      if (st >= blk) dr = bs_mma<2>(tf[st], delta_lds<3>(lu + (st * 64 + lane) * 2, kR), dr);
-    load_square(w.inv, next, tf);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = -grow[r] * (beta[r] * dr[r]);
-    delta_put<3>(lr + own, kR, x);
-    keep(w.dr + sh * kChunk * dvp, wave, dr);
-    {                                // the tile is still in `turn`, by tokens
-      const int t = c * kChunk + delta_row(wave, m), oc = at.slice * 16 + 4 * g;
-      if (t < sp.len) {
-        const float4 d4 = *(const float4*)&turn[wave][m][4 * g];
-        const float* d = (const float*)&d4;
-        T* op = dv + ((sp.batch * plan.tokens + sp.first + t) * in.hv + h) * in.dv + oc;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (oc + r < in.dv) op[r] = bs_from_f32<T>(mine * d[r]);
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < TW; ++i) s[i] *= all;
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const bs_parts<3> a = delta_lds<3>(lg[c & 1] + (st * 64 + lane) * 2, kR);
-      const bs_parts<3> b = delta_lds<3>(lr + (st * 64 + lane) * 2, kR);
-#pragma unroll
-      for (int i = 0; i < TW; ++i) {
-        s[i] = bs_mma<2>(qtf[i][st], a, s[i]);
-        s[i] = bs_mma<2>(ktf[i][st], b, s[i]);
-      }
-    }
-    load_columns(next);
+
+  if (role == 0) {
+    const int col = at.slice * 16 + m;
+    const bool live = col < in.dv;
+    const int out0 = 32 * blk + 8 * g + 4 * (wave & 1);
+    const int own = (blk * 64 + lane) * 2 + (wave & 1);
+    bs_f32x4 s[TW];
+    int d0[TW], sown[TW];
 #pragma unroll
     for (int i = 0; i < TW; ++i) {
       const int t = TW * wave + i;
-      delta_put<3>(ls + ((t >> 1) * 64 + lane) * 2 + (t & 1), kS, s[i]);
-    }
-    if (c) {
-      stage(next);
-      load_grad(max(c - 2, 0));
-    }
-    __syncthreads();
-  }
-  if (dstate && live) {
-#pragma unroll
-    for (int i = 0; i < TW; ++i)
+      d0[i] = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
+      sown[i] = ((t >> 1) * 64 + lane) * 2 + (t & 1);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (d0[i] + r < in.dk)
-          dstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] = s[i][r];
+        s[i][r] = gstate && d0[i] + r < in.dk && live
+            ? gstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] : 0.f;
+      delta_put<3>(ls + sown[i], kS, s[i]);
+    }
+    const uint16_t* kp = w.kp + kb + wave * KS * kFrag + lane * 8;
+    const int64_t tb = kb + wave * TW * 2 * kFrag + lane * 8;
+    const DeltaRows<T> rows(go + ((sp.batch * plan.tokens + sp.first) * in.hv + h) * in.dv,
+                            (int64_t)in.hv * in.dv, out0, col, in.dv);
+    bs_parts<PI> kf[KS], ktf[TW][2], qtf[TW][2];
+    bs_parts<3> tf[2], af[2];
+    float gr[4], total, all = 0.f;
+    float4 coef[3], now[3];
+    auto load_keys = [&](int c) {
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+        kf[st] = delta_frags<PI>(kp + c * keys + st * kFrag, kChunk * DK);
+    };
+    auto load_grad = [&](int c) {
+      const float* co = cp + (int64_t)c * in.hv * kCoef;
+      rows.load(c, sp.len, gr);
+      coef[0] = *(const float4*)(co + kGrow * kChunk + out0);
+      coef[1] = *(const float4*)(co + kLeft * kChunk + out0);
+      coef[2] = *(const float4*)(co + kBeta * kChunk + out0);
+      total = co[kTotal * kChunk];
+    };
+    auto load_columns = [&](int c) {
+#pragma unroll
+      for (int i = 0; i < 2 * TW; ++i) {
+        ktf[i >> 1][i & 1] = delta_frags<PI>(w.kt + tb + c * keys + i * kFrag, kChunk * DK);
+        qtf[i >> 1][i & 1] = delta_frags<PI>(w.qt + tb + c * keys + i * kFrag, kChunk * DK);
+      }
+    };
+    // dO of the chunk that was loaded, and scale G dO, into LDS; its factors are the next ones
+    auto stage = [&](int buf) {
+      bs_f32x4 x, y;
+      const float* gw = (const float*)&coef[0];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[r] = rows.value(gr[r]);
+        y[r] = in.scale * gw[r] * x[r];
+      }
+      delta_put<PI>(lo + own, kR, x);
+      delta_put<3>(lg[buf] + own, kR, y);
+      now[0] = coef[0], now[1] = coef[1], now[2] = coef[2], all = total;
+    };
+    if (const int c = sp.chunks - 1; c >= 0) {
+      load_grad(c);
+      load_keys(c);
+      load_square(w.att, c, af);
+      load_square(w.inv, c, tf);
+      load_columns(c);
+      stage(c & 1);
+      load_grad(max(c - 1, 0));
+    }
+    __syncthreads();
+    for (int c = sp.chunks - 1; c >= 0; --c) {
+      const int next = max(c - 1, 0);
+      bs_f32x4 du = zero4(), dr = zero4();
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+        du = bs_mma<2>(kf[st], delta_lds<3>(ls + (st * 64 + lane) * 2, kS), du);
+      const float* lf = (const float*)&now[1];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) du[r] *= lf[r];
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+        if (st >= blk) du = bs_mma<2>(af[st], delta_lds<PI>(lo + (st * 64 + lane) * 2, kR), du);
+      delta_put<3>(lu + own, kR, du);
+      __builtin_amdgcn_sched_barrier(0);
+      load_keys(next);
+      load_square(w.att, next, af);
+      __syncthreads();                     // dU; dO's last readers are through
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+        if (st >= blk) dr = bs_mma<2>(tf[st], delta_lds<3>(lu + (st * 64 + lane) * 2, kR), dr);
+      const float* gw = (const float*)&now[0];
+      const float* be = (const float*)&now[2];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) dr[r] *= -gw[r] * be[r];
+      delta_put<3>(lr + own, kR, dr);
+      __builtin_amdgcn_sched_barrier(0);
+      load_square(w.inv, next, tf);
+      __syncthreads();                     // dR; the state's last readers are through
+#pragma unroll
+      for (int i = 0; i < TW; ++i) s[i] *= all;
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const bs_parts<3> a = delta_lds<3>(lg[c & 1] + (st * 64 + lane) * 2, kR);
+        const bs_parts<3> b = delta_lds<3>(lr + (st * 64 + lane) * 2, kR);
+#pragma unroll
+        for (int i = 0; i < TW; ++i) {
+          s[i] = bs_mma<2>(qtf[i][st], a, s[i]);
+          s[i] = bs_mma<2>(ktf[i][st], b, s[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < TW; ++i) delta_put<3>(ls + sown[i], kS, s[i]);
+      stage((c - 1) & 1);                  // past chunk 0: what no one reads
+      __builtin_amdgcn_sched_barrier(0);
+      load_columns(next);
+      load_grad(max(c - 2, 0));
+      __syncthreads();                     // the state
+    }
+    if (dstate && live) {
+#pragma unroll
+      for (int i = 0; i < TW; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (d0[i] + r < in.dk)
+            dstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] = s[i][r];
+    }
+  } else {
+    const int ocol = at.slice * 16 + 4 * g;
+    bs_parts<3> tf[2];
+    float beta;
+    T* op = dv + ((sp.batch * plan.tokens + sp.first + tok) * in.hv + h) * in.dv + ocol;
+    if (const int c = sp.chunks - 1; c >= 0) {
+      load_square(w.inv, c, tf);
+      beta = cp[(int64_t)c * in.hv * kCoef + kBeta * kChunk + tok];
+    }
+    __syncthreads();
+    for (int c = sp.chunks - 1; c >= 0; --c) {
+      const int next = max(c - 1, 0);
+      const int64_t sh = hb + (int64_t)c * in.hv;
+#pragma unroll
+      for (int i = 0; i < TW; ++i) {
+        const int t = TW * wave + i;
+        const bs_f32x4 x = delta_turn(delta_lds<3>(ls + ((t >> 1) * 64 + lane) * 2, kS), t & 1, lane);
+        *(bs_f32x4*)(w.ds + sh * DK * dvp + delta_kept(t, at.slice, lane, dvp)) = x;
+      }
+      __syncthreads();                     // dU
+      bs_f32x4 dr = zero4();
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+        if (st >= blk) dr = bs_mma<2>(delta_lds<3>(lu + (st * 64 + lane) * 2, kR), tf[st], dr);
+      load_square(w.inv, next, tf);
+      *(bs_f32x4*)(w.dr + sh * kChunk * dvp + delta_kept(wave, at.slice, lane, dvp)) = dr;
+      if (c * kChunk + tok < sp.len) {
+        T* p = op + (int64_t)c * kChunk * in.hv * in.dv;
+        T z[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[r] = bs_from_f32<T>(beta * dr[r]);
+        if (vec) {
+          if (ocol < in.dv)
+            __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(T)), z, sizeof(z));
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (ocol + r < in.dv) p[r] = z[r];
+        }
+      }
+      beta = cp[(int64_t)next * in.hv * kCoef + kBeta * kChunk + tok];
+      __syncthreads();                     // dR
+      __syncthreads();                     // the state
+    }
   }
 }
 
@@ -297,8 +315,8 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
     const double* run = (const double*)(co + kRun * kChunk);
     const float* us = keep_u + sh * kChunk * dvp;
     const float* dr = w.dr + sh * kChunk * dvp;
-    const float* s0 = keep_s + (sh * DK + half * (DK / 2)) * dvp;
-    const float* ds = w.ds + (sh * DK + half * (DK / 2)) * dvp;
+    const float* s0 = keep_s + sh * DK * dvp;
+    const float* ds = w.ds + sh * DK * dvp;
     const T* gp = go + ((sp.batch * plan.tokens + t0 + (live ? tok : 0)) * in.hv + h) * in.dv;
     const T* vp = (const T*)in.v + bs_delta_at(in.v_stride, sp.batch, t0 + (live ? tok : 0), h);
     bs_f32x4 xq[CT], xs[CT], xr[CT], da[2], dl[2];
@@ -310,10 +328,11 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
     for (int e = 0; e < dvp; e += 32) {
       const int d = e + 8 * g, left = live ? in.dv - d : 0;
       const bs_parts<PI> of = load_parts<PI>(gp + d, left, vec);
-      const float4 r0 = *(const float4*)(dr + tok * dvp + d),
-                   r1 = *(const float4*)(dr + tok * dvp + d + 4);
+      const float* rp = delta_kept_frag(dr, t, e >> 5, lane, dvp);
+      const float* up = delta_kept_frag(us, t, e >> 5, lane, dvp);
+      const float4 r0 = *(const float4*)rp, r1 = *(const float4*)(rp + 256);
       const bs_parts<3> rf = row_parts(r0, r1);
-      const bs_parts<3> uf = row_parts(us + tok * dvp + d);
+      const bs_parts<3> uf = row_parts(*(const float4*)up, *(const float4*)(up + 256));
       if (((e >> 5) & 1) == half) {
         const float rr[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
@@ -322,9 +341,10 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
       }
 #pragma unroll
       for (int i = 0; i < CT; ++i) {
-        const int64_t at = (int64_t)delta_row(i, m) * dvp + d;
-        const float4 a0 = *(const float4*)(s0 + at), a1 = *(const float4*)(s0 + at + 4);
-        const float4 b0 = *(const float4*)(ds + at), b1 = *(const float4*)(ds + at + 4);
+        const float* sp0 = delta_kept_frag(s0, half * CT + i, e >> 5, lane, dvp);
+        const float* sp1 = delta_kept_frag(ds, half * CT + i, e >> 5, lane, dvp);
+        const float4 a0 = *(const float4*)sp0, a1 = *(const float4*)(sp0 + 256);
+        const float4 b0 = *(const float4*)sp1, b1 = *(const float4*)(sp1 + 256);
         if (i == t) {
           float x = a0.x * b0.x;
           x = fmaf(a0.y, b0.y, x), x = fmaf(a0.z, b0.z, x), x = fmaf(a0.w, b0.w, x);
@@ -339,7 +359,8 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         if (j < nj) {
-          const bs_parts<3> a = row_parts(us + delta_row(j0 + j, m) * dvp + d);
+          const float* jp = delta_kept_frag(us, j0 + j, e >> 5, lane, dvp);
+          const bs_parts<3> a = row_parts(*(const float4*)jp, *(const float4*)(jp + 256));
           da[j] = bs_mma<2>(a, of, da[j]);
           dl[j] = bs_mma<2>(a, rf, dl[j]);
         }
@@ -478,8 +499,9 @@ void launch_grad(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork& 
                  const float* keep_u, const GradOut& o, hipStream_t st) {
   const unsigned extra = plan.offsets ? 1 : 0;
   const int units = (plan.seqs + (int)extra) * in.hv;
-  grad_chain_kernel<T, PI, KS><<<delta_grid(units, z.dvp / 16), 256, 0, st>>>(
-      in, plan, w, (const T*)go, gstate, (T*)o.dv, o.dstate, z.dvp, units);
+  grad_chain_kernel<T, PI, KS><<<delta_grid(units, z.dvp / 16), 512, 0, st>>>(
+      in, plan, w, (const T*)go, gstate, (T*)o.dv, o.dstate, z.dvp, units,
+      in.dv % 4 == 0 && (uintptr_t)o.dv % (4 * sizeof(T)) == 0);
   if (plan.slots + extra == 0) return;
   const int vec = in.dv % 8 == 0 && (uintptr_t)go % 16 == 0;
   grad_chunk_kernel<T, PI, KS><<<dim3(plan.slots + extra, in.hk), 512, 0, st>>>(
