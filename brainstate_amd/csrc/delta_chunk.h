@@ -3,6 +3,8 @@
 
 #include "delta.h"
 
+#include <type_traits>
+
 constexpr int kChunk = 64;   // tokens of a chunk
 constexpr int kCoef = 6 * kChunk;
 
@@ -21,13 +23,15 @@ __device__ __forceinline__ int delta_offset(const DeltaPlan& p, int n) {
   return min(max(p.offsets[n], 0), p.tokens);
 }
 
-// Sequence n: its first slot, batch row, first token and length.
+// Sequence n (the same in every lane): its first slot, batch row, first token and length.
 __device__ __forceinline__ DeltaSpan delta_span(const DeltaPlan& p, int n) {
+  n = __builtin_amdgcn_readfirstlane(n);
   DeltaSpan s;
   s.seq = n;
   if (p.offsets) {
-    const int a = delta_offset(p, n);
-    s.batch = 0, s.first = a, s.len = max(delta_offset(p, n + 1) - a, 0);
+    const int a = __builtin_amdgcn_readfirstlane(delta_offset(p, n));
+    const int b = __builtin_amdgcn_readfirstlane(delta_offset(p, n + 1));
+    s.batch = 0, s.first = a, s.len = max(b - a, 0);
     s.slot = a / kChunk + n;
     s.chunks = (s.len + kChunk - 1) / kChunk;
   } else {
@@ -142,12 +146,15 @@ int delta_prepare(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork&
 // branch every load in flight is waited for).
 template <typename T>
 struct DeltaRows {
-  const char* base;        // the first chunk's first row
+  using Raw = typename std::conditional<sizeof(T) == 4, float, uint16_t>::type;
+  uint64_t base;           // the first chunk's first row
   int64_t step;            // bytes of a chunk's rows
   int bytes, row;          // of a row's columns; from row to row
   uint32_t at[4];
   __device__ __forceinline__ DeltaRows(const T* first, int64_t stride, int out0, int col, int dv) {
-    base = (const char*)first;
+    const uint64_t p = (uint64_t)first;      // the same in every lane
+    base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_readfirstlane((int)p);
     row = (int)(stride * sizeof(T));
     step = (int64_t)kChunk * stride * sizeof(T);
     bytes = dv * (int)sizeof(T);
@@ -156,8 +163,8 @@ struct DeltaRows {
       at[r] = col < dv ? (uint32_t)(out0 + r) * (uint32_t)row + col * (uint32_t)sizeof(T)
                        : 0xFFFFFFF0u;
   }
-  // of chunk c of a sequence of `len`, raw
-  __device__ __forceinline__ void load(int c, int len, float* x) const {
+  // of chunk c of a sequence of `len`
+  __device__ __forceinline__ void load(int c, int len, Raw* x) const {
     const int rows = min(len - c * kChunk, kChunk);
     const uint32_t n = (uint32_t)(rows - 1) * (uint32_t)row + (uint32_t)bytes;
     __amdgpu_buffer_rsrc_t rs =
@@ -167,13 +174,13 @@ struct DeltaRows {
       if constexpr (sizeof(T) == 4)
         x[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, at[r], 0, 0));
       else
-        x[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b16(rs, at[r], 0, 0));
+        x[r] = __builtin_amdgcn_raw_buffer_load_b16(rs, at[r], 0, 0);
     }
   }
   // what load gave, as numbers
-  static __device__ __forceinline__ float value(float x) {
+  static __device__ __forceinline__ float value(Raw x) {
     if constexpr (sizeof(T) == 4) return x;
-    else return bs_to_f32(T{(uint16_t)__float_as_uint(x)});
+    else return bs_to_f32(T{x});
   }
 };
 
@@ -191,6 +198,10 @@ __device__ __forceinline__ const float* delta_kept_frag(const float* p, int t, i
                                                         int dvp) {
   return p + ((t * (dvp >> 5) + s) * 2 * 64 + lane) * 4;
 }
+
+// Waits for every load so far.  Ahead of a loop that keeps loads in flight: where the loop is
+// entered with loads of its own in flight, the compiler has to wait in it as if it always were.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
 __device__ __forceinline__ bs_f32x4 zero4() { return bs_f32x4{0.f, 0.f, 0.f, 0.f}; }
 
@@ -229,9 +240,9 @@ __device__ __forceinline__ bs_parts<PI> load_parts(const T* p, int left, bool ve
 // Workgroup of a grid of units x slices: the slices of a unit (one sequence and head) read the
 // same chunks, so they are given to one of the 8 XCDs, whose L2 then reads each chunk once.
 struct DeltaPlace { int unit, slice; };
-__device__ __forceinline__ DeltaPlace delta_place(int slices) {
+__device__ __forceinline__ DeltaPlace delta_place(int units, int slices) {
   const int k = blockIdx.x >> 3;
-  return {k / slices * 8 + (int)(blockIdx.x & 7), k % slices};
+  return {(int)(blockIdx.x & 7) * ((units + 7) >> 3) + k / slices, k % slices};
 }
 static inline unsigned delta_grid(int64_t units, int slices) {
   return (unsigned)((units + 7) / 8 * 8 * slices);
@@ -239,7 +250,8 @@ static inline unsigned delta_grid(int64_t units, int slices) {
 
 // The 16 columns' rows of tile 2s + odd of an operand over 32 rows, transposed: its product with
 // 1, exact.  A lane receives 4 columns of row delta_row(.., m).
-__device__ __forceinline__ bs_f32x4 delta_turn(const bs_parts<3>& x, int odd, int lane) {
+template <int P>
+__device__ __forceinline__ bs_f32x4 delta_turn(const bs_parts<P>& x, int odd, int lane) {
   const int m = lane & 15, g = lane >> 4;
   bs_u16x8 one;
 #pragma unroll
@@ -247,7 +259,7 @@ __device__ __forceinline__ bs_f32x4 delta_turn(const bs_parts<3>& x, int odd, in
   const bs_bf16x8 b = __builtin_bit_cast(bs_bf16x8, one);
   bs_f32x4 r = zero4();
 #pragma unroll
-  for (int p = 2; p >= 0; --p)
+  for (int p = P - 1; p >= 0; --p)
     r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[p], b, r, 0, 0, 0);
   return r;
 }

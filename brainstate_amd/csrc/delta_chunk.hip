@@ -199,20 +199,21 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
 // swapped; for the state, times 1), which leaves 4 neighbouring columns of a row in a lane.  So
 // no wave of the recurrence waits for a store, and a SIMD has two waves to issue from: the
 // recurrence's own arithmetic (products of 3 parts, splitting) leaves it idle half the time.
-// Operands that do not depend on the state are loaded into registers a chunk ahead.
+// Operands that do not depend on the state are loaded into registers one or two chunks ahead.
 template <typename T, int PI, int KS, bool KEEP>
-__global__ __launch_bounds__(512, PI == 1 ? 4 : 2) void chain_kernel(
+__global__ __launch_bounds__(512, 2) void chain_kernel(
     bs_delta_in in, DeltaPlan plan, DeltaWork w, const float* state0, float* state1, T* o,
     float* keep_s, float* keep_u, int dvp, int units, int vec) {
-  constexpr int DK = KS * 32, TW = KS / 2, PO = PI == 3 ? 3 : 2;
+  constexpr int DK = KS * 32, TW = KS / 2, PO = PI == 3 ? 3 : 2, PV = KEEP ? 3 : PO;
   constexpr int kS = KS * 128, kR = 2 * 128;       // words of a part
   __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];     // the state
   __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];     // R
   __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];     // exp(total - run) U
-  __shared__ __attribute__((aligned(16))) uint2 lv[PO * kR];    // U
-  const DeltaPlace at = delta_place(dvp / 16);
+  __shared__ __attribute__((aligned(16))) uint2 lv[PV * kR];    // U
+  const DeltaPlace at = delta_place(units, dvp / 16);
   if (at.unit >= units) return;
-  const int h = at.unit % in.hv, n = at.unit / in.hv, hk = h / (in.hv / in.hk);
+  const int h = __builtin_amdgcn_readfirstlane(at.unit % in.hv);
+  const int n = __builtin_amdgcn_readfirstlane(at.unit / in.hv), hk = h / (in.hv / in.hk);
   if (n >= plan.seqs) {
     zero_outside(plan, o, in.hv, in.dv, h, at.slice * 16, 16);
     return;
@@ -252,20 +253,19 @@ __global__ __launch_bounds__(512, PI == 1 ? 4 : 2) void chain_kernel(
                             in.v_stride[1], out0, col, in.dv);
     bs_parts<PI> kf[KS], ktf[TW][2];
     bs_parts<3> tf[2];
-    float vr[4], total;
-    float4 grow, left, beta;
+    struct Values { typename DeltaRows<T>::Raw v[4]; float total; float4 grow, left, beta; } values[2];
     auto load_keys = [&](int c) {
 #pragma unroll
       for (int st = 0; st < KS; ++st)
         kf[st] = delta_frags<PI>(kp + c * keys + st * kFrag, kChunk * DK);
     };
-    auto load_values = [&](int c) {
+    auto load_values = [&](int c, Values& x) {
       const float* co = cp + (int64_t)c * in.hv * kCoef;
-      rows.load(c, sp.len, vr);
-      grow = *(const float4*)(co + kGrow * kChunk + out0);
-      left = *(const float4*)(co + kLeft * kChunk + out0);
-      beta = *(const float4*)(co + kBeta * kChunk + out0);
-      total = co[kTotal * kChunk];
+      rows.load(c, sp.len, x.v);
+      x.grow = *(const float4*)(co + kGrow * kChunk + out0);
+      x.left = *(const float4*)(co + kLeft * kChunk + out0);
+      x.beta = *(const float4*)(co + kBeta * kChunk + out0);
+      x.total = co[kTotal * kChunk];
     };
     auto load_inverse = [&](int c) {
 #pragma unroll
@@ -278,44 +278,44 @@ __global__ __launch_bounds__(512, PI == 1 ? 4 : 2) void chain_kernel(
       for (int i = 0; i < 2 * TW; ++i)
         ktf[i >> 1][i & 1] = delta_frags<PI>(kt + c * keys + i * kFrag, kChunk * DK);
     };
+    const int last = sp.chunks - 1;
     if (sp.chunks) {
+      load_values(0, values[0]);
       load_keys(0);
-      load_values(0);
       load_inverse(0);
       load_columns(0);
+      load_values(min(1, last), values[1]);
     }
+    wait_loads();
     __syncthreads();
-    for (int c = 0; c < sp.chunks; ++c) {
-      const int next = min(c + 1, sp.chunks - 1);
+    auto step = [&](int c, Values& now) {
+      const int next = min(c + 1, last);
       bs_f32x4 x = zero4(), u = zero4();
 #pragma unroll
       for (int st = 0; st < KS; ++st)
         x = bs_mma<2>(kf[st], delta_lds<3>(ls + (st * 64 + lane) * 2, kS), x);
-      const float* gr = (const float*)&grow;
-      const float* be = (const float*)&beta;
+      const float* gr = (const float*)&now.grow;
+      const float* be = (const float*)&now.beta;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = be[r] * fmaf(-gr[r], x[r], rows.value(vr[r]));
+      for (int r = 0; r < 4; ++r) x[r] = be[r] * fmaf(-gr[r], x[r], rows.value(now.v[r]));
       delta_put<3>(lr + own, kR, x);
       __builtin_amdgcn_sched_barrier(0);   // loads after what the others wait for
-      const float4 lf4 = left;
-      const float all = total;
-      load_values(next);
       load_keys(next);
       __syncthreads();                     // R
 #pragma unroll
       for (int st = 0; st < 2; ++st)
         if (st <= blk)
           u = bs_mma<2>(tf[st], delta_lds<3>(lr + (st * 64 + lane) * 2, kR), u);
-      const float* lf = (const float*)&lf4;
+      const float* lf = (const float*)&now.left;
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = lf[r] * u[r];
       delta_put<3>(lu + own, kR, x);
-      delta_put<PO>(lv + own, kR, u);
+      delta_put<PV>(lv + own, kR, u);
       __builtin_amdgcn_sched_barrier(0);
       load_inverse(next);
       __syncthreads();                     // U; the state's last readers are through
 #pragma unroll
-      for (int i = 0; i < TW; ++i) s[i] *= all;
+      for (int i = 0; i < TW; ++i) s[i] *= now.total;
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         const bs_parts<3> b = delta_lds<3>(lu + (st * 64 + lane) * 2, kR);
@@ -326,8 +326,15 @@ __global__ __launch_bounds__(512, PI == 1 ? 4 : 2) void chain_kernel(
       for (int i = 0; i < TW; ++i) delta_put<3>(ls + sown[i], kS, s[i]);
       __builtin_amdgcn_sched_barrier(0);
       load_columns(next);
+      load_values(min(c + 2, last), now);
       __syncthreads();                     // the state
+    };
+    // two steps a turn, without a way out between them (see wait_loads)
+    for (int c = 0; c + 1 < sp.chunks; c += 2) {
+      step(c, values[0]);
+      step(c + 1, values[1]);
     }
+    if (sp.chunks & 1) step(last, values[0]);
     if (state1 && live) {
 #pragma unroll
       for (int i = 0; i < TW; ++i)
@@ -340,79 +347,72 @@ __global__ __launch_bounds__(512, PI == 1 ? 4 : 2) void chain_kernel(
     const int ocol = at.slice * 16 + 4 * g;
     const uint16_t* qp = w.qp + kb + wave * KS * kFrag + lane * 8;
     const uint16_t* ap = w.att + hb * PO * kSquare + lane * 8;
-    bs_parts<PI> qf[KS];
-    bs_parts<PO> af[2];
-    bs_parts<3> tf[2];
-    float scale;
-    auto load_keys = [&](int c) {
+    struct Operands { bs_parts<PI> q[KS]; bs_parts<PO> a[2]; float scale; } operands[2];
+    auto load = [&](int c, Operands& x) {
+      const int64_t ch = (int64_t)c * in.hv;
 #pragma unroll
       for (int st = 0; st < KS; ++st)
-        qf[st] = delta_frags<PI>(qp + c * keys + st * kFrag, kChunk * DK);
-      scale = in.scale * cp[(int64_t)c * in.hv * kCoef + kGrow * kChunk + tok];
-    };
-    auto load_squares = [&](int c) {
+        x.q[st] = delta_frags<PI>(qp + c * keys + st * kFrag, kChunk * DK);
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const int f = delta_lower(wave, min(st, blk)) * kFrag;
-        af[st] = delta_frags<PO>(ap + (int64_t)c * in.hv * PO * kSquare + f, kSquare);
-        if (KEEP) tf[st] = delta_frags<3>(ip + (int64_t)c * in.hv * 3 * kSquare + f, kSquare);
-      }
+      for (int st = 0; st < 2; ++st)
+        x.a[st] = delta_frags<PO>(ap + ch * PO * kSquare +
+                                      delta_lower(wave, min(st, blk)) * kFrag, kSquare);
+      x.scale = in.scale * cp[ch * kCoef + kGrow * kChunk + tok];
     };
+    const int last = sp.chunks - 1;
     if (sp.chunks) {
-      load_keys(0);
-      load_squares(0);
+      load(0, operands[0]);
+      load(min(1, last), operands[1]);
     }
     T* op = o + ((sp.batch * plan.tokens + sp.first + tok) * in.hv + h) * in.dv + ocol;
+    wait_loads();
     __syncthreads();
-    for (int c = 0; c < sp.chunks; ++c) {
-      const int next = min(c + 1, sp.chunks - 1);
+    // loads two chunks ahead: a load is not seen to arrive before the stores issued before it
+    auto step = [&](int c, Operands& now) {
       const int64_t sh = hb + (int64_t)c * in.hv;
+      __syncthreads();                     // R: from here the recurrence leaves the state alone
       bs_f32x4 y = zero4();
 #pragma unroll
       for (int st = 0; st < KS; ++st)
-        y = bs_mma<PO - 1>(delta_lds<PO>(ls + (st * 64 + lane) * 2, kS), qf[st], y);
+        y = bs_mma<PO - 1>(delta_lds<PO>(ls + (st * 64 + lane) * 2, kS), now.q[st], y);
+      y *= now.scale;
       if (KEEP) {
 #pragma unroll
         for (int i = 0; i < TW; ++i) {
           const int t = TW * wave + i;
-          const bs_f32x4 x = delta_turn(delta_lds<3>(ls + ((t >> 1) * 64 + lane) * 2, kS), t & 1, lane);
+          const bs_f32x4 x =
+              delta_turn(delta_lds<3>(ls + ((t >> 1) * 64 + lane) * 2, kS), t & 1, lane);
           *(bs_f32x4*)(keep_s + sh * DK * dvp + delta_kept(t, at.slice, lane, dvp)) = x;
         }
       }
-      const float f = scale;
-      load_keys(next);
-      __syncthreads();                     // R
-      if (KEEP) {
-        bs_f32x4 u = zero4();
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-          if (st <= blk)
-            u = bs_mma<2>(delta_lds<3>(lr + (st * 64 + lane) * 2, kR), tf[st], u);
-        *(bs_f32x4*)(keep_u + sh * kChunk * dvp + delta_kept(wave, at.slice, lane, dvp)) = u;
-      }
-      y *= f;
       __syncthreads();                     // U
 #pragma unroll
       for (int st = 0; st < 2; ++st)
         if (st <= blk)
-          y = bs_mma<PO - 1>(delta_lds<PO>(lv + (st * 64 + lane) * 2, kR), af[st], y);
-      load_squares(next);
+          y = bs_mma<PO - 1>(delta_lds<PO>(lv + (st * 64 + lane) * 2, kR), now.a[st], y);
+      load(min(c + 2, last), now);
+      if (KEEP) {
+        const bs_f32x4 u = delta_turn(delta_lds<PV>(lv + (blk * 64 + lane) * 2, kR), wave & 1, lane);
+        *(bs_f32x4*)(keep_u + sh * kChunk * dvp + delta_kept(wave, at.slice, lane, dvp)) = u;
+      }
       if (c * kChunk + tok < sp.len) {
         T* p = op + (int64_t)c * kChunk * in.hv * in.dv;
-        T z[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) z[r] = bs_from_f32<T>(y[r]);
         if (vec) {
-          if (ocol < in.dv)
-            __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(T)), z, sizeof(z));
+          if (ocol < in.dv) bs_store4(p, y);
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (ocol + r < in.dv) p[r] = z[r];
+            if (ocol + r < in.dv) p[r] = bs_from_f32<T>(y[r]);
         }
       }
       __syncthreads();                     // the state
+    };
+    // two steps a turn, without a way out between them (see wait_loads)
+    for (int c = 0; c + 1 < sp.chunks; c += 2) {
+      step(c, operands[0]);
+      step(c + 1, operands[1]);
     }
+    if (sp.chunks & 1) step(last, operands[0]);
   }
 }
 

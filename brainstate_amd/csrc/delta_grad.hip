@@ -38,9 +38,10 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
   __shared__ __attribute__((aligned(16))) uint2 lg[2][3 * kR];     // scale G dO
   __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];        // dU
   __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];        // -beta G dR
-  const DeltaPlace at = delta_place(dvp / 16);
+  const DeltaPlace at = delta_place(units, dvp / 16);
   if (at.unit >= units) return;
-  const int h = at.unit % in.hv, n = at.unit / in.hv, hk = h / (in.hv / in.hk);
+  const int h = __builtin_amdgcn_readfirstlane(at.unit % in.hv);
+  const int n = __builtin_amdgcn_readfirstlane(at.unit / in.hv), hk = h / (in.hv / in.hk);
   if (n >= plan.seqs) {
     zero_outside(plan, dv, in.hv, in.dv, h, at.slice * 16, 16);
     return;
@@ -85,20 +86,21 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
                             (int64_t)in.hv * in.dv, out0, col, in.dv);
     bs_parts<PI> kf[KS], ktf[TW][2], qtf[TW][2];
     bs_parts<3> tf[2], af[2];
-    float gr[4], total, all = 0.f;
-    float4 coef[3], now[3];
+    struct Values { typename DeltaRows<T>::Raw v[4]; float total; float4 coef[3]; } values[2];
+    float all = 0.f;
+    float4 now[3];
     auto load_keys = [&](int c) {
 #pragma unroll
       for (int st = 0; st < KS; ++st)
         kf[st] = delta_frags<PI>(kp + c * keys + st * kFrag, kChunk * DK);
     };
-    auto load_grad = [&](int c) {
+    auto load_grad = [&](int c, Values& x) {
       const float* co = cp + (int64_t)c * in.hv * kCoef;
-      rows.load(c, sp.len, gr);
-      coef[0] = *(const float4*)(co + kGrow * kChunk + out0);
-      coef[1] = *(const float4*)(co + kLeft * kChunk + out0);
-      coef[2] = *(const float4*)(co + kBeta * kChunk + out0);
-      total = co[kTotal * kChunk];
+      rows.load(c, sp.len, x.v);
+      x.coef[0] = *(const float4*)(co + kGrow * kChunk + out0);
+      x.coef[1] = *(const float4*)(co + kLeft * kChunk + out0);
+      x.coef[2] = *(const float4*)(co + kBeta * kChunk + out0);
+      x.total = co[kTotal * kChunk];
     };
     auto load_columns = [&](int c) {
 #pragma unroll
@@ -108,29 +110,32 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
       }
     };
     // dO of the chunk that was loaded, and scale G dO, into LDS; its factors are the next ones
-    auto stage = [&](int buf) {
+    auto stage = [&](int buf, const Values& v) {
       bs_f32x4 x, y;
-      const float* gw = (const float*)&coef[0];
+      const float* gw = (const float*)&v.coef[0];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[r] = rows.value(gr[r]);
+        x[r] = rows.value(v.v[r]);
         y[r] = in.scale * gw[r] * x[r];
       }
       delta_put<PI>(lo + own, kR, x);
       delta_put<3>(lg[buf] + own, kR, y);
-      now[0] = coef[0], now[1] = coef[1], now[2] = coef[2], all = total;
+      now[0] = v.coef[0], now[1] = v.coef[1], now[2] = v.coef[2], all = v.total;
     };
     if (const int c = sp.chunks - 1; c >= 0) {
-      load_grad(c);
+      load_grad(c, values[1]);
+      load_grad(max(c - 1, 0), values[0]);
       load_keys(c);
       load_square(w.att, c, af);
       load_square(w.inv, c, tf);
       load_columns(c);
-      stage(c & 1);
-      load_grad(max(c - 1, 0));
+      stage(c & 1, values[1]);
+      load_grad(max(c - 2, 0), values[1]);
     }
+    wait_loads();
     __syncthreads();
-    for (int c = sp.chunks - 1; c >= 0; --c) {
+    // `v` holds chunk c - 1, and then c - 3
+    auto step = [&](int c, Values& v) {
       const int next = max(c - 1, 0);
       bs_f32x4 du = zero4(), dr = zero4();
 #pragma unroll
@@ -172,12 +177,17 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
       }
 #pragma unroll
       for (int i = 0; i < TW; ++i) delta_put<3>(ls + sown[i], kS, s[i]);
-      stage((c - 1) & 1);                  // past chunk 0: what no one reads
+      stage((c - 1) & 1, v);               // past chunk 0: what no one reads
       __builtin_amdgcn_sched_barrier(0);
       load_columns(next);
-      load_grad(max(c - 2, 0));
+      load_grad(max(c - 3, 0), v);
       __syncthreads();                     // the state
+    };
+    for (int c = sp.chunks - 1; c > 0; c -= 2) {
+      step(c, values[0]);
+      step(c - 1, values[1]);
     }
+    if (sp.chunks & 1) step(0, values[0]);
     if (dstate && live) {
 #pragma unroll
       for (int i = 0; i < TW; ++i)
@@ -188,48 +198,55 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
     }
   } else {
     const int ocol = at.slice * 16 + 4 * g;
-    bs_parts<3> tf[2];
-    float beta;
+    struct Operands { bs_parts<3> t[2]; float beta; } operands[2];
+    auto load = [&](int c, Operands& x) {
+      load_square(w.inv, c, x.t);
+      x.beta = cp[(int64_t)c * in.hv * kCoef + kBeta * kChunk + tok];
+    };
     T* op = dv + ((sp.batch * plan.tokens + sp.first + tok) * in.hv + h) * in.dv + ocol;
     if (const int c = sp.chunks - 1; c >= 0) {
-      load_square(w.inv, c, tf);
-      beta = cp[(int64_t)c * in.hv * kCoef + kBeta * kChunk + tok];
+      load(c, operands[0]);
+      load(max(c - 1, 0), operands[1]);
     }
+    wait_loads();
     __syncthreads();
-    for (int c = sp.chunks - 1; c >= 0; --c) {
-      const int next = max(c - 1, 0);
+    auto step = [&](int c, Operands& now) {
       const int64_t sh = hb + (int64_t)c * in.hv;
 #pragma unroll
       for (int i = 0; i < TW; ++i) {
         const int t = TW * wave + i;
-        const bs_f32x4 x = delta_turn(delta_lds<3>(ls + ((t >> 1) * 64 + lane) * 2, kS), t & 1, lane);
+        const bs_f32x4 x =
+            delta_turn(delta_lds<3>(ls + ((t >> 1) * 64 + lane) * 2, kS), t & 1, lane);
         *(bs_f32x4*)(w.ds + sh * DK * dvp + delta_kept(t, at.slice, lane, dvp)) = x;
       }
       __syncthreads();                     // dU
       bs_f32x4 dr = zero4();
 #pragma unroll
       for (int st = 0; st < 2; ++st)
-        if (st >= blk) dr = bs_mma<2>(delta_lds<3>(lu + (st * 64 + lane) * 2, kR), tf[st], dr);
-      load_square(w.inv, next, tf);
+        if (st >= blk)
+          dr = bs_mma<2>(delta_lds<3>(lu + (st * 64 + lane) * 2, kR), now.t[st], dr);
+      const float beta = now.beta;
+      load(max(c - 2, 0), now);
       *(bs_f32x4*)(w.dr + sh * kChunk * dvp + delta_kept(wave, at.slice, lane, dvp)) = dr;
       if (c * kChunk + tok < sp.len) {
         T* p = op + (int64_t)c * kChunk * in.hv * in.dv;
-        T z[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) z[r] = bs_from_f32<T>(beta * dr[r]);
+        const bs_f32x4 y = beta * dr;
         if (vec) {
-          if (ocol < in.dv)
-            __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(T)), z, sizeof(z));
+          if (ocol < in.dv) bs_store4(p, y);
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (ocol + r < in.dv) p[r] = z[r];
+            if (ocol + r < in.dv) p[r] = bs_from_f32<T>(y[r]);
         }
       }
-      beta = cp[(int64_t)next * in.hv * kCoef + kBeta * kChunk + tok];
       __syncthreads();                     // dR
       __syncthreads();                     // the state
+    };
+    for (int c = sp.chunks - 1; c > 0; c -= 2) {
+      step(c, operands[0]);
+      step(c - 1, operands[1]);
     }
+    if (sp.chunks & 1) step(0, operands[0]);
   }
 }
 

@@ -36,6 +36,19 @@ __device__ __forceinline__ bs_f16 bs_from_f32<bs_f16>(float x) {
   return bs_f16{__builtin_bit_cast(uint16_t, (_Float16)x)};
 }
 
+// Four neighbouring values in one store; p is aligned to all four.
+template <typename T>
+__device__ __forceinline__ void bs_store4(T* p, const bs_f32x4& x) {
+  if constexpr (sizeof(T) == 4) {
+    *(bs_f32x4*)p = x;
+  } else {
+    uint2 v;
+    v.x = bs_from_f32<T>(x[0]).u | (uint32_t)bs_from_f32<T>(x[1]).u << 16;
+    v.y = bs_from_f32<T>(x[2]).u | (uint32_t)bs_from_f32<T>(x[3]).u << 16;
+    *(uint2*)p = v;
+  }
+}
+
 // Element i of an array whose type is known at run time (gates, norm weights).
 __device__ __forceinline__ float bs_load_any(const void* p, int dtype, int64_t i) {
   if (dtype == BS_F32) return ((const float*)p)[i];
