@@ -54,8 +54,7 @@ def _delta_operands(q, k, v, g, beta, scale):
     if any(x.device != dev for x in (k, v, g, beta)):
         raise ValueError('q, k, v, g and beta must be on one device')
     q, k, v = (x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous() for x in (q, k, v))
-    if v.stride(1) >= 1 << 23:
-        v = v.contiguous()
+    q, k, v = (x if x.stride(1) < 1 << 23 else x.contiguous() for x in (q, k, v))
     scale = dk ** -0.5 if scale is None else float(scale)
     packed = _DELTA_IN.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),

@@ -141,16 +141,16 @@ int delta_check_chunked(const bs_delta_in* in, int seqs, int tokens, const int32
 int delta_prepare(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork& w,
                   const DeltaSizes& z, int backward, hipStream_t st);
 
-// Four rows of one column of a chunk, 0 past the last row and past the last column: buffer loads,
+// Four rows of NT columns (16 apart) of a chunk, 0 past the last row and column: buffer loads,
 // whose bounds the hardware checks, so that the loads of a chunk stay free of branches (at a
 // branch every load in flight is waited for).
-template <typename T>
+template <typename T, int NT>
 struct DeltaRows {
   using Raw = typename std::conditional<sizeof(T) == 4, float, uint16_t>::type;
   uint64_t base;           // the first chunk's first row
   int64_t step;            // bytes of a chunk's rows
   int bytes, row;          // of a row's columns; from row to row
-  uint32_t at[4];
+  uint32_t at[NT][4];
   __device__ __forceinline__ DeltaRows(const T* first, int64_t stride, int out0, int col, int dv) {
     const uint64_t p = (uint64_t)first;      // the same in every lane
     base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
@@ -159,23 +159,27 @@ struct DeltaRows {
     step = (int64_t)kChunk * stride * sizeof(T);
     bytes = dv * (int)sizeof(T);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      at[r] = col < dv ? (uint32_t)(out0 + r) * (uint32_t)row + col * (uint32_t)sizeof(T)
-                       : 0xFFFFFFF0u;
+    for (int i = 0; i < NT; ++i, col += 16)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        at[i][r] = col < dv ? (uint32_t)(out0 + r) * (uint32_t)row + col * (uint32_t)sizeof(T)
+                            : 0xFFFFFFF0u;
   }
   // of chunk c of a sequence of `len`
-  __device__ __forceinline__ void load(int c, int len, Raw* x) const {
+  __device__ __forceinline__ void load(int c, int len, Raw (*x)[4]) const {
     const int rows = min(len - c * kChunk, kChunk);
     const uint32_t n = (uint32_t)(rows - 1) * (uint32_t)row + (uint32_t)bytes;
     __amdgpu_buffer_rsrc_t rs =
         __builtin_amdgcn_make_buffer_rsrc((void*)(base + c * step), 0, n, 0x00027000);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (sizeof(T) == 4)
-        x[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, at[r], 0, 0));
-      else
-        x[r] = __builtin_amdgcn_raw_buffer_load_b16(rs, at[r], 0, 0);
-    }
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (sizeof(T) == 4)
+          x[i][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, at[i][r], 0, 0));
+        else
+          x[i][r] = __builtin_amdgcn_raw_buffer_load_b16(rs, at[i][r], 0, 0);
+      }
   }
   // what load gave, as numbers
   static __device__ __forceinline__ float value(Raw x) {
@@ -214,28 +218,68 @@ __device__ __forceinline__ bs_parts<3> row_parts(const float* p) {
   return row_parts(*(const float4*)p, *(const float4*)(p + 4));
 }
 
-// 8 values of a row as parts, 0 past `left`.
-template <int PI, typename T>
-__device__ __forceinline__ bs_parts<PI> load_parts(const T* p, int left, bool vec) {
-  if constexpr (PI == 1) {
-    bs_u16x8 r = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (vec && left >= 8) {
-      r = *(const bs_u16x8*)p;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < left) r[j] = p[j].u;
-    }
-    bs_parts<1> o;
-    o.p[0] = __builtin_bit_cast(bs_bf16x8, r);
-    return o;
-  } else {
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < left ? bs_to_f32(p[j]) : 0.f;
-    return bs_split8<PI>(x);
+// Rows of a chunk, a lane one row: 8 neighbouring values of it, 0 past the row's end and past the
+// last row.  Buffer loads, whose bounds the hardware checks: no branches, so nothing waits.
+template <typename T>
+struct DeltaRow {
+  __amdgpu_buffer_rsrc_t rs;
+  uint32_t at;
+  int dim;              // 0 for a lane without a row
+  bool vec;             // rows start on 16 bytes and end on 8 values
+  __device__ __forceinline__ DeltaRow(const T* first, int64_t stride, int row, int rows, int d,
+                                      bool v) {
+    const uint32_t step = (uint32_t)(stride * sizeof(T));
+    const uint64_t p = (uint64_t)first;
+    const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((int)p);
+    rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)base, 0, (uint32_t)(rows - 1) * step + (uint32_t)(d * sizeof(T)), 0x00027000);
+    at = (uint32_t)row * step, dim = row < rows ? d : 0, vec = v;
   }
-}
+  // values d .. d + 7
+  __device__ __forceinline__ void raw(int d, uint4* x) const {
+    constexpr int W = sizeof(T) / 2;           // vectors of 16 bytes
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        x[i] = __builtin_bit_cast(
+            uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                       rs, d < dim ? at + d * (uint32_t)sizeof(T) + 16 * i : 0xFFFFFFF0u, 0, 0));
+    } else {
+      uint32_t e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t o = d + j < dim ? at + (d + j) * (uint32_t)sizeof(T) : 0xFFFFFFF0u;
+        if constexpr (W == 1) e[j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, o, 0, 0);
+        else e[j] = __builtin_amdgcn_raw_buffer_load_b32(rs, o, 0, 0);
+      }
+      if constexpr (W == 1) {
+        x[0] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16,
+                          e[6] | e[7] << 16);
+      } else {
+        x[0] = make_uint4(e[0], e[1], e[2], e[3]);
+        x[1] = make_uint4(e[4], e[5], e[6], e[7]);
+      }
+    }
+  }
+  static __device__ __forceinline__ void values(const uint4* x, float* f) {
+    const T* t = (const T*)x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = bs_to_f32(t[j]);
+  }
+  template <int PI>
+  static __device__ __forceinline__ bs_parts<PI> parts(const uint4* x) {
+    if constexpr (PI == 1) {
+      bs_parts<1> o;
+      o.p[0] = __builtin_bit_cast(bs_bf16x8, x[0]);
+      return o;
+    } else {
+      float f[8];
+      values(x, f);
+      return bs_split8<PI>(f);
+    }
+  }
+};
 
 // Workgroup of a grid of units x slices: the slices of a unit (one sequence and head) read the
 // same chunks, so they are given to one of the 8 XCDs, whose L2 then reads each chunk once.
@@ -262,6 +306,11 @@ __device__ __forceinline__ bs_f32x4 delta_turn(const bs_parts<P>& x, int odd, in
   for (int p = P - 1; p >= 0; --p)
     r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.p[p], b, r, 0, 0, 0);
   return r;
+}
+
+// Whether a workgroup of the recurrences takes 32 value columns instead of 16.
+static inline bool delta_wide(int64_t units, int dvp) {
+  return units * (dvp / 16) > bs_num_cus();
 }
 
 // Rows of a packed batch before the first sequence and after the last one are no sequence's:

@@ -64,15 +64,20 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
   const int row = delta_row(wave, m);
   bs_parts<PI> qf[KS], kf[KS];
   {
-    const bool live = row < len;
-    const int64_t t = live ? t0 + row : t0;
-    const T* kp = (const T*)in.k + bs_delta_at(in.k_stride, sp.batch, t, hk);
-    const T* qp = (const T*)in.q + bs_delta_at(in.q_stride, sp.batch, t, hk);
+    const DeltaRow<T> kr((const T*)in.k + bs_delta_at(in.k_stride, sp.batch, t0, hk),
+                         in.k_stride[1], row, len, in.dk, vec);
+    const DeltaRow<T> qr((const T*)in.q + bs_delta_at(in.q_stride, sp.batch, t0, hk),
+                         in.q_stride[1], row, len, in.dk, vec);
+    uint4 kx[KS][sizeof(T) / 2], qx[KS][sizeof(T) / 2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) kr.raw(32 * s + 8 * g, kx[s]);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qr.raw(32 * s + 8 * g, qx[s]);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int d = 32 * s + 8 * g, left = live ? in.dk - d : 0;
-      kf[s] = load_parts<PI>(kp + d, left, vec);
-      qf[s] = load_parts<PI>(qp + d, left, vec);
+      const int d = 32 * s + 8 * g;
+      kf[s] = kr.template parts<PI>(kx[s]);
+      qf[s] = qr.template parts<PI>(qx[s]);
 #pragma unroll
       for (int p = 0; p < PI; ++p) {
         *(bs_bf16x8*)&kl[p][row][d] = kf[s].p[p];
@@ -191,8 +196,8 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
   }
 }
 
-// Forward over the chunks of one sequence, value head and slice of 16 value columns, by two sets
-// of 4 waves.  The first has the recurrence: each wave 16 tokens of a chunk and a quarter of the
+// Forward over the chunks of one sequence, value head and slice of 16 NT value columns, by two
+// sets of 4 waves.  The first has the recurrence: each wave 16 tokens of a chunk and a quarter of the
 // state's rows; what the others need goes through LDS, as parts and in the lane that takes it.
 // The second forms from the same LDS what the recurrence does not wait for: the output and, for
 // the backward pass, U and the state before the chunk, transposed (the operands of a product
@@ -200,22 +205,22 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
 // no wave of the recurrence waits for a store, and a SIMD has two waves to issue from: the
 // recurrence's own arithmetic (products of 3 parts, splitting) leaves it idle half the time.
 // Operands that do not depend on the state are loaded into registers one or two chunks ahead.
-template <typename T, int PI, int KS, bool KEEP>
+template <typename T, int PI, int KS, int NT, bool KEEP>
 __global__ __launch_bounds__(512, 2) void chain_kernel(
     bs_delta_in in, DeltaPlan plan, DeltaWork w, const float* state0, float* state1, T* o,
     float* keep_s, float* keep_u, int dvp, int units, int vec) {
   constexpr int DK = KS * 32, TW = KS / 2, PO = PI == 3 ? 3 : 2, PV = KEEP ? 3 : PO;
-  constexpr int kS = KS * 128, kR = 2 * 128;       // words of a part
+  constexpr int kS = KS * NT * 128, kR = 2 * NT * 128;       // words of a part
   __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];     // the state
   __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];     // R
   __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];     // exp(total - run) U
   __shared__ __attribute__((aligned(16))) uint2 lv[PV * kR];    // U
-  const DeltaPlace at = delta_place(units, dvp / 16);
+  const DeltaPlace at = delta_place(units, dvp / (16 * NT));
   if (at.unit >= units) return;
   const int h = __builtin_amdgcn_readfirstlane(at.unit % in.hv);
   const int n = __builtin_amdgcn_readfirstlane(at.unit / in.hv), hk = h / (in.hv / in.hk);
   if (n >= plan.seqs) {
-    zero_outside(plan, o, in.hv, in.dv, h, at.slice * 16, 16);
+    zero_outside(plan, o, in.hv, in.dv, h, at.slice * 16 * NT, 16 * NT);
     return;
   }
   const DeltaSpan sp = delta_span(plan, n);
@@ -230,30 +235,37 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(
   const uint16_t* ip = w.inv + hb * 3 * kSquare + lane * 8;
 
   if (role == 0) {
-    const int col = at.slice * 16 + m;
-    const bool live = col < in.dv;
+    const int col = at.slice * 16 * NT + m;
     const int out0 = 32 * blk + 8 * g + 4 * (wave & 1);    // the 4 rows it receives
-    const int own = (blk * 64 + lane) * 2 + (wave & 1);
-    bs_f32x4 s[TW];
+    const int own = (blk * NT * 64 + lane) * 2 + (wave & 1);     // and 128 on for each column tile
+    bs_f32x4 s[TW][NT];
     int d0[TW], sown[TW];
 #pragma unroll
     for (int i = 0; i < TW; ++i) {
       const int t = TW * wave + i;
       d0[i] = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
-      sown[i] = ((t >> 1) * 64 + lane) * 2 + (t & 1);
+      sown[i] = ((t >> 1) * NT * 64 + lane) * 2 + (t & 1);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        s[i][r] = state0 && d0[i] + r < in.dk && live
-            ? state0[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] : 0.f;
-      delta_put<3>(ls + sown[i], kS, s[i]);
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[i][j][r] = state0 && d0[i] + r < in.dk && col + 16 * j < in.dv
+              ? state0[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col + 16 * j]
+              : 0.f;
+        delta_put<3>(ls + sown[i] + 128 * j, kS, s[i][j]);
+      }
     }
     const uint16_t* kp = w.kp + kb + wave * KS * kFrag + lane * 8;
     const uint16_t* kt = w.kt + kb + wave * TW * 2 * kFrag + lane * 8;
-    const DeltaRows<T> rows((const T*)in.v + bs_delta_at(in.v_stride, sp.batch, sp.first, h),
-                            in.v_stride[1], out0, col, in.dv);
+    const DeltaRows<T, NT> rows((const T*)in.v + bs_delta_at(in.v_stride, sp.batch, sp.first, h),
+                                in.v_stride[1], out0, col, in.dv);
     bs_parts<PI> kf[KS], ktf[TW][2];
     bs_parts<3> tf[2];
-    struct Values { typename DeltaRows<T>::Raw v[4]; float total; float4 grow, left, beta; } values[2];
+    struct Values {
+      typename DeltaRows<T, NT>::Raw v[NT][4];
+      float total;
+      float4 grow, left, beta;
+    } values[2];
     auto load_keys = [&](int c) {
 #pragma unroll
       for (int st = 0; st < KS; ++st)
@@ -290,40 +302,60 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(
     __syncthreads();
     auto step = [&](int c, Values& now) {
       const int next = min(c + 1, last);
-      bs_f32x4 x = zero4(), u = zero4();
+      bs_f32x4 x[NT], u[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) x[j] = u[j] = zero4();
 #pragma unroll
       for (int st = 0; st < KS; ++st)
-        x = bs_mma<2>(kf[st], delta_lds<3>(ls + (st * 64 + lane) * 2, kS), x);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          x[j] = bs_mma<2>(kf[st], delta_lds<3>(ls + ((st * NT + j) * 64 + lane) * 2, kS), x[j]);
       const float* gr = (const float*)&now.grow;
       const float* be = (const float*)&now.beta;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = be[r] * fmaf(-gr[r], x[r], rows.value(now.v[r]));
-      delta_put<3>(lr + own, kR, x);
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[j][r] = be[r] * fmaf(-gr[r], x[j][r], rows.value(now.v[j][r]));
+        delta_put<3>(lr + own + 128 * j, kR, x[j]);
+      }
       __builtin_amdgcn_sched_barrier(0);   // loads after what the others wait for
       load_keys(next);
       __syncthreads();                     // R
 #pragma unroll
       for (int st = 0; st < 2; ++st)
-        if (st <= blk)
-          u = bs_mma<2>(tf[st], delta_lds<3>(lr + (st * 64 + lane) * 2, kR), u);
+        if (st <= blk) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            u[j] = bs_mma<2>(tf[st], delta_lds<3>(lr + ((st * NT + j) * 64 + lane) * 2, kR), u[j]);
+        }
       const float* lf = (const float*)&now.left;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = lf[r] * u[r];
-      delta_put<3>(lu + own, kR, x);
-      delta_put<PV>(lv + own, kR, u);
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[j][r] = lf[r] * u[j][r];
+        delta_put<3>(lu + own + 128 * j, kR, x[j]);
+        delta_put<PV>(lv + own + 128 * j, kR, u[j]);
+      }
       __builtin_amdgcn_sched_barrier(0);
       load_inverse(next);
       __syncthreads();                     // U; the state's last readers are through
 #pragma unroll
-      for (int i = 0; i < TW; ++i) s[i] *= now.total;
+      for (int i = 0; i < TW; ++i)
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const bs_parts<3> b = delta_lds<3>(lu + (st * 64 + lane) * 2, kR);
+        for (int j = 0; j < NT; ++j) s[i][j] *= now.total;
 #pragma unroll
-        for (int i = 0; i < TW; ++i) s[i] = bs_mma<2>(ktf[i][st], b, s[i]);
-      }
+      for (int st = 0; st < 2; ++st)
 #pragma unroll
-      for (int i = 0; i < TW; ++i) delta_put<3>(ls + sown[i], kS, s[i]);
+        for (int j = 0; j < NT; ++j) {
+          const bs_parts<3> b = delta_lds<3>(lu + ((st * NT + j) * 64 + lane) * 2, kR);
+#pragma unroll
+          for (int i = 0; i < TW; ++i) s[i][j] = bs_mma<2>(ktf[i][st], b, s[i][j]);
+        }
+#pragma unroll
+      for (int i = 0; i < TW; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) delta_put<3>(ls + sown[i] + 128 * j, kS, s[i][j]);
       __builtin_amdgcn_sched_barrier(0);
       load_columns(next);
       load_values(min(c + 2, last), now);
@@ -335,16 +367,19 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(
       step(c + 1, values[1]);
     }
     if (sp.chunks & 1) step(last, values[0]);
-    if (state1 && live) {
+    if (state1) {
 #pragma unroll
       for (int i = 0; i < TW; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (d0[i] + r < in.dk)
-            state1[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] = s[i][r];
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (d0[i] + r < in.dk && col + 16 * j < in.dv)
+              state1[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col + 16 * j] =
+                  s[i][j][r];
     }
   } else {
-    const int ocol = at.slice * 16 + 4 * g;
+    const int ocol = at.slice * 16 * NT + 4 * g;
     const uint16_t* qp = w.qp + kb + wave * KS * kFrag + lane * 8;
     const uint16_t* ap = w.att + hb * PO * kSquare + lane * 8;
     struct Operands { bs_parts<PI> q[KS]; bs_parts<PO> a[2]; float scale; } operands[2];
@@ -371,38 +406,56 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(
     auto step = [&](int c, Operands& now) {
       const int64_t sh = hb + (int64_t)c * in.hv;
       __syncthreads();                     // R: from here the recurrence leaves the state alone
-      bs_f32x4 y = zero4();
+      bs_f32x4 y[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) y[j] = zero4();
 #pragma unroll
       for (int st = 0; st < KS; ++st)
-        y = bs_mma<PO - 1>(delta_lds<PO>(ls + (st * 64 + lane) * 2, kS), now.q[st], y);
-      y *= now.scale;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          y[j] = bs_mma<PO - 1>(delta_lds<PO>(ls + ((st * NT + j) * 64 + lane) * 2, kS), now.q[st],
+                                y[j]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) y[j] *= now.scale;
       if (KEEP) {
 #pragma unroll
-        for (int i = 0; i < TW; ++i) {
-          const int t = TW * wave + i;
-          const bs_f32x4 x =
-              delta_turn(delta_lds<3>(ls + ((t >> 1) * 64 + lane) * 2, kS), t & 1, lane);
-          *(bs_f32x4*)(keep_s + sh * DK * dvp + delta_kept(t, at.slice, lane, dvp)) = x;
-        }
+        for (int i = 0; i < TW; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const int t = TW * wave + i;
+            const bs_f32x4 x = delta_turn(
+                delta_lds<3>(ls + (((t >> 1) * NT + j) * 64 + lane) * 2, kS), t & 1, lane);
+            *(bs_f32x4*)(keep_s + sh * DK * dvp + delta_kept(t, at.slice * NT + j, lane, dvp)) = x;
+          }
       }
       __syncthreads();                     // U
 #pragma unroll
       for (int st = 0; st < 2; ++st)
-        if (st <= blk)
-          y = bs_mma<PO - 1>(delta_lds<PO>(lv + (st * 64 + lane) * 2, kR), now.a[st], y);
-      load(min(c + 2, last), now);
-      if (KEEP) {
-        const bs_f32x4 u = delta_turn(delta_lds<PV>(lv + (blk * 64 + lane) * 2, kR), wave & 1, lane);
-        *(bs_f32x4*)(keep_u + sh * kChunk * dvp + delta_kept(wave, at.slice, lane, dvp)) = u;
-      }
-      if (c * kChunk + tok < sp.len) {
-        T* p = op + (int64_t)c * kChunk * in.hv * in.dv;
-        if (vec) {
-          if (ocol < in.dv) bs_store4(p, y);
-        } else {
+        if (st <= blk) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (ocol + r < in.dv) p[r] = bs_from_f32<T>(y[r]);
+          for (int j = 0; j < NT; ++j)
+            y[j] = bs_mma<PO - 1>(delta_lds<PO>(lv + ((st * NT + j) * 64 + lane) * 2, kR),
+                                  now.a[st], y[j]);
+        }
+      load(min(c + 2, last), now);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if (KEEP) {
+          const bs_f32x4 u = delta_turn(delta_lds<PV>(lv + ((blk * NT + j) * 64 + lane) * 2, kR),
+                                        wave & 1, lane);
+          *(bs_f32x4*)(keep_u + sh * kChunk * dvp +
+                       delta_kept(wave, at.slice * NT + j, lane, dvp)) = u;
+        }
+        if (c * kChunk + tok < sp.len) {
+          T* p = op + (int64_t)c * kChunk * in.hv * in.dv + 16 * j;
+          const int oc = ocol + 16 * j;
+          if (vec) {
+            if (oc < in.dv) bs_store4(p, y[j]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (oc + r < in.dv) p[r] = bs_from_f32<T>(y[j][r]);
+          }
         }
       }
       __syncthreads();                     // the state
@@ -420,7 +473,7 @@ template <typename T, int PI, int KS>
 void launch_prepare(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork& w,
                     int backward, hipStream_t st) {
   const dim3 grid(plan.slots, in.hv);
-  int vec = (uintptr_t)in.q % 16 == 0 && (uintptr_t)in.k % 16 == 0;
+  int vec = in.dk % 8 == 0 && (uintptr_t)in.q % 16 == 0 && (uintptr_t)in.k % 16 == 0;
   for (int i = 0; i < 3; ++i) vec = vec && in.q_stride[i] % 8 == 0 && in.k_stride[i] % 8 == 0;
   if (backward) prepare_kernel<T, PI, KS, true, 3><<<grid, 256, 0, st>>>(in, plan, w, vec);
   else prepare_kernel<T, PI, KS, false, PI == 3 ? 3 : 2><<<grid, 256, 0, st>>>(in, plan, w, vec);
@@ -432,13 +485,20 @@ void launch_chain(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork&
                   float* keep_u, hipStream_t st) {
   const int units = (plan.seqs + (plan.offsets ? 1 : 0)) * in.hv;
   const int vec = in.dv % 4 == 0 && (uintptr_t)o % (4 * sizeof(T)) == 0;
-  const unsigned grid = delta_grid(units, z.dvp / 16);
-  if (keep_s)
-    chain_kernel<T, PI, KS, true><<<grid, 512, 0, st>>>(in, plan, w, s0, s1, (T*)o, keep_s,
-                                                        keep_u, z.dvp, units, vec);
-  else
-    chain_kernel<T, PI, KS, false><<<grid, 512, 0, st>>>(in, plan, w, s0, s1, (T*)o, keep_s,
-                                                         keep_u, z.dvp, units, vec);
+  auto run = [&](auto nt, auto keep) {
+    chain_kernel<T, PI, KS, nt.value, keep.value>
+        <<<delta_grid(units, z.dvp / (16 * nt.value)), 512, 0, st>>>(
+            in, plan, w, s0, s1, (T*)o, keep_s, keep_u, z.dvp, units, vec);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (delta_wide(units, z.dvp)) {
+    if (keep_s) run(Two(), std::true_type());
+    else run(Two(), std::false_type());
+  } else {
+    if (keep_s) run(One(), std::true_type());
+    else run(One(), std::false_type());
+  }
 }
 
 template <typename T, int PI>
@@ -473,8 +533,9 @@ int delta_check_chunked(const bs_delta_in* in, int seqs, int tokens, const int32
   if (int rc = bs_delta_check(in, who)) return rc;
   BS_CHECK_ARG(seqs >= 0 && tokens >= 0, "%s: %d sequences, %d tokens", who, seqs, tokens);
   // a chunk's rows are addressed in 32 bits
-  BS_CHECK_ARG(in->v_stride[1] >= 0 && in->v_stride[1] < (1 << 23) && in->hv * in->dv < (1 << 23),
-               "%s: %lld elements from token to token", who, (long long)in->v_stride[1]);
+  for (const int64_t* st : {in->q_stride, in->k_stride, in->v_stride})
+    BS_CHECK_ARG(st[1] >= 0 && st[1] < (1 << 23) && in->hv * in->dv < (1 << 23),
+                 "%s: %lld elements from token to token", who, (long long)st[1]);
   const int64_t slots = offsets ? (int64_t)tokens / kChunk + seqs
                                 : (int64_t)seqs * ((tokens + kChunk - 1) / kChunk);
   BS_CHECK_ARG(slots <= 0x7FFFFFFF / kChunk && in->hv <= 65535 &&

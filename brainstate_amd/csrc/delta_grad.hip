@@ -24,26 +24,26 @@
 
 namespace {
 
-// Chunks of one sequence, value head and slice of 16 value columns, last to first, by two sets of
-// 4 waves as in the forward pass: the first has the recurrence, the second forms dR again for the
+// Chunks of one sequence, value head and slice of 16 NT value columns, last to first, by two sets
+// of 4 waves as in the forward pass: the first has the recurrence, the second forms dR again for the
 // gradient of v and the chunk's gradients, and keeps the gradient of the state.
-template <typename T, int PI, int KS>
+template <typename T, int PI, int KS, int NT>
 __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
     bs_delta_in in, DeltaPlan plan, DeltaWork w, const T* go, const float* gstate, T* dv,
     float* dstate, int dvp, int units, int vec) {
   constexpr int DK = KS * 32, TW = KS / 2;
-  constexpr int kS = KS * 128, kR = 2 * 128;       // words of a part
+  constexpr int kS = KS * NT * 128, kR = 2 * NT * 128;       // words of a part
   __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];        // dS
   __shared__ __attribute__((aligned(16))) uint2 lo[PI * kR];       // dO
   __shared__ __attribute__((aligned(16))) uint2 lg[2][3 * kR];     // scale G dO
   __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];        // dU
   __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];        // -beta G dR
-  const DeltaPlace at = delta_place(units, dvp / 16);
+  const DeltaPlace at = delta_place(units, dvp / (16 * NT));
   if (at.unit >= units) return;
   const int h = __builtin_amdgcn_readfirstlane(at.unit % in.hv);
   const int n = __builtin_amdgcn_readfirstlane(at.unit / in.hv), hk = h / (in.hv / in.hk);
   if (n >= plan.seqs) {
-    zero_outside(plan, dv, in.hv, in.dv, h, at.slice * 16, 16);
+    zero_outside(plan, dv, in.hv, in.dv, h, at.slice * 16 * NT, 16 * NT);
     return;
   }
   const DeltaSpan sp = delta_span(plan, n);
@@ -63,30 +63,37 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
   };
 
   if (role == 0) {
-    const int col = at.slice * 16 + m;
-    const bool live = col < in.dv;
+    const int col = at.slice * 16 * NT + m;
     const int out0 = 32 * blk + 8 * g + 4 * (wave & 1);
-    const int own = (blk * 64 + lane) * 2 + (wave & 1);
-    bs_f32x4 s[TW];
+    const int own = (blk * NT * 64 + lane) * 2 + (wave & 1);
+    bs_f32x4 s[TW][NT];
     int d0[TW], sown[TW];
 #pragma unroll
     for (int i = 0; i < TW; ++i) {
       const int t = TW * wave + i;
       d0[i] = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
-      sown[i] = ((t >> 1) * 64 + lane) * 2 + (t & 1);
+      sown[i] = ((t >> 1) * NT * 64 + lane) * 2 + (t & 1);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        s[i][r] = gstate && d0[i] + r < in.dk && live
-            ? gstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] : 0.f;
-      delta_put<3>(ls + sown[i], kS, s[i]);
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[i][j][r] = gstate && d0[i] + r < in.dk && col + 16 * j < in.dv
+              ? gstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col + 16 * j]
+              : 0.f;
+        delta_put<3>(ls + sown[i] + 128 * j, kS, s[i][j]);
+      }
     }
     const uint16_t* kp = w.kp + kb + wave * KS * kFrag + lane * 8;
     const int64_t tb = kb + wave * TW * 2 * kFrag + lane * 8;
-    const DeltaRows<T> rows(go + ((sp.batch * plan.tokens + sp.first) * in.hv + h) * in.dv,
-                            (int64_t)in.hv * in.dv, out0, col, in.dv);
+    const DeltaRows<T, NT> rows(go + ((sp.batch * plan.tokens + sp.first) * in.hv + h) * in.dv,
+                                (int64_t)in.hv * in.dv, out0, col, in.dv);
     bs_parts<PI> kf[KS], ktf[TW][2], qtf[TW][2];
     bs_parts<3> tf[2], af[2];
-    struct Values { typename DeltaRows<T>::Raw v[4]; float total; float4 coef[3]; } values[2];
+    struct Values {
+      typename DeltaRows<T, NT>::Raw v[NT][4];
+      float total;
+      float4 coef[3];
+    } values[2];
     float all = 0.f;
     float4 now[3];
     auto load_keys = [&](int c) {
@@ -111,15 +118,18 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
     };
     // dO of the chunk that was loaded, and scale G dO, into LDS; its factors are the next ones
     auto stage = [&](int buf, const Values& v) {
-      bs_f32x4 x, y;
       const float* gw = (const float*)&v.coef[0];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[r] = rows.value(v.v[r]);
-        y[r] = in.scale * gw[r] * x[r];
+      for (int j = 0; j < NT; ++j) {
+        bs_f32x4 x, y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[r] = rows.value(v.v[j][r]);
+          y[r] = in.scale * gw[r] * x[r];
+        }
+        delta_put<PI>(lo + own + 128 * j, kR, x);
+        delta_put<3>(lg[buf] + own + 128 * j, kR, y);
       }
-      delta_put<PI>(lo + own, kR, x);
-      delta_put<3>(lg[buf] + own, kR, y);
       now[0] = v.coef[0], now[1] = v.coef[1], now[2] = v.coef[2], all = v.total;
     };
     if (const int c = sp.chunks - 1; c >= 0) {
@@ -137,46 +147,73 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
     // `v` holds chunk c - 1, and then c - 3
     auto step = [&](int c, Values& v) {
       const int next = max(c - 1, 0);
-      bs_f32x4 du = zero4(), dr = zero4();
+      bs_f32x4 du[NT], dr[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) du[j] = dr[j] = zero4();
 #pragma unroll
       for (int st = 0; st < KS; ++st)
-        du = bs_mma<2>(kf[st], delta_lds<3>(ls + (st * 64 + lane) * 2, kS), du);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          du[j] = bs_mma<2>(kf[st], delta_lds<3>(ls + ((st * NT + j) * 64 + lane) * 2, kS), du[j]);
       const float* lf = (const float*)&now[1];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) du[r] *= lf[r];
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) du[j][r] *= lf[r];
 #pragma unroll
       for (int st = 0; st < 2; ++st)
-        if (st >= blk) du = bs_mma<2>(af[st], delta_lds<PI>(lo + (st * 64 + lane) * 2, kR), du);
-      delta_put<3>(lu + own, kR, du);
+        if (st >= blk) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            du[j] = bs_mma<2>(af[st], delta_lds<PI>(lo + ((st * NT + j) * 64 + lane) * 2, kR),
+                              du[j]);
+        }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) delta_put<3>(lu + own + 128 * j, kR, du[j]);
       __builtin_amdgcn_sched_barrier(0);
       load_keys(next);
       load_square(w.att, next, af);
       __syncthreads();                     // dU; dO's last readers are through
 #pragma unroll
       for (int st = 0; st < 2; ++st)
-        if (st >= blk) dr = bs_mma<2>(tf[st], delta_lds<3>(lu + (st * 64 + lane) * 2, kR), dr);
+        if (st >= blk) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            dr[j] = bs_mma<2>(tf[st], delta_lds<3>(lu + ((st * NT + j) * 64 + lane) * 2, kR),
+                              dr[j]);
+        }
       const float* gw = (const float*)&now[0];
       const float* be = (const float*)&now[2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) dr[r] *= -gw[r] * be[r];
-      delta_put<3>(lr + own, kR, dr);
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dr[j][r] *= -gw[r] * be[r];
+        delta_put<3>(lr + own + 128 * j, kR, dr[j]);
+      }
       __builtin_amdgcn_sched_barrier(0);
       load_square(w.inv, next, tf);
       __syncthreads();                     // dR; the state's last readers are through
 #pragma unroll
-      for (int i = 0; i < TW; ++i) s[i] *= all;
+      for (int i = 0; i < TW; ++i)
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const bs_parts<3> a = delta_lds<3>(lg[c & 1] + (st * 64 + lane) * 2, kR);
-        const bs_parts<3> b = delta_lds<3>(lr + (st * 64 + lane) * 2, kR);
+        for (int j = 0; j < NT; ++j) s[i][j] *= all;
 #pragma unroll
-        for (int i = 0; i < TW; ++i) {
-          s[i] = bs_mma<2>(qtf[i][st], a, s[i]);
-          s[i] = bs_mma<2>(ktf[i][st], b, s[i]);
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const int at2 = ((st * NT + j) * 64 + lane) * 2;
+          const bs_parts<3> a = delta_lds<3>(lg[c & 1] + at2, kR);
+          const bs_parts<3> b = delta_lds<3>(lr + at2, kR);
+#pragma unroll
+          for (int i = 0; i < TW; ++i) {
+            s[i][j] = bs_mma<2>(qtf[i][st], a, s[i][j]);
+            s[i][j] = bs_mma<2>(ktf[i][st], b, s[i][j]);
+          }
         }
-      }
 #pragma unroll
-      for (int i = 0; i < TW; ++i) delta_put<3>(ls + sown[i], kS, s[i]);
+      for (int i = 0; i < TW; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) delta_put<3>(ls + sown[i] + 128 * j, kS, s[i][j]);
       stage((c - 1) & 1, v);               // past chunk 0: what no one reads
       __builtin_amdgcn_sched_barrier(0);
       load_columns(next);
@@ -188,16 +225,19 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
       step(c - 1, values[1]);
     }
     if (sp.chunks & 1) step(0, values[0]);
-    if (dstate && live) {
+    if (dstate) {
 #pragma unroll
       for (int i = 0; i < TW; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (d0[i] + r < in.dk)
-            dstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col] = s[i][r];
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (d0[i] + r < in.dk && col + 16 * j < in.dv)
+              dstate[(((int64_t)n * in.hv + h) * in.dk + d0[i] + r) * in.dv + col + 16 * j] =
+                  s[i][j][r];
     }
   } else {
-    const int ocol = at.slice * 16 + 4 * g;
+    const int ocol = at.slice * 16 * NT + 4 * g;
     struct Operands { bs_parts<3> t[2]; float beta; } operands[2];
     auto load = [&](int c, Operands& x) {
       load_square(w.inv, c, x.t);
@@ -213,30 +253,43 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
     auto step = [&](int c, Operands& now) {
       const int64_t sh = hb + (int64_t)c * in.hv;
 #pragma unroll
-      for (int i = 0; i < TW; ++i) {
-        const int t = TW * wave + i;
-        const bs_f32x4 x =
-            delta_turn(delta_lds<3>(ls + ((t >> 1) * 64 + lane) * 2, kS), t & 1, lane);
-        *(bs_f32x4*)(w.ds + sh * DK * dvp + delta_kept(t, at.slice, lane, dvp)) = x;
-      }
+      for (int i = 0; i < TW; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const int t = TW * wave + i;
+          const bs_f32x4 x = delta_turn(
+              delta_lds<3>(ls + (((t >> 1) * NT + j) * 64 + lane) * 2, kS), t & 1, lane);
+          *(bs_f32x4*)(w.ds + sh * DK * dvp + delta_kept(t, at.slice * NT + j, lane, dvp)) = x;
+        }
       __syncthreads();                     // dU
-      bs_f32x4 dr = zero4();
+      bs_f32x4 dr[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) dr[j] = zero4();
 #pragma unroll
       for (int st = 0; st < 2; ++st)
-        if (st >= blk)
-          dr = bs_mma<2>(delta_lds<3>(lu + (st * 64 + lane) * 2, kR), now.t[st], dr);
+        if (st >= blk) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            dr[j] = bs_mma<2>(delta_lds<3>(lu + ((st * NT + j) * 64 + lane) * 2, kR), now.t[st],
+                              dr[j]);
+        }
       const float beta = now.beta;
       load(max(c - 2, 0), now);
-      *(bs_f32x4*)(w.dr + sh * kChunk * dvp + delta_kept(wave, at.slice, lane, dvp)) = dr;
-      if (c * kChunk + tok < sp.len) {
-        T* p = op + (int64_t)c * kChunk * in.hv * in.dv;
-        const bs_f32x4 y = beta * dr;
-        if (vec) {
-          if (ocol < in.dv) bs_store4(p, y);
-        } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (ocol + r < in.dv) p[r] = bs_from_f32<T>(y[r]);
+      for (int j = 0; j < NT; ++j) {
+        *(bs_f32x4*)(w.dr + sh * kChunk * dvp +
+                     delta_kept(wave, at.slice * NT + j, lane, dvp)) = dr[j];
+        if (c * kChunk + tok < sp.len) {
+          T* p = op + (int64_t)c * kChunk * in.hv * in.dv + 16 * j;
+          const int oc = ocol + 16 * j;
+          const bs_f32x4 y = beta * dr[j];
+          if (vec) {
+            if (oc < in.dv) bs_store4(p, y);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (oc + r < in.dv) p[r] = bs_from_f32<T>(y[r]);
+          }
         }
       }
       __syncthreads();                     // dR
@@ -282,6 +335,7 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
   __shared__ __attribute__((aligned(16))) float lp[kChunk][kChunk + 4];
   __shared__ __attribute__((aligned(16))) float lm[kChunk][kChunk + 4];
   __shared__ float rows[2][kChunk], betas[2][kChunk], tot[8];
+  __shared__ __attribute__((aligned(16))) uint4 lst[2][2][2 * KS][3][64];    // states' parts
   const int slot = blockIdx.x, hk = blockIdx.y, group = in.hv / in.hk;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), t = wave & 3, half = wave >> 2;
@@ -334,53 +388,81 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
     const float* dr = w.dr + sh * kChunk * dvp;
     const float* s0 = keep_s + sh * DK * dvp;
     const float* ds = w.ds + sh * DK * dvp;
-    const T* gp = go + ((sp.batch * plan.tokens + t0 + (live ? tok : 0)) * in.hv + h) * in.dv;
-    const T* vp = (const T*)in.v + bs_delta_at(in.v_stride, sp.batch, t0 + (live ? tok : 0), h);
+    const DeltaRow<T> gr(go + ((sp.batch * plan.tokens + t0) * in.hv + h) * in.dv,
+                         (int64_t)in.hv * in.dv, tok, len, in.dv, vec & 1);
+    const DeltaRow<T> vr((const T*)in.v + bs_delta_at(in.v_stride, sp.batch, t0, h),
+                         in.v_stride[1], tok, len, in.dv, vec & 2);
     bs_f32x4 xq[CT], xs[CT], xr[CT], da[2], dl[2];
     float dot_s = 0.f, dot_v = 0.f;
 #pragma unroll
     for (int i = 0; i < CT; ++i) xq[i] = xs[i] = xr[i] = zero4();
 #pragma unroll
     for (int j = 0; j < 2; ++j) da[j] = dl[j] = zero4();
-    for (int e = 0; e < dvp; e += 32) {
-      const int d = e + 8 * g, left = live ? in.dv - d : 0;
-      const bs_parts<PI> of = load_parts<PI>(gp + d, left, vec);
-      const float* rp = delta_kept_frag(dr, t, e >> 5, lane, dvp);
-      const float* up = delta_kept_frag(us, t, e >> 5, lane, dvp);
-      const float4 r0 = *(const float4*)rp, r1 = *(const float4*)(rp + 256);
-      const bs_parts<3> rf = row_parts(r0, r1);
-      const bs_parts<3> uf = row_parts(*(const float4*)up, *(const float4*)(up + 256));
-      if (((e >> 5) & 1) == half) {
-        const float rr[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+    // Steps of 32 value columns.  The states' parts are cut once for all waves: wave w loads tile
+    // w of both, a step ahead, and leaves them in LDS, two steps deep.
+    float4 sw[4], rw[2], uw[2], jw[2][2];
+    uint4 gw[sizeof(T) / 2], vw[sizeof(T) / 2];
+    auto load_step = [&](int e) {
+      gr.raw(e + 8 * g, gw);
+      vr.raw(e + 8 * g, vw);
+      const float* p = delta_kept_frag(s0, min(wave, 2 * KS - 1), e >> 5, lane, dvp);
+      const float* q = delta_kept_frag(ds, min(wave, 2 * KS - 1), e >> 5, lane, dvp);
+      sw[0] = *(const float4*)p, sw[1] = *(const float4*)(p + 256);
+      sw[2] = *(const float4*)q, sw[3] = *(const float4*)(q + 256);
+      p = delta_kept_frag(dr, t, e >> 5, lane, dvp);
+      rw[0] = *(const float4*)p, rw[1] = *(const float4*)(p + 256);
+      p = delta_kept_frag(us, t, e >> 5, lane, dvp);
+      uw[0] = *(const float4*)p, uw[1] = *(const float4*)(p + 256);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < left) dot_v = fmaf(rr[j], bs_to_f32(vp[d + j]), dot_v);
+      for (int j = 0; j < 2; ++j) {
+        p = delta_kept_frag(us, j0 + min(j, nj - 1), e >> 5, lane, dvp);
+        jw[j][0] = *(const float4*)p, jw[j][1] = *(const float4*)(p + 256);
       }
+    };
+    load_step(0);
+    for (int e = 0; e < dvp; e += 32) {
+      const int buf = (e >> 5) & 1;
+      if (wave < 2 * KS) {
+        const bs_parts<3> a = row_parts(sw[0], sw[1]), b = row_parts(sw[2], sw[3]);
 #pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        const float* sp0 = delta_kept_frag(s0, half * CT + i, e >> 5, lane, dvp);
-        const float* sp1 = delta_kept_frag(ds, half * CT + i, e >> 5, lane, dvp);
-        const float4 a0 = *(const float4*)sp0, a1 = *(const float4*)(sp0 + 256);
-        const float4 b0 = *(const float4*)sp1, b1 = *(const float4*)(sp1 + 256);
-        if (i == t) {
-          float x = a0.x * b0.x;
-          x = fmaf(a0.y, b0.y, x), x = fmaf(a0.z, b0.z, x), x = fmaf(a0.w, b0.w, x);
-          x = fmaf(a1.x, b1.x, x), x = fmaf(a1.y, b1.y, x), x = fmaf(a1.z, b1.z, x);
-          dot_s += fmaf(a1.w, b1.w, x);
+        for (int p = 0; p < 3; ++p) {
+          *(bs_bf16x8*)&lst[buf][0][wave][p][lane] = a.p[p];
+          *(bs_bf16x8*)&lst[buf][1][wave][p][lane] = b.p[p];
         }
-        const bs_parts<3> sf = row_parts(a0, a1), df = row_parts(b0, b1);
-        xq[i] = bs_mma<2>(sf, of, xq[i]);
-        xr[i] = bs_mma<2>(sf, rf, xr[i]);
-        xs[i] = bs_mma<2>(df, uf, xs[i]);
+        const float* x = (const float*)sw;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot_s = fmaf(x[i], x[8 + i], dot_s);
+      }
+      const bs_parts<PI> of = gr.template parts<PI>(gw);
+      const bs_parts<3> rf = row_parts(rw[0], rw[1]), uf = row_parts(uw[0], uw[1]);
+      if (buf == half) {
+        const float* x = (const float*)rw;
+        float f[8];
+        vr.values(vw, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dot_v = fmaf(x[j], f[j], dot_v);
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         if (j < nj) {
-          const float* jp = delta_kept_frag(us, j0 + j, e >> 5, lane, dvp);
-          const bs_parts<3> a = row_parts(*(const float4*)jp, *(const float4*)(jp + 256));
+          const bs_parts<3> a = row_parts(jw[j][0], jw[j][1]);
           da[j] = bs_mma<2>(a, of, da[j]);
           dl[j] = bs_mma<2>(a, rf, dl[j]);
         }
+      load_step(min(e + 32, dvp - 32));
+      __syncthreads();                // the parts of this step
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        bs_parts<3> sf, df;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          sf.p[p] = *(const bs_bf16x8*)&lst[buf][0][half * CT + i][p][lane];
+          df.p[p] = *(const bs_bf16x8*)&lst[buf][1][half * CT + i][p][lane];
+        }
+        xq[i] = bs_mma<2>(sf, of, xq[i]);
+        xr[i] = bs_mma<2>(sf, rf, xr[i]);
+        xs[i] = bs_mma<2>(df, uf, xs[i]);
+      }
     }
     // the masked products of this wave, to LDS by rows
     const float grow = co[kGrow * kChunk + tok], beta = co[kBeta * kChunk + tok];
@@ -516,11 +598,20 @@ void launch_grad(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWork& 
                  const float* keep_u, const GradOut& o, hipStream_t st) {
   const unsigned extra = plan.offsets ? 1 : 0;
   const int units = (plan.seqs + (int)extra) * in.hv;
-  grad_chain_kernel<T, PI, KS><<<delta_grid(units, z.dvp / 16), 512, 0, st>>>(
-      in, plan, w, (const T*)go, gstate, (T*)o.dv, o.dstate, z.dvp, units,
-      in.dv % 4 == 0 && (uintptr_t)o.dv % (4 * sizeof(T)) == 0);
+  const int wide = in.dv % 4 == 0 && (uintptr_t)o.dv % (4 * sizeof(T)) == 0;
+  auto run = [&](auto nt) {
+    grad_chain_kernel<T, PI, KS, nt.value>
+        <<<delta_grid(units, z.dvp / (16 * nt.value)), 512, 0, st>>>(
+            in, plan, w, (const T*)go, gstate, (T*)o.dv, o.dstate, z.dvp, units, wide);
+  };
+  if (delta_wide(units, z.dvp)) run(std::integral_constant<int, 2>());
+  else run(std::integral_constant<int, 1>());
   if (plan.slots + extra == 0) return;
-  const int vec = in.dv % 8 == 0 && (uintptr_t)go % 16 == 0;
+  int vec = in.dv % 8 == 0 ? 3 : 0;           // bit 0: grad_o's rows, bit 1: v's
+  if ((uintptr_t)go % 16) vec &= 2;
+  if ((uintptr_t)in.v % 16) vec &= 1;
+  for (int i = 0; i < 3; ++i)
+    if (in.v_stride[i] % 8) vec &= 1;
   grad_chunk_kernel<T, PI, KS><<<dim3(plan.slots + extra, in.hk), 512, 0, st>>>(
       in, plan, w, (const T*)go, keep_s, keep_u, (T*)o.dq, (T*)o.dk, o.dg, o.dbeta, z.dvp, vec);
 }
