@@ -10,9 +10,11 @@
 // Few tokens (skinny_kernel): bound by the weights' bytes.  Each workgroup has 16 channels and its
 // waves share k; weights go straight from memory to the matrix instruction, whose operand is 16
 // rows x 64 bytes.  Many tokens (tile_kernel): bound by the matrix cores; tiles of both operands
-// are staged in LDS by direct loads, two deep, 16-byte pieces in an order (piece ^ row) that
-// keeps the reads off each other's banks.
+// are staged in LDS by direct loads, two deep, 16-byte pieces in an order that keeps the reads off
+// each other's banks.
 #include "lane_types.h"
+
+#include <type_traits>
 
 namespace {
 
@@ -22,23 +24,36 @@ using i32x16 = __attribute__((__vector_size__(16 * sizeof(int)))) int;
 constexpr int kStep = 128;    // bytes of k in one step of the kernels
 
 // ------------------------------------------------------------------ tokens to 8 bits
-template <typename T>
+// A row to a workgroup; V vectors of 8 values of it to a lane's registers (the rest, if any, is
+// read again for the second pass).
+template <typename T, int V>
 __global__ __launch_bounds__(256) void quant_kernel(const T* x, int64_t stride, int k, int ld,
                                                     int8_t* x8, float* scale) {
   __shared__ uint32_t sh[4];
   const int64_t row = blockIdx.x;
   const T* p = x + row * stride;
-  uint32_t top = 0;     // of |x| as bits: ordered like the values, NaN above infinity
-  for (int c = threadIdx.x * 8; c < k; c += 2048) {
+  T held[V][8];
+  auto load = [&](int c, T* t) {
     if (c + 8 <= k) {
-      T t[8];
-      __builtin_memcpy(t, p + c, sizeof(t));
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        top = max(top, __float_as_uint(bs_to_f32(t[j])) & 0x7FFFFFFFu);
+      __builtin_memcpy(t, p + c, 8 * sizeof(T));
     } else {
-      for (int j = c; j < k; ++j) top = max(top, __float_as_uint(bs_to_f32(p[j])) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = c + j < k ? p[c + j] : T{};
     }
+  };
+  uint32_t top = 0;     // of |x| as bits: ordered like the values, NaN above infinity
+  auto raise = [&](const T* t) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(bs_to_f32(t[j])) & 0x7FFFFFFFu);
+  };
+#pragma unroll
+  for (int v = 0; v < V; ++v) load(threadIdx.x * 8 + 2048 * v, held[v]);
+#pragma unroll
+  for (int v = 0; v < V; ++v) raise(held[v]);
+  for (int c = threadIdx.x * 8 + 2048 * V; c < k; c += 2048) {
+    T t[8];
+    load(c, t);
+    raise(t);
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
@@ -54,16 +69,28 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* x, int64_t stride, 
   const bool ok = a > 0.f && a < INFINITY;    // a row of 0, or with NaN or infinity, is 0: its
                                               // scale makes the result 0 or NaN
   int8_t* q = x8 + row * ld;
-  for (int c = threadIdx.x * 8; c < ld; c += 2048) {
-    int8_t r[8];
+  auto store = [&](int c, const T* t) {
+    uint32_t r[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      r[j] = ok && c + j < k ? (int8_t)rintf(up * bs_to_f32(p[c + j]) / den) : (int8_t)0;
+    for (int j = 0; j < 8; ++j) {
+      const int n = ok ? (int)rintf(up * bs_to_f32(t[j]) / den) : 0;
+      r[j >> 2] |= (uint32_t)(n & 255) << 8 * (j & 3);
+    }
     if (c + 8 <= ld) {
       __builtin_memcpy(q + c, r, 8);
     } else {
-      for (int j = 0; c + j < ld; ++j) q[c + j] = r[j];
+      for (int j = 0; c + j < ld; ++j) q[c + j] = (int8_t)(r[j >> 2] >> 8 * (j & 3));
     }
+  };
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = threadIdx.x * 8 + 2048 * v;
+    if (c < ld) store(c, held[v]);
+  }
+  for (int c = threadIdx.x * 8 + 2048 * V; c < ld; c += 2048) {
+    T t[8];
+    load(c, t);
+    store(c, t);
   }
 }
 
@@ -77,6 +104,7 @@ struct Out {
   const float *a, *w;       // scales
   const void* bias;
   int y_dtype, bias_dtype, m, n;
+  bool wide;                // rows of y start on 4 values
 };
 
 __device__ __forceinline__ void put(const Out& o, int m, int n, int acc, float w, float b) {
@@ -152,42 +180,52 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const int8_t* x8, in
                                                             int tiles_m, int tiles_n) {
   constexpr int W = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
   constexpr int LA = BM * kStep / 1024 / W, LB = BN * kStep / 1024 / W;   // 1 KB loads a wave
-  __shared__ __attribute__((aligned(16))) int8_t sa[2][BM * kStep];
-  __shared__ __attribute__((aligned(16))) int8_t sb[2][BN * kStep];
-  // workgroups go round the 8 XCDs: each gets a run of tiles, so that its L2 keeps their rows
+  // two steps of both operands, as arrays of their own: a read of one then does not wait for the
+  // loads into the other
+  __shared__ __attribute__((aligned(16))) int8_t sa0[BM * kStep];
+  __shared__ __attribute__((aligned(16))) int8_t sb0[BN * kStep];
+  __shared__ __attribute__((aligned(16))) int8_t sa1[BM * kStep];
+  __shared__ __attribute__((aligned(16))) int8_t sb1[BN * kStep];
+  __shared__ float scales[BM];
+  // workgroups go round the 8 XCDs: each gets a run of tiles, 8 rows of tiles deep, so that the 32
+  // tiles it works on at a time share 8 + 4 runs of rows in its L2
   const int tiles = tiles_m * tiles_n, per = (tiles + 7) / 8;
   const int tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((blockIdx.x >> 3) >= per || tile >= tiles) return;
-  const int m0 = tile % tiles_m * BM, n0 = tile / tiles_m * BN;
+  const int band = tile / (8 * tiles_n), in_band = tile % (8 * tiles_n);
+  const int deep = min(8, tiles_m - 8 * band);
+  const int m0 = (8 * band + in_band % deep) * BM, n0 = in_band / deep * BN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / WN, wn = wave % WN, r = lane & 31, g = lane >> 5;
 
   // Load i of a wave fills rows 8 (wave LA + i) .. + 7; lane: row lane / 8, place lane % 8, which
-  // holds piece (place ^ row % 8).
-  const int piece = (lane & 7) ^ (lane >> 3);
+  // holds piece (place ^ (row / 2) % 8): 16 rows' pieces then lie on different banks.
+  auto key = [](int row) { return row >> 1 & 7; };
+  auto piece = [&](int i) { return (lane & 7) ^ key(8 * i + (lane >> 3)); };
   const int8_t* ga[LA];
   const int8_t* gb[LB];
 #pragma unroll
   for (int i = 0; i < LA; ++i)
-    ga[i] = x8 + (int64_t)min(m0 + 8 * (wave * LA + i) + (lane >> 3), o.m - 1) * ld + 16 * piece;
+    ga[i] = x8 + (int64_t)min(m0 + 8 * (wave * LA + i) + (lane >> 3), o.m - 1) * ld +
+            16 * piece(wave * LA + i);
 #pragma unroll
   for (int i = 0; i < LB; ++i)
     gb[i] = w8 + (int64_t)min(n0 + 8 * (wave * LB + i) + (lane >> 3), o.n - 1) * k_len;
   const int last = max(k_len - 16, 0);     // DIRECT: the last whole piece of a row
 
-  auto stage = [&](int k, int buf) {
+  auto stage = [&](int k, int8_t* sa, int8_t* sb) {
 #pragma unroll
     for (int i = 0; i < LA; ++i)
       __builtin_amdgcn_global_load_lds((GlobalPtr)(ga[i] + k),
-                                       (LdsPtr)(sa[buf] + (wave * LA + i) * 1024), 16, 0, 0);
+                                       (LdsPtr)(sa + (wave * LA + i) * 1024), 16, 0, 0);
 #pragma unroll
     for (int i = 0; i < LB; ++i) {
       if constexpr (DIRECT) {
-        __builtin_amdgcn_global_load_lds((GlobalPtr)(gb[i] + min(k + 16 * piece, last)),
-                                         (LdsPtr)(sb[buf] + (wave * LB + i) * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((GlobalPtr)(gb[i] + min(k + 16 * piece(wave * LB + i), last)),
+                                         (LdsPtr)(sb + (wave * LB + i) * 1024), 16, 0, 0);
       } else {
-        *(i32x4*)(sb[buf] + (wave * LB + i) * 1024 + lane * 16) =
-            load_w(gb[i], k + 16 * piece, k_len);
+        *(i32x4*)(sb + (wave * LB + i) * 1024 + lane * 16) =
+            load_w(gb[i], k + 16 * piece(wave * LB + i), k_len);
       }
     }
   };
@@ -198,44 +236,100 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const int8_t* x8, in
     for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-  stage(0, 0);
-  int buf = 0;
-  for (int k = 0; k < ld; k += kStep, buf ^= 1) {
-    __syncthreads();
-    if (k + kStep < ld) stage(k + kStep, buf ^ 1);
-#pragma unroll
-    for (int s = 0; s < kStep / 32; ++s) {
-      i32x4 a[TM], b[TN];
+  // a step's four products, the operands of each read while the one before runs
+  auto multiply = [&](const int8_t* sa, const int8_t* sb) {
+    i32x4 a[2][TM], b[2][TN];
+    auto read = [&](int s) {
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int row = (wm * TM + i) * 32 + r;
-        a[i] = *(const i32x4*)(sa[buf] + row * kStep + 16 * ((2 * s + g) ^ (row & 7)));
+        a[s & 1][i] = *(const i32x4*)(sa + row * kStep + 16 * ((2 * s + g) ^ key(row)));
       }
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int row = (wn * TN + j) * 32 + r;
-        b[j] = *(const i32x4*)(sb[buf] + row * kStep + 16 * ((2 * s + g) ^ (row & 7)));
+        b[s & 1][j] = *(const i32x4*)(sb + row * kStep + 16 * ((2 * s + g) ^ key(row)));
       }
+    };
+    read(0);
+#pragma unroll
+    for (int s = 0; s < kStep / 32; ++s) {
+      if (s + 1 < kStep / 32) read(s + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+          acc[i][j] =
+              __builtin_amdgcn_mfma_i32_32x32x32_i8(a[s & 1][i], b[s & 1][j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // every wave's direct loads have to be in LDS before any wave passes the barrier
+  auto arrive = [&]() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt 0
+    __syncthreads();
+  };
+  for (int i = threadIdx.x; i < BM; i += 64 * W) scales[i] = o.a[min(m0 + i, o.m - 1)];
+  stage(0, sa0, sb0);
+  for (int k = 0; k < ld; k += 2 * kStep) {
+    arrive();
+    if (k + kStep < ld) stage(k + kStep, sa1, sb1);
+    multiply(sa0, sb0);
+    if (k + kStep < ld) {
+      arrive();
+      if (k + 2 * kStep < ld) stage(k + 2 * kStep, sa0, sb0);
+      multiply(sa1, sb1);
     }
   }
+  // 16 rows at a time through a wave's own part of sa0, so that a lane stores 4 neighbouring
+  // channels and 8 or 16 lanes a whole run of a row; groups of 4 in an order (group ^ row) that
+  // spreads the banks
+  constexpr int C = TN * 32, L = C / 4;
+  __syncthreads();
+  int* turn = (int*)(sa0 + wave * 16 * C * 4);
+  const int cg = lane % L, n = n0 + wn * C + 4 * cg;
+  float w[4], bias[4];
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int n = n0 + (wn * TN + j) * 32 + r;
-    if (n >= o.n) continue;
-    const float w = o.w[n], b = o.bias ? bs_load_any(o.bias, o.bias_dtype, n) : 0.f;
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int m = m0 + (wm * TM + i) * 32 + 8 * (e >> 2) + 4 * g + (e & 3);
-        if (m < o.m) put(o, m, n, acc[i][j][e], w, b);
-      }
+  for (int i = 0; i < 4; ++i) {
+    w[i] = n + i < o.n ? o.w[n + i] : 0.f;
+    bias[i] = o.bias && n + i < o.n ? bs_load_any(o.bias, o.bias_dtype, n + i) : 0.f;
   }
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int row = 8 * (e >> 2) + 4 * g + (e & 3), col = 32 * j + r;
+          turn[row * C + ((((col >> 2) ^ row) & (L - 1)) << 2) + (col & 3)] = acc[i][j][8 * h + e];
+        }
+      __builtin_amdgcn_wave_barrier();     // one wave's LDS accesses are done in order
+#pragma unroll
+      for (int q = 0; q < 16 * L / 64; ++q) {
+        const int row = q * (64 / L) + lane / L;
+        const int mi = (wm * TM + i) * 32 + 16 * h + row, m = m0 + mi;
+        const i32x4 v = *(const i32x4*)(turn + row * C + (((cg ^ row) & (L - 1)) << 2));
+        if (m >= o.m) continue;
+        const float am = scales[mi];
+        bs_f32x4 y;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) y[x] = fmaf((float)v[x], am * w[x], bias[x]);
+        const int64_t at = (int64_t)m * o.n + n;
+        if (o.wide && n < o.n) {
+          if (o.y_dtype == BS_F32) bs_store4((float*)o.y + at, y);
+          else if (o.y_dtype == BS_BF16) bs_store4((bs_bf16*)o.y + at, y);
+          else bs_store4((bs_f16*)o.y + at, y);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (n + x < o.n) bs_store_any(o.y, o.y_dtype, at + x, y[x]);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
 }
 
 template <int BM, int BN, int WM, int WN>
@@ -275,12 +369,17 @@ int check(int64_t m, int32_t k, int32_t n, const char* who) {
 
 int quantize(const void* x, int dtype, int64_t m, int k, int64_t stride, int ld, int8_t* x8,
              float* scale, hipStream_t st) {
-  if (dtype == BS_F32)
-    quant_kernel<<<(unsigned)m, 256, 0, st>>>((const float*)x, stride, k, ld, x8, scale);
-  else if (dtype == BS_BF16)
-    quant_kernel<<<(unsigned)m, 256, 0, st>>>((const bs_bf16*)x, stride, k, ld, x8, scale);
-  else
-    quant_kernel<<<(unsigned)m, 256, 0, st>>>((const bs_f16*)x, stride, k, ld, x8, scale);
+  auto run = [&](auto* p) {
+    if (ld <= 2048)
+      quant_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, 1>
+          <<<(unsigned)m, 256, 0, st>>>(p, stride, k, ld, x8, scale);
+    else
+      quant_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, 4>
+          <<<(unsigned)m, 256, 0, st>>>(p, stride, k, ld, x8, scale);
+  };
+  if (dtype == BS_F32) run((const float*)x);
+  else if (dtype == BS_BF16) run((const bs_bf16*)x);
+  else run((const bs_f16*)x);
   BS_CHECK_LAUNCH();
   return BS_OK;
 }
@@ -324,7 +423,8 @@ extern "C" int bs_int8_linear(const void* x, int32_t x_dtype, int64_t stride, co
   } else if (int rc = quantize(x, x_dtype, m, k, stride, ld, x8, a, st)) {
     return rc;
   }
-  const Out o = {y, x_scale ? x_scale : a, w_scale, bias, y_dtype, bias_dtype, (int)m, n};
+  const Out o = {y, x_scale ? x_scale : a, w_scale, bias, y_dtype, bias_dtype, (int)m, n,
+                 n % 4 == 0 && (uintptr_t)y % 16 == 0};
   product(x8, ld, w8, k, o, st);
   BS_CHECK_LAUNCH();
   return BS_OK;
