@@ -5,109 +5,190 @@
 //
 // (a part that is not given is left out).  Bound by bytes: a row is read once into registers,
 // where both norms' sums are taken in 32 bits, and its results are written once; s is rounded
-// only when it is stored.  A row belongs to TPR lanes with 8 NV values each, so a norm over a
-// head of 128 values shares a wave with three others and one of 16,384 takes 1,024 threads.
+// only when it is stored.  A row belongs to as many lanes as it has
+// runs of 8 values, so a norm over a head of 128 values shares a wave with three others and one of
+// 2,050 takes 5 waves.
 // Workgroups stay for many rows: a lane's columns are the same in each, so the weights are read
 // once and the weights' gradients are summed in registers, then over the workgroups in their
 // order (grad_sum_kernel): the same bits every time.
 #include "lane_types.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int kVec = 8;
 
-// Rows start at any element: 16-byte loads of any alignment, single ones at a row's end.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int left, float* x) {
-  if (left >= kVec) {
-    T t[kVec];
-    __builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) x[j] = bs_to_f32(t[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) x[j] = j < left ? bs_to_f32(p[j]) : 0.f;
-  }
-}
+// How a lane's 8 columns lie: rows of whole runs; rows whose last lane takes the row's last 8
+// columns, some of them a second time (it stores the same values there and leaves them out of
+// sums); rows of fewer than 8 columns.  Either way a row's loads have no branch and are in flight
+// together; they and the stores are of 16 bytes and any alignment.
+enum Mode { kWhole, kTail, kSmall };
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int left, const float* x) {
-  if (left >= kVec) {
-    T t[kVec];
+template <int MODE>
+struct Cols {
+  int c, at;              // the first column, and where its 8 are loaded
+  bool in;
+  float m[MODE == kTail ? kVec : 1];
+  __device__ __forceinline__ Cols() {}
+  __device__ __forceinline__ Cols(int first, int dim) {
+    c = first, in = c < dim;
+    at = MODE == kSmall ? c : min(c, dim - kVec);
+    if (MODE == kTail)
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) t[j] = bs_from_f32<T>(x[j]);
-    __builtin_memcpy(p, t, sizeof(t));
-  } else {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j)
-      if (j < left) p[j] = bs_from_f32<T>(x[j]);
+      for (int j = 0; j < kVec; ++j) m[j] = in && at + j >= c ? 1.f : 0.f;
   }
-}
+  __device__ __forceinline__ float once(int j, float x) const {    // x, where column j counts
+    return MODE == kTail ? m[j] * x : x;
+  }
+};
 
-template <int NV>
-__device__ __forceinline__ void load_weight(const void* p, int dtype, int c0, int step, int dim,
-                                            float fill, float (*w)[kVec]) {
+template <typename T, int MODE>
+struct Vec8 {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* row, const Cols<MODE>& k, int dim) {
+    if (MODE != kSmall) {
+      __builtin_memcpy(w, row + k.at, sizeof(w));
+    } else {
+      T t[kVec];
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const int c = c0 + v * step + j;
-      w[v][j] = p && c < dim ? bs_load_any(p, dtype, c) : fill;
+      for (int j = 0; j < kVec; ++j) t[j] = k.at + j < dim ? row[k.at + j] : T{};
+      __builtin_memcpy(w, t, sizeof(w));
     }
+  }
+  // as numbers; 0 for a lane past the row
+  __device__ __forceinline__ void values(bool in, float* x) const {
+    T t[kVec];
+    __builtin_memcpy(t, w, sizeof(w));
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) x[j] = in ? bs_to_f32(t[j]) : 0.f;
+  }
+  static __device__ __forceinline__ void store(T* row, const Cols<MODE>& k, int dim,
+                                               const float* x) {
+    if (!k.in) return;
+    if (MODE != kSmall) {
+      uint4 o[sizeof(T) / 2];
+      if constexpr (sizeof(T) == 4) {
+        o[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                          __float_as_uint(x[3]));
+        o[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]),
+                          __float_as_uint(x[7]));
+      } else {
+        uint32_t* u = (uint32_t*)o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          u[j] = bs_from_f32<T>(x[2 * j]).u | (uint32_t)bs_from_f32<T>(x[2 * j + 1]).u << 16;
+      }
+      __builtin_memcpy(row + k.at, o, sizeof(o));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (k.at + j < dim) row[k.at + j] = bs_from_f32<T>(x[j]);
+    }
+  }
+};
+
+template <typename W, int NV, int MODE>
+__device__ __forceinline__ void load_typed(const W* p, const Cols<MODE>* k, int dim,
+                                           float (*w)[kVec]) {
+  Vec8<W, MODE> v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i].load(p, k[i], dim);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i].values(k[i].in, w[i]);
 }
 
-// Sums over the TPR lanes of a row; `turn` alternates so that one barrier a sum is enough.
+template <int NV, int MODE>
+__device__ __forceinline__ void load_weight(const void* p, int dtype, const Cols<MODE>* k, int dim,
+                                            float fill, float (*w)[kVec]) {
+  if (!p) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) w[v][j] = fill;
+  } else if (dtype == BS_F32) {
+    load_typed<float, NV>((const float*)p, k, dim, w);
+  } else if (dtype == BS_BF16) {
+    load_typed<bs_bf16, NV>((const bs_bf16*)p, k, dim, w);
+  } else {
+    load_typed<bs_f16, NV>((const bs_f16*)p, k, dim, w);
+  }
+}
+
+// Sums over the lanes of a row: TPR of a wave, or (TPR = 0) the whole workgroup, where `turn`
+// alternates so that one barrier a sum is enough.
 template <int TPR, int N>
 __device__ __forceinline__ void row_sum(float* x, float (*sh)[16][N], int& turn) {
 #pragma unroll
-  for (int d = 1; d < (TPR < 64 ? TPR : 64); d <<= 1)
+  for (int d = 1; d < (TPR ? TPR : 64); d <<= 1)
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] += __shfl_xor(x[i], d);
-  if (TPR > 64) {
-    const int wave = threadIdx.x >> 6;
+  if (TPR == 0) {
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) sh[turn][wave][i] = x[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      x[i] = 0.f;
+    for (int i = 0; i < N; ++i) x[i] = 0.f;
+    for (int k = 0; k < waves; ++k)
 #pragma unroll
-      for (int k = 0; k < TPR / 64; ++k) x[i] += sh[turn][k][i];
-    }
+      for (int i = 0; i < N; ++i) x[i] += sh[turn][k][i];
     turn ^= 1;
   }
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
+// 1 / (1 + exp(-z)): the hardware's exponential and reciprocal, each within 1 ulp; the exponent's
+// rounding adds |z| 2^-24 where exp(-z) counts beside 1.
+__device__ __forceinline__ float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z));
+}
 
-template <typename T, int TPR, int NV>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(bs_norm_in in, T* stream,
-                                                                     T* normed) {
-  constexpr int RPB = TPR >= 256 ? 1 : 256 / TPR;
+// TPR lanes to a row and 256 / TPR rows to a workgroup, or (TPR = 0) a row to a workgroup.
+template <typename T, int TPR, int NV, int BLOCK, int MODE>
+__global__ __launch_bounds__(BLOCK) void norm_kernel(bs_norm_in in, T* stream, T* normed) {
+  constexpr int RPB = TPR ? 256 / TPR : 1;
   __shared__ float sh[2][16][1];
-  const int t = threadIdx.x % TPR, c0 = t * kVec, step = TPR * kVec, dim = in.dim;
+  const int lanes = TPR ? TPR : blockDim.x, t = threadIdx.x % lanes;
+  const int step = lanes * kVec, dim = in.dim;
+  Cols<MODE> k[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) k[v] = Cols<MODE>(t * kVec + v * step, dim);
   int turn = 0;
   float post[NV][kVec], scale[NV][kVec], pre[NV][kVec];
-  load_weight<NV>(in.post, in.post_dtype, c0, step, dim, 1.f, post);
-  load_weight<NV>(in.scale, in.scale_dtype, c0, step, dim, in.scale_value, scale);
-  load_weight<NV>(in.pre, in.pre_dtype, c0, step, dim, 1.f, pre);
+  load_weight<NV>(in.post, in.post_dtype, k, dim, 1.f, post);
+  load_weight<NV>(in.scale, in.scale_dtype, k, dim, in.scale_value, scale);
+  load_weight<NV>(in.pre, in.pre_dtype, k, dim, 1.f, pre);
   const float inv = 1.f / (float)dim;
-  const int64_t first = (int64_t)blockIdx.x * RPB, stride = (int64_t)gridDim.x * RPB;
-  for (int64_t base = first; base < in.rows; base += stride) {
-    const int64_t row = base + threadIdx.x / TPR;
+  const int64_t stride = (int64_t)gridDim.x * RPB, last = in.rows - 1;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / lanes;
+  const int64_t turns = (in.rows - (int64_t)blockIdx.x * RPB + stride - 1) / stride;
+  Vec8<T, MODE> yv[NV], zv[NV], sv[NV];
+  // the next row's operands are loaded while this one's sums are taken
+  auto load = [&](int64_t r) {
+    r = r < last ? r : last;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      yv[v].load((const T*)in.y + r * in.y_stride, k[v], dim);
+      if (in.gate) zv[v].load((const T*)in.gate + r * in.gate_stride, k[v], dim);
+      if (in.residual) sv[v].load((const T*)in.residual + r * in.residual_stride, k[v], dim);
+    }
+  };
+  load(row);
+  for (int64_t turn_of = 0; turn_of < turns; ++turn_of, row += stride) {
     const bool live = row < in.rows;
     float x[NV][kVec], z[NV][kVec], s[NV][kVec];
     float sum[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = c0 + v * step, left = live ? dim - c : 0;
-      load8((const T*)in.y + row * in.y_stride + c, left, x[v]);
-      if (in.gate) load8((const T*)in.gate + row * in.gate_stride + c, left, z[v]);
-      if (in.residual) load8((const T*)in.residual + row * in.residual_stride + c, left, s[v]);
+      const bool inside = k[v].in;
+      yv[v].values(inside, x[v]);
+      if (in.gate) zv[v].values(inside, z[v]);
+      if (in.residual) sv[v].values(inside, s[v]);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) sum[0] = fmaf(x[v][j], x[v][j], sum[0]);
+      for (int j = 0; j < kVec; ++j) sum[0] = fmaf(k[v].once(j, x[v][j]), x[v][j], sum[0]);
     }
+    load(row + stride);
     float r1 = 1.f;
     if (in.post) {
       row_sum<TPR, 1>(sum, sh, turn);
@@ -122,10 +203,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(bs_norm_in 
         if (in.gate) a *= z[v][j] * sigmoid(z[v][j]);
         if (in.residual) a += s[v][j];
         s[v][j] = a;
-        sum[0] = fmaf(a, a, sum[0]);
+        sum[0] = fmaf(k[v].once(j, a), a, sum[0]);
       }
-      const int c = c0 + v * step;
-      if (live) store8(stream + row * dim + c, dim - c, s[v]);
+      if (live) yv[v].store(stream + row * dim, k[v], dim, s[v]);
     }
     if (in.pre) {
       row_sum<TPR, 1>(sum, sh, turn);
@@ -134,8 +214,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(bs_norm_in 
       for (int v = 0; v < NV; ++v) {
 #pragma unroll
         for (int j = 0; j < kVec; ++j) s[v][j] *= r2 * pre[v][j];
-        const int c = c0 + v * step;
-        if (live) store8(normed + row * dim + c, dim - c, s[v]);
+        if (live) yv[v].store(normed + row * dim, k[v], dim, s[v]);
       }
     }
   }
@@ -149,20 +228,23 @@ struct NormGrad {
 
 // With n = s r2, dn = grad normed . pre:  ds = grad stream + r2 (dn - n mean(dn n)), and the like
 // for y; sums of a row: y^2, then s^2 and dn s, then what reaches y.
-template <typename T, int TPR, int NV>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_grad_kernel(bs_norm_in in,
-                                                                          NormGrad o) {
-  constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+template <typename T, int TPR, int NV, int BLOCK, int MODE>
+__global__ __launch_bounds__(BLOCK) void norm_grad_kernel(bs_norm_in in, NormGrad o) {
+  constexpr int RPB = TPR ? 256 / TPR : 1;
   __shared__ float sh[2][16][1];
   __shared__ float sh2[2][16][2];
   __shared__ float acc[BLOCK * kVec];
-  const int t = threadIdx.x % TPR, c0 = t * kVec, step = TPR * kVec, dim = in.dim;
+  const int lanes = TPR ? TPR : blockDim.x, t = threadIdx.x % lanes;
+  const int step = lanes * kVec, dim = in.dim;
+  Cols<MODE> k[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) k[v] = Cols<MODE>(t * kVec + v * step, dim);
   int turn = 0, turn2 = 0;
   float post[NV][kVec], scale[NV][kVec], pre[NV][kVec];
   float dw[3][NV][kVec];
-  load_weight<NV>(in.post, in.post_dtype, c0, step, dim, 1.f, post);
-  load_weight<NV>(in.scale, in.scale_dtype, c0, step, dim, in.scale_value, scale);
-  load_weight<NV>(in.pre, in.pre_dtype, c0, step, dim, 1.f, pre);
+  load_weight<NV>(in.post, in.post_dtype, k, dim, 1.f, post);
+  load_weight<NV>(in.scale, in.scale_dtype, k, dim, in.scale_value, scale);
+  load_weight<NV>(in.pre, in.pre_dtype, k, dim, 1.f, pre);
 #pragma unroll
   for (int i = 0; i < 3; ++i)
 #pragma unroll
@@ -170,25 +252,36 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_grad_kernel(bs_nor
 #pragma unroll
       for (int j = 0; j < kVec; ++j) dw[i][v][j] = 0.f;
   const float inv = 1.f / (float)dim;
-  for (int64_t base = (int64_t)blockIdx.x * RPB; base < in.rows;
-       base += (int64_t)gridDim.x * RPB) {
-    const int64_t row = base + threadIdx.x / TPR;
+  const int64_t stride = (int64_t)gridDim.x * RPB, last = in.rows - 1;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / lanes;
+  const int64_t turns = (in.rows - (int64_t)blockIdx.x * RPB + stride - 1) / stride;
+  Vec8<T, MODE> yv[NV], zv[NV], sv[NV], gsv[NV], gnv[NV];
+  auto load = [&](int64_t r) {
+    r = r < last ? r : last;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      yv[v].load((const T*)in.y + r * in.y_stride, k[v], dim);
+      if (in.gate) zv[v].load((const T*)in.gate + r * in.gate_stride, k[v], dim);
+      if (in.residual) sv[v].load((const T*)in.residual + r * in.residual_stride, k[v], dim);
+      if (o.gs) gsv[v].load((const T*)o.gs + r * dim, k[v], dim);
+      if (o.gn) gnv[v].load((const T*)o.gn + r * dim, k[v], dim);
+    }
+  };
+  for (int64_t turn_of = 0; turn_of < turns; ++turn_of, row += stride) {
     const bool live = row < in.rows;
+    load(row);
     float x[NV][kVec], z[NV][kVec], s[NV][kVec], d[NV][kVec], dn[NV][kVec];
     float sum[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = c0 + v * step, left = live ? dim - c : 0;
-      load8((const T*)in.y + row * in.y_stride + c, left, x[v]);
-      if (in.gate) load8((const T*)in.gate + row * in.gate_stride + c, left, z[v]);
-      if (in.residual) load8((const T*)in.residual + row * in.residual_stride + c, left, s[v]);
-      if (o.gs) load8((const T*)o.gs + row * dim + c, left, d[v]);
-      if (o.gn) load8((const T*)o.gn + row * dim + c, left, dn[v]);
+      const bool inside = k[v].in;
+      yv[v].values(inside, x[v]);
+      if (in.gate) zv[v].values(inside, z[v]);
+      if (in.residual) sv[v].values(inside, s[v]);
+      gsv[v].values(o.gs && inside && live, d[v]);       // a row that is not there gives nothing
+      gnv[v].values(o.gn && inside && live, dn[v]);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        sum[0] = fmaf(x[v][j], x[v][j], sum[0]);
-        if (!o.gs) d[v][j] = 0.f;
-      }
+      for (int j = 0; j < kVec; ++j) sum[0] = fmaf(k[v].once(j, x[v][j]), x[v][j], sum[0]);
     }
     float r1 = 1.f;
     if (in.post) {
@@ -206,26 +299,25 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_grad_kernel(bs_nor
         if (in.residual) a += s[v][j];
         s[v][j] = a;
         if (o.gn) {
-          two[0] = fmaf(a, a, two[0]);
-          two[1] = fmaf(dn[v][j] * pre[v][j], a, two[1]);
+          two[0] = fmaf(k[v].once(j, a), a, two[0]);
+          two[1] = fmaf(k[v].once(j, dn[v][j]) * pre[v][j], a, two[1]);
         }
       }
     if (o.gn) {
       row_sum<TPR, 2>(two, sh2, turn2);
-      const float r2 = rsqrtf(two[0] * inv + in.eps), k = two[1] * r2 * r2 * inv;
+      const float r2 = rsqrtf(two[0] * inv + in.eps), off = two[1] * r2 * r2 * inv;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
           dw[2][v][j] = fmaf(dn[v][j], s[v][j] * r2, dw[2][v][j]);
-          d[v][j] += r2 * (dn[v][j] * pre[v][j] - s[v][j] * k);
+          d[v][j] += r2 * (dn[v][j] * pre[v][j] - s[v][j] * off);
         }
     }
     sum[0] = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = c0 + v * step;
-      if (live && o.dresidual) store8((T*)o.dresidual + row * dim + c, dim - c, d[v]);
+      if (live && o.dresidual) yv[v].store((T*)o.dresidual + row * dim, k[v], dim, d[v]);
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
         const float p = x[v][j] * post[v][j];
@@ -240,18 +332,17 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_grad_kernel(bs_nor
         const float dp = d[v][j] * scale[v][j] * act;
         dw[0][v][j] = fmaf(dp, x[v][j], dw[0][v][j]);
         d[v][j] = dp * post[v][j];
-        sum[0] = fmaf(d[v][j], x[v][j], sum[0]);
+        sum[0] = fmaf(k[v].once(j, d[v][j]), x[v][j], sum[0]);
       }
-      if (live && o.dgate) store8((T*)o.dgate + row * dim + c, dim - c, z[v]);
+      if (live && o.dgate) yv[v].store((T*)o.dgate + row * dim, k[v], dim, z[v]);
     }
     if (in.post) row_sum<TPR, 1>(sum, sh, turn);
-    const float k = in.post ? sum[0] * inv : 0.f;
+    const float off = in.post ? sum[0] * inv : 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) d[v][j] = r1 * (d[v][j] - x[v][j] * k);
-      const int c = c0 + v * step;
-      if (live && o.dy) store8((T*)o.dy + row * dim + c, dim - c, d[v]);
+      for (int j = 0; j < kVec; ++j) d[v][j] = r1 * (d[v][j] - x[v][j] * off);
+      if (live && o.dy) yv[v].store((T*)o.dy + row * dim, k[v], dim, d[v]);
     }
   }
   if (!o.part) return;
@@ -261,32 +352,37 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_grad_kernel(bs_nor
     for (int v = 0; v < NV; ++v) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) acc[threadIdx.x * kVec + j] = dw[i][v][j];
+      for (int j = 0; j < kVec; ++j) {
+        const int e = k[v].at + j - v * step;
+        if (MODE != kTail || k[v].m[j] != 0.f)
+          if (k[v].in) acc[threadIdx.x / lanes * step + e] = dw[i][v][j];
+      }
       __syncthreads();
-      for (int e = threadIdx.x; e < TPR * kVec; e += BLOCK) {   // the rows side by side
-        float a = 0.f;
-        for (int k = 0; k < RPB; ++k) a += acc[k * TPR * kVec + e];
+      for (int e = threadIdx.x; e < step; e += blockDim.x) {   // the rows side by side
         const int c = v * step + e;
+        float a = 0.f;
+        if (c < dim)
+          for (int x = 0; x < RPB; ++x) a += acc[x * step + e];
         if (c < dim) o.part[((int64_t)blockIdx.x * 3 + i) * dim + c] = a;
       }
     }
 }
 
-// Column sums of the workgroups' parts: 64 columns a workgroup, 16 waves over the parts.
+// Column sums of the workgroups' parts: 32 columns a workgroup, 32 half waves over the parts.
 __global__ __launch_bounds__(1024) void grad_sum_kernel(const float* part, int parts, int dim,
                                                         bs_norm_in in, void* dpost, void* dscale,
                                                         void* dpre) {
-  __shared__ float sh[16][64];
-  const int which = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  __shared__ float sh[32][33];
+  const int which = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
   void* out = which == 0 ? dpost : which == 1 ? dscale : dpre;
   if (!out) return;
   float a = 0.f;
   if (c < dim)
-    for (int k = w; k < parts; k += 16) a += part[((int64_t)k * 3 + which) * dim + c];
-  sh[w][threadIdx.x & 63] = a;
+    for (int k = w; k < parts; k += 32) a += part[((int64_t)k * 3 + which) * dim + c];
+  sh[w][threadIdx.x & 31] = a;
   __syncthreads();
   if (w == 0 && c < dim) {
-    for (int k = 1; k < 16; ++k) a += sh[k][threadIdx.x & 63];
+    for (int k = 1; k < 32; ++k) a += sh[k][threadIdx.x];
     bs_store_any(out, which == 0 ? in.post_dtype : which == 1 ? in.scale_dtype : in.pre_dtype, c,
                  a);
   }
@@ -303,55 +399,64 @@ int check(const bs_norm_in* in, const char* who) {
   return BS_OK;
 }
 
-struct Shape { int tpr, nv; };
+// Lanes to a row: as many as it has runs of 8 values, a power of two up to a wave, whole waves
+// above; two runs a lane past 4,096 values.
+struct Shape { int lanes, nv; };
 Shape shape_of(int dim) {
-  static const Shape s[] = {{16, 1}, {16, 2}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {1024, 1},
-                            {1024, 2}};
-  for (const Shape& x : s)
-    if (dim <= x.tpr * x.nv * kVec) return x;
-  return s[7];
+  const int runs = (dim + kVec - 1) / kVec;
+  if (runs <= 16) return {16, 1};
+  if (runs <= 32) return {32, 1};
+  const int nv = runs > 512 ? 2 : 1;
+  return {(runs + 64 * nv - 1) / (64 * nv) * 64, nv};
 }
+int block_of(const Shape& s) { return s.lanes <= 64 ? 256 : s.lanes; }
 
-int grid_of(const bs_norm_in& in, const Shape& s, int per_cu) {
-  const int rpb = s.tpr >= 256 ? 1 : 256 / s.tpr;
-  const int64_t need = (in.rows + rpb - 1) / rpb, most = (int64_t)per_cu * bs_num_cus();
+int grid_of(const bs_norm_in& in, const Shape& s, int threads) {   // threads: wanted on a CU
+  const int block = block_of(s), rpb = s.lanes <= 64 ? 256 / s.lanes : 1;
+  const int64_t need = (in.rows + rpb - 1) / rpb;
+  const int64_t most = (int64_t)(threads / block > 1 ? threads / block : 1) * bs_num_cus();
   return (int)(need < most ? need : most);
 }
 
-constexpr int kGradPerCu = 2;
+constexpr int kThreads = 2048, kGradThreads = 1024;
 
-template <typename T, typename F>
-void by_shape(const Shape& s, F&& f) {
-  switch (s.tpr * s.nv) {
-    case 16: f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>()); break;
-    case 32: f(std::integral_constant<int, 16>(), std::integral_constant<int, 2>()); break;
-    case 64: f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>()); break;
-    case 128: f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>()); break;
-    case 256: f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>()); break;
-    case 512: f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>()); break;
-    case 1024: f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>()); break;
-    default: f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
-  }
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+// f(lanes of a row or 0, runs a lane, largest workgroup, mode)
+template <typename F>
+void by_shape(const Shape& s, int dim, F&& f) {
+  auto moded = [&](auto... a) {
+    if (dim % kVec == 0) f(a..., Int<kWhole>());
+    else f(a..., Int<kTail>());
+  };
+  if (dim < kVec) f(Int<16>(), Int<1>(), Int<256>(), Int<kSmall>());
+  else if (s.lanes == 16) moded(Int<16>(), Int<1>(), Int<256>());
+  else if (s.lanes == 32) moded(Int<32>(), Int<1>(), Int<256>());
+  else if (s.lanes == 64) moded(Int<64>(), Int<1>(), Int<256>());
+  else if (s.nv == 1) moded(Int<0>(), Int<1>(), Int<512>());
+  else if (s.lanes <= 512) moded(Int<0>(), Int<2>(), Int<512>());
+  else moded(Int<0>(), Int<2>(), Int<1024>());
 }
 
 template <typename T>
 void launch(const bs_norm_in& in, void* stream, void* normed, hipStream_t st) {
   const Shape s = shape_of(in.dim);
-  const int grid = grid_of(in, s, 8);
-  by_shape<T>(s, [&](auto tpr, auto nv) {
-    norm_kernel<T, tpr.value, nv.value><<<grid, tpr.value > 256 ? tpr.value : 256, 0, st>>>(
-        in, (T*)stream, (T*)normed);
+  const int grid = grid_of(in, s, kThreads);
+  by_shape(s, in.dim, [&](auto tpr, auto nv, auto block, auto mode) {
+    norm_kernel<T, tpr.value, nv.value, block.value, mode.value>
+        <<<grid, block_of(s), 0, st>>>(in, (T*)stream, (T*)normed);
   });
 }
 
 template <typename T>
 void launch_grad(const bs_norm_in& in, const NormGrad& o, hipStream_t st) {
   const Shape s = shape_of(in.dim);
-  const int grid = grid_of(in, s, kGradPerCu);
+  const int grid = grid_of(in, s, kGradThreads);
   if (grid == 0) return;
-  by_shape<T>(s, [&](auto tpr, auto nv) {
-    norm_grad_kernel<T, tpr.value, nv.value><<<grid, tpr.value > 256 ? tpr.value : 256, 0, st>>>(
-        in, o);
+  by_shape(s, in.dim, [&](auto tpr, auto nv, auto block, auto mode) {
+    norm_grad_kernel<T, tpr.value, nv.value, block.value, mode.value>
+        <<<grid, block_of(s), 0, st>>>(in, o);
   });
 }
 
@@ -374,7 +479,7 @@ extern "C" size_t bs_norm_grad_workspace_size(int64_t rows, int32_t dim) {
   bs_norm_in in = {};
   in.rows = rows, in.dim = dim;
   if (rows < 1 || dim < 1 || dim > 16384) return 0;
-  return (size_t)grid_of(in, shape_of(dim), kGradPerCu) * 3 * dim * sizeof(float);
+  return (size_t)grid_of(in, shape_of(dim), kGradThreads) * 3 * dim * sizeof(float);
 }
 
 extern "C" int bs_norm_gate_residual_grad(const bs_norm_in* in, const void* grad_stream,
@@ -400,8 +505,8 @@ extern "C" int bs_norm_gate_residual_grad(const bs_norm_in* in, const void* grad
   else launch_grad<bs_f16>(*in, o, st);
   BS_CHECK_LAUNCH();
   if (weights) {
-    const int parts = grid_of(*in, shape_of(in->dim), kGradPerCu);
-    grad_sum_kernel<<<dim3((in->dim + 63) / 64, 3), 1024, 0, st>>>(
+    const int parts = grid_of(*in, shape_of(in->dim), kGradThreads);
+    grad_sum_kernel<<<dim3((in->dim + 31) / 32, 3), 1024, 0, st>>>(
         (const float*)workspace, parts, in->dim, *in, dpost, dscale, dpre);
     BS_CHECK_LAUNCH();
   }
