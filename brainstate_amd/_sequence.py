@@ -15,56 +15,77 @@ _NORM_IN = struct.Struct('6P4q5i2f')       # bs_norm_in
 
 
 def _floating(name, t, dtype=None):
-    if not torch.is_tensor(t):
+    """Number of the type of ``t`` (enum bs_dtype); raises for what is no floating GPU tensor."""
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f'{name} must be a tensor, not {type(t).__name__}')
-    if t.dtype not in _DTYPES:
+    number = _DTYPES.get(t.dtype)
+    if number is None:
         raise TypeError(f'{name}: dtype {t.dtype} not supported (float32, bfloat16, float16)')
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f'{name} is {t.dtype}, expected {dtype}')
     if not t.is_cuda:
+        N.require_gpu()
         raise ValueError(f'{name} must be on the GPU')
+    return number
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                return True
+    return False
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 # ------------------------------------------------------------------------- gated delta rule
 def _delta_operands(q, k, v, g, beta, scale):
-    """Checked operands as (views, bytes of bs_delta_in, sizes).  A head's values have to lie
-    side by side; any other strides are taken as they are."""
-    _floating('q', q)
-    for name, t in (('k', k), ('v', v)):
-        _floating(name, t, q.dtype)
-    for name, t in (('g', g), ('beta', beta)):
-        _floating(name, t)
-    if q.dim() != 4 or q.shape != k.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2]:
+    """Checked operands as (views, bytes of bs_delta_in, sizes)."""
+    qt = _floating('q', q)
+    _floating('k', k, q.dtype)
+    _floating('v', v, q.dtype)
+    gt, bt = _floating('g', g), _floating('beta', beta)
+    shape, vshape = q.shape, v.shape
+    if len(shape) != 4 or shape != k.shape or len(vshape) != 4 or vshape[:2] != shape[:2]:
         raise ValueError(f'q, k [batch, tokens, key heads, dk] and v [batch, tokens, heads, dv]: '
-                         f'got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
-    b, t, hk, dk = q.shape
-    hv, dv = v.shape[2:]
+                         f'got {tuple(shape)}, {tuple(k.shape)}, {tuple(vshape)}')
+    b, t, hk, dk = shape
+    hv, dv = vshape[2:]
     if hk < 1 or hv < 1 or hv % hk:
         raise ValueError(f'{hv} value heads for {hk} key heads')
     if not 1 <= dk <= 128 or not 1 <= dv <= 128:
         raise ValueError(f'head sizes {dk}, {dv} outside 1..128')
-    if g.shape != v.shape[:3] or beta.shape != v.shape[:3]:
-        raise ValueError(f'g and beta must be {tuple(v.shape[:3])}: got {tuple(g.shape)}, '
+    if g.shape != vshape[:3] or beta.shape != vshape[:3]:
+        raise ValueError(f'g and beta must be {tuple(vshape[:3])}: got {tuple(g.shape)}, '
                          f'{tuple(beta.shape)}')
     dev = q.device
-    if any(x.device != dev for x in (k, v, g, beta)):
+    if not (dev == k.device == v.device == g.device == beta.device):
         raise ValueError('q, k, v, g and beta must be on one device')
-    q, k, v = (x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous() for x in (q, k, v))
-    q, k, v = (x if x.stride(1) < 1 << 23 else x.contiguous() for x in (q, k, v))
-    scale = dk ** -0.5 if scale is None else float(scale)
+    return _delta_pack(q, k, v, g, beta, scale, qt, gt, bt) + ((b, t, hk, hv, dk, dv),)
+
+
+def _heads(x):
+    """``x`` with a head's values side by side; any other strides are taken as they are."""
+    at = x.stride()
+    return x if (at[3] == 1 or x.shape[3] == 1) and at[1] < 1 << 23 else x.contiguous()
+
+
+def _delta_pack(q, k, v, g, beta, scale, qt, gt, bt):
+    q, k, v = _heads(q), _heads(k), _heads(v)
+    dk = q.shape[3]
     packed = _DELTA_IN.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride(),
-        _DTYPES[q.dtype], _DTYPES[g.dtype], _DTYPES[beta.dtype], hk, hv, dk, dv, scale)
-    return (q, k, v, g, beta), packed, (b, t, hk, hv, dk, dv)
+        qt, gt, bt, q.shape[2], v.shape[2], dk, v.shape[3],
+        dk ** -0.5 if scale is None else float(scale))
+    return (q, k, v, g, beta), packed
 
 
 def _states(name, s, n, hv, dk, dv, device):
-    if not torch.is_tensor(s) or s.dtype != torch.float32:
+    if not isinstance(s, torch.Tensor) or s.dtype != torch.float32:
         raise TypeError(f'{name} must be a float32 tensor')
     if s.dim() != 4 or tuple(s.shape[1:]) != (hv, dk, dv) or n is not None and s.shape[0] != n:
         raise ValueError(f'{name} must be [{"n" if n is None else n}, {hv}, {dk}, {dv}]: got '
@@ -84,11 +105,10 @@ def gated_delta_step(q, k, v, g, beta, state, slots=None, scale=None):
     order.  ``state`` [n, heads, dk, dv] float32, contiguous.  ``slots`` [batch] int32 names each
     row's state; a negative one (or one from n on) marks an idle row, whose output is 0.  Without
     it row b has state b.  Not differentiable."""
-    N.require_gpu()
     if _wants_grad(q, k, v, g, beta, state):
         raise ValueError('gated_delta_step updates its state in place and has no gradient: use '
                          'gated_delta_rule, or torch.no_grad()')
-    one = torch.is_tensor(q) and q.dim() == 3
+    one = isinstance(q, torch.Tensor) and q.dim() == 3
     if one:
         if v.dim() != 3 or k.dim() != 3 or g.dim() != 2 or beta.dim() != 2:
             raise ValueError('q, k, v, g and beta must all have a dimension of tokens, or none')
@@ -106,7 +126,7 @@ def gated_delta_step(q, k, v, g, beta, state, slots=None, scale=None):
         slots = slots.contiguous()
     o = torch.empty((b, t, hv, dv), dtype=q.dtype, device=q.device)
     N.check(N.lib().bs_gated_delta_step(packed, b, t, state.data_ptr(), state.shape[0],
-                                        N.ptr(slots), o.data_ptr(), N.raw_stream(q.device)),
+                                        _address(slots), o.data_ptr(), N.raw_stream(q.device)),
             'bs_gated_delta_step')
     return o.squeeze(1) if one else o
 
@@ -140,8 +160,8 @@ def _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, keep):
     nbytes = lib.bs_gated_delta_workspace_size(packed, n, t, seq_offsets is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     N.check(lib.bs_gated_delta_rule(
-        packed, n, t, N.ptr(seq_offsets), N.ptr(initial_state), final.data_ptr(), o.data_ptr(),
-        N.ptr(kept[0]), N.ptr(kept[1]), ws.data_ptr(), nbytes, N.raw_stream(dev)),
+        packed, n, t, _address(seq_offsets), _address(initial_state), final.data_ptr(), o.data_ptr(),
+        _address(kept[0]), _address(kept[1]), ws.data_ptr(), nbytes, N.raw_stream(dev)),
         'bs_gated_delta_rule')
     return o, final, kept
 
@@ -162,7 +182,8 @@ class _DeltaRule(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, go, gstate):
         *x, seq_offsets, kept_s, kept_u = ctx.saved_tensors
-        held, packed, (b, t, hk, hv, dk, dv) = _delta_operands(*x, ctx.scale)
+        held, packed = _delta_pack(*x, ctx.scale, *(_DTYPES[x[i].dtype] for i in (0, 3, 4)))
+        (b, t, hk, dk), (hv, dv) = x[0].shape, x[2].shape[2:]
         dev = x[0].device
         n = b
         if seq_offsets is not None:
@@ -177,8 +198,8 @@ class _DeltaRule(torch.autograd.Function):
         nbytes = lib.bs_gated_delta_grad_workspace_size(packed, n, t, seq_offsets is not None)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         N.check(lib.bs_gated_delta_rule_grad(
-            packed, n, t, N.ptr(seq_offsets), go.data_ptr(), N.ptr(gstate), kept_s.data_ptr(),
-            kept_u.data_ptr(), *(y.data_ptr() for y in grads), N.ptr(ds), ws.data_ptr(), nbytes,
+            packed, n, t, _address(seq_offsets), go.data_ptr(), _address(gstate), kept_s.data_ptr(),
+            kept_u.data_ptr(), *(y.data_ptr() for y in grads), _address(ds), ws.data_ptr(), nbytes,
             N.raw_stream(dev)), 'bs_gated_delta_rule_grad')
         return (*grads, ds, None, None)
 
@@ -192,7 +213,6 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, seq_offse
     ``seq_offsets`` (int32 [sequences + 1], ascending) the sequences are packed end to end into
     one batch row; tokens outside all of them give 0.  Differentiable in everything but
     ``seq_offsets``."""
-    N.require_gpu()
     if _wants_grad(q, k, v, g, beta, initial_state):
         return _DeltaRule.apply(q, k, v, g, beta, initial_state, scale, seq_offsets)
     o, final, _ = _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, False)
@@ -202,41 +222,48 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, seq_offse
 # ------------------------------------------------------------------------- norms around a block
 def _rows(t, dim):
     """``t`` [.., dim] as rows with their values side by side."""
-    t = t.reshape(-1, dim)
+    if t.dim() != 2:
+        t = t.reshape(-1, dim)
     return t if t.stride(1) == 1 or dim == 1 else t.contiguous()
 
 
 def _norm_operands(y, post, gate, scale, residual, pre, eps):
     """Checked operands as (row views, bytes of bs_norm_in, rows, dim)."""
     _floating('y', y)
-    if y.dim() < 1 or not 1 <= y.shape[-1] <= 16384:
-        raise ValueError(f'y [.., dim] with dim in 1..16384: got {tuple(y.shape)}')
-    dim, dev = y.shape[-1], y.device
+    shape, dtype, dev = y.shape, y.dtype, y.device
+    if len(shape) < 1 or not 1 <= shape[-1] <= 16384:
+        raise ValueError(f'y [.., dim] with dim in 1..16384: got {tuple(shape)}')
+    dim = shape[-1]
     for name, t in (('gate', gate), ('residual', residual)):
         if t is not None:
-            _floating(name, t, y.dtype)
-            if t.shape != y.shape or t.device != dev:
-                raise ValueError(f'{name} must be {tuple(y.shape)} on {dev}: got '
+            _floating(name, t, dtype)
+            if t.shape != shape or t.device != dev:
+                raise ValueError(f'{name} must be {tuple(shape)} on {dev}: got '
                                  f'{tuple(t.shape)} on {t.device}')
-    value = 1.0
-    if scale is not None and not torch.is_tensor(scale):
-        scale, value = None, float(scale)
-    weights = []
+    if scale is not None and not isinstance(scale, torch.Tensor):
+        scale = float(scale)
     for name, t in (('post_weight', post), ('scale', scale), ('pre_weight', pre)):
-        if t is not None:
+        if t is not None and t.__class__ is not float:
             _floating(name, t)
             if t.shape != (dim,) or t.device != dev:
                 raise ValueError(f'{name} must be [{dim}] on {dev}: got {tuple(t.shape)} on '
                                  f'{t.device}')
-            t = t.contiguous()
-        weights.append(t)
+    return _norm_pack(y, post, gate, scale, residual, pre, eps)
+
+
+def _norm_pack(y, post, gate, scale, residual, pre, eps):
+    dim, value = y.shape[-1], 1.0
+    if scale.__class__ is float:
+        scale, value = None, scale
     acts = [t if t is None else _rows(t, dim) for t in (y, gate, residual)]
+    weights = [t if t is None else t.contiguous() for t in (post, scale, pre)]
+    y_at, gate_at, residual_at = [0 if t is None else t.data_ptr() for t in acts]
+    post_at, scale_at, pre_at = [0 if t is None else t.data_ptr() for t in weights]
     rows = acts[0].shape[0]
-    at = [0 if t is None else t.data_ptr() for t in acts + weights]
     packed = _NORM_IN.pack(
-        at[0], at[3], at[1], at[4], at[2], at[5],
-        *(0 if t is None else t.stride(0) for t in acts), rows, dim, _DTYPES[y.dtype],
-        *(0 if t is None else _DTYPES[t.dtype] for t in weights), eps, value)
+        y_at, post_at, gate_at, scale_at, residual_at, pre_at,
+        *[0 if t is None else t.stride(0) for t in acts], rows, dim, _DTYPES[y.dtype],
+        *[0 if t is None else _DTYPES[t.dtype] for t in weights], eps, value)
     return (acts, weights), packed, rows, dim
 
 
@@ -244,7 +271,7 @@ def _norm_forward(y, post, gate, scale, residual, pre, eps):
     held, packed, _, _ = _norm_operands(y, post, gate, scale, residual, pre, eps)
     stream = torch.empty(y.shape, dtype=y.dtype, device=y.device)
     normed = torch.empty_like(stream) if pre is not None else None
-    N.check(N.lib().bs_norm_gate_residual(packed, stream.data_ptr(), N.ptr(normed),
+    N.check(N.lib().bs_norm_gate_residual(packed, stream.data_ptr(), _address(normed),
                                           N.raw_stream(y.device)), 'bs_norm_gate_residual')
     return stream, normed
 
@@ -255,7 +282,7 @@ class _NormGateResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, post, gate, scale, residual, pre, eps):
         ctx.eps = eps
-        ctx.value = None if torch.is_tensor(scale) else scale
+        ctx.value = None if scale is None or isinstance(scale, torch.Tensor) else float(scale)
         ctx.save_for_backward(y, post, gate, scale if ctx.value is None else None, residual, pre)
         ctx.set_materialize_grads(False)
         return _norm_forward(y, post, gate, scale, residual, pre, eps)
@@ -264,7 +291,7 @@ class _NormGateResidual(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, gs, gn):
         y, post, gate, scale, residual, pre = x = ctx.saved_tensors
-        held, packed, rows, dim = _norm_operands(
+        held, packed, rows, dim = _norm_pack(
             y, post, gate, scale if ctx.value is None else ctx.value, residual, pre, ctx.eps)
         dev = y.device
         gs, gn = (None if t is None else t.contiguous() for t in (gs, gn))
@@ -276,7 +303,7 @@ class _NormGateResidual(torch.autograd.Function):
             nbytes = lib.bs_norm_grad_workspace_size(rows, dim)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         N.check(lib.bs_norm_gate_residual_grad(
-            packed, N.ptr(gs), N.ptr(gn), *(N.ptr(t) for t in grads), N.ptr(ws), nbytes,
+            packed, _address(gs), _address(gn), *(_address(t) for t in grads), _address(ws), nbytes,
             N.raw_stream(dev)), 'bs_norm_gate_residual_grad')
         return (*grads, None)
 
@@ -293,8 +320,7 @@ def norm_gate_residual(y, post_weight=None, gate=None, scale=None, residual=None
     ``pre_weight`` are [dim] of any floating type, ``scale`` may be a number.  Any of them may be
     left out, with its norm or factor.  Sums are in 32 bits; ``normed`` is formed before
     ``stream`` is rounded.  Differentiable in every tensor."""
-    N.require_gpu()
-    if _wants_grad(y, post_weight, gate, scale if torch.is_tensor(scale) else None, residual,
+    if _wants_grad(y, post_weight, gate, scale if isinstance(scale, torch.Tensor) else None, residual,
                    pre_weight):
         return _NormGateResidual.apply(y, post_weight, gate, scale, residual, pre_weight, eps)
     return _norm_forward(y, post_weight, gate, scale, residual, pre_weight, eps)
@@ -307,7 +333,7 @@ def _no_grad(who, *ts):
 
 
 def _channels(name, t, n, dev):
-    if not torch.is_tensor(t) or t.dtype != torch.float32 or t.shape != (n,) or t.device != dev:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != (n,) or t.device != dev:
         raise ValueError(f'{name} must be float32 [{n}] on {dev}')
     return t.contiguous()
 
@@ -316,7 +342,6 @@ def int8_quantize(x):
     """Rows of ``x`` [.., k] in 8 bits -> (int8 [.., k], float32 scales [..]): scale
     ``max|x| / 127``, integers ``127 x / max|x|`` rounded to nearest (ties to even).  A row of zeros
     has scale 0.  Not differentiable."""
-    N.require_gpu()
     _floating('x', x)
     _no_grad('int8_quantize', x)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 65536:
@@ -333,7 +358,7 @@ def int8_quantize(x):
 
 def _int8_product(x, x_scale, w8, w_scale, bias, out_dtype):
     dev = x.device
-    if not torch.is_tensor(w8) or w8.dtype != torch.int8 or w8.dim() != 2 or w8.device != dev:
+    if not isinstance(w8, torch.Tensor) or w8.dtype != torch.int8 or w8.dim() != 2 or w8.device != dev:
         raise ValueError(f'w8 must be int8 [channels, k] on {dev}')
     n, k = w8.shape
     if x.dim() < 1 or x.shape[-1] != k or not 1 <= k <= 65536:
@@ -357,8 +382,8 @@ def _int8_product(x, x_scale, w8, w_scale, bias, out_dtype):
     nbytes = m * (-(-k // 128) * 128 + 4)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     N.check(N.lib().bs_int8_linear(
-        rows.data_ptr(), _DTYPES.get(x.dtype, 0), rows.stride(0), N.ptr(x_scale), m, k, n,
-        w8.data_ptr(), w_scale.data_ptr(), N.ptr(bias),
+        rows.data_ptr(), _DTYPES.get(x.dtype, 0), rows.stride(0), _address(x_scale), m, k, n,
+        w8.data_ptr(), w_scale.data_ptr(), _address(bias),
         0 if bias is None else _DTYPES[bias.dtype], y.data_ptr(), _DTYPES[out_dtype],
         ws.data_ptr(), nbytes, N.raw_stream(dev)), 'bs_int8_linear')
     return y
@@ -368,8 +393,8 @@ def int8_matmul(x8, x_scale, w8, w_scale, bias=None, out_dtype=torch.float32):
     """``x_scale[m] * w_scale[n] * sum_k x8[m, k] * w8[n, k] + bias[n]`` with exact sums: tokens
     ``x8`` int8 [.., k] with a scale each (:func:`int8_quantize`), weights ``w8`` int8 [n, k] with
     a scale for each channel.  Not differentiable."""
-    N.require_gpu()
-    if not torch.is_tensor(x8) or x8.dtype != torch.int8 or not x8.is_cuda:
+    if not isinstance(x8, torch.Tensor) or x8.dtype != torch.int8 or not x8.is_cuda:
+        N.require_gpu()
         raise TypeError('x8 must be an int8 tensor on the GPU')
     if out_dtype not in _DTYPES:
         raise TypeError(f'out_dtype {out_dtype} not supported (float32, bfloat16, float16)')
@@ -381,7 +406,6 @@ def int8_linear(x, w8, w_scale, bias=None):
     """``x`` [.., k] times 8-bit weights ``w8`` [n, k] with a scale for each channel -> [.., n] of
     the type of ``x``: its rows are quantized on the way (:func:`int8_quantize`), the sums are
     exact, ``bias`` [n] is added in 32 bits.  Not differentiable."""
-    N.require_gpu()
     _floating('x', x)
     _no_grad('int8_linear', x, w_scale, bias)
     return _int8_product(x, None, w8, w_scale, bias, x.dtype)

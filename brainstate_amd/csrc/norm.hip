@@ -418,7 +418,7 @@ int grid_of(const bs_norm_in& in, const Shape& s, int threads) {   // threads: w
   return (int)(need < most ? need : most);
 }
 
-constexpr int kThreads = 2048, kGradThreads = 1024;
+constexpr int kThreads = 2048, kGradThreads = 512;
 
 template <int V>
 using Int = std::integral_constant<int, V>;
