@@ -7,11 +7,14 @@
 // products then need no test of k on that side, and what the weights' side reads past a row's end
 // is multiplied by 0.
 //
-// Few tokens (skinny_kernel): bound by the weights' bytes.  Each workgroup has 16 channels and its
-// waves share k; weights go straight from memory to the matrix instruction, whose operand is 16
-// rows x 64 bytes.  Many tokens (tile_kernel): bound by the matrix cores; tiles of both operands
-// are staged in LDS by direct loads, two deep, 16-byte pieces in an order that keeps the reads off
-// each other's banks.
+// Few tokens (skinny_kernel): bound by the weights' bytes, and below a few MB by the latency of
+// one pass over k.  Each workgroup has 16 channels and its waves share k; weights go straight from
+// memory to the matrix instruction, whose operand is 16 rows x 64 bytes.  One token x 4,096 x
+// 4,096: 6.0 us (2.8 TB/s; 16.9 MB fetched for 16.8), with 3.6 before it for the token's integers.
+// Many tokens (tile_kernel): bound by the matrix cores; tiles of both operands are staged in LDS
+// by direct loads, two deep, 16-byte pieces in an order that keeps the reads off each other's
+// banks (no conflicts counted).  8,192 x 4,096 x 4,096: 140 us in a run of calls (1.96 POP/s; the
+// matrix cores are busy in 49 % of the cycles), a large library product of this type 2.1 POP/s.
 #include "lane_types.h"
 
 #include <type_traits>
@@ -24,8 +27,10 @@ using i32x16 = __attribute__((__vector_size__(16 * sizeof(int)))) int;
 constexpr int kStep = 128;    // bytes of k in one step of the kernels
 
 // ------------------------------------------------------------------ tokens to 8 bits
+// Bound by bytes: 8,192 x 4,096 bfloat16 24 us (4.2 TB/s).
 // A row to a workgroup; V vectors of 8 values of it to a lane's registers (the rest, if any, is
-// read again for the second pass).
+// read again for the second pass).  V is 1 for rows of up to 2,048 values and 4 above: us by 1 / 4
+// at 8,192 rows of 2,048 12.7 / 18.5, of 4,096 22.2 / 24.0, of 8,192 42.5 / 36.5.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void quant_kernel(const T* x, int64_t stride, int k, int ld,
                                                     int8_t* x8, float* scale) {
@@ -343,14 +348,28 @@ void launch_tile(const int8_t* x8, int ld, const int8_t* w8, int k, const Out& o
     tile_kernel<BM, BN, WM, WN, false><<<grid, 64 * WM * WN, 0, st>>>(x8, ld, w8, k, o, tm, tn);
 }
 
+// Skinny while one round of workgroups (one a CU) holds the call, with as few tokens each as that
+// allows: a workgroup's time is its share of k, which more tokens a workgroup only lengthen.  Past
+// that the weights are read again for every 64 tokens and the tiles' LDS pays, but up to 32 tokens
+// a tile of 64 is mostly empty.  us at tokens x k x channels, skinny by 16 / 32 / 64 tokens, tile:
+//   64 x 1,000 x 300    7.4 /  8.0 / 10.0, 12.9      512 x 1,000 x 300   - / - / 10.8, 13.8
+//   32 x 4,096 x 4,096 13.8 / 13.2 / 15.3, 20.2      128 x 4,096 x 4,096 - / - / 25.0, 21.0
+//   64 x 4,096 x 4,096 21.0 / 17.6 / 18.9, 20.5       64 x 2,048 x 8,192 19.3 / 15.8 / 14.1, 12.7
+// Tiles are as large as still give every CU one.  us by 64 / 128 / 256 at 4,096 x 4,096:
+//   512 tokens 26.0 / 33.7 / -, 1,024 37.5 / 36.6 / 65.4, 2,048 68.0 / 57.4 / 70.3,
+//   4,096 123.6 / 100.6 / 83.8, 8,192 236.8 / 192.5 / 159.4
 void product(const int8_t* x8, int ld, const int8_t* w8, int k, const Out& o, hipStream_t st) {
-  const unsigned tn = (o.n + 15) / 16;
-  if (o.m <= 16) skinny_kernel<1><<<dim3(tn, 1), 256, 0, st>>>(x8, ld, w8, k, o);
-  else if (o.m <= 32) skinny_kernel<2><<<dim3(tn, 1), 256, 0, st>>>(x8, ld, w8, k, o);
-  else if (o.m <= 128) skinny_kernel<4><<<dim3(tn, (o.m + 63) / 64), 256, 0, st>>>(x8, ld, w8, k, o);
-  else if ((int64_t)((o.m + 255) / 256) * ((o.n + 255) / 256) >= bs_num_cus())
+  const int64_t tn = (o.n + 15) / 16, tm = (o.m + 15) / 16, cus = bs_num_cus();
+  const auto grid = [&](int mt) { return dim3((unsigned)tn, (unsigned)((tm + mt - 1) / mt)); };
+  if (tm == 1 || tn * tm <= cus)
+    skinny_kernel<1><<<grid(1), 256, 0, st>>>(x8, ld, w8, k, o);
+  else if (tm == 2 || tn * ((tm + 1) / 2) <= cus)
+    skinny_kernel<2><<<grid(2), 256, 0, st>>>(x8, ld, w8, k, o);
+  else if (tn * ((tm + 3) / 4) <= cus)
+    skinny_kernel<4><<<grid(4), 256, 0, st>>>(x8, ld, w8, k, o);
+  else if ((int64_t)((o.m + 255) / 256) * ((o.n + 255) / 256) >= cus)
     launch_tile<256, 256, 2, 4>(x8, ld, w8, k, o, st);
-  else if ((int64_t)((o.m + 127) / 128) * ((o.n + 127) / 128) >= bs_num_cus())
+  else if ((int64_t)((o.m + 127) / 128) * ((o.n + 127) / 128) >= cus)
     launch_tile<128, 128, 2, 2>(x8, ld, w8, k, o, st);
   else
     launch_tile<64, 64, 2, 2>(x8, ld, w8, k, o, st);

@@ -68,6 +68,17 @@ def test_product(size, dtype):
     assert torch.equal(y, ops.int8_linear(x, w8, ws))
 
 
+# tokens around the counts where another form of the product takes over, few and many channels
+@pytest.mark.parametrize('size', [(32, 200, 300), (33, 200, 2100), (64, 1000, 300), (65, 64, 1000),
+                                  (96, 272, 4100), (129, 130, 520), (257, 384, 300),
+                                  (500, 1000, 260), (1000, 128, 17), (4100, 33, 5)])
+def test_product_between_forms(size):
+    m, k, n = size
+    x, w8, ws, bias = _operands(m, k, n, torch.bfloat16, seed=m)
+    x8, a = ops.int8_quantize(x)
+    _close(ops.int8_linear(x, w8, ws, bias=bias), x8, a, w8, ws, bias)
+
+
 def test_against_the_definition():
     x, w8, ws, bias = _operands(90, 500, 210, seed=4)
     y = ops.int8_linear(x, w8, ws, bias=bias)
