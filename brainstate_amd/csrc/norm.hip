@@ -11,6 +11,9 @@
 // Workgroups stay for many rows: a lane's columns are the same in each, so the weights are read
 // once and the weights' gradients are summed in registers, then over the workgroups in their
 // order (grad_sum_kernel): the same bits every time.
+// bfloat16 with every part, beside a large copy's 5.1 TB/s: 8,192 x 4,096 forward 67 us (5.0 TB/s),
+// gradients 129 us (4.2 TB/s; 201 with a row's loads only after the row before); 4,099 x 2,050
+// 26 and 75 us.  Past 8,192 values the gradients' lanes hold more than their registers and spill.
 #include "lane_types.h"
 
 #include <type_traits>
@@ -267,9 +270,12 @@ __global__ __launch_bounds__(BLOCK) void norm_grad_kernel(bs_norm_in in, NormGra
       if (o.gn) gnv[v].load((const T*)o.gn + r * dim, k[v], dim);
     }
   };
+  // the next row is loaded while this one's sums are formed, where registers are left for it
+  constexpr bool kAhead = NV == 1;
+  if (kAhead) load(row);
   for (int64_t turn_of = 0; turn_of < turns; ++turn_of, row += stride) {
     const bool live = row < in.rows;
-    load(row);
+    if (!kAhead) load(row);
     float x[NV][kVec], z[NV][kVec], s[NV][kVec], d[NV][kVec], dn[NV][kVec];
     float sum[1] = {0.f};
 #pragma unroll
@@ -283,6 +289,7 @@ __global__ __launch_bounds__(BLOCK) void norm_grad_kernel(bs_norm_in in, NormGra
 #pragma unroll
       for (int j = 0; j < kVec; ++j) sum[0] = fmaf(k[v].once(j, x[v][j]), x[v][j], sum[0]);
     }
+    if (kAhead) load(row + stride);
     float r1 = 1.f;
     if (in.post) {
       row_sum<TPR, 1>(sum, sh, turn);
@@ -400,7 +407,8 @@ int check(const bs_norm_in* in, const char* who) {
 }
 
 // Lanes to a row: as many as it has runs of 8 values, a power of two up to a wave, whole waves
-// above; two runs a lane past 4,096 values.
+// above; two runs a lane past 4,096 values.  us at 262,144 x 128 by 16 / 64 lanes 62 / 144, at
+// 131,072 x 250 by 32 / 64 63 / 90.
 struct Shape { int lanes, nv; };
 Shape shape_of(int dim) {
   const int runs = (dim + kVec - 1) / kVec;
@@ -408,6 +416,14 @@ Shape shape_of(int dim) {
   if (runs <= 32) return {32, 1};
   const int nv = runs > 512 ? 2 : 1;
   return {(runs + 64 * nv - 1) / (64 * nv) * 64, nv};
+}
+// Forward only: two runs a lane also where one would take 5 or 6 waves, which lie unevenly on a
+// CU's 4 SIMDs (bfloat16, us with one / two: 8,192 x 2,560 48.5 / 44.5, x 3,000 58.8 / 48.0, 4,099 x
+// 2,050 34.0 / 25.5; 4 waves, x 2,048, 32.7 / 35.3; 7 waves, x 3,584, 63.7 / 63.7).  The gradients
+// would leave the registers (4,099 x 2,050 90 / 280).
+Shape forward_shape_of(int dim) {
+  const int runs = (dim + kVec - 1) / kVec;
+  return runs > 256 && runs <= 384 ? Shape{192, 2} : shape_of(dim);
 }
 int block_of(const Shape& s) { return s.lanes <= 64 ? 256 : s.lanes; }
 
@@ -418,6 +434,9 @@ int grid_of(const bs_norm_in& in, const Shape& s, int threads) {   // threads: w
   return (int)(need < most ? need : most);
 }
 
+// Threads a CU: a full one forward (512 / 1,024 / 2,048 / 4,096 at 8,192 x 4,096: 69.7 / 67.0 / 65.8 /
+// 68.2 us); fewer for gradients, whose workgroups each leave three rows of sums (512 / 1,024 / 2,048
+// at 8,192 x 2,048, loads not yet ahead: 96 / 113 / 134 us).
 constexpr int kThreads = 2048, kGradThreads = 512;
 
 template <int V>
@@ -441,7 +460,7 @@ void by_shape(const Shape& s, int dim, F&& f) {
 
 template <typename T>
 void launch(const bs_norm_in& in, void* stream, void* normed, hipStream_t st) {
-  const Shape s = shape_of(in.dim);
+  const Shape s = forward_shape_of(in.dim);
   const int grid = grid_of(in, s, kThreads);
   by_shape(s, in.dim, [&](auto tpr, auto nv, auto block, auto mode) {
     norm_kernel<T, tpr.value, nv.value, block.value, mode.value>

@@ -76,6 +76,12 @@ def test_forward_and_gradients(size, dtype):
             _near(g, wg[n], 4 * F32 + TOL[g.dtype])
 
 
+# rows of 5 and 6 waves' runs, and so many of them that a workgroup takes several
+@pytest.mark.parametrize('size', [(700, 2049), (1100, 2568), (600, 3070), (5, 3080), (1300, 640)])
+def test_many_rows_forward_and_gradients(size):
+    test_forward_and_gradients(size, torch.bfloat16)
+
+
 @pytest.mark.parametrize('w_dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('parts', FORMS)
 def test_parts_left_out(parts, w_dtype):
