@@ -20,6 +20,12 @@
 //
 // since dL = -(1 + L)^-T (dU R^T) (1 + L)^-T = -dR U^T needs no product with the inverse beyond dR.
 // dg is a difference of large sums, so everything that reaches it is in 32 bits.
+//
+// 4 x 2,048 tokens x 16 heads of 128 x 128 in bfloat16: prepare again 58 us (kept from the forward
+// pass it would hold 142 MB more a layer), grad_chain_kernel 157, grad_chunk_kernel 296.  The last
+// is bound by issue: products in three parts and their cutting keep the matrix cores busy in 15 %
+// and the vector units in 26 % of the cycles, with two waves a SIMD to issue from; its 530 MB alone
+// would take 105 us.
 #include "delta_chunk.h"
 
 namespace {

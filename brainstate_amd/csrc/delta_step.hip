@@ -7,7 +7,9 @@
 // written for 8 dk dv operations: bound by HBM), is read once and written once whatever the
 // number of tokens.  A workgroup keeps a slice of 32 columns of one head's state in registers:
 // 8 lanes x 4 columns side by side make 128-byte pieces of a row, 32 rows a pass.  One token of
-// one sequence with 32 heads of 128 x 128 then has 128 workgroups.
+// one sequence with 32 heads of 128 x 128 then has 128 workgroups: 5.8 us, most of it the latency
+// of one read, one sum over the rows and one write.  224 live rows of 256 with such heads: 222 us,
+// 4.3 TB/s beside a large copy's 5.1.
 #include "delta.h"
 
 namespace {
