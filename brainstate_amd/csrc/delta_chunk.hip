@@ -19,7 +19,7 @@
 // One prompt of 8,192 tokens x 32 heads of 128 x 128 in bfloat16: prepare 104 us, of which the 227 MB
 // it writes for chain_kernel are 45 at a large copy's rate; chain 283 us, 2.2 us a chunk: bound by
 // the latency of its three dependent products and barriers (the matrix cores are busy in 16 % of
-// the cycles, 214 MB move).
+// the cycles, 370 MB move).
 #include "delta_chunk.h"
 
 namespace {

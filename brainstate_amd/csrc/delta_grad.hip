@@ -21,11 +21,12 @@
 // since dL = -(1 + L)^-T (dU R^T) (1 + L)^-T = -dR U^T needs no product with the inverse beyond dR.
 // dg is a difference of large sums, so everything that reaches it is in 32 bits.
 //
-// 4 x 2,048 tokens x 16 heads of 128 x 128 in bfloat16: prepare again 58 us (kept from the forward
-// pass it would hold 142 MB more a layer), grad_chain_kernel 157, grad_chunk_kernel 296.  The last
-// is bound by issue: products in three parts and their cutting keep the matrix cores busy in 15 %
-// and the vector units in 26 % of the cycles, with two waves a SIMD to issue from; its 530 MB alone
-// would take 105 us.
+// 4 x 2,048 tokens x 16 heads of 128 x 128 in bfloat16, the whole step 652 us: the forward pass 187
+// (it keeps the states), prepare again 58 us (kept from the forward pass it would hold 142 MB more
+// a layer), grad_chain_kernel 157, grad_chunk_kernel about 260.  The last is bound by its
+// registers: products in three parts and their cutting fill all 256 and spill (184 bytes a lane;
+// 220 and 296 us with U's parts cut by every wave that takes them), two waves a SIMD keep the
+// matrix cores busy in 15 % of the cycles, and its bytes alone would take 105 us.
 #include "delta_chunk.h"
 
 namespace {
@@ -342,6 +343,7 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
   __shared__ __attribute__((aligned(16))) float lm[kChunk][kChunk + 4];
   __shared__ float rows[2][kChunk], betas[2][kChunk], tot[8];
   __shared__ __attribute__((aligned(16))) uint4 lst[2][2][2 * KS][3][64];    // states' parts
+  __shared__ __attribute__((aligned(16))) uint4 lut[2][4][3][64];            // U's
   const int slot = blockIdx.x, hk = blockIdx.y, group = in.hv / in.hk;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), t = wave & 3, half = wave >> 2;
@@ -404,9 +406,10 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
     for (int i = 0; i < CT; ++i) xq[i] = xs[i] = xr[i] = zero4();
 #pragma unroll
     for (int j = 0; j < 2; ++j) da[j] = dl[j] = zero4();
-    // Steps of 32 value columns.  The states' parts are cut once for all waves: wave w loads tile
-    // w of both, a step ahead, and leaves them in LDS, two steps deep.
-    float4 sw[4], rw[2], uw[2], jw[2][2];
+    // Steps of 32 value columns.  The parts of the states and of U are cut once for all waves: wave
+    // w loads tile w of both states, the first four tile w of U, a step ahead, and leaves them in
+    // LDS, two steps deep.
+    float4 sw[4], rw[2], uw[2];
     uint4 gw[sizeof(T) / 2], vw[sizeof(T) / 2];
     auto load_step = [&](int e) {
       gr.raw(e + 8 * g, gw);
@@ -419,14 +422,8 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
       rw[0] = *(const float4*)p, rw[1] = *(const float4*)(p + 256);
       p = delta_kept_frag(us, t, e >> 5, lane, dvp);
       uw[0] = *(const float4*)p, uw[1] = *(const float4*)(p + 256);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        p = delta_kept_frag(us, j0 + min(j, nj - 1), e >> 5, lane, dvp);
-        jw[j][0] = *(const float4*)p, jw[j][1] = *(const float4*)(p + 256);
-      }
     };
-    load_step(0);
-    for (int e = 0; e < dvp; e += 32) {
+    auto step = [&](int e, auto more) {
       const int buf = (e >> 5) & 1;
       if (wave < 2 * KS) {
         const bs_parts<3> a = row_parts(sw[0], sw[1]), b = row_parts(sw[2], sw[3]);
@@ -440,7 +437,12 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
         for (int i = 0; i < 8; ++i) dot_s = fmaf(x[i], x[8 + i], dot_s);
       }
       const bs_parts<PI> of = gr.template parts<PI>(gw);
-      const bs_parts<3> rf = row_parts(rw[0], rw[1]), uf = row_parts(uw[0], uw[1]);
+      const bs_parts<3> rf = row_parts(rw[0], rw[1]);
+      if (half == 0) {
+        const bs_parts<3> u = row_parts(uw[0], uw[1]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *(bs_bf16x8*)&lut[buf][t][p][lane] = u.p[p];
+      }
       if (buf == half) {
         const float* x = (const float*)rw;
         float f[8];
@@ -448,15 +450,20 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
 #pragma unroll
         for (int j = 0; j < 8; ++j) dot_v = fmaf(x[j], f[j], dot_v);
       }
+      if (more.value) load_step(e + 32);
+      __syncthreads();                // the parts of this step
+      bs_parts<3> uf;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) uf.p[p] = *(const bs_bf16x8*)&lut[buf][t][p][lane];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         if (j < nj) {
-          const bs_parts<3> a = row_parts(jw[j][0], jw[j][1]);
+          bs_parts<3> a;
+#pragma unroll
+          for (int p = 0; p < 3; ++p) a.p[p] = *(const bs_bf16x8*)&lut[buf][j0 + j][p][lane];
           da[j] = bs_mma<2>(a, of, da[j]);
           dl[j] = bs_mma<2>(a, rf, dl[j]);
         }
-      load_step(min(e + 32, dvp - 32));
-      __syncthreads();                // the parts of this step
 #pragma unroll
       for (int i = 0; i < CT; ++i) {
         bs_parts<3> sf, df;
@@ -469,7 +476,10 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
         xr[i] = bs_mma<2>(sf, rf, xr[i]);
         xs[i] = bs_mma<2>(df, uf, xs[i]);
       }
-    }
+    };
+    load_step(0);
+    for (int e = 0; e + 32 < dvp; e += 32) step(e, std::true_type());
+    step(dvp - 32, std::false_type());
     // the masked products of this wave, to LDS by rows
     const float grow = co[kGrow * kChunk + tok], beta = co[kBeta * kChunk + tok];
     const double run_i = run[tok];
