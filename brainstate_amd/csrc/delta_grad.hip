@@ -21,12 +21,13 @@
 // since dL = -(1 + L)^-T (dU R^T) (1 + L)^-T = -dR U^T needs no product with the inverse beyond dR.
 // dg is a difference of large sums, so everything that reaches it is in 32 bits.
 //
-// 4 x 2,048 tokens x 16 heads of 128 x 128 in bfloat16, the whole step 652 us: the forward pass 187
+// 4 x 2,048 tokens x 16 heads of 128 x 128 in bfloat16, the whole step 613 us: the forward pass 187
 // (it keeps the states), prepare again 58 us (kept from the forward pass it would hold 142 MB more
-// a layer), grad_chain_kernel 157, grad_chunk_kernel about 260.  The last is bound by its
-// registers: products in three parts and their cutting fill all 256 and spill (184 bytes a lane;
-// 220 and 296 us with U's parts cut by every wave that takes them), two waves a SIMD keep the
-// matrix cores busy in 15 % of the cycles, and its bytes alone would take 105 us.
+// a layer), grad_chain_kernel 158, grad_chunk_kernel the rest.  The last fills its 256 registers with
+// products in three parts and their cutting: whole step 687 us with U's parts cut by every wave that
+// takes them, 652 with the fragments' addresses kept over the heads (184 bytes a lane spilled, 100
+// MB written and read).  Two waves a SIMD to issue from keep the matrix cores busy in a sixth of
+// the cycles.
 #include "delta_chunk.h"
 
 namespace {
@@ -389,6 +390,9 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
       }
   }
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
+    // the key head's fragments are addressed anew for each head: kept, the addresses spill
+    int64_t kbh = kb;
+    asm volatile("" : "+s"(kbh));
     const int64_t sh = (int64_t)slot * in.hv + h;
     const float* co = w.coef + sh * kCoef;
     const double* run = (const double*)(co + kRun * kChunk);
@@ -506,7 +510,7 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
     bs_parts<PI> kf[HS], qf[HS];
 #pragma unroll
     for (int s = 0; s < HS; ++s) {
-      const int64_t at = kb + lane * 8 + (t * KS + half * HS + s) * kFrag;
+      const int64_t at = kbh + lane * 8 + (t * KS + half * HS + s) * kFrag;
       kf[s] = delta_frags<PI>(w.kp + at, kChunk * DK);
       qf[s] = delta_frags<PI>(w.qp + at, kChunk * DK);
     }
@@ -529,7 +533,7 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
           const bs_parts<PI> a = delta_frags<PI>(
-              w.kt + kb + lane * 8 + ((half * CT + i) * 2 + st) * kFrag, kChunk * DK);
+              w.kt + kbh + lane * 8 + ((half * CT + i) * 2 + st) * kFrag, kChunk * DK);
           xq[i] = bs_mma<2>(a, pf, xq[i]);
           xr[i] = bs_mma<2>(a, mf, xr[i]);
         }
@@ -541,7 +545,7 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
         const bs_parts<3> pf = bs_split8<3>(p), mf = bs_split8<3>(q);
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
-          const int64_t at = kb + lane * 8 + ((half * CT + i) * 2 + st) * kFrag;
+          const int64_t at = kbh + lane * 8 + ((half * CT + i) * 2 + st) * kFrag;
           xs[i] = bs_mma<2>(delta_frags<PI>(w.qt + at, kChunk * DK), pf, xs[i]);
           xs[i] = bs_mma<2>(delta_frags<PI>(w.kt + at, kChunk * DK), mf, xs[i]);
         }
