@@ -23,7 +23,7 @@
 //
 // 4 x 2,048 tokens x 16 heads of 128 x 128 in bfloat16, the whole step 613 us: the forward pass 187
 // (it keeps the states), prepare again 58 us (kept from the forward pass it would hold 142 MB more
-// a layer), grad_chain_kernel 158, grad_chunk_kernel the rest.  The last fills its 256 registers with
+// a layer), grad_chain_kernel 160, grad_chunk_kernel 232.  The last fills its 256 registers with
 // products in three parts and their cutting: whole step 687 us with U's parts cut by every wave that
 // takes them, 652 with the fragments' addresses kept over the heads (184 bytes a lane spilled, 100
 // MB written and read).  Two waves a SIMD to issue from keep the matrix cores busy in a sixth of
