@@ -42,7 +42,8 @@ __device__ __forceinline__ DeltaSpan delta_span(const DeltaPlan& p, int n) {
   return s;
 }
 
-// The sequence that owns a slot: the last one whose first slot is not past it.
+// The sequence that owns a slot: the last one whose first slot is not past it, or the first one
+// where every first slot is (no sequence's chunk lies there then).
 __device__ __forceinline__ int delta_owner(const DeltaPlan& p, int slot) {
   if (!p.offsets) return slot / ((p.tokens + kChunk - 1) / kChunk);
   int lo = 0, hi = p.seqs - 1;

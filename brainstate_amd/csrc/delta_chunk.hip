@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
   const int group = in.hv / in.hk, hk = h / group;
   const DeltaSpan sp = delta_span(plan, delta_owner(plan, slot));
   const int c = slot - sp.slot;
-  if (c >= sp.chunks) return;
+  if (c < 0 || c >= sp.chunks) return;      // c < 0: ahead of the first sequence
   const int64_t t0 = sp.first + (int64_t)c * kChunk;
   const int len = min(sp.len - c * kChunk, kChunk);
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;

@@ -362,7 +362,7 @@ __global__ __launch_bounds__(512) void grad_chunk_kernel(bs_delta_in in, DeltaPl
   }
   const DeltaSpan sp = delta_span(plan, delta_owner(plan, slot));
   const int c = slot - sp.slot;
-  if (c >= sp.chunks) return;
+  if (c < 0 || c >= sp.chunks) return;
   const int64_t t0 = sp.first + (int64_t)c * kChunk;
   const int len = min(sp.len - c * kChunk, kChunk);
   const int64_t kb = ((int64_t)slot * in.hk + hk) * PI * kChunk * DK;
