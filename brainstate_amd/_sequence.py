@@ -151,7 +151,7 @@ def _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, keep):
     final = torch.empty((n, hv, dk, dv), dtype=torch.float32, device=dev)
     kept = (None, None)
     if keep:
-        slots = t // _CHUNK + n if seq_offsets is not None else n * -(-t // _CHUNK)
+        slots = n * -(-t // _CHUNK) if seq_offsets is None else t // _CHUNK + n if n else 0
         dvp = -(-dv // 32) * 32
         kept = (torch.empty((slots, hv, 64 if dk <= 64 else 128, dvp), dtype=torch.float32,
                             device=dev),

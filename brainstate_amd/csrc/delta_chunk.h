@@ -133,7 +133,8 @@ static inline DeltaWork delta_work(void* ws, const DeltaSizes& s, int backward) 
 static inline DeltaPlan delta_plan(int seqs, int tokens, const int32_t* offsets) {
   DeltaPlan p;
   p.seqs = seqs, p.tokens = tokens, p.offsets = offsets;
-  p.slots = offsets ? tokens / kChunk + seqs : seqs * ((tokens + kChunk - 1) / kChunk);
+  p.slots = !seqs ? 0 : offsets ? tokens / kChunk + seqs
+                                : seqs * ((tokens + kChunk - 1) / kChunk);
   return p;
 }
 

@@ -666,7 +666,8 @@ extern "C" int bs_gated_delta_rule_grad(const bs_delta_in* in, int32_t seqs, int
   const DeltaPlan plan = delta_plan(seqs, tokens, seq_offsets);
   const DeltaSizes z = delta_sizes(*in, plan.slots, 1);
   BS_CHECK_ARG(tokens == 0 || (in->q && in->k && in->v && in->g && in->beta && grad_o &&
-                               kept_states && kept_u && dq && dk && dv && dg && dbeta),
+                               (plan.slots == 0 || (kept_states && kept_u)) && dq && dk && dv &&
+                               dg && dbeta),
                "bs_gated_delta_rule_grad: NULL pointer");
   BS_CHECK_ARG(z.bytes == 0 || (workspace && workspace_bytes >= (size_t)z.bytes),
                "bs_gated_delta_rule_grad: workspace of %lld bytes needed, %lld given",

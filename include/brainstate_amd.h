@@ -566,8 +566,8 @@ BS_API int bs_gated_delta_step(const bs_delta_in* in, int32_t batch, int32_t tok
  * `tokens` tokens (batch strides unused); rows outside all of them give 0.  States are
  * [seqs, hv, dk, dv], NULL where not given or not wanted.  kept_states [slots, hv, dkp, dvp] and
  * kept_u [slots, hv, 64, dvp] (both or neither) are written for the backward pass, with
- * slots = seqs ceil(tokens / 64), or tokens / 64 + seqs when packed, dkp = 64 or 128 and
- * dvp = dv rounded up to 32. */
+ * slots = seqs ceil(tokens / 64), or tokens / 64 + seqs when packed (0 without a sequence, where
+ * they may be NULL), dkp = 64 or 128 and dvp = dv rounded up to 32. */
 BS_API size_t bs_gated_delta_workspace_size(const bs_delta_in* in, int32_t seqs, int32_t tokens,
                                             int32_t packed);
 BS_API int bs_gated_delta_rule(const bs_delta_in* in, int32_t seqs, int32_t tokens,

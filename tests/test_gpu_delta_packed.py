@@ -60,3 +60,18 @@ def test_late_first_sequences(cuts, dtype):
         _near(got, w, 8 * F32 + UNIT[got.dtype])
     for got in (o, *grads[:5]):
         assert (got[:, :cuts[0]] == 0).all() and (got[:, cuts[-1]:] == 0).all()
+
+
+@pytest.mark.parametrize('tokens', [0, 10, 100])
+def test_no_sequence_at_all(tokens):
+    """Offsets of one entry: every token is outside."""
+    x, do = _operands(tokens, torch.float32, seed=1)
+    s0 = torch.zeros(0, H, DK, DV, device='cuda')
+    offsets = torch.tensor([min(tokens, 3)], dtype=torch.int32).cuda()
+    o, s1 = ops.gated_delta_rule(*x, seq_offsets=offsets)
+    assert o.shape == (1, tokens, H, DV) and (o == 0).all() and s1.shape == (0, H, DK, DV)
+    leaves = [y.requires_grad_() for y in (*x, s0)]
+    o, s1 = ops.gated_delta_rule(*x, initial_state=s0, seq_offsets=offsets)
+    assert (o == 0).all()
+    for got, y in zip(torch.autograd.grad((o, s1), leaves, (do, s1.detach())), leaves):
+        assert got.shape == y.shape and (got == 0).all()
