@@ -569,6 +569,8 @@ extern "C" int bs_gated_delta_rule(const bs_delta_in* in, int32_t seqs, int32_t 
   const DeltaSizes z = delta_sizes(*in, plan.slots, 0);
   BS_CHECK_ARG(tokens == 0 || (in->q && in->k && in->v && in->g && in->beta && o),
                "bs_gated_delta_rule: NULL pointer");
+  BS_CHECK_ARG(!kept_states == !kept_u,
+               "bs_gated_delta_rule: one of kept_states and kept_u is NULL");
   BS_CHECK_ARG(z.bytes == 0 || (workspace && workspace_bytes >= (size_t)z.bytes),
                "bs_gated_delta_rule: workspace of %lld bytes needed, %lld given",
                (long long)z.bytes, (long long)(workspace ? workspace_bytes : 0));
