@@ -11,7 +11,7 @@ from . import _native as N
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # enum bs_dtype
 _CHUNK = 64
 _DELTA_IN = struct.Struct('5P15q7if')      # bs_delta_in
-_NORM_IN = struct.Struct('6P4q5i2f')       # bs_norm_in
+_NORM_IN = struct.Struct('6P4q5i2f4x')     # bs_norm_in, to its whole 8 bytes
 
 
 def _floating(name, t, dtype=None):

@@ -1,6 +1,7 @@
 """Checks of the sequence-layer entry points that come before any device work (CPU)."""
 import ctypes
 import os
+import struct
 
 import pytest
 
@@ -28,3 +29,30 @@ def test_kept_matrices_are_both_given_or_neither(lib):
     for kept in ((at, None), (None, at)):
         rc = lib.bs_gated_delta_rule(_delta_in(), 1, 64, None, None, at, at, *kept, at, need, None)
         assert rc == N.BS_ERR_INVALID and b'kept_u' in lib.bs_last_error()
+
+
+def test_packed_operands_are_the_compiled_headers_structs(tmp_path):
+    """Sizes, padding included, and where the fields past the pointers lie."""
+    import shutil
+    import subprocess
+    cc = shutil.which('gcc')
+    if cc is None:
+        pytest.skip('no host C compiler')
+    fields = {'bs_delta_in': ['q_stride', 'beta_stride', 'dtype', 'hk', 'dv', 'scale'],
+              'bs_norm_in': ['y_stride', 'rows', 'dim', 'pre_dtype', 'eps', 'scale_value']}
+    src = tmp_path / 'sizes.c'
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "brainstate_amd.h"\n'
+                   'int main(void) {\n' + ''.join(
+                       f'printf("%zu ", sizeof({s}));' + ''.join(
+                           f'printf("%zu ", offsetof({s}, {f}));' for f in fs)
+                       for s, fs in fields.items()) + 'return 0; }\n')
+    exe = tmp_path / 'sizes'
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([cc, '-I', os.path.join(root, 'include'), str(src), '-o', str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True,
+                                          check=True).stdout.split()]
+    delta, norm = struct.calcsize('@5P'), struct.calcsize('@6P')
+    assert got == [_sequence._DELTA_IN.size, delta, delta + 12 * 8, delta + 15 * 8,
+                   delta + 15 * 8 + 12, delta + 15 * 8 + 24, delta + 15 * 8 + 28,
+                   _sequence._NORM_IN.size, norm, norm + 3 * 8, norm + 4 * 8, norm + 4 * 8 + 16,
+                   norm + 4 * 8 + 20, norm + 4 * 8 + 24]
