@@ -543,8 +543,10 @@ int delta_check_chunked(const bs_delta_in* in, int seqs, int tokens, const int32
                  "%s: %lld elements from token to token", who, (long long)st[1]);
   const int64_t slots = offsets ? (int64_t)tokens / kChunk + seqs
                                 : (int64_t)seqs * ((tokens + kChunk - 1) / kChunk);
-  BS_CHECK_ARG(slots <= 0x7FFFFFFF / kChunk && in->hv <= 65535 &&
-                   ((int64_t)seqs + 1) * in->hv <= 0x7FFFFFFF / 64,
+  // launches of 512 threads a slot, or a unit and slice of 32 columns (16 only where those are at
+  // most one a CU), have fewer than 2^32 threads; past that the count wraps without an error
+  BS_CHECK_ARG(slots < (1 << 23) - 1 && in->hv <= 65535 &&
+                   (((int64_t)seqs + 1) * in->hv + 7) * ((in->dv + 31) / 32) < 1 << 23,
                "%s: %d sequences of %d tokens, %d heads exceed one launch", who, seqs, tokens,
                in->hv);
   return BS_OK;

@@ -172,7 +172,8 @@ extern "C" int bs_gated_delta_step(const bs_delta_in* in, int32_t batch, int32_t
   BS_CHECK_ARG(batch >= 0 && tokens >= 0 && n_states >= 0,
                "bs_gated_delta_step: batch %d, tokens %d, states %lld", batch, tokens,
                (long long)n_states);
-  BS_CHECK_ARG((int64_t)batch * in->hv * 4 <= 0x7FFFFFFF,
+  // a launch has fewer than 2^32 threads; past that the count wraps without an error
+  BS_CHECK_ARG((int64_t)batch * in->hv * ((in->dv + kCols - 1) / kCols) < 1 << 24,
                "bs_gated_delta_step: batch %d x %d heads exceeds one launch", batch, in->hv);
   if (batch == 0 || tokens == 0) return BS_OK;
   BS_CHECK_ARG(in->q && in->k && in->v && in->g && in->beta && state && o,

@@ -378,23 +378,36 @@ void product(const int8_t* x8, int ld, const int8_t* w8, int k, const Out& o, hi
 int padded(int k) { return (k + kStep - 1) / kStep * kStep; }
 
 int check(int64_t m, int32_t k, int32_t n, const char* who) {
-  BS_CHECK_ARG(m >= 0 && m <= 0x7FFFFF00 && k >= 1 && k <= 65536 && n >= 0 && n <= 0x7FFFFF00,
+  BS_CHECK_ARG(m >= 0 && m <= 0x7FFFF000 && k >= 1 && k <= 65536 && n >= 0 && n <= 0x0FFFFF00,
                "%s: %lld tokens of %d values (1..65536), %d channels", who, (long long)m, k, n);
-  const int64_t tiles = ((m + 63) / 64) * (((int64_t)n + 63) / 64);
-  BS_CHECK_ARG(tiles < 0x7FFFFF00, "%s: %lld tokens x %d channels exceed one launch", who,
+  // the largest tiles' and the skinny form's workgroups, rounded up, stay below 2^32 threads
+  const int64_t tiles = ((m + 255) / 256) * (((int64_t)n + 255) / 256);
+  BS_CHECK_ARG(tiles < (1 << 23) - 8, "%s: %lld tokens x %d channels exceed one launch", who,
                (long long)m, n);
   return BS_OK;
+}
+
+// A launch has fewer than 2^32 threads (past that the count wraps without an error), so rows that
+// take a workgroup each go in pieces of this many: f(first row, rows).
+constexpr int64_t kRowsAtOnce = 1 << 23;
+template <typename F>
+void row_pieces(int64_t m, F&& f) {
+  for (int64_t r = 0; r < m; r += kRowsAtOnce)
+    f(r, (unsigned)(m - r < kRowsAtOnce ? m - r : kRowsAtOnce));
 }
 
 int quantize(const void* x, int dtype, int64_t m, int k, int64_t stride, int ld, int8_t* x8,
              float* scale, hipStream_t st) {
   auto run = [&](auto* p) {
-    if (ld <= 2048)
-      quant_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, 1>
-          <<<(unsigned)m, 256, 0, st>>>(p, stride, k, ld, x8, scale);
-    else
-      quant_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, 4>
-          <<<(unsigned)m, 256, 0, st>>>(p, stride, k, ld, x8, scale);
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+    row_pieces(m, [&](int64_t r, unsigned rows) {
+      if (ld <= 2048)
+        quant_kernel<T, 1><<<rows, 256, 0, st>>>(p + r * stride, stride, k, ld, x8 + r * ld,
+                                                 scale + r);
+      else
+        quant_kernel<T, 4><<<rows, 256, 0, st>>>(p + r * stride, stride, k, ld, x8 + r * ld,
+                                                 scale + r);
+    });
   };
   if (dtype == BS_F32) run((const float*)x);
   else if (dtype == BS_BF16) run((const bs_bf16*)x);
@@ -437,7 +450,9 @@ extern "C" int bs_int8_linear(const void* x, int32_t x_dtype, int64_t stride, co
   int8_t* x8 = (int8_t*)workspace;
   float* a = (float*)(x8 + (size_t)m * ld);
   if (x_scale) {
-    pad_kernel<<<(unsigned)m, 256, 0, st>>>((const int8_t*)x, k, ld, x8);
+    row_pieces(m, [&](int64_t r, unsigned rows) {
+      pad_kernel<<<rows, 256, 0, st>>>((const int8_t*)x + r * k, k, ld, x8 + r * ld);
+    });
     BS_CHECK_LAUNCH();
   } else if (int rc = quantize(x, x_dtype, m, k, stride, ld, x8, a, st)) {
     return rc;

@@ -56,3 +56,24 @@ def test_packed_operands_are_the_compiled_headers_structs(tmp_path):
                    delta + 15 * 8 + 12, delta + 15 * 8 + 24, delta + 15 * 8 + 28,
                    _sequence._NORM_IN.size, norm, norm + 3 * 8, norm + 4 * 8, norm + 4 * 8 + 16,
                    norm + 4 * 8 + 20, norm + 4 * 8 + 24]
+
+
+def test_launches_of_too_many_threads_are_refused(lib):
+    """A grid of 2^32 threads or more wraps: what would need one is an invalid argument."""
+    at = ctypes.c_void_p(4096)
+
+    def refused(rc):
+        return rc == N.BS_ERR_INVALID and b'exceed' in lib.bs_last_error()
+
+    one = _delta_in(hv=1, dv=128)              # 4 workgroups of 256 a row
+    assert refused(lib.bs_gated_delta_step(one, 1 << 22, 1, at, 1 << 22, None, at, None))
+    assert lib.bs_gated_delta_workspace_size(one, 1 << 21, 1, 0) == 0
+    assert refused(lib.bs_gated_delta_rule(one, 1 << 21, 1, None, None, at, at, None, None, at,
+                                           1 << 62, None))
+    assert lib.bs_gated_delta_workspace_size(one, (1 << 21) - 16, 1, 0) > 0
+    assert lib.bs_gated_delta_grad_workspace_size(_delta_in(), 1, 1 << 29, 0) == 0
+    assert lib.bs_gated_delta_grad_workspace_size(_delta_in(), 1, (1 << 29) - 128, 0) > 0
+    linear = (at, F32, 8, None, 1 << 30, 8, 1 << 20, at, at, None, F32, at, F32, at, 1 << 62, None)
+    assert refused(lib.bs_int8_linear(*linear))
+    assert lib.bs_int8_linear(at, F32, 8, None, 1, 8, 1 << 28, at, at, None, F32, at, F32, at,
+                              1 << 62, None) == N.BS_ERR_INVALID
