@@ -70,7 +70,10 @@ def _delta_operands(q, k, v, g, beta, scale):
 def _heads(x):
     """``x`` with a head's values side by side; any other strides are taken as they are."""
     at = x.stride()
-    return x if (at[3] == 1 or x.shape[3] == 1) and at[1] < 1 << 23 else x.contiguous()
+    if (at[3] == 1 or x.shape[3] == 1) and at[1] < 1 << 23:
+        return x
+    # of one token the stride does not count, and contiguous() alone would leave it
+    return x.squeeze(1).contiguous().unsqueeze(1) if x.shape[1] == 1 else x.contiguous()
 
 
 def _delta_pack(q, k, v, g, beta, scale, qt, gt, bt):
