@@ -5,6 +5,7 @@ in brainstate; :mod:`brainstate_amd.ops` exports them.
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -37,8 +38,39 @@ def _wants_grad(*ts):
     return False
 
 
+def _tangent(*ts):
+    """Whether one of the operands carries a forward-mode tangent or is wrapped by a torch.func
+    transform: there is no rule for either here, and the kernels would drop it."""
+    active = getattr(torch._C, '_are_functorch_transforms_active', None)
+    inside = active is None or active()
+    if not inside and getattr(forward_ad, '_current_level', 0) < 0:
+        return False
+    for t in ts:
+        if isinstance(t, torch.Tensor):
+            if inside and torch._C._functorch.is_functorch_wrapped_tensor(t):
+                return True
+            if forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return False
+
+
+def _recorded(who, *ts):
+    """Whether autograd records a call on the tensors ``ts``."""
+    if _tangent(*ts):
+        raise NotImplementedError(f'{who} has neither a forward-mode derivative nor a rule for '
+                                  f'torch.func transforms: use torch.autograd')
+    return _wants_grad(*ts)
+
+
 def _address(t):
-    return None if t is None else t.data_ptr()
+    if t is None:
+        return None
+    try:
+        return t.data_ptr()
+    except RuntimeError:        # a new tensor inside a torch.func transform, or a batched gradient
+        if not torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise NotImplementedError('no rule for batched gradients: take them one by one')
+        return N.ptr(t).value
 
 
 # ------------------------------------------------------------------------- gated delta rule
@@ -80,7 +112,7 @@ def _delta_pack(q, k, v, g, beta, scale, qt, gt, bt):
     q, k, v = _heads(q), _heads(k), _heads(v)
     dk = q.shape[3]
     packed = _DELTA_IN.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+        _address(q), _address(k), _address(v), _address(g), _address(beta),
         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride(),
         qt, gt, bt, q.shape[2], v.shape[2], dk, v.shape[3],
         dk ** -0.5 if scale is None else float(scale))
@@ -108,7 +140,7 @@ def gated_delta_step(q, k, v, g, beta, state, slots=None, scale=None):
     order.  ``state`` [n, heads, dk, dv] float32, contiguous.  ``slots`` [batch] int32 names each
     row's state; a negative one (or one from n on) marks an idle row, whose output is 0.  Without
     it row b has state b.  Not differentiable."""
-    if _wants_grad(q, k, v, g, beta, state):
+    if _wants_grad(q, k, v, g, beta, state) or _tangent(q, k, v, g, beta, state, slots):
         raise ValueError('gated_delta_step updates its state in place and has no gradient: use '
                          'gated_delta_rule, or torch.no_grad()')
     one = isinstance(q, torch.Tensor) and q.dim() == 3
@@ -128,8 +160,8 @@ def gated_delta_step(q, k, v, g, beta, state, slots=None, scale=None):
     else:
         slots = slots.contiguous()
     o = torch.empty((b, t, hv, dv), dtype=q.dtype, device=q.device)
-    N.check(N.lib().bs_gated_delta_step(packed, b, t, state.data_ptr(), state.shape[0],
-                                        _address(slots), o.data_ptr(), N.raw_stream(q.device)),
+    N.check(N.lib().bs_gated_delta_step(packed, b, t, _address(state), state.shape[0],
+                                        _address(slots), _address(o), N.raw_stream(q.device)),
             'bs_gated_delta_step')
     return o.squeeze(1) if one else o
 
@@ -163,8 +195,8 @@ def _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, keep):
     nbytes = lib.bs_gated_delta_workspace_size(packed, n, t, seq_offsets is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     N.check(lib.bs_gated_delta_rule(
-        packed, n, t, _address(seq_offsets), _address(initial_state), final.data_ptr(), o.data_ptr(),
-        _address(kept[0]), _address(kept[1]), ws.data_ptr(), nbytes, N.raw_stream(dev)),
+        packed, n, t, _address(seq_offsets), _address(initial_state), _address(final), _address(o),
+        _address(kept[0]), _address(kept[1]), _address(ws), nbytes, N.raw_stream(dev)),
         'bs_gated_delta_rule')
     return o, final, kept
 
@@ -184,6 +216,7 @@ class _DeltaRule(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, go, gstate):
+        _recorded('gated_delta_rule', go, gstate)
         *x, seq_offsets, kept_s, kept_u = ctx.saved_tensors
         held, packed = _delta_pack(*x, ctx.scale, *(_DTYPES[x[i].dtype] for i in (0, 3, 4)))
         (b, t, hk, dk), (hv, dv) = x[0].shape, x[2].shape[2:]
@@ -201,8 +234,8 @@ class _DeltaRule(torch.autograd.Function):
         nbytes = lib.bs_gated_delta_grad_workspace_size(packed, n, t, seq_offsets is not None)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         N.check(lib.bs_gated_delta_rule_grad(
-            packed, n, t, _address(seq_offsets), go.data_ptr(), _address(gstate), kept_s.data_ptr(),
-            kept_u.data_ptr(), *(y.data_ptr() for y in grads), _address(ds), ws.data_ptr(), nbytes,
+            packed, n, t, _address(seq_offsets), _address(go), _address(gstate), _address(kept_s),
+            _address(kept_u), *(_address(y) for y in grads), _address(ds), _address(ws), nbytes,
             N.raw_stream(dev)), 'bs_gated_delta_rule_grad')
         return (*grads, ds, None, None)
 
@@ -216,7 +249,7 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, seq_offse
     ``seq_offsets`` (int32 [sequences + 1], ascending) the sequences are packed end to end into
     one batch row; tokens outside all of them give 0.  Differentiable in everything but
     ``seq_offsets``."""
-    if _wants_grad(q, k, v, g, beta, initial_state):
+    if _recorded('gated_delta_rule', q, k, v, g, beta, initial_state, seq_offsets):
         return _DeltaRule.apply(q, k, v, g, beta, initial_state, scale, seq_offsets)
     o, final, _ = _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, False)
     return o, final
@@ -260,8 +293,8 @@ def _norm_pack(y, post, gate, scale, residual, pre, eps):
         scale, value = None, scale
     acts = [t if t is None else _rows(t, dim) for t in (y, gate, residual)]
     weights = [t if t is None else t.contiguous() for t in (post, scale, pre)]
-    y_at, gate_at, residual_at = [0 if t is None else t.data_ptr() for t in acts]
-    post_at, scale_at, pre_at = [0 if t is None else t.data_ptr() for t in weights]
+    y_at, gate_at, residual_at = [_address(t) or 0 for t in acts]
+    post_at, scale_at, pre_at = [_address(t) or 0 for t in weights]
     rows = acts[0].shape[0]
     packed = _NORM_IN.pack(
         y_at, post_at, gate_at, scale_at, residual_at, pre_at,
@@ -274,7 +307,7 @@ def _norm_forward(y, post, gate, scale, residual, pre, eps):
     held, packed, _, _ = _norm_operands(y, post, gate, scale, residual, pre, eps)
     stream = torch.empty(y.shape, dtype=y.dtype, device=y.device)
     normed = torch.empty_like(stream) if pre is not None else None
-    N.check(N.lib().bs_norm_gate_residual(packed, stream.data_ptr(), _address(normed),
+    N.check(N.lib().bs_norm_gate_residual(packed, _address(stream), _address(normed),
                                           N.raw_stream(y.device)), 'bs_norm_gate_residual')
     return stream, normed
 
@@ -293,6 +326,7 @@ class _NormGateResidual(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gs, gn):
+        _recorded('norm_gate_residual', gs, gn)
         y, post, gate, scale, residual, pre = x = ctx.saved_tensors
         held, packed, rows, dim = _norm_pack(
             y, post, gate, scale if ctx.value is None else ctx.value, residual, pre, ctx.eps)
@@ -323,16 +357,16 @@ def norm_gate_residual(y, post_weight=None, gate=None, scale=None, residual=None
     ``pre_weight`` are [dim] of any floating type, ``scale`` may be a number.  Any of them may be
     left out, with its norm or factor.  Sums are in 32 bits; ``normed`` is formed before
     ``stream`` is rounded.  Differentiable in every tensor."""
-    if _wants_grad(y, post_weight, gate, scale if isinstance(scale, torch.Tensor) else None, residual,
-                   pre_weight):
+    if _recorded('norm_gate_residual', y, post_weight, gate, scale, residual, pre_weight):
         return _NormGateResidual.apply(y, post_weight, gate, scale, residual, pre_weight, eps)
     return _norm_forward(y, post_weight, gate, scale, residual, pre_weight, eps)
 
 
 # ------------------------------------------------------------------------- 8-bit integer product
 def _no_grad(who, *ts):
-    if _wants_grad(*ts):
-        raise ValueError(f'{who} has no gradient: detach its operands or use torch.no_grad()')
+    if _wants_grad(*ts) or _tangent(*ts):
+        raise ValueError(f'{who} has no gradient, nor a rule for torch.func transforms: detach its '
+                         f'operands or use torch.no_grad()')
 
 
 def _channels(name, t, n, dev):
@@ -353,8 +387,8 @@ def int8_quantize(x):
     rows = _rows(x, k)
     x8 = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    N.check(N.lib().bs_int8_quantize(rows.data_ptr(), _DTYPES[x.dtype], rows.shape[0], k,
-                                     rows.stride(0), x8.data_ptr(), scale.data_ptr(),
+    N.check(N.lib().bs_int8_quantize(_address(rows), _DTYPES[x.dtype], rows.shape[0], k,
+                                     rows.stride(0), _address(x8), _address(scale),
                                      N.raw_stream(x.device)), 'bs_int8_quantize')
     return x8, scale
 
@@ -385,10 +419,10 @@ def _int8_product(x, x_scale, w8, w_scale, bias, out_dtype):
     nbytes = m * (-(-k // 128) * 128 + 4)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     N.check(N.lib().bs_int8_linear(
-        rows.data_ptr(), _DTYPES.get(x.dtype, 0), rows.stride(0), _address(x_scale), m, k, n,
-        w8.data_ptr(), w_scale.data_ptr(), _address(bias),
-        0 if bias is None else _DTYPES[bias.dtype], y.data_ptr(), _DTYPES[out_dtype],
-        ws.data_ptr(), nbytes, N.raw_stream(dev)), 'bs_int8_linear')
+        _address(rows), _DTYPES.get(x.dtype, 0), rows.stride(0), _address(x_scale), m, k, n,
+        _address(w8), _address(w_scale), _address(bias),
+        0 if bias is None else _DTYPES[bias.dtype], _address(y), _DTYPES[out_dtype],
+        _address(ws), nbytes, N.raw_stream(dev)), 'bs_int8_linear')
     return y
 
 
@@ -401,7 +435,7 @@ def int8_matmul(x8, x_scale, w8, w_scale, bias=None, out_dtype=torch.float32):
         raise TypeError('x8 must be an int8 tensor on the GPU')
     if out_dtype not in _DTYPES:
         raise TypeError(f'out_dtype {out_dtype} not supported (float32, bfloat16, float16)')
-    _no_grad('int8_matmul', x_scale, w_scale, bias)
+    _no_grad('int8_matmul', x8, x_scale, w8, w_scale, bias)
     return _int8_product(x8, x_scale, w8, w_scale, bias, out_dtype)
 
 
@@ -410,5 +444,5 @@ def int8_linear(x, w8, w_scale, bias=None):
     the type of ``x``: its rows are quantized on the way (:func:`int8_quantize`), the sums are
     exact, ``bias`` [n] is added in 32 bits.  Not differentiable."""
     _floating('x', x)
-    _no_grad('int8_linear', x, w_scale, bias)
+    _no_grad('int8_linear', x, w8, w_scale, bias)
     return _int8_product(x, None, w8, w_scale, bias, x.dtype)
