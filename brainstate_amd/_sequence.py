@@ -163,6 +163,7 @@ def gated_delta_step(q, k, v, g, beta, state, slots=None, scale=None):
     N.check(N.lib().bs_gated_delta_step(packed, b, t, _address(state), state.shape[0],
                                         _address(slots), _address(o), N.raw_stream(q.device)),
             'bs_gated_delta_step')
+    torch.autograd.graph.increment_version(state)     # autograd does not see the kernel's stores
     return o.squeeze(1) if one else o
 
 
