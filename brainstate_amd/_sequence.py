@@ -8,6 +8,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _native as N
+from . import _trace
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # enum bs_dtype
 _CHUNK = 64
@@ -140,6 +141,8 @@ def gated_delta_step(q, k, v, g, beta, state, slots=None, scale=None):
     order.  ``state`` [n, heads, dk, dv] float32, contiguous.  ``slots`` [batch] int32 names each
     row's state; a negative one (or one from n on) marks an idle row, whose output is 0.  Without
     it row b has state b.  Not differentiable."""
+    if _trace.active() is not None:      # a for_loop's recording pass: state must not advance in it
+        _trace.not_fusable()
     if _wants_grad(q, k, v, g, beta, state) or _tangent(q, k, v, g, beta, state, slots):
         raise ValueError('gated_delta_step updates its state in place and has no gradient: use '
                          'gated_delta_rule, or torch.no_grad()')

@@ -103,6 +103,11 @@ def active():
     return _active.trace
 
 
+def not_fusable():
+    """Ends the recording in progress: called by operators that change an operand in place."""
+    _abort(NotFusable())
+
+
 # operations allowed on a marked tensor: each maps a 0/1 (or bool) vector with ones exactly at
 # the spikes to another such vector (or only reads metadata)
 _META = {'shape', 'dtype', 'device', 'ndim', 'is_cuda', 'layout', 'requires_grad'}
