@@ -290,7 +290,12 @@ __global__ __launch_bounds__(512, 2) void grad_chain_kernel(
         if (c * kChunk + tok < sp.len) {
           T* p = op + (int64_t)c * kChunk * in.hv * in.dv + 16 * j;
           const int oc = ocol + 16 * j;
-          const bs_f32x4 y = beta * dr[j];
+          bs_f32x4 y = beta * dr[j];
+          // rounded to 32 bits in every form: in some of them the compiler folds the product into the
+          // conversion to fp16, which then rounds once, and a row's last bit would go by how many
+          // heads and sequences run beside it
+#pragma unroll
+          for (int r = 0; r < 4; ++r) asm volatile("" : "+v"(y[r]));
           if (vec) {
             if (oc < in.dv) bs_store4(p, y);
           } else {
