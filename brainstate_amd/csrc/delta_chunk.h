@@ -71,8 +71,8 @@ struct DeltaWork {
   uint16_t *kp, *qp;          // [slot][hk][parts][4][dkp / 32]: k and q, 0 past the end
   uint16_t *kt, *qt;          // [slot][hk][parts][dkp / 16][2]: their transposes
   uint16_t *inv;              // [slot][hv][3][6]: (1 + L)^-1 without its 32 x 32 block of zeros
-  uint16_t *att;              // [slot][hv][att parts][6]: the masked q k^T; in the backward pass
-                              // the transposes of both
+  uint16_t *att;              // [slot][hv][3][6]: the masked q k^T; in the backward pass the
+                              // transposes of both
   float *coef;                // [slot][hv][kCoef], see delta_coef
   float *ds, *dr;             // backward: [slot][hv][dkp][dvp], the gradient of the state after
                               // the chunk, and [slot][hv][64][dvp], that of R
@@ -89,14 +89,12 @@ __device__ __forceinline__ int delta_upper(int t, int s) { return t < 2 ? 2 * t 
 
 struct DeltaSizes {
   int64_t keys, square, coef, state, rows, bytes;
-  int parts, att_parts, dkp, dvp, ks;
+  int parts, dkp, dvp, ks;
 };
 
 static inline DeltaSizes delta_sizes(const bs_delta_in& in, int slots, int backward) {
   DeltaSizes s;
   s.parts = in.dtype == BS_BF16 ? 1 : in.dtype == BS_F16 ? 2 : 3;
-  // outputs in 16 bits take two parts of the masked product, gradients three
-  s.att_parts = backward || in.dtype == BS_F32 ? 3 : 2;
   s.ks = in.dk <= 64 ? 2 : 4;
   s.dkp = 32 * s.ks;
   s.dvp = (in.dv + 31) / 32 * 32;
@@ -105,7 +103,7 @@ static inline DeltaSizes delta_sizes(const bs_delta_in& in, int slots, int backw
   s.coef = (int64_t)slots * in.hv * kCoef;
   s.state = backward ? (int64_t)slots * in.hv * s.dkp * s.dvp : 0;
   s.rows = backward ? (int64_t)slots * in.hv * kChunk * s.dvp : 0;
-  s.bytes = s.keys * 2 * (backward ? 4 : 3) + s.square * 2 * (3 + s.att_parts) +
+  s.bytes = s.keys * 2 * (backward ? 4 : 3) + s.square * 2 * 6 +
             (s.coef + s.state + s.rows) * 4;
   return s;
 }
@@ -119,7 +117,7 @@ static inline DeltaWork delta_work(void* ws, const DeltaSizes& s, int backward) 
     return r;
   };
   w.inv = (uint16_t*)take(s.square * 6);
-  w.att = (uint16_t*)take(s.square * 2 * s.att_parts);
+  w.att = (uint16_t*)take(s.square * 6);
   w.coef = (float*)take(s.coef * 4);
   w.kp = (uint16_t*)take(s.keys * 2);
   w.qp = (uint16_t*)take(s.keys * 2);

@@ -27,7 +27,7 @@ namespace {
 // One chunk and value head: 4 waves, wave w has tile w's rows.
 // The inverse is formed by blocks of 16 tokens: the four on the diagonal by substitution, one
 // column a lane, the ones below by X_ij = -X_ii sum_k L_ik X_kj in 32-bit matrix instructions.
-template <typename T, int PI, int KS, bool BWD, int PA>
+template <typename T, int PI, int KS, bool BWD>
 __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan plan, DeltaWork w,
                                                       int vec) {
   constexpr int DK = KS * 32, LD = DK + 8;
@@ -190,14 +190,12 @@ __global__ __launch_bounds__(256) void prepare_kernel(bs_delta_in in, DeltaPlan 
       x[e] = BWD ? xm[j + e][i] : xm[i][j + e];
       y[e] = BWD ? lm[j + e][i] : lm[i][j + e];
     }
-    const bs_parts<3> xp = bs_split8<3>(x);
-    const bs_parts<PA> yp = bs_split8<PA>(y);
+    const bs_parts<3> xp = bs_split8<3>(x), yp = bs_split8<3>(y);
 #pragma unroll
-    for (int p = 0; p < 3; ++p)
+    for (int p = 0; p < 3; ++p) {
       *(bs_bf16x8*)(w.inv + (sh * 3 + p) * kSquare + f * kFrag + lane * 8) = xp.p[p];
-#pragma unroll
-    for (int p = 0; p < PA; ++p)
-      *(bs_bf16x8*)(w.att + (sh * PA + p) * kSquare + f * kFrag + lane * 8) = yp.p[p];
+      *(bs_bf16x8*)(w.att + (sh * 3 + p) * kSquare + f * kFrag + lane * 8) = yp.p[p];
+    }
   }
 }
 
@@ -214,12 +212,12 @@ template <typename T, int PI, int KS, int NT, bool KEEP>
 __global__ __launch_bounds__(512, 2) void chain_kernel(
     bs_delta_in in, DeltaPlan plan, DeltaWork w, const float* state0, float* state1, T* o,
     float* keep_s, float* keep_u, int dvp, int units, int vec) {
-  constexpr int DK = KS * 32, TW = KS / 2, PO = PI == 3 ? 3 : 2, PV = KEEP ? 3 : PO;
+  constexpr int DK = KS * 32, TW = KS / 2;
   constexpr int kS = KS * NT * 128, kR = 2 * NT * 128;       // words of a part
   __shared__ __attribute__((aligned(16))) uint2 ls[3 * kS];     // the state
   __shared__ __attribute__((aligned(16))) uint2 lr[3 * kR];     // R
   __shared__ __attribute__((aligned(16))) uint2 lu[3 * kR];     // exp(total - run) U
-  __shared__ __attribute__((aligned(16))) uint2 lv[PV * kR];    // U
+  __shared__ __attribute__((aligned(16))) uint2 lv[3 * kR];     // U
   const DeltaPlace at = delta_place(units, dvp / (16 * NT));
   if (at.unit >= units) return;
   const int h = __builtin_amdgcn_readfirstlane(at.unit % in.hv);
@@ -340,7 +338,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[j][r] = lf[r] * u[j][r];
         delta_put<3>(lu + own + 128 * j, kR, x[j]);
-        delta_put<PV>(lv + own + 128 * j, kR, u[j]);
+        delta_put<3>(lv + own + 128 * j, kR, u[j]);
       }
       __builtin_amdgcn_sched_barrier(0);
       load_inverse(next);
@@ -386,8 +384,8 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(
   } else {
     const int ocol = at.slice * 16 * NT + 4 * g;
     const uint16_t* qp = w.qp + kb + wave * KS * kFrag + lane * 8;
-    const uint16_t* ap = w.att + hb * PO * kSquare + lane * 8;
-    struct Operands { bs_parts<PI> q[KS]; bs_parts<PO> a[2]; float scale; } operands[2];
+    const uint16_t* ap = w.att + hb * 3 * kSquare + lane * 8;
+    struct Operands { bs_parts<PI> q[KS]; bs_parts<3> a[2]; float scale; } operands[2];
     auto load = [&](int c, Operands& x) {
       const int64_t ch = (int64_t)c * in.hv;
 #pragma unroll
@@ -395,8 +393,8 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(
         x.q[st] = delta_frags<PI>(qp + c * keys + st * kFrag, kChunk * DK);
 #pragma unroll
       for (int st = 0; st < 2; ++st)
-        x.a[st] = delta_frags<PO>(ap + ch * PO * kSquare +
-                                      delta_lower(wave, min(st, blk)) * kFrag, kSquare);
+        x.a[st] = delta_frags<3>(ap + ch * 3 * kSquare +
+                                     delta_lower(wave, min(st, blk)) * kFrag, kSquare);
       x.scale = in.scale * cp[ch * kCoef + kGrow * kChunk + tok];
     };
     const int last = sp.chunks - 1;
@@ -418,8 +416,7 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(
       for (int st = 0; st < KS; ++st)
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-          y[j] = bs_mma<PO - 1>(delta_lds<PO>(ls + ((st * NT + j) * 64 + lane) * 2, kS), now.q[st],
-                                y[j]);
+          y[j] = bs_mma<2>(delta_lds<3>(ls + ((st * NT + j) * 64 + lane) * 2, kS), now.q[st], y[j]);
 #pragma unroll
       for (int j = 0; j < NT; ++j) y[j] *= now.scale;
       if (KEEP) {
@@ -439,14 +436,14 @@ __global__ __launch_bounds__(512, 2) void chain_kernel(
         if (st <= blk) {
 #pragma unroll
           for (int j = 0; j < NT; ++j)
-            y[j] = bs_mma<PO - 1>(delta_lds<PO>(lv + ((st * NT + j) * 64 + lane) * 2, kR),
-                                  now.a[st], y[j]);
+            y[j] = bs_mma<2>(delta_lds<3>(lv + ((st * NT + j) * 64 + lane) * 2, kR), now.a[st],
+                             y[j]);
         }
       load(min(c + 2, last), now);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         if (KEEP) {
-          const bs_f32x4 u = delta_turn(delta_lds<PV>(lv + ((blk * NT + j) * 64 + lane) * 2, kR),
+          const bs_f32x4 u = delta_turn(delta_lds<3>(lv + ((blk * NT + j) * 64 + lane) * 2, kR),
                                         wave & 1, lane);
           *(bs_f32x4*)(keep_u + sh * kChunk * dvp +
                        delta_kept(wave, at.slice * NT + j, lane, dvp)) = u;
@@ -480,8 +477,8 @@ void launch_prepare(const bs_delta_in& in, const DeltaPlan& plan, const DeltaWor
   const dim3 grid(plan.slots, in.hv);
   int vec = in.dk % 8 == 0 && (uintptr_t)in.q % 16 == 0 && (uintptr_t)in.k % 16 == 0;
   for (int i = 0; i < 3; ++i) vec = vec && in.q_stride[i] % 8 == 0 && in.k_stride[i] % 8 == 0;
-  if (backward) prepare_kernel<T, PI, KS, true, 3><<<grid, 256, 0, st>>>(in, plan, w, vec);
-  else prepare_kernel<T, PI, KS, false, PI == 3 ? 3 : 2><<<grid, 256, 0, st>>>(in, plan, w, vec);
+  if (backward) prepare_kernel<T, PI, KS, true><<<grid, 256, 0, st>>>(in, plan, w, vec);
+  else prepare_kernel<T, PI, KS, false><<<grid, 256, 0, st>>>(in, plan, w, vec);
 }
 
 template <typename T, int PI, int KS>

@@ -71,8 +71,6 @@ static inline int bs_dtype_size(int d) { return d == BS_F32 ? 4 : 2; }
 // weight 2^-8p, and pairs with p + q > 2 are left out.  A pair costs one instruction, so a
 // 32-bit operand against a bf16 one costs 3 and two of them 6, where the fp32 matrix
 // instruction costs 16.
-// Where the result is rounded to 16 bits at once, pairs with p + q > 1 are left out as well
-// (error 2^-15 against the result's own 2^-9).
 template <int P>
 struct bs_parts { bs_bf16x8 p[P]; };
 
