@@ -39,11 +39,14 @@ def _wants_grad(*ts):
     return False
 
 
+# a torch that cannot tell whether a transform is active has every operand looked at
+_transforms_active = getattr(torch._C, '_are_functorch_transforms_active', lambda: True)
+
+
 def _tangent(*ts):
     """Whether one of the operands carries a forward-mode tangent or is wrapped by a torch.func
     transform: there is no rule for either here, and the kernels would drop it."""
-    active = getattr(torch._C, '_are_functorch_transforms_active', None)
-    inside = active is None or active()
+    inside = _transforms_active()
     if not inside and getattr(forward_ad, '_current_level', 0) < 0:
         return False
     for t in ts:
