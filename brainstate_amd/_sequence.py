@@ -142,8 +142,8 @@ def gated_delta_step(q, k, v, g, beta, state, slots=None, scale=None):
     ``q``, ``k`` [batch, key heads, dk], ``v`` [batch, heads, dv], ``g`` (log decay) and ``beta``
     [batch, heads]; each may have a dimension of tokens after the batch, which are taken in
     order.  ``state`` [n, heads, dk, dv] float32, contiguous.  ``slots`` [batch] int32 names each
-    row's state; a negative one (or one from n on) marks an idle row, whose output is 0.  Without
-    it row b has state b.  Not differentiable."""
+    row's state, each its own; a negative one (or one from n on) marks an idle row, whose output is
+    0.  Without it row b has state b.  Not differentiable."""
     if _trace.active() is not None:      # a for_loop's recording pass: state must not advance in it
         _trace.not_fusable()
     if _wants_grad(q, k, v, g, beta, state) or _tangent(q, k, v, g, beta, state, slots):
@@ -255,7 +255,7 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, seq_offse
     ``beta`` [batch, tokens, heads]; ``initial_state`` float32, None for zeros.  With
     ``seq_offsets`` (int32 [sequences + 1], ascending) the sequences are packed end to end into
     one batch row; tokens outside all of them give 0.  Differentiable in everything but
-    ``seq_offsets``."""
+    ``seq_offsets``, in reverse mode."""
     if _recorded('gated_delta_rule', q, k, v, g, beta, initial_state, seq_offsets):
         return _DeltaRule.apply(q, k, v, g, beta, initial_state, scale, seq_offsets)
     o, final, _ = _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, False)
@@ -363,7 +363,7 @@ def norm_gate_residual(y, post_weight=None, gate=None, scale=None, residual=None
     ``y``, ``gate`` and ``residual`` have one shape and type; ``post_weight``, ``scale`` and
     ``pre_weight`` are [dim] of any floating type, ``scale`` may be a number.  Any of them may be
     left out, with its norm or factor.  Sums are in 32 bits; ``normed`` is formed before
-    ``stream`` is rounded.  Differentiable in every tensor."""
+    ``stream`` is rounded.  Differentiable in every tensor, in reverse mode."""
     if _recorded('norm_gate_residual', y, post_weight, gate, scale, residual, pre_weight):
         return _NormGateResidual.apply(y, post_weight, gate, scale, residual, pre_weight, eps)
     return _norm_forward(y, post_weight, gate, scale, residual, pre_weight, eps)

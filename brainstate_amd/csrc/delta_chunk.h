@@ -311,8 +311,8 @@ __device__ __forceinline__ bs_f32x4 delta_turn(const bs_parts<P>& x, int odd, in
 // Whether a workgroup of the recurrences takes 32 value columns instead of 16: where 16 would not
 // leave every workgroup a CU of its own.  A chunk's latency grows less than the columns do, and
 // half the workgroups then take turns on a CU.  Whole forward call in us with 16 / 32 columns,
-// heads of 128 x 128: 8,192 tokens x 32 heads (256 workgroups of 16) 406 / 461, x 40 heads 686 /
-// 496, 2 x 4,096 x 16 172 / 205, 4 x 2,048 x 16 177 / 142.
+// heads of 128 x 128: 8,192 tokens x 32 heads (256 workgroups of 16) 434 / 506, x 40 heads 735 /
+// 542, 2 x 4,096 x 16 186 / 231, 4 x 2,048 x 16 194 / 156.
 static inline bool delta_wide(int64_t units, int dvp) {
   return units * (dvp / 16) > bs_num_cus();
 }

@@ -21,13 +21,17 @@
 // since dL = -(1 + L)^-T (dU R^T) (1 + L)^-T = -dR U^T needs no product with the inverse beyond dR.
 // dg is a difference of large sums, so everything that reaches it is in 32 bits.
 //
-// 4 x 2,048 tokens x 16 heads of 128 x 128 in bfloat16, the whole step 613 us: the forward pass 187
-// (it keeps the states), prepare again 58 us (kept from the forward pass it would hold 142 MB more
-// a layer), grad_chain_kernel 160, grad_chunk_kernel 232.  The last fills its 256 registers with
-// products in three parts and their cutting: whole step 687 us with U's parts cut by every wave that
-// takes them, 652 with the fragments' addresses kept over the heads (184 bytes a lane spilled, 100
-// MB written and read).  Two waves a SIMD to issue from keep the matrix cores busy in a sixth of
-// the cycles.
+// 4 x 2,048 tokens x 16 heads of 128 x 128 in bfloat16, the whole step 625 us.  Its kernels under
+// the tracer, 643 in all: forward prepare 55 and chain 140 (it keeps the states), prepare again 58
+// (all of it kept from the forward pass would hold 146 MB more a layer), grad_chain_kernel 158,
+// grad_chunk_kernel 232.  The last fills its 256 registers with products in three parts and their
+// cutting (16 bytes a lane spill): beside 613 for the whole step then, 687 with U's parts cut by
+// every wave that takes them, 652 with the fragments' addresses kept over the heads (184 bytes
+// spilled, 100 MB written and read).  Two waves a SIMD to issue from keep the matrix cores busy in
+// a fifth of the cycles, in both kernels.
+// Keys past 64 values in fp16 and in 32 bits do not fit the registers: grad_chain_kernel spills 180
+// bytes a lane in fp16 (with 32 columns) and 248 or 344 in 32 bits, grad_chunk_kernel 80 and 220;
+// the gradients of the same layer take 591 and 974 us there, 451 in bfloat16.
 #include "delta_chunk.h"
 
 namespace {

@@ -10,11 +10,12 @@
 // Few tokens (skinny_kernel): bound by the weights' bytes, and below a few MB by the latency of
 // one pass over k.  Each workgroup has 16 channels and its waves share k; weights go straight from
 // memory to the matrix instruction, whose operand is 16 rows x 64 bytes.  One token x 4,096 x
-// 4,096: 6.0 us (2.8 TB/s; 16.9 MB fetched for 16.8), with 3.6 before it for the token's integers.
+// 4,096: 6.0 us (2.8 TB/s; 16.9 MB fetched for 16.8), with 3.7 before it for the token's integers.
 // Many tokens (tile_kernel): bound by the matrix cores; tiles of both operands are staged in LDS
 // by direct loads, two deep, 16-byte pieces in an order that keeps the reads off each other's
-// banks (no conflicts counted).  8,192 x 4,096 x 4,096: 140 us in a run of calls (1.96 POP/s; the
-// matrix cores are busy in 49 % of the cycles), a large library product of this type 2.1 POP/s.
+// banks (no conflicts counted).  8,192 x 4,096 x 4,096: in a run of calls 162 us with the 24 of
+// quant_kernel, so 138 (2.0 POP/s; a large library product of this type 2.1), under the tracer 157
+// (1.75 POP/s); the matrix cores are busy in 49 % of the cycles.
 #include "lane_types.h"
 
 #include <type_traits>

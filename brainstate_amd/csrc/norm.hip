@@ -11,9 +11,14 @@
 // Workgroups stay for many rows: a lane's columns are the same in each, so the weights are read
 // once and the weights' gradients are summed in registers, then over the workgroups in their
 // order (grad_sum_kernel): the same bits every time.
-// bfloat16 with every part, beside a large copy's 5.1 TB/s: 8,192 x 4,096 forward 67 us (5.0 TB/s),
-// gradients 129 us (4.2 TB/s; 201 with a row's loads only after the row before); 4,099 x 2,050
-// 26 and 75 us.  Past 8,192 values the gradients' lanes hold more than their registers and spill.
+// bfloat16 with every part, beside a large copy's 5.1 TB/s: 8,192 x 4,096 forward 68 us (4.9 TB/s),
+// gradients 136 us with the weights' sums (3.9 TB/s; the kernel alone 129, 201 with a row's loads
+// only after the row before); 4,099 x 2,050 29 and 76 us.
+// Two runs a lane (past 4,096 values) do not fit the gradients' registers, which spill 340 to 436
+// bytes a lane, 856 to 892 in workgroups of 1,024 (past 8,192), where the forward kernel spills 92
+// to 256 as well: 4,096 x 5,120 forward 70 us (3.0 TB/s: 5 waves lie unevenly on 4 SIMDs),
+// gradients 444 (0.8); 8,192 x 8,192 143 (4.7) and 1,026 (1.0); 4,096 x 16,384 245 (2.7) and 2,046
+// (0.5).
 #include "lane_types.h"
 
 #include <type_traits>

@@ -23,8 +23,8 @@ class GatedDelta(Dynamics):
         y = (norm(o) head_norm silu(z)) weight_out^T
         stream + scale y,  norm(stream + scale y) next_norm
 
-    [batch, in_size] is one token of every row and advances ``S`` in place (no gradient: for
-    ``for_loop``-like stepping and serving); [batch, tokens, in_size] runs whole sequences in
+    [batch, in_size] is one token of every row and advances ``S`` in place (no gradient: for serving,
+    one by one or in a ``for_loop`` under ``torch.no_grad()``); [batch, tokens, in_size] runs whole sequences in
     chunks, is differentiable in the parameters and both inputs, and leaves the last states in
     ``S`` (with their graph where one is recorded: ``init_state`` starts the next sequence).
 
