@@ -167,6 +167,12 @@ SIGNATURES = {
     'bs_gated_delta_grad_workspace_size': (c_size, [c_vp, c_i32, c_i32, c_i32]),
     'bs_gated_delta_rule_grad': (ctypes.c_int, [c_vp, c_i32, c_i32] + [c_vp] * 12 + [c_size,
                                                                                    c_vp]),
+    'bs_decay_attention_step': (ctypes.c_int, [c_vp, c_i32, c_i32, c_vp, ctypes.c_int64, c_vp,
+                                               c_vp, c_vp]),
+    'bs_decay_attention_segments': (c_size, [c_vp, c_i32, c_i32, c_i32, c_i32]),
+    'bs_decay_attention_workspace_size': (c_size, [c_vp, c_i32, c_i32, c_i32, c_i32]),
+    'bs_decay_attention': (ctypes.c_int, [c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32,
+                                          c_vp, c_size, c_vp]),
     'bs_norm_gate_residual': (ctypes.c_int, [c_vp] * 4),
     'bs_norm_grad_workspace_size': (c_size, [ctypes.c_int64, c_i32]),
     'bs_norm_gate_residual_grad': (ctypes.c_int, [c_vp] * 10 + [c_size, c_vp]),

@@ -1,0 +1,818 @@
+// Decay attention over chunks of 64 tokens: the walk over a sequence's chunks, forward and for the
+// gradients (decay.h has its formulas), and the carry of states from segment to segment.
+//
+// A chunk costs two products with the state and two within the chunk.  A workgroup walks the
+// chunks of one segment and head; each of its 4 waves has 32 value columns of the state in
+// registers, so the state never leaves them inside a segment:
+//
+//   att^T = K Q^T          rows j, columns i: a lane has 16 neighbouring j of one i
+//   O^T   = S^T Q^T + V^T att^T     rows are value columns, a lane has 16 neighbouring of one token
+//   S     = K^T V          a lane has one value column and runs of 8 rows, which is what the next
+//                          S^T Q^T takes from it
+//
+// Rows of a tile are dealt so that a product leaves in a lane what the next one takes from it; the
+// transposed operands (K^T, V^T) are read from LDS by its transposing reads.
+//
+// Numbers: the state and all sums are 32-bit; products take 32-bit operands as three exact bf16
+// parts (lane_types.h).  Sums of log decays are 64-bit, since their differences are exponents.
+#include "decay.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPitch = 128;      // values of a row of V in LDS
+
+template <typename T> constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
+template <> constexpr int kParts<bs_bf16> = 1;
+
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
+typedef __attribute__((address_space(3))) i16x4* LdsTile;
+
+// 4 rows x 16 columns of 16-bit values for 16 lanes, transposed: lane l gives the place of the 4
+// columns 4 (l % 4) .. of row l / 4 % 4 and receives the 4 rows of column l % 16.
+__device__ __forceinline__ uint2 turn4(const uint16_t* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTile)p));
+}
+
+// acc += a b over 16 products: parts p, q with p + q <= 2.
+template <int PA, int PB>
+__device__ __forceinline__ bs_f32x16 mma(const bs_parts<PA>& a, const bs_parts<PB>& b,
+                                         bs_f32x16 acc) {
+#pragma unroll
+  for (int s = 2; s >= 0; --s)
+#pragma unroll
+    for (int p = 0; p <= s; ++p)
+      if (p < PA && s - p < PB)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[p], b.p[s - p], acc, 0, 0, 0);
+  return acc;
+}
+
+__device__ __forceinline__ bs_f32x16 zero16() {
+  bs_f32x16 r;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = 0.f;
+  return r;
+}
+
+// Where value d of row `row` lies in a tile of rows of D values: pieces of 8 in an order that
+// spreads 16 rows' pieces over the banks.
+template <int D>
+__device__ __forceinline__ int place(int row, int d) {
+  const int key = D == 128 ? row & 15 : row >> 1 & 7;
+  return row * D + (((d >> 3) ^ key) << 3) + (d & 7);
+}
+
+// The rows of a chunk in processing order, 8 neighbouring values at a time, 0 past the last row and
+// the row's end: buffer loads, whose bounds the hardware checks.
+template <typename T>
+struct ChunkRows {
+  __amdgpu_buffer_rsrc_t rs;
+  uint32_t step;
+  int dim, rows, back;
+  bool vec;
+  __device__ __forceinline__ ChunkRows(const DecayOperand& x, const DecayChunk& c, int h, int d,
+                                       int v, int b) {
+    step = (uint32_t)(x.stride[1] * sizeof(T));
+    const uint64_t p = (uint64_t)((const T*)x.p + bs_delta_at(x.stride, c.batch, c.token,
+                                                              h / x.rep));
+    const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((int)p);
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0,
+                                           (uint32_t)(c.rows - 1) * step + d * (int)sizeof(T),
+                                           0x00027000);
+    dim = d, rows = c.rows, vec = v, back = b;
+  }
+  __device__ __forceinline__ void raw(int row, int d, uint4* x) const {
+    constexpr int W = sizeof(T) / 2;
+    const int have = row < rows ? dim : 0;
+    const uint32_t at = (uint32_t)(back ? rows - 1 - row : row) * step;
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        x[i] = __builtin_bit_cast(
+            uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                       rs, d < have ? at + d * (uint32_t)sizeof(T) + 16 * i : 0xFFFFFFF0u, 0, 0));
+    } else {
+      uint32_t e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t o = d + j < have ? at + (d + j) * (uint32_t)sizeof(T) : 0xFFFFFFF0u;
+        if constexpr (W == 1) e[j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, o, 0, 0);
+        else e[j] = __builtin_amdgcn_raw_buffer_load_b32(rs, o, 0, 0);
+      }
+      if constexpr (W == 1) {
+        x[0] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16,
+                          e[6] | e[7] << 16);
+      } else {
+        x[0] = make_uint4(e[0], e[1], e[2], e[3]);
+        x[1] = make_uint4(e[4], e[5], e[6], e[7]);
+      }
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void floats(const uint4* x, float* f) {
+  T t[8];
+  __builtin_memcpy(t, x, sizeof(t));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = bs_to_f32(t[j]);
+}
+
+template <typename T>
+__device__ __forceinline__ bs_parts<kParts<T>> parts_of(const uint4* x) {
+  if constexpr (kParts<T> == 1) {
+    bs_parts<1> o;
+    o.p[0] = __builtin_bit_cast(bs_bf16x8, x[0]);
+    return o;
+  } else {
+    float f[8];
+    floats<T>(x, f);
+    return bs_split8<kParts<T>>(f);
+  }
+}
+
+// A chunk's rows of D padded values on their way into LDS.
+template <typename T, int D>
+struct Staged {
+  static constexpr int kPer = D / 8, kRows = kThreads / kPer, kN = 64 / kRows, W = sizeof(T) / 2;
+  uint4 x[kN][W];
+  __device__ __forceinline__ void load(const ChunkRows<T>& r) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      r.raw(threadIdx.x / kPer + i * kRows, threadIdx.x % kPer * 8, x[i]);
+  }
+  // as bf16 parts, [part][64][D]
+  __device__ __forceinline__ void put(uint16_t* to) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const bs_parts<kParts<T>> p = parts_of<T>(x[i]);
+      const int at = place<D>(threadIdx.x / kPer + i * kRows, threadIdx.x % kPer * 8);
+#pragma unroll
+      for (int k = 0; k < kParts<T>; ++k) *(bs_bf16x8*)(to + k * 64 * D + at) = p.p[k];
+    }
+  }
+  // as they are, [64][D]: 16-bit values in the order of place(), 32-bit ones in a row's order
+  __device__ __forceinline__ void put_raw(void* to) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int row = threadIdx.x / kPer + i * kRows, d = threadIdx.x % kPer * 8;
+      if constexpr (W == 1) {
+        *(uint4*)((uint16_t*)to + place<D>(row, d)) = x[i][0];
+      } else {
+        *(uint4*)((float*)to + row * D + d) = x[i][0];
+        *(uint4*)((float*)to + row * D + d + 4) = x[i][W - 1];
+      }
+    }
+  }
+};
+
+// Coefficients of a chunk, by processing order.
+struct Coef {
+  float grow[64], left[64];      // exp(run_i), exp(total - run_i)
+  double run[64];                // times log2 e
+  float total;                   // exp(total)
+};
+
+constexpr double kLog2e = 1.4426950408889634;
+
+__device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
+
+// By one wave, lane = row.  Returns total (times log2 e).
+__device__ __forceinline__ double coefficients(const DecayPlan& p, const DecayChunk& c, int back,
+                                               int h, Coef& o) {
+  const int lane = threadIdx.x & 63;
+  // from the last token to the first, a decay belongs to the row after its token
+  const int at = back ? c.rows - lane : lane;
+  float g = 0.f;
+  if (lane < c.rows && (!back || lane > 0 || c.next_g))
+    g = bs_load_any(p.g, p.g_dtype, bs_delta_at(p.g_stride, c.batch, c.token + at, h));
+  g = g < BS_DELTA_G_MIN ? BS_DELTA_G_MIN : g;
+  double x = (double)g * kLog2e;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  const double total = __shfl(x, 63);
+  o.run[lane] = x;
+  o.grow[lane] = exp_of(x);
+  o.left[lane] = exp_of(total - x);
+  if (lane == 0) o.total = exp_of(total);
+  return total;
+}
+
+// The slots of a segment in processing order, those with a chunk.
+struct Chunks {
+  int slot, end, step, back;
+  DeltaSpan span;
+  __device__ __forceinline__ Chunks(const DeltaPlan& p, int from, int to, int b) {
+    back = b, step = b ? -1 : 1;
+    slot = b ? to - 1 : from;
+    end = b ? from - 1 : to;
+    span.slot = -1, span.chunks = 0;
+  }
+  // `empty`: called for a sequence without tokens
+  template <typename F>
+  __device__ __forceinline__ bool next(const DeltaPlan& p, DecayChunk& c, F&& empty) {
+    for (; slot != end; slot += step) {
+      if (slot < span.slot || slot >= span.slot + span.chunks) {
+        span = delta_span(p, delta_owner(p, slot));
+        if (span.chunks == 0 && slot == span.slot) empty(span.seq);
+      }
+      const int k = slot - span.slot;
+      if (k < 0 || k >= span.chunks) continue;
+      c.seq = span.seq, c.batch = span.batch;
+      c.token = span.first + (int64_t)k * kChunk;
+      c.rows = min(span.len - k * kChunk, kChunk);
+      c.next_g = k < span.chunks - 1;
+      c.first = back ? k == span.chunks - 1 : k == 0;
+      c.last = back ? k == 0 : k == span.chunks - 1;
+      slot += step;
+      return true;
+    }
+    return false;
+  }
+};
+
+// What the segment [from, to) leaves to the next one, and the slots it takes.
+__device__ __forceinline__ DecayLink link_of(const DeltaPlan& p, int back, int& from, int& to) {
+  const int edge = back ? from : to - 1;
+  const DeltaSpan s = delta_span(p, delta_owner(p, edge));
+  const int k = edge - s.slot;
+  if (k < 0 || k >= s.chunks || k == (back ? 0 : s.chunks - 1)) return {-1, 0};
+  const int first = back ? s.slot + s.chunks <= to : s.slot >= from;
+  if (back) to = min(to, s.slot + s.chunks);
+  else from = max(from, s.slot);
+  return {s.seq, first};
+}
+
+struct Place {                   // a lane's place in the products of 32 x 32
+  int m, g, x, y, half;
+  __device__ __forceinline__ Place() {
+    const int lane = threadIdx.x & 63;
+    m = lane & 31, g = lane >> 5, x = lane & 3, y = lane >> 2 & 3, half = lane >> 4 & 1;
+  }
+};
+
+// Row m of a tile of value columns (and of att^T): lane group g then has 16 neighbouring ones.
+__device__ __forceinline__ int value_row(int m) {
+  return 16 * (m >> 2 & 1) + 4 * (m >> 3) + (m & 3);
+}
+
+// K^T of rows 32 rt .. and tokens 16 ks ..: part `part` of the tile [part][64][DC].
+template <int DC>
+__device__ __forceinline__ bs_bf16x8 turned_k(const uint16_t* k, int rt, int ks, const Place& l) {
+  const int d = 32 * rt + 16 * l.half + 8 * (l.x & 1) + 4 * (l.x >> 1), t = 16 * ks + 8 * l.g + l.y;
+  const uint2 a = turn4(k + place<DC>(t, d)), b = turn4(k + place<DC>(t + 4, d));
+  return __builtin_bit_cast(bs_bf16x8, make_uint4(a.x, a.y, b.x, b.y));
+}
+
+// V^T of 32 value columns from `col` and tokens 16 ks ..: 8 values.
+template <typename T>
+__device__ __forceinline__ void turned_v(const void* v, int col, int ks, const Place& l, uint4* r) {
+  if constexpr (sizeof(T) == 2) {
+    const int d = col + 16 * (l.x & 1) + 4 * (2 * l.half + (l.x >> 1)), t = 16 * ks + 8 * l.g + l.y;
+    const uint2 a = turn4((const uint16_t*)v + place<kPitch>(t, d)),
+                b = turn4((const uint16_t*)v + place<kPitch>(t + 4, d));
+    r[0] = make_uint4(a.x, a.y, b.x, b.y);
+  } else {
+    const uint32_t* p = (const uint32_t*)v + (16 * ks + 8 * l.g) * kPitch + col + value_row(l.m);
+    r[0] = make_uint4(p[0], p[kPitch], p[2 * kPitch], p[3 * kPitch]);
+    r[1] = make_uint4(p[4 * kPitch], p[5 * kPitch], p[6 * kPitch], p[7 * kPitch]);
+  }
+}
+
+// The wave's 32 columns of a state: element e of tile rt is row 32 rt + 16 (e / 8) + 8 g + e % 8.
+template <int RT>
+struct Columns {
+  bs_f32x16 s[RT];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) s[i] = zero16();
+  }
+  template <typename F>
+  static __device__ __forceinline__ void each(const DecayRun& r, int col, const Place& l, F&& f) {
+    const int c = col + value_row(l.m);
+    if (c >= r.dv) return;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int d = 32 * i + 16 * (e >> 3) + 8 * l.g + (e & 7);
+        if (d < r.dc) f(i, e, d, c);
+      }
+  }
+  __device__ __forceinline__ void load(const DecayRun& r, const DecayState& st, int64_t at, int col,
+                                       const Place& l) {
+    clear();
+    if (!st.p) return;
+    const float* p = st.p + at * r.dc * r.dv;
+    each(r, col, l, [&](int i, int e, int d, int c) { s[i][e] = p[d * st.row + c * st.col]; });
+  }
+  __device__ __forceinline__ void store(const DecayRun& r, const DecayState& st, int64_t at,
+                                        float scale, int col, const Place& l) const {
+    float* p = st.p + at * r.dc * r.dv;
+    each(r, col, l,
+         [&](int i, int e, int d, int c) { p[d * st.row + c * st.col] = scale * s[i][e]; });
+  }
+  // s = decay s + K^T (left V) with V's turned fragments of 16 tokens each
+  template <typename T, int DC>
+  __device__ __forceinline__ void add(const uint16_t* k, const uint4 (*v)[sizeof(T) / 2],
+                                      const Coef& co, float scale, const Place& l) {
+    const float total = co.total;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) s[i] *= total;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      float f[8];
+      floats<T>(v[ks], f);
+      const float* lf = co.left + 16 * ks + 8 * l.g;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= scale * lf[j];
+      const bs_parts<3> vp = bs_split8<3>(f);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        bs_parts<kParts<T>> kp;
+#pragma unroll
+        for (int p = 0; p < kParts<T>; ++p) kp.p[p] = turned_k<DC>(k + p * 64 * DC, i, ks, l);
+        s[i] = mma(kp, vp, s[i]);
+      }
+    }
+  }
+};
+
+struct Carry {
+  float* factor;               // [segs][hv]: decay of a state over the slots a segment takes
+  DecayLink* link;             // [segs]
+};
+
+// What the slots of a segment that the next one goes on with add to the state, from zero.
+template <typename T, int RT>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void sum_kernel(DecayRun run,
+                                                                             DecayPlan plan,
+                                                                             Carry carry) {
+  constexpr int DC = 32 * RT, PI = kParts<T>;
+  __shared__ __attribute__((aligned(16))) uint16_t lk[PI * 64 * DC];
+  __shared__ __attribute__((aligned(16))) T lv[64 * kPitch];
+  __shared__ Coef coef[2];
+  const int seg = blockIdx.x, h = blockIdx.y;
+  int from = seg * plan.per, to = min(from + plan.per, plan.seq.slots);
+  const DecayLink link = link_of(plan.seq, run.back, from, to);
+  if (h == 0 && threadIdx.x == 0) carry.link[seg] = link;
+  if (link.seq < 0) return;
+  const Place l;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = 32 * wave;
+  const bool live = col < run.dv;
+  Chunks chunks(plan.seq, from, to, run.back);
+  DecayChunk c;
+  auto none = [](int) {};
+  Staged<T, DC> k;
+  Staged<T, kPitch> v;
+  auto load = [&](const DecayChunk& at) {
+    k.load(ChunkRows<T>(run.k, at, h, run.dc, run.vec_k, run.back));
+    v.load(ChunkRows<T>(run.v, at, h, run.dv, run.vec_v, run.back));
+  };
+  double decay = 0.0;
+  bool more = chunks.next(plan.seq, c, none);
+  if (more) {
+    load(c);
+    if (wave == 3) decay += coefficients(plan, c, run.back, h, coef[0]);
+  }
+  Columns<RT> s;
+  s.clear();
+  for (int at = 0; more; at ^= 1) {
+    __syncthreads();
+    k.put(lk);
+    v.put_raw(lv);
+    more = chunks.next(plan.seq, c, none);
+    __syncthreads();
+    if (more) {
+      load(c);
+      if (wave == 3) decay += coefficients(plan, c, run.back, h, coef[at ^ 1]);
+    }
+    if (live) {
+      uint4 vf[4][sizeof(T) / 2];
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) turned_v<T>(lv, col, ks, l, vf[ks]);
+      s.template add<T, DC>(lk, vf, coef[at], run.add_scale, l);
+    }
+  }
+  if (live) s.store(run, run.start, (int64_t)seg * plan.hv + h, 1.f, col, l);
+  if (threadIdx.x == 192) carry.factor[seg * plan.hv + h] = exp_of(decay);
+}
+
+// The states before the segments, in place of the segments' sums: a lane has one element of a
+// head's state.
+__global__ __launch_bounds__(256) void scan_kernel(DecayRun run, DecayPlan plan, Carry carry) {
+  const int n = run.dc * run.dv, e = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+  if (e >= n) return;
+  const int r = e / run.dv, c = e % run.dv;
+  float* p = run.start.p + (int64_t)h * n + e;
+  const int64_t step = (int64_t)plan.hv * n;
+  float state = 0.f;
+  constexpr int kAhead = 8;
+  for (int i0 = 0; i0 < plan.segs; i0 += kAhead) {
+    float x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int seg = min(i0 + i, plan.segs - 1);
+      x[i] = p[(run.back ? plan.segs - 1 - seg : seg) * step];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i0 + i >= plan.segs) break;
+      const int seg = run.back ? plan.segs - 1 - i0 - i : i0 + i;
+      p[seg * step] = state;
+      const DecayLink link = carry.link[seg];
+      if (link.seq < 0) continue;
+      if (link.first)
+        state = run.first.p ? run.first.p[((int64_t)link.seq * plan.hv + h) * n +
+                                          r * run.first.row + c * run.first.col]
+                            : 0.f;
+      state = fmaf(carry.factor[seg * plan.hv + h], state, x[i]);
+    }
+  }
+}
+
+struct Runs { DecayRun r[3]; };
+
+template <typename T>
+__device__ void zero_rows(const DecayPlan& plan, T* o, int dv, int h) {
+  zero_outside(plan.seq, o, plan.hv, dv, h, 0, kPitch);
+}
+
+template <typename T, int RT>
+__global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(Runs runs,
+                                                                              DecayPlan plan) {
+  constexpr int DC = 32 * RT, PI = kParts<T>, W = sizeof(T) / 2;
+  __shared__ __attribute__((aligned(16))) uint16_t lq[PI * 64 * DC];
+  __shared__ __attribute__((aligned(16))) uint16_t lk[PI * 64 * DC];
+  __shared__ __attribute__((aligned(16))) T lv[64 * kPitch];
+  __shared__ __attribute__((aligned(16))) uint16_t la[3 * 64 * 64];     // att, [part][i][j]
+  __shared__ Coef coef[2];
+  __shared__ float dots[4][64];
+  const DecayRun& run = runs.r[blockIdx.z];
+  const int seg = blockIdx.x, h = blockIdx.y;
+  if (seg >= plan.segs) {
+    if (run.o_f32) zero_rows(plan, (float*)run.o, run.dv, h);
+    else zero_rows(plan, (T*)run.o, run.dv, h);
+    return;
+  }
+  const int from = seg * plan.per, to = min(from + plan.per, plan.seq.slots);
+  const Place l;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = 32 * wave;
+  const bool live = col < run.dv;
+  Chunks chunks(plan.seq, from, to, run.back);
+  const int n = run.dc * run.dv;
+  auto empty = [&](int seq) {                 // a sequence without tokens keeps its state
+    if (!run.last.p) return;
+    const int64_t at = ((int64_t)seq * plan.hv + h) * n;
+    for (int e = threadIdx.x; e < n; e += kThreads) {
+      const int r = e / run.dv, c = e % run.dv;
+      run.last.p[at + r * run.last.row + c * run.last.col] =
+          run.first.p ? run.first.p[at + r * run.first.row + c * run.first.col] : 0.f;
+    }
+  };
+  Staged<T, DC> q, k;
+  Staged<T, kPitch> v;
+  auto load = [&](const DecayChunk& at) {
+    q.load(ChunkRows<T>(run.q, at, h, run.dc, run.vec_q, run.back));
+    k.load(ChunkRows<T>(run.k, at, h, run.dc, run.vec_k, run.back));
+    v.load(ChunkRows<T>(run.v, at, h, run.dv, run.vec_v, run.back));
+  };
+  auto put = [&]() {
+    q.put(lq);
+    k.put(lk);
+    v.put_raw(lv);
+  };
+  DecayChunk c;
+  if (!chunks.next(plan.seq, c, empty)) return;
+  load(c);
+  if (wave == 3) coefficients(plan, c, run.back, h, coef[0]);
+  Columns<RT> s;
+  if (live && !c.first) s.load(run, run.start, (int64_t)seg * plan.hv + h, col, l);
+  put();
+  __syncthreads();
+  for (int at = 0;; at ^= 1) {
+    DecayChunk next;
+    const bool more = chunks.next(plan.seq, next, empty);
+    if (more) load(next);
+    const Coef& co = coef[at];
+    if (live && c.first) s.load(run, run.first, (int64_t)c.seq * plan.hv + h, col, l);
+    if (wave < 3) {                           // att^T: the tiles (0, 0), (0, 1), (1, 1)
+      const int jt = wave >> 1, it = (wave + 1) >> 1, i = 32 * it + l.m;
+      bs_f32x16 a = zero16();
+      const int j = 32 * jt + value_row(l.m);
+#pragma unroll
+      for (int s = 0; s < DC / 16; ++s) {
+        bs_parts<PI> kp, qp;
+#pragma unroll
+        for (int p = 0; p < PI; ++p) {
+          kp.p[p] = *(const bs_bf16x8*)(lk + p * 64 * DC + place<DC>(j, 16 * s + 8 * l.g));
+          qp.p[p] = *(const bs_bf16x8*)(lq + p * 64 * DC + place<DC>(i, 16 * s + 8 * l.g));
+        }
+        a = mma(kp, qp, a);
+      }
+      const double ri = co.run[i];
+      const int j0 = 32 * jt + 16 * l.g;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int je = j0 + 8 * half + e;
+          f[e] = je <= i ? run.att_scale * exp_of(ri - co.run[je]) * a[8 * half + e] : 0.f;
+        }
+        const bs_parts<3> p = bs_split8<3>(f);
+#pragma unroll
+        for (int x = 0; x < 3; ++x)
+          *(bs_bf16x8*)(la + x * 64 * 64 + place<64>(i, j0 + 8 * half)) = p.p[x];
+      }
+    } else if (more) {
+      coefficients(plan, next, run.back, h, coef[at ^ 1]);
+    }
+    bs_f32x16 o[2] = {zero16(), zero16()};
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = s.s[i][8 * half + e];
+          const bs_parts<3> sp = bs_split8<3>(f);
+#pragma unroll
+          for (int it = 0; it < 2; ++it) {
+            bs_parts<PI> qp;
+#pragma unroll
+            for (int p = 0; p < PI; ++p)
+              qp.p[p] = *(const bs_bf16x8*)(lq + p * 64 * DC +
+                                            place<DC>(32 * it + l.m, 32 * i + 16 * half + 8 * l.g));
+            o[it] = mma(sp, qp, o[it]);
+          }
+        }
+#pragma unroll
+      for (int it = 0; it < 2; ++it) o[it] *= run.grow_scale * co.grow[32 * it + l.m];
+    }
+    __syncthreads();                          // att
+    if (live) {
+      uint4 vf[4][W];
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) turned_v<T>(lv, col, ks, l, vf[ks]);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const bs_parts<PI> vp = parts_of<T>(vf[ks]);
+#pragma unroll
+        for (int it = ks >> 1; it < 2; ++it) {
+          bs_parts<3> ap;
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+            ap.p[p] = *(const bs_bf16x8*)(la + p * 64 * 64 +
+                                          place<64>(32 * it + l.m, 16 * ks + 8 * l.g));
+          o[it] = mma(vp, ap, o[it]);
+        }
+      }
+      s.template add<T, DC>(lk, vf, co, run.add_scale, l);
+      const int oc = col + 16 * l.g;
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const int i = 32 * it + l.m;
+        if (run.dot.p) {
+          const ChunkRows<T> rows(run.dot, c, h, run.dv, run.vec_o, run.back);
+          float sum = 0.f;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint4 x[W];
+            float f[8];
+            rows.raw(i, oc + 8 * half, x);
+            floats<T>(x, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], o[it][8 * half + e], sum);
+          }
+          sum += __shfl_xor(sum, 32);
+          if (l.g == 0) dots[wave][i] = sum;
+        }
+        if (i >= c.rows) continue;
+        const int64_t row = c.batch * plan.seq.tokens + c.token + (run.back ? c.rows - 1 - i : i);
+        const int64_t base = (row * plan.hv + h) * run.dv + oc;
+        auto put_out = [&](auto* p) {
+          if (run.vec_o) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              if (oc + e < run.dv)
+                bs_store4(p + e, bs_f32x4{o[it][e], o[it][e + 1], o[it][e + 2], o[it][e + 3]});
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (oc + e < run.dv)
+                p[e] = bs_from_f32<typename std::remove_pointer<decltype(p)>::type>(o[it][e]);
+          }
+        };
+        if (run.o_f32) put_out((float*)run.o + base);
+        else put_out((T*)run.o + base);
+      }
+      if (c.last && run.last.p) {
+        float scale = 1.f;
+        if (run.back) {
+          const float g = bs_load_any(plan.g, plan.g_dtype,
+                                      bs_delta_at(plan.g_stride, c.batch, c.token, h));
+          scale = exp_of((g < BS_DELTA_G_MIN ? BS_DELTA_G_MIN : g) * kLog2e);
+        }
+        s.store(run, run.last, (int64_t)c.seq * plan.hv + h, scale, col, l);
+      }
+    }
+    __syncthreads();                          // the chunk's last readers are through
+    if (run.dot.p && threadIdx.x < c.rows) {
+      float sum = dots[0][threadIdx.x];
+      for (int w = 1; 32 * w < run.dv; ++w) sum += dots[w][threadIdx.x];
+      const int64_t row = c.batch * plan.seq.tokens + c.token +
+                          (run.back ? c.rows - 1 - (int)threadIdx.x : threadIdx.x);
+      run.dots[row * plan.hv + h] = sum;
+    }
+    if (!more) return;
+    put();
+    c = next;
+    __syncthreads();
+  }
+}
+
+// Sequences without tokens keep their states.
+__global__ __launch_bounds__(256) void keep_kernel(const float* from, float* to, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    to[i] = from ? from[i] : 0.f;
+}
+
+template <typename F>
+void by_type(int dtype, int wide, F&& f) {
+  using Two = std::integral_constant<int, 2>;
+  using Four = std::integral_constant<int, 4>;
+  auto sized = [&](auto t) {
+    if (wide) f(t, Four());
+    else f(t, Two());
+  };
+  if (dtype == BS_F32) sized(float());
+  else if (dtype == BS_BF16) sized(bs_bf16());
+  else sized(bs_f16());
+}
+
+int vectors(const DecayOperand& x, int dim, int dtype) {
+  const int per = 16 / bs_dtype_size(dtype);
+  int ok = dim % 8 == 0 && (uintptr_t)x.p % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && x.stride[i] % per == 0;
+  return ok;
+}
+
+int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+
+DecayPlan decay_plan(const bs_delta_in& in, int seqs, int tokens, const int32_t* offsets,
+                     int train) {
+  DecayPlan p;
+  p.seq = delta_plan(seqs, tokens, offsets);
+  p.hv = in.hv, p.g = in.g, p.g_dtype = in.g_dtype;
+  for (int i = 0; i < 3; ++i) p.g_stride[i] = in.g_stride[i];
+  // as many segments as the card takes workgroups at a time, of 4 chunks at least; for gradients
+  // of 16 at most, since sums over a segment's tokens are differences (decay_grad.hip)
+  const int64_t units = (int64_t)p.seq.slots * in.hv;
+  const int64_t at_once = (in.dtype == BS_BF16 ? 2 : 1) * bs_num_cus();
+  int64_t per = (units + at_once - 1) / at_once;
+  per = per < 4 ? 4 : per;
+  if (train && per > 16) per = 16;
+  p.carry = 1;
+  const int whole = (tokens + kChunk - 1) / kChunk;       // chunks of a sequence
+  if (!offsets && whole && per >= whole) {
+    per = per / whole * whole;
+    p.carry = 0;
+  }
+  if (per >= p.seq.slots) {
+    per = p.seq.slots;
+    p.carry = 0;
+  }
+  p.per = (int)per;
+  p.segs = p.seq.slots ? (int)((p.seq.slots + per - 1) / per) : 0;
+  return p;
+}
+
+int decay_check(const bs_delta_in* in, int seqs, int tokens, const int32_t* offsets,
+                const char* who) {
+  if (int rc = delta_check_chunked(in, seqs, tokens, offsets, who)) return rc;
+  BS_CHECK_ARG(in->hv <= 65535, "%s: %d heads exceed one launch", who, in->hv);
+  const int64_t slots = offsets ? (int64_t)tokens / kChunk + seqs
+                                : (int64_t)seqs * ((tokens + kChunk - 1) / kChunk);
+  BS_CHECK_ARG((slots + 1) * in->hv < 1 << 22 && (int64_t)seqs * in->hv < 1 << 22,
+               "%s: %d sequences of %d tokens, %d heads exceed one launch", who, seqs, tokens,
+               in->hv);
+  return BS_OK;
+}
+
+DecayRun decay_run(const bs_delta_in& in, const DecayOperand& q, const DecayOperand& k,
+                   const DecayOperand& v, int dc, int dv) {
+  DecayRun r = {};
+  r.q = q, r.k = k, r.v = v, r.dc = dc, r.dv = dv;
+  r.dot = DecayOperand{nullptr, {0, 0, 0}, 1};
+  r.first = r.last = r.start = DecayState{nullptr, dv, 1};
+  r.vec_q = vectors(q, dc, in.dtype), r.vec_k = vectors(k, dc, in.dtype);
+  r.vec_v = vectors(v, dv, in.dtype);
+  r.att_scale = r.grow_scale = in.scale, r.add_scale = 1.f;
+  return r;
+}
+
+int64_t decay_carry_bytes(const bs_delta_in& in, const DecayPlan& plan) {
+  if (!plan.carry) return 0;
+  return align16((int64_t)plan.segs * in.hv * 4) + align16((int64_t)plan.segs * sizeof(DecayLink));
+}
+
+void decay_carry(const DecayRun& run, const DecayPlan& plan, int dtype, void* scratch,
+                 hipStream_t st) {
+  Carry c;
+  c.factor = (float*)scratch;
+  c.link = (DecayLink*)((char*)scratch + align16((int64_t)plan.segs * plan.hv * 4));
+  by_type(dtype, run.dc > 64, [&](auto t, auto rt) {
+    sum_kernel<decltype(t), rt.value><<<dim3(plan.segs, plan.hv), kThreads, 0, st>>>(run, plan, c);
+  });
+  scan_kernel<<<dim3((run.dc * run.dv + 255) / 256, plan.hv), 256, 0, st>>>(run, plan, c);
+}
+
+void decay_walk(const DecayRun* runs, int n, const DecayPlan& plan, int dtype, hipStream_t st) {
+  Runs r = {};
+  int wide = 0;
+  for (int i = 0; i < n; ++i) {
+    r.r[i] = runs[i];
+    wide |= runs[i].dc > 64;
+  }
+  const dim3 grid(plan.segs + (plan.seq.offsets ? 1 : 0), plan.hv, n);
+  if (grid.x == 0) return;
+  by_type(dtype, wide, [&](auto t, auto rt) {
+    walk_kernel<decltype(t), rt.value><<<grid, kThreads, 0, st>>>(r, plan);
+  });
+}
+
+extern "C" size_t bs_decay_attention_segments(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                                              int32_t packed, int32_t train) {
+  static const int32_t dummy[1] = {0};
+  const int32_t* off = packed ? dummy : nullptr;
+  if (decay_check(in, seqs, tokens, off, "bs_decay_attention_segments")) return 0;
+  const DecayPlan p = decay_plan(*in, seqs, tokens, off, train);
+  return p.carry ? (size_t)p.segs : 0;
+}
+
+extern "C" size_t bs_decay_attention_workspace_size(const bs_delta_in* in, int32_t seqs,
+                                                    int32_t tokens, int32_t packed,
+                                                    int32_t train) {
+  static const int32_t dummy[1] = {0};
+  const int32_t* off = packed ? dummy : nullptr;
+  if (decay_check(in, seqs, tokens, off, "bs_decay_attention_workspace_size")) return 0;
+  const DecayPlan p = decay_plan(*in, seqs, tokens, off, train);
+  int64_t bytes = decay_carry_bytes(*in, p);
+  if (p.carry && !train) bytes += align16((int64_t)p.segs * in->hv * in->dk * in->dv * 4);
+  return (size_t)bytes;
+}
+
+extern "C" int bs_decay_attention(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                                  const int32_t* seq_offsets, const float* initial_state,
+                                  float* final_state, void* o, float* kept_states, int32_t train,
+                                  void* workspace, size_t workspace_bytes, bs_stream_t stream) {
+  static const char* who = "bs_decay_attention";
+  if (int rc = decay_check(in, seqs, tokens, seq_offsets, who)) return rc;
+  if (seqs == 0 && !seq_offsets) return BS_OK;
+  const DecayPlan plan = decay_plan(*in, seqs, tokens, seq_offsets, train);
+  const size_t need =
+      bs_decay_attention_workspace_size(in, seqs, tokens, seq_offsets != nullptr, train);
+  BS_CHECK_ARG(tokens == 0 || (in->q && in->k && in->v && in->g && o), "%s: NULL pointer", who);
+  BS_CHECK_ARG(!train || !plan.carry || kept_states, "%s: kept_states is NULL", who);
+  BS_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
+               "%s: workspace of %zu bytes needed, %zu given", who, need,
+               workspace ? workspace_bytes : (size_t)0);
+  hipStream_t st = bs_stream(stream);
+  const int64_t states = (int64_t)seqs * in->hv * in->dk * in->dv;
+  if (plan.seq.slots == 0) {
+    if (final_state && states) {
+      const int64_t blocks = (states + 255) / 256;
+      keep_kernel<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, st>>>(
+          initial_state, final_state, states);
+      BS_CHECK_LAUNCH();
+    }
+    if (!seq_offsets || tokens == 0) return BS_OK;
+  }
+  const int group = in->hv / in->hk;
+  auto op = [](const void* p, const int64_t* s, int rep) {
+    return DecayOperand{p, {s[0], s[1], s[2]}, rep};
+  };
+  DecayRun run = decay_run(*in, op(in->q, in->q_stride, group), op(in->k, in->k_stride, group),
+                           op(in->v, in->v_stride, 1), in->dk, in->dv);
+  run.o = o;
+  run.vec_o = in->dv % 4 == 0 && (uintptr_t)o % (4 * bs_dtype_size(in->dtype)) == 0;
+  run.first.p = const_cast<float*>(initial_state);
+  run.last.p = final_state;
+  if (plan.carry) {
+    run.start.p = train ? kept_states
+                        : (float*)((char*)workspace + decay_carry_bytes(*in, plan));
+    decay_carry(run, plan, in->dtype, workspace, st);
+    BS_CHECK_LAUNCH();
+  }
+  decay_walk(&run, 1, plan, in->dtype, st);
+  BS_CHECK_LAUNCH();
+  return BS_OK;
+}

@@ -799,5 +799,6 @@ def ctypes_ref(s):
     return ctypes.byref(s)
 
 
+from ._decay import decay_attention, decay_attention_step  # noqa: E402,F401
 from ._sequence import (gated_delta_rule, gated_delta_step,  # noqa: E402,F401
                         int8_linear, int8_matmul, int8_quantize, norm_gate_residual)

@@ -588,6 +588,31 @@ BS_API int bs_gated_delta_rule_grad(const bs_delta_in* in, int32_t seqs, int32_t
                                     void* dbeta, float* dstate, void* workspace,
                                     size_t workspace_bytes, bs_stream_t stream);
 
+/* ---------------------------------------------------------------- decay attention
+ * Linear attention whose state fades at a rate of its own for each head (no counterpart in the
+ * reference):
+ *   S = exp(g) S + k v^T,  o = scale S^T q.
+ * Operands as for the gated delta rule, beta unused; g [.., hv], or one value for each head with
+ * batch and token strides of 0.
+ *
+ * Tokens of running sequences, o [batch, tokens, hv, dv]; state and slots as in
+ * bs_gated_delta_step. */
+BS_API int bs_decay_attention_step(const bs_delta_in* in, int32_t batch, int32_t tokens,
+                                   float* state, int64_t n_states, const int32_t* slots, void* o,
+                                   bs_stream_t stream);
+
+/* Whole sequences, over chunks of 64 tokens; sequences, seq_offsets and states as in
+ * bs_gated_delta_rule.  With `train`, kept_states [bs_decay_attention_segments, hv, dk, dv] is
+ * written for the backward pass (NULL where that is 0). */
+BS_API size_t bs_decay_attention_segments(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                                          int32_t packed, int32_t train);
+BS_API size_t bs_decay_attention_workspace_size(const bs_delta_in* in, int32_t seqs,
+                                                int32_t tokens, int32_t packed, int32_t train);
+BS_API int bs_decay_attention(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                              const int32_t* seq_offsets, const float* initial_state,
+                              float* final_state, void* o, float* kept_states, int32_t train,
+                              void* workspace, size_t workspace_bytes, bs_stream_t stream);
+
 /* ---------------------------------------------------------------- norms around a block
  * Over rows of `dim` values (1..16384), with r(x) = (mean x^2 + eps)^-1/2 (no counterpart in
  * the reference):

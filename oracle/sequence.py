@@ -47,6 +47,43 @@ def gated_delta(q, k, v, g, beta, scale=None, state=None, grad_o=None, grad_stat
     return (o, s), (fold(dqh), fold(dkh), dvv, dg, db, ds)
 
 
+def decay_attention(q, k, v, g, scale=None, state=None, grad_o=None, grad_state=None):
+    """One sequence through decay attention, token by token: q, k [T, Hk, dk], v [T, H, dv], g [T, H]
+    or [H], state [H, dk, dv].  -> (o, final state), and with ``grad_o`` (and ``grad_state``) the
+    gradients (dq, dk, dv, dg, dstate) of their weighted sum."""
+    q, k, v, g = (np.asarray(x, np.float64) for x in (q, k, v, g))
+    T, hk, dk = q.shape
+    h, dv = v.shape[1:]
+    group, each = h // hk, g.ndim == 2
+    g = np.broadcast_to(g, (T, h))
+    scale = dk ** -0.5 if scale is None else scale
+    s = np.zeros((h, dk, dv)) if state is None else np.asarray(state, np.float64).copy()
+    qh, kh = np.repeat(q, group, 1), np.repeat(k, group, 1)
+    o, kept = np.zeros_like(v), []
+    for t in range(T):
+        kept.append(s)
+        with np.errstate(under='ignore'):
+            s = np.exp(g[t])[:, None, None] * s + kh[t][:, :, None] * v[t][:, None]
+        o[t] = scale * np.einsum('hde,hd->he', s, qh[t])
+    if grad_o is None:
+        return o, s
+    do = np.asarray(grad_o, np.float64)
+    ds = np.zeros_like(s) if grad_state is None else np.asarray(grad_state, np.float64).copy()
+    dqh, dkh = np.zeros_like(qh), np.zeros_like(kh)
+    dvv, dg = np.zeros_like(v), np.zeros((T, h))
+    for t in reversed(range(T)):
+        decay = np.exp(g[t])[:, None, None]
+        old = decay * kept[t]
+        st = old + kh[t][:, :, None] * v[t][:, None]
+        dqh[t] = scale * np.einsum('hde,he->hd', st, do[t])
+        ds = ds + scale * qh[t][:, :, None] * do[t][:, None]
+        dkh[t], dvv[t] = np.einsum('hde,he->hd', ds, v[t]), np.einsum('hde,hd->he', ds, kh[t])
+        dg[t] = (ds * old).sum((1, 2))
+        ds = decay * ds
+    fold = lambda x: x.reshape(T, hk, group, dk).sum(2)                       # noqa: E731
+    return (o, s), (fold(dqh), fold(dkh), dvv, dg if each else dg.sum(0), ds)
+
+
 def norm_gate_residual(y, post=None, gate=None, scale=None, residual=None, pre=None, eps=1e-6,
                        grad_stream=None, grad_normed=None):
     """Norm, gate, scale, residual and the next norm over rows [R, D] -> (stream, normed or None),
