@@ -76,16 +76,15 @@ def decay_attention_step(q, k, v, g, state, slots=None, scale=None):
     else:
         slots = slots.contiguous()
     o = torch.empty((b, t, hv, dv), dtype=q.dtype, device=q.device)
-    N.check(N.lib().bs_decay_attention_step(packed, b, t, _address(state), state.shape[0],
-                                            _address(slots), _address(o),
-                                            N.raw_stream(q.device)),
-            'bs_decay_attention_step')
+    N.call('bs_decay_attention_step', q.device, packed, b, t, _address(state), state.shape[0],
+           _address(slots), _address(o))
     torch.autograd.graph.increment_version(state)     # autograd does not see the kernel's stores
     return o.squeeze(1) if one else o
 
 
-def _forward(q, k, v, g, scale, initial_state, seq_offsets, train):
-    """(o, final state, the segments' states that the backward pass starts from)."""
+def _forward(q, k, v, g, scale, initial_state, seq_offsets, keep):
+    """(o, final state, what the backward pass needs of it: ``keep`` 0 nothing, 1 without the
+    gradient of g, 2 with it)."""
     held, packed, (b, t, hk, hv, dk, dv) = _operands(q, k, v, g, scale)
     dev = q.device
     n = b
@@ -103,16 +102,57 @@ def _forward(q, k, v, g, scale, initial_state, seq_offsets, train):
     o = torch.empty((b, t, hv, dv), dtype=q.dtype, device=dev)
     final = torch.empty((n, hv, dk, dv), dtype=torch.float32, device=dev)
     lib, is_packed = N.lib(), seq_offsets is not None
-    kept = None
-    if train:
-        segs = lib.bs_decay_attention_segments(packed, n, t, is_packed, True)
-        kept = torch.empty((segs, hv, dk, dv), dtype=torch.float32, device=dev) if segs else None
-    nbytes = lib.bs_decay_attention_workspace_size(packed, n, t, is_packed, train)
+    nbytes = lib.bs_decay_attention_kept_size(packed, n, t, is_packed, keep)
+    kept = torch.empty(nbytes, dtype=torch.uint8, device=dev) if keep else None
+    nbytes = lib.bs_decay_attention_workspace_size(packed, n, t, is_packed, keep)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    N.check(lib.bs_decay_attention(
-        packed, n, t, _address(seq_offsets), _address(initial_state), _address(final), _address(o),
-        _address(kept), train, _address(ws), nbytes, N.raw_stream(dev)), 'bs_decay_attention')
+    N.call('bs_decay_attention', dev, packed, n, t, _address(seq_offsets), _address(initial_state),
+           _address(final), _address(o), _address(kept), keep, _address(ws), nbytes)
     return o, final, kept
+
+
+class _DecayAttention(torch.autograd.Function):
+    """decay_attention with its gradients, formed from the operands and the states between the
+    forward pass's segments."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, initial_state, scale, seq_offsets):
+        o, final, kept = _forward(q, k, v, g, scale, initial_state, seq_offsets,
+                                  2 if ctx.needs_input_grad[3] else 1)
+        ctx.save_for_backward(q, k, v, g, initial_state, seq_offsets, kept)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return o, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go, gstate):
+        _recorded('decay_attention', go, gstate)
+        *x, initial_state, seq_offsets, kept = ctx.saved_tensors
+        held, packed = _pack(*x, ctx.scale)
+        (b, t, hk, dk), (hv, dv) = x[0].shape, x[2].shape[2:]
+        dev = x[0].device
+        n = b
+        if seq_offsets is not None:
+            seq_offsets, n = seq_offsets.contiguous(), seq_offsets.numel() - 1
+        if initial_state is not None:
+            initial_state = initial_state.contiguous()
+        go = torch.zeros(x[2].shape, dtype=x[2].dtype, device=dev) if go is None else \
+            go.contiguous()
+        gstate = None if gstate is None else gstate.contiguous()
+        decays = ctx.needs_input_grad[3]
+        grads = [torch.empty(y.shape, dtype=y.dtype, device=dev) for y in x[:3 + decays]]
+        ds = torch.empty((n, hv, dk, dv), dtype=torch.float32, device=dev) \
+            if ctx.needs_input_grad[4] else None
+        nbytes = N.lib().bs_decay_attention_grad_workspace_size(
+            packed, n, t, seq_offsets is not None, decays)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        if not decays:
+            grads.append(None)
+        N.call('bs_decay_attention_grad', dev, packed, n, t, _address(seq_offsets), _address(go),
+               _address(gstate), _address(initial_state), _address(kept),
+               *(_address(y) for y in grads), x[3].dim() == 1, _address(ds), _address(ws), nbytes)
+        return (*grads, ds, None, None)
 
 
 def decay_attention(q, k, v, g, scale=None, initial_state=None, seq_offsets=None):
@@ -124,5 +164,7 @@ def decay_attention(q, k, v, g, scale=None, initial_state=None, seq_offsets=None
     zeros.  With ``seq_offsets`` (int32 [sequences + 1], ascending) the sequences are packed end to
     end into one batch row; tokens outside all of them give 0.  Differentiable in everything but
     ``seq_offsets``, in reverse mode."""
+    if _recorded('decay_attention', q, k, v, g, initial_state, seq_offsets):
+        return _DecayAttention.apply(q, k, v, g, initial_state, scale, seq_offsets)
     o, final, _ = _forward(q, k, v, g, scale, initial_state, seq_offsets, False)
     return o, final

@@ -169,10 +169,13 @@ SIGNATURES = {
                                                                                    c_vp]),
     'bs_decay_attention_step': (ctypes.c_int, [c_vp, c_i32, c_i32, c_vp, ctypes.c_int64, c_vp,
                                                c_vp, c_vp]),
-    'bs_decay_attention_segments': (c_size, [c_vp, c_i32, c_i32, c_i32, c_i32]),
+    'bs_decay_attention_kept_size': (c_size, [c_vp, c_i32, c_i32, c_i32, c_i32]),
     'bs_decay_attention_workspace_size': (c_size, [c_vp, c_i32, c_i32, c_i32, c_i32]),
     'bs_decay_attention': (ctypes.c_int, [c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32,
                                           c_vp, c_size, c_vp]),
+    'bs_decay_attention_grad_workspace_size': (c_size, [c_vp, c_i32, c_i32, c_i32, c_i32]),
+    'bs_decay_attention_grad': (ctypes.c_int, [c_vp, c_i32, c_i32] + [c_vp] * 9 + [
+        c_i32, c_vp, c_vp, c_size, c_vp]),
     'bs_norm_gate_residual': (ctypes.c_int, [c_vp] * 4),
     'bs_norm_grad_workspace_size': (c_size, [ctypes.c_int64, c_i32]),
     'bs_norm_gate_residual_grad': (ctypes.c_int, [c_vp] * 10 + [c_size, c_vp]),
@@ -253,3 +256,16 @@ def raw_stream(device=None):
 
 def stream_handle(device=None):
     return ctypes.c_void_p(raw_stream(device))
+
+
+def call(name, device, *args):
+    """Entry point ``name`` on the current stream of ``device``, which need not be the current
+    device."""
+    import torch
+    f = getattr(lib(), name)
+    if device.index is None or device.index == torch.cuda.current_device():
+        rc = f(*args, raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = f(*args, raw_stream(device))
+    check(rc, name)

@@ -26,13 +26,20 @@ struct DecayState {           // element (r, c) of sequence or segment n's state
 
 struct DecayRun {
   DecayOperand q, k, v;
-  DecayOperand dot;           // rows like o's whose product with them goes to dots, or p = NULL
+  DecayOperand dot;           // rows like o's whose product with o's first term goes to dots, or
+                              // p = NULL
   DecayState first;           // states before the sequences, p = NULL for zeros
   DecayState last;            // and after them, p = NULL if not wanted
   DecayState start;           // states before the segments that go on with a sequence
   void* o;                    // [.., hv, dv] of the operands' type, or in 32 bits (o_f32)
-  float* dots;                // [batch, tokens, hv]
-  int dc, dv, back, o_f32, vec_q, vec_k, vec_v, vec_o;
+  double* dots;               // [hv][rows], rows of all sequences
+  int pairs;                  // dots have the second term's too, less what it gives as key: with
+                              // P_ij = att_ij (dot_i.v_j), sum_j P_ij - sum_j P_ji
+  float* save;                // states before the chunks but a sequence's first, see decay_saved;
+  const float* saved;         // from the last token to the first: the ones that a run has saved,
+  float* edge;                // [slots][hv]: and their product with the state at a chunk's end
+  int64_t rows;
+  int dc, dv, back, o_f32, vec_q, vec_k, vec_v, vec_dot, vec_o;
   float att_scale, grow_scale, add_scale;
 };
 
@@ -55,16 +62,24 @@ struct DecayLink {
 // A chunk: sequence, batch row, its first token and rows, and whether it is the sequence's first
 // or last in processing order.
 struct DecayChunk {
-  int seq, rows, first, last;
+  int seq, slot, rows, first, last;
   int64_t batch, token;
   int next_g;                 // back: whether a token follows the chunk in its sequence
 };
 
-DecayPlan decay_plan(const bs_delta_in& in, int seqs, int tokens, const int32_t* offsets,
-                     int train);
+// Values of a saved state: its columns in tiles of 32, in the order of the registers.
+static inline __host__ __device__ int decay_saved(int dc, int dv) {
+  return (dc + 31) / 32 * ((dv + 31) / 32) * 1024;
+}
+
+DecayPlan decay_plan(const bs_delta_in& in, int seqs, int tokens, const int32_t* offsets);
 int decay_check(const bs_delta_in* in, int seqs, int tokens, const int32_t* offsets,
                 const char* who);
-// States, decays and links of the segments: the workspace of one run's carry.
+// What the forward call keeps for the gradients: the segments' states and, for those of the decays,
+// a state a chunk (at decay_kept_saved); `keep` is enum-like: 0 nothing, 1 without them, 2 with.
+int64_t decay_kept_bytes(const bs_delta_in& in, const DecayPlan& plan, int keep);
+float* decay_kept_saved(const bs_delta_in& in, const DecayPlan& plan, void* kept);
+// Decays and links of the segments: the workspace of one run's carry.
 int64_t decay_carry_bytes(const bs_delta_in& in, const DecayPlan& plan);
 // Fills run.start (sums, then their scan over the segments); `scratch` holds decays and links.
 void decay_carry(const DecayRun& run, const DecayPlan& plan, int dtype, void* scratch,
@@ -72,4 +87,6 @@ void decay_carry(const DecayRun& run, const DecayPlan& plan, int dtype, void* sc
 // The walks, all in one launch.
 void decay_walk(const DecayRun* runs, int n, const DecayPlan& plan, int dtype, hipStream_t st);
 DecayRun decay_run(const bs_delta_in& in, const DecayOperand& q, const DecayOperand& k,
-                   const DecayOperand& v, int dc, int dv);
+                   const DecayOperand& v, const DecayOperand& dot, int dc, int dv);
+// Copies n floats, zeros from NULL.
+void decay_keep(const float* from, float* to, int64_t n, hipStream_t st);

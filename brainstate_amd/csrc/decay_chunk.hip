@@ -16,6 +16,7 @@
 // Numbers: the state and all sums are 32-bit; products take 32-bit operands as three exact bf16
 // parts (lane_types.h).  Sums of log decays are 64-bit, since their differences are exponents.
 #include "decay.h"
+#include "decay_slots.h"
 
 namespace {
 
@@ -202,51 +203,6 @@ __device__ __forceinline__ double coefficients(const DecayPlan& p, const DecayCh
   return total;
 }
 
-// The slots of a segment in processing order, those with a chunk.
-struct Chunks {
-  int slot, end, step, back;
-  DeltaSpan span;
-  __device__ __forceinline__ Chunks(const DeltaPlan& p, int from, int to, int b) {
-    back = b, step = b ? -1 : 1;
-    slot = b ? to - 1 : from;
-    end = b ? from - 1 : to;
-    span.slot = -1, span.chunks = 0;
-  }
-  // `empty`: called for a sequence without tokens
-  template <typename F>
-  __device__ __forceinline__ bool next(const DeltaPlan& p, DecayChunk& c, F&& empty) {
-    for (; slot != end; slot += step) {
-      if (slot < span.slot || slot >= span.slot + span.chunks) {
-        span = delta_span(p, delta_owner(p, slot));
-        if (span.chunks == 0 && slot == span.slot) empty(span.seq);
-      }
-      const int k = slot - span.slot;
-      if (k < 0 || k >= span.chunks) continue;
-      c.seq = span.seq, c.batch = span.batch;
-      c.token = span.first + (int64_t)k * kChunk;
-      c.rows = min(span.len - k * kChunk, kChunk);
-      c.next_g = k < span.chunks - 1;
-      c.first = back ? k == span.chunks - 1 : k == 0;
-      c.last = back ? k == 0 : k == span.chunks - 1;
-      slot += step;
-      return true;
-    }
-    return false;
-  }
-};
-
-// What the segment [from, to) leaves to the next one, and the slots it takes.
-__device__ __forceinline__ DecayLink link_of(const DeltaPlan& p, int back, int& from, int& to) {
-  const int edge = back ? from : to - 1;
-  const DeltaSpan s = delta_span(p, delta_owner(p, edge));
-  const int k = edge - s.slot;
-  if (k < 0 || k >= s.chunks || k == (back ? 0 : s.chunks - 1)) return {-1, 0};
-  const int first = back ? s.slot + s.chunks <= to : s.slot >= from;
-  if (back) to = min(to, s.slot + s.chunks);
-  else from = max(from, s.slot);
-  return {s.seq, first};
-}
-
 struct Place {                   // a lane's place in the products of 32 x 32
   int m, g, x, y, half;
   __device__ __forceinline__ Place() {
@@ -315,6 +271,38 @@ struct Columns {
     float* p = st.p + at * r.dc * r.dv;
     each(r, col, l,
          [&](int i, int e, int d, int c) { p[d * st.row + c * st.col] = scale * s[i][e]; });
+  }
+  // as saved states lie: tile by tile, 4 values of a lane side by side
+  static __device__ __forceinline__ int64_t saved_at(const DecayRun& r, int64_t slot_head, int wave) {
+    return slot_head * decay_saved(r.dc, r.dv) + wave * ((r.dc + 31) / 32 * 1024) +
+           (threadIdx.x & 63) * 4;
+  }
+  __device__ __forceinline__ void save(const DecayRun& r, int64_t slot_head, int wave) const {
+    float* p = r.save + saved_at(r, slot_head, wave);
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+      if (32 * i < r.dc) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *(float4*)(p + (4 * i + e) * 256) = make_float4(s[i][4 * e], s[i][4 * e + 1],
+                                                          s[i][4 * e + 2], s[i][4 * e + 3]);
+      }
+  }
+  // this lane's part of the product with a saved state
+  __device__ __forceinline__ float product(const DecayRun& r, int64_t slot_head, int wave) const {
+    const float* p = r.saved + saved_at(r, slot_head, wave);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+      if (32 * i < r.dc) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 x = *(const float4*)(p + (4 * i + e) * 256);
+          sum = fmaf(x.x, s[i][4 * e], sum), sum = fmaf(x.y, s[i][4 * e + 1], sum);
+          sum = fmaf(x.z, s[i][4 * e + 2], sum), sum = fmaf(x.w, s[i][4 * e + 3], sum);
+        }
+      }
+    return sum;
   }
   // s = decay s + K^T (left V) with V's turned fragments of 16 tokens each
   template <typename T, int DC>
@@ -442,7 +430,41 @@ __device__ void zero_rows(const DecayPlan& plan, T* o, int dv, int h) {
   zero_outside(plan.seq, o, plan.hv, dv, h, 0, kPitch);
 }
 
-template <typename T, int RT>
+// sum_j P_ij for row i and sum_i P_ij for column j of a 32 x 32 tile, of which a lane has 16 j of
+// one i: the first in lane i of either group, the second of j = 16 g + m / 2.
+__device__ __forceinline__ void pair_sums(const float* p, const Place& l, double& row,
+                                          double& col) {
+  double v[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = p[e];
+  row = 0.0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) row += v[e];
+  row += __shfl_xor(row, 32);
+#pragma unroll
+  for (int w = 8; w >= 1; w >>= 1) {     // lanes 2 w apart share out their values
+    const bool up = l.m & 2 * w;
+#pragma unroll
+    for (int k = 0; k < w; ++k) {
+      const double mine = up ? v[k + w] : v[k], other = up ? v[k] : v[k + w];
+      v[k] = mine + __shfl_xor(other, 2 * w);
+    }
+  }
+  col = v[0] + __shfl_xor(v[0], 1);
+}
+
+// 8 values of a row of V as it lies in LDS.
+template <typename T>
+__device__ __forceinline__ void straight_v(const T* v, int row, int d, uint4* x) {
+  if constexpr (sizeof(T) == 2) {
+    x[0] = *(const uint4*)((const uint16_t*)v + place<kPitch>(row, d));
+  } else {
+    x[0] = *(const uint4*)(v + row * kPitch + d);
+    x[1] = *(const uint4*)(v + row * kPitch + d + 4);
+  }
+}
+
+template <typename T, int RT, bool GRAD>
 __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(Runs runs,
                                                                               DecayPlan plan) {
   constexpr int DC = 32 * RT, PI = kParts<T>, W = sizeof(T) / 2;
@@ -451,7 +473,9 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
   __shared__ __attribute__((aligned(16))) T lv[64 * kPitch];
   __shared__ __attribute__((aligned(16))) uint16_t la[3 * 64 * 64];     // att, [part][i][j]
   __shared__ Coef coef[2];
-  __shared__ float dots[4][64];
+  __shared__ float dots[GRAD ? 4 : 1][64];
+  __shared__ float edge[4];
+  __shared__ double sums[GRAD ? 3 : 1][2][32];       // of P's tiles
   const DecayRun& run = runs.r[blockIdx.z];
   const int seg = blockIdx.x, h = blockIdx.y;
   if (seg >= plan.segs) {
@@ -516,23 +540,44 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
       }
       const double ri = co.run[i];
       const int j0 = 32 * jt + 16 * l.g;
+      float w[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        w[e] = j0 + e <= i ? run.att_scale * exp_of(ri - co.run[j0 + e]) * a[e] : 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float f[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int je = j0 + 8 * half + e;
-          f[e] = je <= i ? run.att_scale * exp_of(ri - co.run[je]) * a[8 * half + e] : 0.f;
-        }
-        const bs_parts<3> p = bs_split8<3>(f);
+        const bs_parts<3> p = bs_split8<3>(w + 8 * half);
 #pragma unroll
         for (int x = 0; x < 3; ++x)
           *(bs_bf16x8*)(la + x * 64 * 64 + place<64>(i, j0 + 8 * half)) = p.p[x];
+      }
+      if (GRAD && run.pairs) {
+        const ChunkRows<T> rows(run.dot, c, h, run.dv, run.vec_dot, run.back);
+        a = zero16();
+        for (int d = 8 * l.g; d - 8 * l.g < run.dv; d += 16) {
+          uint4 x[W], y[W];
+          rows.raw(i, d, x);
+          straight_v(lv, j, d, y);
+          a = mma(parts_of<T>(y), parts_of<T>(x), a);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] *= a[e];
+        double row, column;
+        pair_sums(w, l, row, column);
+        if (l.g == 0) sums[wave][0][l.m] = row;
+        if (!(l.m & 1)) sums[wave][1][16 * l.g + l.m / 2] = column;
       }
     } else if (more) {
       coefficients(plan, next, run.back, h, coef[at ^ 1]);
     }
     bs_f32x16 o[2] = {zero16(), zero16()};
+    if (!GRAD && live && run.save && !c.first) s.save(run, (int64_t)c.slot * plan.hv + h, wave);
+    if (GRAD && live && run.saved && !c.first) {
+      float sum = s.product(run, (int64_t)(c.slot + 1) * plan.hv + h, wave);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+      if ((threadIdx.x & 63) == 0) edge[wave] = sum;
+    }
     if (live) {
 #pragma unroll
       for (int i = 0; i < RT; ++i)
@@ -553,7 +598,25 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
           }
         }
 #pragma unroll
-      for (int it = 0; it < 2; ++it) o[it] *= run.grow_scale * co.grow[32 * it + l.m];
+      for (int it = 0; it < 2; ++it) {
+        const int i = 32 * it + l.m;
+        o[it] *= run.grow_scale * co.grow[i];
+        if (GRAD && run.dot.p) {
+          const ChunkRows<T> rows(run.dot, c, h, run.dv, run.vec_dot, run.back);
+          float sum = 0.f;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint4 x[W];
+            float f[8];
+            rows.raw(i, col + 16 * l.g + 8 * half, x);
+            floats<T>(x, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], o[it][8 * half + e], sum);
+          }
+          sum += __shfl_xor(sum, 32);
+          if (l.g == 0) dots[wave][i] = sum;
+        }
+      }
     }
     __syncthreads();                          // att
     if (live) {
@@ -578,21 +641,6 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
         const int i = 32 * it + l.m;
-        if (run.dot.p) {
-          const ChunkRows<T> rows(run.dot, c, h, run.dv, run.vec_o, run.back);
-          float sum = 0.f;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint4 x[W];
-            float f[8];
-            rows.raw(i, oc + 8 * half, x);
-            floats<T>(x, f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], o[it][8 * half + e], sum);
-          }
-          sum += __shfl_xor(sum, 32);
-          if (l.g == 0) dots[wave][i] = sum;
-        }
         if (i >= c.rows) continue;
         const int64_t row = c.batch * plan.seq.tokens + c.token + (run.back ? c.rows - 1 - i : i);
         const int64_t base = (row * plan.hv + h) * run.dv + oc;
@@ -623,12 +671,21 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
       }
     }
     __syncthreads();                          // the chunk's last readers are through
-    if (run.dot.p && threadIdx.x < c.rows) {
-      float sum = dots[0][threadIdx.x];
-      for (int w = 1; 32 * w < run.dv; ++w) sum += dots[w][threadIdx.x];
-      const int64_t row = c.batch * plan.seq.tokens + c.token +
-                          (run.back ? c.rows - 1 - (int)threadIdx.x : threadIdx.x);
-      run.dots[row * plan.hv + h] = sum;
+    if (GRAD && run.dot.p && threadIdx.x < c.rows) {
+      const int i = threadIdx.x, m = i & 31;
+      double sum = dots[0][i];
+      for (int w = 1; 32 * w < run.dv; ++w) sum += dots[w][i];
+      if (run.pairs)
+        sum += i < 32 ? sums[0][0][m] - sums[0][1][m] - sums[1][1][m]
+                      : sums[1][0][m] + sums[2][0][m] - sums[2][1][m];
+      const int64_t row = c.batch * plan.seq.tokens + c.token + (run.back ? c.rows - 1 - i : i);
+      run.dots[(int64_t)h * run.rows + row] = sum;
+    }
+    if (GRAD && run.saved && !c.first && threadIdx.x == 0) {
+      float sum = edge[0];
+      for (int w = 1; 32 * w < run.dv; ++w) sum += edge[w];
+      // the decay of the next chunk's first token stands between
+      run.edge[(int64_t)c.slot * plan.hv + h] = co.grow[0] * sum;
     }
     if (!more) return;
     put();
@@ -667,19 +724,16 @@ int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
 
 }  // namespace
 
-DecayPlan decay_plan(const bs_delta_in& in, int seqs, int tokens, const int32_t* offsets,
-                     int train) {
+DecayPlan decay_plan(const bs_delta_in& in, int seqs, int tokens, const int32_t* offsets) {
   DecayPlan p;
   p.seq = delta_plan(seqs, tokens, offsets);
   p.hv = in.hv, p.g = in.g, p.g_dtype = in.g_dtype;
   for (int i = 0; i < 3; ++i) p.g_stride[i] = in.g_stride[i];
-  // as many segments as the card takes workgroups at a time, of 4 chunks at least; for gradients
-  // of 16 at most, since sums over a segment's tokens are differences (decay_grad.hip)
+  // as many segments as the card takes workgroups at a time, of 4 chunks at least
   const int64_t units = (int64_t)p.seq.slots * in.hv;
   const int64_t at_once = (in.dtype == BS_BF16 ? 2 : 1) * bs_num_cus();
   int64_t per = (units + at_once - 1) / at_once;
   per = per < 4 ? 4 : per;
-  if (train && per > 16) per = 16;
   p.carry = 1;
   const int whole = (tokens + kChunk - 1) / kChunk;       // chunks of a sequence
   if (!offsets && whole && per >= whole) {
@@ -708,10 +762,10 @@ int decay_check(const bs_delta_in* in, int seqs, int tokens, const int32_t* offs
 }
 
 DecayRun decay_run(const bs_delta_in& in, const DecayOperand& q, const DecayOperand& k,
-                   const DecayOperand& v, int dc, int dv) {
+                   const DecayOperand& v, const DecayOperand& dot, int dc, int dv) {
   DecayRun r = {};
-  r.q = q, r.k = k, r.v = v, r.dc = dc, r.dv = dv;
-  r.dot = DecayOperand{nullptr, {0, 0, 0}, 1};
+  r.q = q, r.k = k, r.v = v, r.dot = dot, r.dc = dc, r.dv = dv;
+  r.vec_dot = vectors(dot, dv, in.dtype);
   r.first = r.last = r.start = DecayState{nullptr, dv, 1};
   r.vec_q = vectors(q, dc, in.dtype), r.vec_k = vectors(k, dc, in.dtype);
   r.vec_v = vectors(v, dv, in.dtype);
@@ -736,6 +790,7 @@ void decay_carry(const DecayRun& run, const DecayPlan& plan, int dtype, void* sc
 }
 
 void decay_walk(const DecayRun* runs, int n, const DecayPlan& plan, int dtype, hipStream_t st) {
+  const bool grad = n > 1;     // the gradients' walks, else the forward one
   Runs r = {};
   int wide = 0;
   for (int i = 0; i < n; ++i) {
@@ -745,43 +800,57 @@ void decay_walk(const DecayRun* runs, int n, const DecayPlan& plan, int dtype, h
   const dim3 grid(plan.segs + (plan.seq.offsets ? 1 : 0), plan.hv, n);
   if (grid.x == 0) return;
   by_type(dtype, wide, [&](auto t, auto rt) {
-    walk_kernel<decltype(t), rt.value><<<grid, kThreads, 0, st>>>(r, plan);
+    if (grad) walk_kernel<decltype(t), rt.value, true><<<grid, kThreads, 0, st>>>(r, plan);
+    else walk_kernel<decltype(t), rt.value, false><<<grid, kThreads, 0, st>>>(r, plan);
   });
 }
 
-extern "C" size_t bs_decay_attention_segments(const bs_delta_in* in, int32_t seqs, int32_t tokens,
-                                              int32_t packed, int32_t train) {
+void decay_keep(const float* from, float* to, int64_t n, hipStream_t st) {
+  const int64_t blocks = (n + 255) / 256;
+  keep_kernel<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, st>>>(from, to, n);
+}
+
+int64_t decay_kept_bytes(const bs_delta_in& in, const DecayPlan& plan, int keep) {
+  if (!keep) return 0;
+  const int64_t start = plan.carry ? (int64_t)plan.segs * in.hv * in.dk * in.dv * 4 : 0;
+  return align16(start) +
+         (keep > 1 ? (int64_t)plan.seq.slots * in.hv * decay_saved(in.dk, in.dv) * 4 : 0);
+}
+
+float* decay_kept_saved(const bs_delta_in& in, const DecayPlan& plan, void* kept) {
+  return (float*)((char*)kept + decay_kept_bytes(in, plan, 1));
+}
+
+extern "C" size_t bs_decay_attention_kept_size(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                                               int32_t packed, int32_t keep) {
   static const int32_t dummy[1] = {0};
   const int32_t* off = packed ? dummy : nullptr;
-  if (decay_check(in, seqs, tokens, off, "bs_decay_attention_segments")) return 0;
-  const DecayPlan p = decay_plan(*in, seqs, tokens, off, train);
-  return p.carry ? (size_t)p.segs : 0;
+  if (decay_check(in, seqs, tokens, off, "bs_decay_attention_kept_size")) return 0;
+  return (size_t)decay_kept_bytes(*in, decay_plan(*in, seqs, tokens, off), keep);
 }
 
 extern "C" size_t bs_decay_attention_workspace_size(const bs_delta_in* in, int32_t seqs,
-                                                    int32_t tokens, int32_t packed,
-                                                    int32_t train) {
+                                                    int32_t tokens, int32_t packed, int32_t keep) {
   static const int32_t dummy[1] = {0};
   const int32_t* off = packed ? dummy : nullptr;
   if (decay_check(in, seqs, tokens, off, "bs_decay_attention_workspace_size")) return 0;
-  const DecayPlan p = decay_plan(*in, seqs, tokens, off, train);
-  int64_t bytes = decay_carry_bytes(*in, p);
-  if (p.carry && !train) bytes += align16((int64_t)p.segs * in->hv * in->dk * in->dv * 4);
-  return (size_t)bytes;
+  const DecayPlan p = decay_plan(*in, seqs, tokens, off);
+  return (size_t)(decay_carry_bytes(*in, p) + (keep ? 0 : decay_kept_bytes(*in, p, 1)));
 }
 
 extern "C" int bs_decay_attention(const bs_delta_in* in, int32_t seqs, int32_t tokens,
                                   const int32_t* seq_offsets, const float* initial_state,
-                                  float* final_state, void* o, float* kept_states, int32_t train,
+                                  float* final_state, void* o, void* kept, int32_t keep,
                                   void* workspace, size_t workspace_bytes, bs_stream_t stream) {
   static const char* who = "bs_decay_attention";
   if (int rc = decay_check(in, seqs, tokens, seq_offsets, who)) return rc;
   if (seqs == 0 && !seq_offsets) return BS_OK;
-  const DecayPlan plan = decay_plan(*in, seqs, tokens, seq_offsets, train);
+  const DecayPlan plan = decay_plan(*in, seqs, tokens, seq_offsets);
   const size_t need =
-      bs_decay_attention_workspace_size(in, seqs, tokens, seq_offsets != nullptr, train);
+      bs_decay_attention_workspace_size(in, seqs, tokens, seq_offsets != nullptr, keep);
   BS_CHECK_ARG(tokens == 0 || (in->q && in->k && in->v && in->g && o), "%s: NULL pointer", who);
-  BS_CHECK_ARG(!train || !plan.carry || kept_states, "%s: kept_states is NULL", who);
+  BS_CHECK_ARG(keep >= 0 && keep <= 2 && (kept || !decay_kept_bytes(*in, plan, keep)),
+               "%s: keep %d, kept is NULL", who, keep);
   BS_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                "%s: workspace of %zu bytes needed, %zu given", who, need,
                workspace ? workspace_bytes : (size_t)0);
@@ -789,9 +858,7 @@ extern "C" int bs_decay_attention(const bs_delta_in* in, int32_t seqs, int32_t t
   const int64_t states = (int64_t)seqs * in->hv * in->dk * in->dv;
   if (plan.seq.slots == 0) {
     if (final_state && states) {
-      const int64_t blocks = (states + 255) / 256;
-      keep_kernel<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, st>>>(
-          initial_state, final_state, states);
+      decay_keep(initial_state, final_state, states, st);
       BS_CHECK_LAUNCH();
     }
     if (!seq_offsets || tokens == 0) return BS_OK;
@@ -801,17 +868,18 @@ extern "C" int bs_decay_attention(const bs_delta_in* in, int32_t seqs, int32_t t
     return DecayOperand{p, {s[0], s[1], s[2]}, rep};
   };
   DecayRun run = decay_run(*in, op(in->q, in->q_stride, group), op(in->k, in->k_stride, group),
-                           op(in->v, in->v_stride, 1), in->dk, in->dv);
+                           op(in->v, in->v_stride, 1), op(nullptr, in->v_stride, 1), in->dk,
+                           in->dv);
   run.o = o;
   run.vec_o = in->dv % 4 == 0 && (uintptr_t)o % (4 * bs_dtype_size(in->dtype)) == 0;
   run.first.p = const_cast<float*>(initial_state);
   run.last.p = final_state;
   if (plan.carry) {
-    run.start.p = train ? kept_states
-                        : (float*)((char*)workspace + decay_carry_bytes(*in, plan));
+    run.start.p = (float*)(keep ? kept : (char*)workspace + decay_carry_bytes(*in, plan));
     decay_carry(run, plan, in->dtype, workspace, st);
     BS_CHECK_LAUNCH();
   }
+  if (keep > 1) run.save = decay_kept_saved(*in, plan, kept);
   decay_walk(&run, 1, plan, in->dtype, st);
   BS_CHECK_LAUNCH();
   return BS_OK;

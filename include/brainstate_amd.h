@@ -602,16 +602,30 @@ BS_API int bs_decay_attention_step(const bs_delta_in* in, int32_t batch, int32_t
                                    bs_stream_t stream);
 
 /* Whole sequences, over chunks of 64 tokens; sequences, seq_offsets and states as in
- * bs_gated_delta_rule.  With `train`, kept_states [bs_decay_attention_segments, hv, dk, dv] is
- * written for the backward pass (NULL where that is 0). */
-BS_API size_t bs_decay_attention_segments(const bs_delta_in* in, int32_t seqs, int32_t tokens,
-                                          int32_t packed, int32_t train);
+ * bs_gated_delta_rule.  keep: 0, 1 for a backward pass without a gradient of g, 2 for one with it;
+ * `kept` (bs_decay_attention_kept_size bytes, on 16 bytes, like the workspace) is written for it. */
+BS_API size_t bs_decay_attention_kept_size(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                                           int32_t packed, int32_t keep);
 BS_API size_t bs_decay_attention_workspace_size(const bs_delta_in* in, int32_t seqs,
-                                                int32_t tokens, int32_t packed, int32_t train);
+                                                int32_t tokens, int32_t packed, int32_t keep);
 BS_API int bs_decay_attention(const bs_delta_in* in, int32_t seqs, int32_t tokens,
                               const int32_t* seq_offsets, const float* initial_state,
-                              float* final_state, void* o, float* kept_states, int32_t train,
+                              float* final_state, void* o, void* kept, int32_t keep,
                               void* workspace, size_t workspace_bytes, bs_stream_t stream);
+
+/* Gradients of bs_decay_attention given those of o (grad_o [seqs, tokens, hv, dv]) and of the final
+ * states (grad_state, NULL for none): dq, dk, dv, dg laid out side by side and of their operands'
+ * types, dg [seqs, tokens, hv], or [hv] with dg_heads, or NULL where `kept` was written with keep 1
+ * (`decays` 0); dstate that of the initial states (NULL if not wanted). */
+BS_API size_t bs_decay_attention_grad_workspace_size(const bs_delta_in* in, int32_t seqs,
+                                                     int32_t tokens, int32_t packed,
+                                                     int32_t decays);
+BS_API int bs_decay_attention_grad(const bs_delta_in* in, int32_t seqs, int32_t tokens,
+                                   const int32_t* seq_offsets, const void* grad_o,
+                                   const float* grad_state, const float* initial_state,
+                                   const void* kept, void* dq, void* dk, void* dv, void* dg,
+                                   int32_t dg_heads, float* dstate, void* workspace,
+                                   size_t workspace_bytes, bs_stream_t stream);
 
 /* ---------------------------------------------------------------- norms around a block
  * Over rows of `dim` values (1..16384), with r(x) = (mean x^2 + eps)^-1/2 (no counterpart in
