@@ -651,6 +651,42 @@ BS_API int bs_norm_gate_residual_grad(const bs_norm_in* in, const void* grad_str
                                       void* dscale, void* dresidual, void* dpre, void* workspace,
                                       size_t workspace_bytes, bs_stream_t stream);
 
+/* ---------------------------------------------------------------- dropout and layer norm
+ * Dropout keeps element (row, column) of [rows, dim], times `scale`, where word column % 4 of the
+ * Philox 4x32-10 generator with counter (column / 4, site, row mod 2^32, row / 2^32) and key (seed
+ * mod 2^32, seed / 2^32) is at least `drop` (p 2^32), and gives 0 elsewhere, whatever lies there.
+ * The seed is *seed_at (device memory, read when the kernel runs) where that is given.  x has rows
+ * `stride` elements apart, y [rows, dim] is of the same type.  The gradient is the same call. */
+BS_API int bs_dropout(const void* x, int32_t dtype, int64_t rows, int32_t dim, int64_t stride,
+                      uint64_t seed, const int64_t* seed_at, uint32_t site, uint32_t drop,
+                      float scale, void* y, bs_stream_t stream);
+
+/* Layer norm of a residual stream and a dropped-out branch, over rows of `dim` values (1..16384):
+ *   stream = residual + dropout(x),  normed = (stream - mean) r weight + bias,
+ * r = (variance + eps)^-1/2.  A NULL residual is 0, drop = 0 keeps everything, NULL weight and bias
+ * are 1 and 0.  x and residual are of `dtype`, their rows *_stride elements apart; outputs are
+ * [rows, dim].  stream_out may be NULL; stats [rows, 2] takes mean and r for the gradients, or is
+ * NULL. */
+typedef struct bs_layer_norm_in {
+  const void *x, *residual, *weight, *bias;
+  const int64_t* seed_at;
+  int64_t x_stride, residual_stride, rows;
+  uint64_t seed;
+  int32_t dim, dtype, weight_dtype, bias_dtype;
+  uint32_t site, drop;
+  float keep_scale, eps;
+} bs_layer_norm_in;
+
+BS_API int bs_layer_norm(const bs_layer_norm_in* in, void* stream_out, void* normed_out,
+                         float* stats, bs_stream_t stream);
+/* Gradients, given those of stream and normed ([rows, dim], NULL: none); a NULL output is not
+ * wanted.  Weights' gradients are of their weights' types and need the workspace. */
+BS_API size_t bs_layer_norm_grad_workspace_size(int64_t rows, int32_t dim);
+BS_API int bs_layer_norm_grad(const bs_layer_norm_in* in, const void* grad_stream,
+                              const void* grad_normed, const float* stats, void* dx,
+                              void* dresidual, void* dweight, void* dbias, void* workspace,
+                              size_t workspace_bytes, bs_stream_t stream);
+
 /* ---------------------------------------------------------------- 8-bit integer products
  * Tokens x [m, k] (rows `stride` elements apart) to 8 bits with a scale each (no counterpart in
  * the reference): scale = max|x| / 127, x8 = 127 x / max|x| rounded to nearest, ties to even, in

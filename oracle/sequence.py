@@ -124,6 +124,47 @@ def norm_gate_residual(y, post=None, gate=None, scale=None, residual=None, pre=N
     return (stream, normed), out
 
 
+def philox(seed, site, rows, dim):
+    """The generator's word for every element of [rows, dim] (Philox 4x32-10, Salmon et al. 2011)."""
+    u, low = np.uint64, np.uint64(0xFFFFFFFF)
+    row, quad = np.meshgrid(np.asarray(rows, np.uint64), np.arange(-(-dim // 4), dtype=np.uint64),
+                            indexing='ij')
+    c = [quad, np.full_like(quad, site), row & low, row >> u(32)]
+    k = [int(seed) & 0xFFFFFFFF, int(seed) >> 32]
+    for _ in range(10):
+        a, b = u(0xD2511F53) * c[0], u(0xCD9E8D57) * c[2]
+        c = [(b >> u(32)) ^ c[1] ^ u(k[0]), b & low, (a >> u(32)) ^ c[3] ^ u(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return np.stack(c, -1).reshape(len(row), -1)[:, :dim]
+
+
+def dropout_mask(seed, site, rows, dim, p):
+    """1 / (1 - p) where dropout keeps an element of rows 0 .. rows - 1, 0 elsewhere."""
+    return (philox(seed, site, np.arange(rows), dim) >= int(p * 2 ** 32)) / (1 - p)
+
+
+def layer_norm(x, residual=None, weight=None, bias=None, mask=None, eps=1e-5, grad_stream=None,
+               grad_normed=None):
+    """Dropped-out branch, residual and layer norm over rows [R, D] -> (stream, normed), and with
+    ``grad_normed`` the gradients (dx, dresidual, dweight, dbias)."""
+    f = lambda t: None if t is None else np.asarray(t, np.float64)             # noqa: E731
+    x, residual, weight, bias, mask = map(f, (x, residual, weight, bias, mask))
+    m = 1.0 if mask is None else mask
+    stream = np.where(np.broadcast_to(m, x.shape) > 0, x * m, 0.0)
+    stream = stream if residual is None else residual + stream
+    d = stream - stream.mean(1, keepdims=True)
+    r = (np.mean(d * d, 1, keepdims=True) + eps) ** -0.5
+    h, w = d * r, 1.0 if weight is None else weight
+    normed = h * w + (0.0 if bias is None else bias)
+    if grad_normed is None:
+        return stream, normed
+    gn = f(grad_normed)
+    dh = gn * w
+    g = r * (dh - dh.mean(1, keepdims=True) - h * (dh * h).mean(1, keepdims=True))
+    g = g if grad_stream is None else g + f(grad_stream)
+    return (stream, normed), (g * m, g, (gn * h).sum(0), gn.sum(0))
+
+
 def int8_quantize(x):
     """Rows of x in 8 bits: a = max|x| / 127 and round-half-even of x / a = 127 x / max|x| (one
     rounding, so halves of 16-bit values are met exactly); 0 for a row of 0."""
