@@ -191,6 +191,11 @@ SIGNATURES = {
     'bs_int8_linear': (ctypes.c_int, [c_vp, c_i32, ctypes.c_int64, c_vp, ctypes.c_int64, c_i32,
                                       c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_i32, c_vp, c_size,
                                       c_vp]),
+    'bs_int4_quantize': (ctypes.c_int, [c_vp, c_i32, ctypes.c_int64, c_i32, ctypes.c_int64, c_i32,
+                                        c_vp, c_vp, c_vp]),
+    'bs_int4_workspace_size': (c_size, [c_vp, c_i32, ctypes.c_int64, ctypes.c_int64, c_i32, c_i32]),
+    'bs_int4_linear': (ctypes.c_int, [c_vp, c_i32, ctypes.c_int64, ctypes.c_int64, c_i32, c_i32,
+                                      c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_size, c_vp]),
     'bs_net_seed_spikes': (ctypes.c_int, [c_vp, c_vp, ctypes.c_int64, c_vp, c_vp]),
 }
 

@@ -22,7 +22,8 @@ LIB = os.path.join(LIBDIR, 'libbsamd.so')
 SOURCES = ['runtime.hip', 'compact.hip', 'event_sparse.hip', 'event_bucket.hip', 'event_dense.hip',
            'event_dense_packed.hip', 'neuron.hip', 'network.hip', 'delay.hip', 'conn.hip',
            'delta_step.hip', 'delta_chunk.hip', 'delta_grad.hip', 'norm.hip', 'int8.hip',
-           'decay_step.hip', 'decay_chunk.hip', 'decay_grad.hip', 'layer_norm.hip']
+           'decay_step.hip', 'decay_chunk.hip', 'decay_grad.hip', 'layer_norm.hip',
+           'int4.hip']
 ARCH = 'gfx950'
 
 

@@ -801,5 +801,6 @@ def ctypes_ref(s):
 
 from ._decay import decay_attention, decay_attention_step  # noqa: E402,F401
 from ._dropout import add_layer_norm, dropout, layer_norm  # noqa: E402,F401
+from ._int4 import int4_linear, int4_quantize  # noqa: E402,F401
 from ._sequence import (gated_delta_rule, gated_delta_step,  # noqa: E402,F401
                         int8_linear, int8_matmul, int8_quantize, norm_gate_residual)

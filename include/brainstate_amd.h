@@ -704,6 +704,24 @@ BS_API int bs_int8_linear(const void* x, int32_t x_dtype, int64_t stride, const 
                           int32_t y_dtype, void* workspace, size_t workspace_bytes,
                           bs_stream_t stream);
 
+/* ---------------------------------------------------------------- products with 4-bit weights
+ * Weights w [n, k] (rows `stride` elements apart) to 4 bits with a scale for each channel and group
+ * of `group` values (32, 64 or 128): scale = max|w| / 7, u = 8 + (7 w / max|w| rounded to nearest,
+ * ties to even), in 1..15.  w4 [n, (k + 1) / 2] holds them two to a byte, the even one in the low
+ * half; w_scale is [n, ceil(k / group)].  A group of zeros gives 8 and scale 0, one with NaN or
+ * infinity gives 8 and that scale.  k in 1..65536. */
+BS_API int bs_int4_quantize(const void* w, int32_t dtype, int64_t n, int32_t k, int64_t stride,
+                            int32_t group, uint8_t* w4, float* scale, bs_stream_t stream);
+/* y [m, n] = sum_k x[m, k] (u[n, k] - 8) w_scale[n, k / group] + bias[n], u in 0..15; x (rows
+ * `stride` elements apart) and y are of `dtype`, bias may be NULL.  The workspace starts on 16
+ * bytes; few tokens, and some layouts of x, need none. */
+BS_API size_t bs_int4_workspace_size(const void* x, int32_t dtype, int64_t stride, int64_t m,
+                                     int32_t k, int32_t n);
+BS_API int bs_int4_linear(const void* x, int32_t dtype, int64_t stride, int64_t m, int32_t k,
+                          int32_t n, int32_t group, const uint8_t* w4, const float* w_scale,
+                          const void* bias, int32_t bias_dtype, void* y, void* workspace,
+                          size_t workspace_bytes, bs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

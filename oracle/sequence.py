@@ -178,3 +178,28 @@ def int8_linear(x, w8, w_scale, bias=None):
     x8, a = int8_quantize(x)
     y = (x8 @ np.asarray(w8, np.float64).T) * a[:, None] * np.asarray(w_scale, np.float64)
     return y if bias is None else y + np.asarray(bias, np.float64)
+
+
+def int4_quantize(w, group):
+    """Weights in 4 bits: (integers 1..15 [n, k], scales [n, groups]), a = max|w| / 7 of a group and
+    round-half-even of 7 w / max|w|, plus 8; 8 for a group of 0."""
+    w = np.asarray(w, np.float64)
+    n, k = w.shape
+    groups = -(-k // group)
+    g = np.pad(w, ((0, 0), (0, groups * group - k))).reshape(n, groups, group)
+    top = np.abs(g).max(2, keepdims=True)
+    u = np.where(top > 0, np.rint(7 * g / np.where(top > 0, top, 1)), 0.0) + 8
+    return u.reshape(n, -1)[:, :k], top[:, :, 0] / 7
+
+
+def int4_pack(u):
+    """Integers 0..15 [n, k] two to a byte, the even one in the low half (8 past an odd end)."""
+    u = np.asarray(u, np.uint8)
+    u = np.pad(u, ((0, 0), (0, u.shape[1] % 2)), constant_values=8)
+    return u[:, ::2] | u[:, 1::2] << 4
+
+
+def int4_linear(x, u, scale, group, bias=None):
+    x, u, scale = (np.asarray(t, np.float64) for t in (x, u, scale))
+    y = x @ ((u - 8) * np.repeat(scale, group, 1)[:, :u.shape[1]]).T
+    return y if bias is None else y + np.asarray(bias, np.float64)
