@@ -39,7 +39,8 @@ struct DecayRun {
   const float* saved;         // from the last token to the first: the ones that a run has saved,
   float* edge;                // [slots][hv]: and their product with the state at a chunk's end
   int64_t rows;
-  int dc, dv, back, o_f32, vec_q, vec_k, vec_v, vec_dot, vec_o;
+  int dc, dv, back, o_f32;
+  int vec, vec_o;             // operands' rows start on 16 bytes and end on 8 values; o's on 4
   float att_scale, grow_scale, add_scale;
 };
 

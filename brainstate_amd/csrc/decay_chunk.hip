@@ -65,14 +65,13 @@ __device__ __forceinline__ int place(int row, int d) {
 
 // The rows of a chunk in processing order, 8 neighbouring values at a time, 0 past the last row and
 // the row's end: buffer loads, whose bounds the hardware checks.
-template <typename T>
+template <typename T, bool VEC>     // VEC: rows start on 16 bytes and end on 8 values
 struct ChunkRows {
   __amdgpu_buffer_rsrc_t rs;
   uint32_t step;
   int dim, rows, back;
-  bool vec;
   __device__ __forceinline__ ChunkRows(const DecayOperand& x, const DecayChunk& c, int h, int d,
-                                       int v, int b) {
+                                       int b) {
     step = (uint32_t)(x.stride[1] * sizeof(T));
     const uint64_t p = (uint64_t)((const T*)x.p + bs_delta_at(x.stride, c.batch, c.token,
                                                               h / x.rep));
@@ -81,13 +80,13 @@ struct ChunkRows {
     rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0,
                                            (uint32_t)(c.rows - 1) * step + d * (int)sizeof(T),
                                            0x00027000);
-    dim = d, rows = c.rows, vec = v, back = b;
+    dim = d, rows = c.rows, back = b;
   }
   __device__ __forceinline__ void raw(int row, int d, uint4* x) const {
     constexpr int W = sizeof(T) / 2;
     const int have = row < rows ? dim : 0;
     const uint32_t at = (uint32_t)(back ? rows - 1 - row : row) * step;
-    if (vec) {
+    if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < W; ++i)
         x[i] = __builtin_bit_cast(
@@ -138,7 +137,8 @@ template <typename T, int D>
 struct Staged {
   static constexpr int kPer = D / 8, kRows = kThreads / kPer, kN = 64 / kRows, W = sizeof(T) / 2;
   uint4 x[kN][W];
-  __device__ __forceinline__ void load(const ChunkRows<T>& r) {
+  template <bool VEC>
+  __device__ __forceinline__ void load(const ChunkRows<T, VEC>& r) {
 #pragma unroll
     for (int i = 0; i < kN; ++i)
       r.raw(threadIdx.x / kPer + i * kRows, threadIdx.x % kPer * 8, x[i]);
@@ -205,8 +205,11 @@ __device__ __forceinline__ double coefficients(const DecayPlan& p, const DecayCh
 
 struct Place {                   // a lane's place in the products of 32 x 32
   int m, g, x, y, half;
-  __device__ __forceinline__ Place() {
-    const int lane = threadIdx.x & 63;
+  // fresh: formed anew where it stands, so that what follows from it is not kept in registers over
+  // a loop (LDS places of a hundred fragments, which would spill)
+  __device__ __forceinline__ explicit Place(bool fresh = false) {
+    int lane = threadIdx.x & 63;
+    if (fresh) asm volatile("" : "+v"(lane));
     m = lane & 31, g = lane >> 5, x = lane & 3, y = lane >> 2 & 3, half = lane >> 4 & 1;
   }
 };
@@ -247,30 +250,44 @@ struct Columns {
 #pragma unroll
     for (int i = 0; i < RT; ++i) s[i] = zero16();
   }
+  // f(tile, element, its offset in bytes): a buffer's bounds leave out what the lane does not have,
+  // so the offset is whole in the one register that they are checked against
   template <typename F>
-  static __device__ __forceinline__ void each(const DecayRun& r, int col, const Place& l, F&& f) {
-    const int c = col + value_row(l.m);
-    if (c >= r.dv) return;
+  static __device__ __forceinline__ void each(const DecayRun& r, const DecayState& st, int col,
+                                              const Place& l, F&& f) {
+    const int c = col + value_row(l.m), have = c < r.dv ? r.dc - 8 * l.g : 0;
+    const uint32_t at = 4u * (c * st.col + 8 * l.g * st.row), row = 4u * st.row;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int d = 32 * i + 16 * (e >> 3) + 8 * l.g + (e & 7);
-        if (d < r.dc) f(i, e, d, c);
+        const int d = 32 * i + 16 * (e >> 3) + (e & 7);
+        f(i, e, d < have ? at + d * row : 0x80000000u);
       }
+  }
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t place_of(const DecayRun& r,
+                                                                   const DecayState& st,
+                                                                   int64_t at) {
+    const uint64_t p = (uint64_t)(st.p + at * r.dc * r.dv);
+    const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((int)p);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 4 * r.dc * r.dv, 0x00027000);
   }
   __device__ __forceinline__ void load(const DecayRun& r, const DecayState& st, int64_t at, int col,
                                        const Place& l) {
     clear();
     if (!st.p) return;
-    const float* p = st.p + at * r.dc * r.dv;
-    each(r, col, l, [&](int i, int e, int d, int c) { s[i][e] = p[d * st.row + c * st.col]; });
+    const __amdgpu_buffer_rsrc_t rs = place_of(r, st, at);
+    each(r, st, col, l, [&](int i, int e, uint32_t at) {
+      s[i][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0));
+    });
   }
   __device__ __forceinline__ void store(const DecayRun& r, const DecayState& st, int64_t at,
                                         float scale, int col, const Place& l) const {
-    float* p = st.p + at * r.dc * r.dv;
-    each(r, col, l,
-         [&](int i, int e, int d, int c) { p[d * st.row + c * st.col] = scale * s[i][e]; });
+    const __amdgpu_buffer_rsrc_t rs = place_of(r, st, at);
+    each(r, st, col, l, [&](int i, int e, uint32_t at) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(scale * s[i][e]), rs, at, 0, 0);
+    });
   }
   // as saved states lie: tile by tile, 4 values of a lane side by side
   static __device__ __forceinline__ int64_t saved_at(const DecayRun& r, int64_t slot_head, int wave) {
@@ -326,6 +343,7 @@ struct Columns {
         for (int p = 0; p < kParts<T>; ++p) kp.p[p] = turned_k<DC>(k + p * 64 * DC, i, ks, l);
         s[i] = mma(kp, vp, s[i]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -336,7 +354,7 @@ struct Carry {
 };
 
 // What the slots of a segment that the next one goes on with add to the state, from zero.
-template <typename T, int RT>
+template <typename T, int RT, bool VEC>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void sum_kernel(DecayRun run,
                                                                              DecayPlan plan,
                                                                              Carry carry) {
@@ -349,7 +367,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void sum_kernel(D
   const DecayLink link = link_of(plan.seq, run.back, from, to);
   if (h == 0 && threadIdx.x == 0) carry.link[seg] = link;
   if (link.seq < 0) return;
-  const Place l;
+  const Place l(false);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = 32 * wave;
   const bool live = col < run.dv;
   Chunks chunks(plan.seq, from, to, run.back);
@@ -358,8 +376,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void sum_kernel(D
   Staged<T, DC> k;
   Staged<T, kPitch> v;
   auto load = [&](const DecayChunk& at) {
-    k.load(ChunkRows<T>(run.k, at, h, run.dc, run.vec_k, run.back));
-    v.load(ChunkRows<T>(run.v, at, h, run.dv, run.vec_v, run.back));
+    k.load(ChunkRows<T, VEC>(run.k, at, h, run.dc, run.back));
+    v.load(ChunkRows<T, VEC>(run.v, at, h, run.dv, run.back));
   };
   double decay = 0.0;
   bool more = chunks.next(plan.seq, c, none);
@@ -380,6 +398,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void sum_kernel(D
       if (wave == 3) decay += coefficients(plan, c, run.back, h, coef[at ^ 1]);
     }
     if (live) {
+      const Place l(true);
       uint4 vf[4][sizeof(T) / 2];
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) turned_v<T>(lv, col, ks, l, vf[ks]);
@@ -464,7 +483,7 @@ __device__ __forceinline__ void straight_v(const T* v, int row, int d, uint4* x)
   }
 }
 
-template <typename T, int RT, bool GRAD>
+template <typename T, int RT, bool VEC, bool GRAD>
 __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(Runs runs,
                                                                               DecayPlan plan) {
   constexpr int DC = 32 * RT, PI = kParts<T>, W = sizeof(T) / 2;
@@ -484,7 +503,7 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
     return;
   }
   const int from = seg * plan.per, to = min(from + plan.per, plan.seq.slots);
-  const Place l;
+  const Place l(false);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = 32 * wave;
   const bool live = col < run.dv;
   Chunks chunks(plan.seq, from, to, run.back);
@@ -501,9 +520,9 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
   Staged<T, DC> q, k;
   Staged<T, kPitch> v;
   auto load = [&](const DecayChunk& at) {
-    q.load(ChunkRows<T>(run.q, at, h, run.dc, run.vec_q, run.back));
-    k.load(ChunkRows<T>(run.k, at, h, run.dc, run.vec_k, run.back));
-    v.load(ChunkRows<T>(run.v, at, h, run.dv, run.vec_v, run.back));
+    q.load(ChunkRows<T, VEC>(run.q, at, h, run.dc, run.back));
+    k.load(ChunkRows<T, VEC>(run.k, at, h, run.dc, run.back));
+    v.load(ChunkRows<T, VEC>(run.v, at, h, run.dv, run.back));
   };
   auto put = [&]() {
     q.put(lq);
@@ -519,6 +538,7 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
   put();
   __syncthreads();
   for (int at = 0;; at ^= 1) {
+    const Place l(true);
     DecayChunk next;
     const bool more = chunks.next(plan.seq, next, empty);
     if (more) load(next);
@@ -528,6 +548,15 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
       const int jt = wave >> 1, it = (wave + 1) >> 1, i = 32 * it + l.m;
       bs_f32x16 a = zero16();
       const int j = 32 * jt + value_row(l.m);
+      constexpr int kPairs = GRAD ? kPitch / 32 : 1;     // fragments loaded together
+      uint4 px[kPairs][W];
+      auto load_pairs = [&](int half) {
+        const ChunkRows<T, VEC> rows(run.dot, c, h, run.dv, run.back);
+#pragma unroll
+        for (int s = 0; s < kPairs; ++s)
+          rows.raw(i, 16 * (kPairs * half + s) + 8 * l.g, px[s]);
+      };
+      if (GRAD && run.pairs) load_pairs(0);
 #pragma unroll
       for (int s = 0; s < DC / 16; ++s) {
         bs_parts<PI> kp, qp;
@@ -552,13 +581,15 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
           *(bs_bf16x8*)(la + x * 64 * 64 + place<64>(i, j0 + 8 * half)) = p.p[x];
       }
       if (GRAD && run.pairs) {
-        const ChunkRows<T> rows(run.dot, c, h, run.dv, run.vec_dot, run.back);
         a = zero16();
-        for (int d = 8 * l.g; d - 8 * l.g < run.dv; d += 16) {
-          uint4 x[W], y[W];
-          rows.raw(i, d, x);
-          straight_v(lv, j, d, y);
-          a = mma(parts_of<T>(y), parts_of<T>(x), a);
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int s = 0; s < kPairs; ++s) {
+            uint4 y[W];
+            straight_v(lv, j, 16 * (kPairs * half + s) + 8 * l.g, y);
+            a = mma(parts_of<T>(y), parts_of<T>(px[s]), a);
+          }
+          if (half == 0) load_pairs(1);
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] *= a[e];
@@ -570,6 +601,7 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
     } else if (more) {
       coefficients(plan, next, run.back, h, coef[at ^ 1]);
     }
+    __builtin_amdgcn_sched_barrier(0);        // phase by phase: registers for one at a time
     bs_f32x16 o[2] = {zero16(), zero16()};
     if (!GRAD && live && run.save && !c.first) s.save(run, (int64_t)c.slot * plan.hv + h, wave);
     if (GRAD && live && run.saved && !c.first) {
@@ -579,6 +611,15 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
       if ((threadIdx.x & 63) == 0) edge[wave] = sum;
     }
     if (live) {
+      uint4 dx[2][2][W];
+      if (GRAD && run.dot.p) {
+        const ChunkRows<T, VEC> rows(run.dot, c, h, run.dv, run.back);
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            rows.raw(32 * it + l.m, col + 16 * l.g + 8 * half, dx[it][half]);
+      }
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -596,20 +637,18 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
                                             place<DC>(32 * it + l.m, 32 * i + 16 * half + 8 * l.g));
             o[it] = mma(sp, qp, o[it]);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
         const int i = 32 * it + l.m;
         o[it] *= run.grow_scale * co.grow[i];
         if (GRAD && run.dot.p) {
-          const ChunkRows<T> rows(run.dot, c, h, run.dv, run.vec_dot, run.back);
           float sum = 0.f;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            uint4 x[W];
             float f[8];
-            rows.raw(i, col + 16 * l.g + 8 * half, x);
-            floats<T>(x, f);
+            floats<T>(dx[it][half], f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum = fmaf(f[e], o[it][8 * half + e], sum);
           }
@@ -635,6 +674,7 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
                                           place<64>(32 * it + l.m, 16 * ks + 8 * l.g));
           o[it] = mma(vp, ap, o[it]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
       s.template add<T, DC>(lk, vf, co, run.add_scale, l);
       const int oc = col + 16 * l.g;
@@ -700,13 +740,19 @@ __global__ __launch_bounds__(256) void keep_kernel(const float* from, float* to,
     to[i] = from ? from[i] : 0.f;
 }
 
+// f(element, tiles of 32 rows of a state, whether operands' rows start on 16 bytes and end on 8
+// values)
 template <typename F>
-void by_type(int dtype, int wide, F&& f) {
+void by_type(int dtype, int wide, int vec, F&& f) {
   using Two = std::integral_constant<int, 2>;
   using Four = std::integral_constant<int, 4>;
   auto sized = [&](auto t) {
-    if (wide) f(t, Four());
-    else f(t, Two());
+    auto placed = [&](auto rt) {
+      if (vec) f(t, rt, std::true_type());
+      else f(t, rt, std::false_type());
+    };
+    if (wide) placed(Four());
+    else placed(Two());
   };
   if (dtype == BS_F32) sized(float());
   else if (dtype == BS_BF16) sized(bs_bf16());
@@ -765,10 +811,9 @@ DecayRun decay_run(const bs_delta_in& in, const DecayOperand& q, const DecayOper
                    const DecayOperand& v, const DecayOperand& dot, int dc, int dv) {
   DecayRun r = {};
   r.q = q, r.k = k, r.v = v, r.dot = dot, r.dc = dc, r.dv = dv;
-  r.vec_dot = vectors(dot, dv, in.dtype);
   r.first = r.last = r.start = DecayState{nullptr, dv, 1};
-  r.vec_q = vectors(q, dc, in.dtype), r.vec_k = vectors(k, dc, in.dtype);
-  r.vec_v = vectors(v, dv, in.dtype);
+  r.vec = vectors(q, dc, in.dtype) && vectors(k, dc, in.dtype) && vectors(v, dv, in.dtype) &&
+          (!dot.p || vectors(dot, dv, in.dtype));
   r.att_scale = r.grow_scale = in.scale, r.add_scale = 1.f;
   return r;
 }
@@ -783,8 +828,8 @@ void decay_carry(const DecayRun& run, const DecayPlan& plan, int dtype, void* sc
   Carry c;
   c.factor = (float*)scratch;
   c.link = (DecayLink*)((char*)scratch + align16((int64_t)plan.segs * plan.hv * 4));
-  by_type(dtype, run.dc > 64, [&](auto t, auto rt) {
-    sum_kernel<decltype(t), rt.value><<<dim3(plan.segs, plan.hv), kThreads, 0, st>>>(run, plan, c);
+  by_type(dtype, run.dc > 64, run.vec, [&](auto t, auto rt, auto vec) {
+    sum_kernel<decltype(t), rt.value, vec.value><<<dim3(plan.segs, plan.hv), kThreads, 0, st>>>(run, plan, c);
   });
   scan_kernel<<<dim3((run.dc * run.dv + 255) / 256, plan.hv), 256, 0, st>>>(run, plan, c);
 }
@@ -792,16 +837,18 @@ void decay_carry(const DecayRun& run, const DecayPlan& plan, int dtype, void* sc
 void decay_walk(const DecayRun* runs, int n, const DecayPlan& plan, int dtype, hipStream_t st) {
   const bool grad = n > 1;     // the gradients' walks, else the forward one
   Runs r = {};
-  int wide = 0;
+  int wide = 0, aligned = 1;
   for (int i = 0; i < n; ++i) {
     r.r[i] = runs[i];
     wide |= runs[i].dc > 64;
+    aligned &= runs[i].vec;
   }
   const dim3 grid(plan.segs + (plan.seq.offsets ? 1 : 0), plan.hv, n);
   if (grid.x == 0) return;
-  by_type(dtype, wide, [&](auto t, auto rt) {
-    if (grad) walk_kernel<decltype(t), rt.value, true><<<grid, kThreads, 0, st>>>(r, plan);
-    else walk_kernel<decltype(t), rt.value, false><<<grid, kThreads, 0, st>>>(r, plan);
+  by_type(dtype, wide, aligned, [&](auto t, auto rt, auto vec) {
+    if (grad)
+      walk_kernel<decltype(t), rt.value, vec.value, true><<<grid, kThreads, 0, st>>>(r, plan);
+    else walk_kernel<decltype(t), rt.value, vec.value, false><<<grid, kThreads, 0, st>>>(r, plan);
   });
 }
 
