@@ -40,7 +40,7 @@ struct DecayRun {
   float* edge;                // [slots][hv]: and their product with the state at a chunk's end
   int64_t rows;
   int dc, dv, back, o_f32;
-  int vec, vec_o;             // operands' rows start on 16 bytes and end on 8 values; o's on 4
+  int vec, vec_o;             // operands' rows start on 16 bytes and end on 8 values, and o's
   float att_scale, grow_scale, add_scale;
 };
 

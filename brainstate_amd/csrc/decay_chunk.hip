@@ -28,11 +28,13 @@ template <> constexpr int kParts<bs_bf16> = 1;
 
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
 typedef __attribute__((address_space(3))) i16x4* LdsTile;
+using bs_u32x4 = __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t;
 
 // 4 rows x 16 columns of 16-bit values for 16 lanes, transposed: lane l gives the place of the 4
 // columns 4 (l % 4) .. of row l / 4 % 4 and receives the 4 rows of column l % 16.
-__device__ __forceinline__ uint2 turn4(const uint16_t* p) {
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTile)p));
+__device__ __forceinline__ uint2 turn4(const void* tile, int bytes) {
+  return __builtin_bit_cast(
+      uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTile)((const char*)tile + bytes)));
 }
 
 // acc += a b over 16 products: parts p, q with p + q <= 2.
@@ -55,13 +57,60 @@ __device__ __forceinline__ bs_f32x16 zero16() {
   return r;
 }
 
-// Where value d of row `row` lies in a tile of rows of D values: pieces of 8 in an order that
-// spreads 16 rows' pieces over the banks.
+// Where piece `piece` (8 values) of row `row` lies in a tile of rows of D values, in bytes.  Pieces are
+// in an order that spreads over the banks both the same piece of 16 rows and, for the transposing
+// reads, 4 neighbouring pieces of 4 rows.  Piece c ^ piece lies at place ^ (16 c), and rows 16 (of 128
+// values) or 32 apart have one order.
 template <int D>
-__device__ __forceinline__ int place(int row, int d) {
-  const int key = D == 128 ? row & 15 : row >> 1 & 7;
-  return row * D + (((d >> 3) ^ key) << 3) + (d & 7);
+__device__ __forceinline__ int place(int row, int piece) {
+  const int key = D == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
+  return row * (2 * D) + ((piece ^ key) << 4);
 }
+__device__ __forceinline__ bs_bf16x8 piece_at(const uint16_t* tile, int bytes) {
+  return *(const bs_bf16x8*)((const char*)tile + bytes);
+}
+
+// Three bf16 parts of 8 floats (lane_types.h), what a part leaves by the exact sum x - part.
+struct Splitter {
+  uint32_t low, high;           // -1 in either half, in scalar registers
+  __device__ __forceinline__ Splitter() : low(0x0000BF80u), high(0xBF800000u) {
+    asm volatile("" : "+s"(low), "+s"(high));
+  }
+  template <int P>
+  __device__ __forceinline__ bs_parts<P> split(const float* x) const {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    uint32_t w[P][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        w[p][i] = bs_pack_hi(a, b);
+        if (p + 1 < P) {
+          const bf16x2 v = __builtin_bit_cast(bf16x2, w[p][i]);
+          a = __builtin_amdgcn_fdot2_f32_bf16(v, __builtin_bit_cast(bf16x2, low), a, false);
+          b = __builtin_amdgcn_fdot2_f32_bf16(v, __builtin_bit_cast(bf16x2, high), b, false);
+        }
+      }
+    }
+    bs_parts<P> o;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      o.p[p] = __builtin_bit_cast(bs_bf16x8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
+    return o;
+  }
+};
+
+// An operand's rows of one head; strides in bytes.
+struct HeadRows {
+  const char* p;
+  int64_t batch, token;
+  template <typename T>
+  static __device__ __forceinline__ HeadRows of(const DecayOperand& x, int h) {
+    constexpr int64_t n = sizeof(T);
+    return {(const char*)x.p + (h / x.rep) * x.stride[2] * n, x.stride[0] * n, x.stride[1] * n};
+  }
+};
 
 // The rows of a chunk in processing order, 8 neighbouring values at a time, 0 past the last row and
 // the row's end: buffer loads, whose bounds the hardware checks.
@@ -70,11 +119,9 @@ struct ChunkRows {
   __amdgpu_buffer_rsrc_t rs;
   uint32_t step;
   int dim, rows, back;
-  __device__ __forceinline__ ChunkRows(const DecayOperand& x, const DecayChunk& c, int h, int d,
-                                       int b) {
-    step = (uint32_t)(x.stride[1] * sizeof(T));
-    const uint64_t p = (uint64_t)((const T*)x.p + bs_delta_at(x.stride, c.batch, c.token,
-                                                              h / x.rep));
+  __device__ __forceinline__ ChunkRows(const HeadRows& x, const DecayChunk& c, int d, int b) {
+    step = (uint32_t)x.token;
+    const uint64_t p = (uint64_t)(x.p + c.batch * x.batch + c.token * x.token);
     const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
                           (uint32_t)__builtin_amdgcn_readfirstlane((int)p);
     rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0,
@@ -87,11 +134,11 @@ struct ChunkRows {
     const int have = row < rows ? dim : 0;
     const uint32_t at = (uint32_t)(back ? rows - 1 - row : row) * step;
     if constexpr (VEC) {
+      const uint32_t o = d < have ? at + d * (uint32_t)sizeof(T) : 0xFFFFFF00u;
 #pragma unroll
       for (int i = 0; i < W; ++i)
-        x[i] = __builtin_bit_cast(
-            uint4, __builtin_amdgcn_raw_buffer_load_b128(
-                       rs, d < have ? at + d * (uint32_t)sizeof(T) + 16 * i : 0xFFFFFFF0u, 0, 0));
+        x[i] = __builtin_bit_cast(uint4,
+                                  __builtin_amdgcn_raw_buffer_load_b128(rs, o + 16 * i, 0, 0));
     } else {
       uint32_t e[8];
 #pragma unroll
@@ -120,7 +167,7 @@ __device__ __forceinline__ void floats(const uint4* x, float* f) {
 }
 
 template <typename T>
-__device__ __forceinline__ bs_parts<kParts<T>> parts_of(const uint4* x) {
+__device__ __forceinline__ bs_parts<kParts<T>> parts_of(const Splitter& sp, const uint4* x) {
   if constexpr (kParts<T> == 1) {
     bs_parts<1> o;
     o.p[0] = __builtin_bit_cast(bs_bf16x8, x[0]);
@@ -128,7 +175,7 @@ __device__ __forceinline__ bs_parts<kParts<T>> parts_of(const uint4* x) {
   } else {
     float f[8];
     floats<T>(x, f);
-    return bs_split8<kParts<T>>(f);
+    return sp.split<kParts<T>>(f);
   }
 }
 
@@ -144,22 +191,24 @@ struct Staged {
       r.raw(threadIdx.x / kPer + i * kRows, threadIdx.x % kPer * 8, x[i]);
   }
   // as bf16 parts, [part][64][D]
-  __device__ __forceinline__ void put(uint16_t* to) const {
+  __device__ __forceinline__ void put(uint16_t* to, const Splitter& sp) const {
+    const int at = place<D>(threadIdx.x / kPer, threadIdx.x % kPer);
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const bs_parts<kParts<T>> p = parts_of<T>(x[i]);
-      const int at = place<D>(threadIdx.x / kPer + i * kRows, threadIdx.x % kPer * 8);
+      const bs_parts<kParts<T>> p = parts_of<T>(sp, x[i]);
 #pragma unroll
-      for (int k = 0; k < kParts<T>; ++k) *(bs_bf16x8*)(to + k * 64 * D + at) = p.p[k];
+      for (int k = 0; k < kParts<T>; ++k)
+        *(bs_bf16x8*)((char*)to + (k * 64 + i * kRows) * 2 * D + at) = p.p[k];
     }
   }
   // as they are, [64][D]: 16-bit values in the order of place(), 32-bit ones in a row's order
   __device__ __forceinline__ void put_raw(void* to) const {
+    const int at = place<D>(threadIdx.x / kPer, threadIdx.x % kPer);
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int row = threadIdx.x / kPer + i * kRows, d = threadIdx.x % kPer * 8;
       if constexpr (W == 1) {
-        *(uint4*)((uint16_t*)to + place<D>(row, d)) = x[i][0];
+        *(uint4*)((char*)to + i * kRows * 2 * D + at) = x[i][0];
       } else {
         *(uint4*)((float*)to + row * D + d) = x[i][0];
         *(uint4*)((float*)to + row * D + d + 4) = x[i][W - 1];
@@ -171,7 +220,7 @@ struct Staged {
 // Coefficients of a chunk, by processing order.
 struct Coef {
   float grow[64], left[64];      // exp(run_i), exp(total - run_i)
-  double run[64];                // times log2 e
+  float high[64], low[64];       // run_i log2 e = high + low
   float total;                   // exp(total)
 };
 
@@ -179,15 +228,19 @@ constexpr double kLog2e = 1.4426950408889634;
 
 __device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
-// By one wave, lane = row.  Returns total (times log2 e).
-__device__ __forceinline__ double coefficients(const DecayPlan& p, const DecayChunk& c, int back,
-                                               int h, Coef& o) {
+// The log decay of the lane's row.
+__device__ __forceinline__ float decay_of(const DecayPlan& p, const DecayChunk& c, int back, int h) {
   const int lane = threadIdx.x & 63;
   // from the last token to the first, a decay belongs to the row after its token
   const int at = back ? c.rows - lane : lane;
-  float g = 0.f;
   if (lane < c.rows && (!back || lane > 0 || c.next_g))
-    g = bs_load_any(p.g, p.g_dtype, bs_delta_at(p.g_stride, c.batch, c.token + at, h));
+    return bs_load_any(p.g, p.g_dtype, bs_delta_at(p.g_stride, c.batch, c.token + at, h));
+  return 0.f;
+}
+
+// By one wave, lane = row, from decay_of.  Returns total (times log2 e).
+__device__ __forceinline__ double coefficients(float g, Coef& o) {
+  const int lane = threadIdx.x & 63;
   g = g < BS_DELTA_G_MIN ? BS_DELTA_G_MIN : g;
   double x = (double)g * kLog2e;
 #pragma unroll
@@ -196,7 +249,8 @@ __device__ __forceinline__ double coefficients(const DecayPlan& p, const DecayCh
     if (lane >= d) x += y;
   }
   const double total = __shfl(x, 63);
-  o.run[lane] = x;
+  o.high[lane] = (float)x;
+  o.low[lane] = (float)(x - (double)(float)x);
   o.grow[lane] = exp_of(x);
   o.left[lane] = exp_of(total - x);
   if (lane == 0) o.total = exp_of(total);
@@ -204,13 +258,20 @@ __device__ __forceinline__ double coefficients(const DecayPlan& p, const DecayCh
 }
 
 struct Place {                   // a lane's place in the products of 32 x 32
-  int m, g, x, y, half;
+  int m, g;
   // fresh: formed anew where it stands, so that what follows from it is not kept in registers over
-  // a loop (LDS places of a hundred fragments, which would spill)
-  __device__ __forceinline__ explicit Place(bool fresh = false) {
+  // a loop (places in LDS, which would spill)
+  __device__ __forceinline__ explicit Place(bool fresh) {
     int lane = threadIdx.x & 63;
     if (fresh) asm volatile("" : "+v"(lane));
-    m = lane & 31, g = lane >> 5, x = lane & 3, y = lane >> 2 & 3, half = lane >> 4 & 1;
+    m = lane & 31, g = lane >> 5;
+  }
+  // Where this lane reads 4 rows 16 ks + 8 g + 4 second .. (and 32 D ks further on) x 4 columns of a
+  // 16-bit tile for the transposing read: `piece` and the upper or lower half of it, by what column
+  // of 4 (lane % 4) it gives for the 16 lanes it reads with.
+  template <int D>
+  __device__ __forceinline__ int turn(int piece, int upper, int second) const {
+    return place<D>(8 * g + 4 * second + (m >> 2 & 3), piece) + 8 * upper;
   }
 };
 
@@ -219,26 +280,25 @@ __device__ __forceinline__ int value_row(int m) {
   return 16 * (m >> 2 & 1) + 4 * (m >> 3) + (m & 3);
 }
 
-// K^T of rows 32 rt .. and tokens 16 ks ..: part `part` of the tile [part][64][DC].
-template <int DC>
-__device__ __forceinline__ bs_bf16x8 turned_k(const uint16_t* k, int rt, int ks, const Place& l) {
-  const int d = 32 * rt + 16 * l.half + 8 * (l.x & 1) + 4 * (l.x >> 1), t = 16 * ks + 8 * l.g + l.y;
-  const uint2 a = turn4(k + place<DC>(t, d)), b = turn4(k + place<DC>(t + 4, d));
-  return __builtin_bit_cast(bs_bf16x8, make_uint4(a.x, a.y, b.x, b.y));
-}
-
-// V^T of 32 value columns from `col` and tokens 16 ks ..: 8 values.
+// V^T of 32 value columns from `col`: fragments of 16 tokens each, 8 values a lane.
 template <typename T>
-__device__ __forceinline__ void turned_v(const void* v, int col, int ks, const Place& l, uint4* r) {
+__device__ __forceinline__ void turned_v(const void* v, int col, const Place& l,
+                                         uint4 (*r)[sizeof(T) / 2]) {
   if constexpr (sizeof(T) == 2) {
-    const int d = col + 16 * (l.x & 1) + 4 * (2 * l.half + (l.x >> 1)), t = 16 * ks + 8 * l.g + l.y;
-    const uint2 a = turn4((const uint16_t*)v + place<kPitch>(t, d)),
-                b = turn4((const uint16_t*)v + place<kPitch>(t + 4, d));
-    r[0] = make_uint4(a.x, a.y, b.x, b.y);
+    const int x = l.m & 3, half = l.m >> 4, piece = col / 8 + 2 * (x & 1) + half;
+    const int a = l.turn<kPitch>(piece, x >> 1, 0), b = l.turn<kPitch>(piece, x >> 1, 1);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const uint2 p = turn4(v, a + ks * 32 * kPitch), q = turn4(v, b + ks * 32 * kPitch);
+      r[ks][0] = make_uint4(p.x, p.y, q.x, q.y);
+    }
   } else {
-    const uint32_t* p = (const uint32_t*)v + (16 * ks + 8 * l.g) * kPitch + col + value_row(l.m);
-    r[0] = make_uint4(p[0], p[kPitch], p[2 * kPitch], p[3 * kPitch]);
-    r[1] = make_uint4(p[4 * kPitch], p[5 * kPitch], p[6 * kPitch], p[7 * kPitch]);
+    const uint32_t* p = (const uint32_t*)v + 8 * l.g * kPitch + col + value_row(l.m);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks, p += 16 * kPitch) {
+      r[ks][0] = make_uint4(p[0], p[kPitch], p[2 * kPitch], p[3 * kPitch]);
+      r[ks][1] = make_uint4(p[4 * kPitch], p[5 * kPitch], p[6 * kPitch], p[7 * kPitch]);
+    }
   }
 }
 
@@ -324,10 +384,14 @@ struct Columns {
   // s = decay s + K^T (left V) with V's turned fragments of 16 tokens each
   template <typename T, int DC>
   __device__ __forceinline__ void add(const uint16_t* k, const uint4 (*v)[sizeof(T) / 2],
-                                      const Coef& co, float scale, const Place& l) {
+                                      const Coef& co, float scale, const Place& l,
+                                      const Splitter& sp) {
+    constexpr int PI = kParts<T>;
     const float total = co.total;
 #pragma unroll
     for (int i = 0; i < RT; ++i) s[i] *= total;
+    const int x = l.m & 3, piece = 2 * (l.m >> 4) + (x & 1);
+    const int first = l.turn<DC>(piece, x >> 1, 0), second = l.turn<DC>(piece, x >> 1, 1);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       float f[8];
@@ -335,15 +399,18 @@ struct Columns {
       const float* lf = co.left + 16 * ks + 8 * l.g;
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] *= scale * lf[j];
-      const bs_parts<3> vp = bs_split8<3>(f);
+      const bs_parts<3> vp = sp.split<3>(f);
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        bs_parts<kParts<T>> kp;
+        bs_parts<PI> kp;
 #pragma unroll
-        for (int p = 0; p < kParts<T>; ++p) kp.p[p] = turned_k<DC>(k + p * 64 * DC, i, ks, l);
+        for (int p = 0; p < PI; ++p) {
+          const int at = (p * 64 + 16 * ks) * 2 * DC;
+          const uint2 a = turn4(k, (first ^ 64 * i) + at), b = turn4(k, (second ^ 64 * i) + at);
+          kp.p[p] = __builtin_bit_cast(bs_bf16x8, make_uint4(a.x, a.y, b.x, b.y));
+        }
         s[i] = mma(kp, vp, s[i]);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -373,36 +440,43 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void sum_kernel(D
   Chunks chunks(plan.seq, from, to, run.back);
   DecayChunk c;
   auto none = [](int) {};
+  const Splitter sp;
+  const HeadRows kh = HeadRows::of<T>(run.k, h), vh = HeadRows::of<T>(run.v, h);
   Staged<T, DC> k;
   Staged<T, kPitch> v;
   auto load = [&](const DecayChunk& at) {
-    k.load(ChunkRows<T, VEC>(run.k, at, h, run.dc, run.back));
-    v.load(ChunkRows<T, VEC>(run.v, at, h, run.dv, run.back));
+    k.load(ChunkRows<T, VEC>(kh, at, run.dc, run.back));
+    v.load(ChunkRows<T, VEC>(vh, at, run.dv, run.back));
   };
   double decay = 0.0;
+  float g = 0.f;                  // of the chunk that is loaded next, a chunk ahead of its use
   bool more = chunks.next(plan.seq, c, none);
   if (more) {
     load(c);
-    if (wave == 3) decay += coefficients(plan, c, run.back, h, coef[0]);
+    if (wave == 3) decay += coefficients(decay_of(plan, c, run.back, h), coef[0]);
   }
+  bool ahead = more && chunks.next(plan.seq, c, none);
+  if (ahead && wave == 3) g = decay_of(plan, c, run.back, h);
   Columns<RT> s;
   s.clear();
   for (int at = 0; more; at ^= 1) {
+    const Place l(true);
     __syncthreads();
-    k.put(lk);
+    k.put(lk, sp);
     v.put_raw(lv);
-    more = chunks.next(plan.seq, c, none);
     __syncthreads();
+    more = ahead;
     if (more) {
       load(c);
-      if (wave == 3) decay += coefficients(plan, c, run.back, h, coef[at ^ 1]);
+      if (wave == 3) decay += coefficients(g, coef[at ^ 1]);
+      ahead = chunks.next(plan.seq, c, none);
+      if (ahead && wave == 3) g = decay_of(plan, c, run.back, h);
     }
     if (live) {
       const Place l(true);
       uint4 vf[4][sizeof(T) / 2];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) turned_v<T>(lv, col, ks, l, vf[ks]);
-      s.template add<T, DC>(lk, vf, coef[at], run.add_scale, l);
+      turned_v<T>(lv, col, l, vf);
+      s.template add<T, DC>(lk, vf, coef[at], run.add_scale, l, sp);
     }
   }
   if (live) s.store(run, run.start, (int64_t)seg * plan.hv + h, 1.f, col, l);
@@ -418,26 +492,26 @@ __global__ __launch_bounds__(256) void scan_kernel(DecayRun run, DecayPlan plan,
   float* p = run.start.p + (int64_t)h * n + e;
   const int64_t step = (int64_t)plan.hv * n;
   float state = 0.f;
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 8;      // segments whose loads are in flight together
   for (int i0 = 0; i0 < plan.segs; i0 += kAhead) {
-    float x[kAhead];
+    float x[kAhead], factor[kAhead];
+    DecayLink link[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int seg = min(i0 + i, plan.segs - 1);
-      x[i] = p[(run.back ? plan.segs - 1 - seg : seg) * step];
+      const int at = min(i0 + i, plan.segs - 1), seg = run.back ? plan.segs - 1 - at : at;
+      x[i] = p[seg * step];
+      link[i] = carry.link[seg], factor[i] = carry.factor[seg * plan.hv + h];
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (i0 + i >= plan.segs) break;
-      const int seg = run.back ? plan.segs - 1 - i0 - i : i0 + i;
-      p[seg * step] = state;
-      const DecayLink link = carry.link[seg];
-      if (link.seq < 0) continue;
-      if (link.first)
-        state = run.first.p ? run.first.p[((int64_t)link.seq * plan.hv + h) * n +
+      p[(run.back ? plan.segs - 1 - i0 - i : i0 + i) * step] = state;
+      if (link[i].seq < 0) continue;
+      if (link[i].first)
+        state = run.first.p ? run.first.p[((int64_t)link[i].seq * plan.hv + h) * n +
                                           r * run.first.row + c * run.first.col]
                             : 0.f;
-      state = fmaf(carry.factor[seg * plan.hv + h], state, x[i]);
+      state = fmaf(factor[i], state, x[i]);
     }
   }
 }
@@ -472,14 +546,14 @@ __device__ __forceinline__ void pair_sums(const float* p, const Place& l, double
   col = v[0] + __shfl_xor(v[0], 1);
 }
 
-// 8 values of a row of V as it lies in LDS.
+// 8 values of a row of V as it lies in LDS; `at`: where the row's piece g lies (16-bit), or value 8 g.
 template <typename T>
-__device__ __forceinline__ void straight_v(const T* v, int row, int d, uint4* x) {
+__device__ __forceinline__ void straight_v(const T* v, int at, int step, uint4* x) {
   if constexpr (sizeof(T) == 2) {
-    x[0] = *(const uint4*)((const uint16_t*)v + place<kPitch>(row, d));
+    x[0] = *(const uint4*)((const char*)v + (at ^ 32 * step));
   } else {
-    x[0] = *(const uint4*)(v + row * kPitch + d);
-    x[1] = *(const uint4*)(v + row * kPitch + d + 4);
+    x[0] = *(const uint4*)(v + at + 16 * step);
+    x[1] = *(const uint4*)(v + at + 16 * step + 4);
   }
 }
 
@@ -517,30 +591,34 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
           run.first.p ? run.first.p[at + r * run.first.row + c * run.first.col] : 0.f;
     }
   };
+  const Splitter sp;
+  const HeadRows qh = HeadRows::of<T>(run.q, h), kh = HeadRows::of<T>(run.k, h),
+                 vh = HeadRows::of<T>(run.v, h), dh = HeadRows::of<T>(run.dot, h);
   Staged<T, DC> q, k;
   Staged<T, kPitch> v;
   auto load = [&](const DecayChunk& at) {
-    q.load(ChunkRows<T, VEC>(run.q, at, h, run.dc, run.back));
-    k.load(ChunkRows<T, VEC>(run.k, at, h, run.dc, run.back));
-    v.load(ChunkRows<T, VEC>(run.v, at, h, run.dv, run.back));
+    q.load(ChunkRows<T, VEC>(qh, at, run.dc, run.back));
+    k.load(ChunkRows<T, VEC>(kh, at, run.dc, run.back));
+    v.load(ChunkRows<T, VEC>(vh, at, run.dv, run.back));
   };
   auto put = [&]() {
-    q.put(lq);
-    k.put(lk);
+    q.put(lq, sp);
+    k.put(lk, sp);
     v.put_raw(lv);
   };
-  DecayChunk c;
+  DecayChunk c, next;
+  float g = 0.f;                  // of the next chunk, loaded an iteration ahead of its use
   if (!chunks.next(plan.seq, c, empty)) return;
   load(c);
-  if (wave == 3) coefficients(plan, c, run.back, h, coef[0]);
+  if (wave == 3) coefficients(decay_of(plan, c, run.back, h), coef[0]);
+  bool more = chunks.next(plan.seq, next, empty);
+  if (more && wave == 3) g = decay_of(plan, next, run.back, h);
   Columns<RT> s;
   if (live && !c.first) s.load(run, run.start, (int64_t)seg * plan.hv + h, col, l);
   put();
   __syncthreads();
   for (int at = 0;; at ^= 1) {
     const Place l(true);
-    DecayChunk next;
-    const bool more = chunks.next(plan.seq, next, empty);
     if (more) load(next);
     const Coef& co = coef[at];
     if (live && c.first) s.load(run, run.first, (int64_t)c.seq * plan.hv + h, col, l);
@@ -551,34 +629,38 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
       constexpr int kPairs = GRAD ? kPitch / 32 : 1;     // fragments loaded together
       uint4 px[kPairs][W];
       auto load_pairs = [&](int half) {
-        const ChunkRows<T, VEC> rows(run.dot, c, h, run.dv, run.back);
+        const ChunkRows<T, VEC> rows(dh, c, run.dv, run.back);
 #pragma unroll
         for (int s = 0; s < kPairs; ++s)
           rows.raw(i, 16 * (kPairs * half + s) + 8 * l.g, px[s]);
       };
       if (GRAD && run.pairs) load_pairs(0);
+      const int ka = place<DC>(j, l.g), qa = place<DC>(i, l.g);
 #pragma unroll
       for (int s = 0; s < DC / 16; ++s) {
         bs_parts<PI> kp, qp;
 #pragma unroll
         for (int p = 0; p < PI; ++p) {
-          kp.p[p] = *(const bs_bf16x8*)(lk + p * 64 * DC + place<DC>(j, 16 * s + 8 * l.g));
-          qp.p[p] = *(const bs_bf16x8*)(lq + p * 64 * DC + place<DC>(i, 16 * s + 8 * l.g));
+          kp.p[p] = piece_at(lk, (ka ^ 32 * s) + p * 128 * DC);
+          qp.p[p] = piece_at(lq, (qa ^ 32 * s) + p * 128 * DC);
         }
         a = mma(kp, qp, a);
       }
-      const double ri = co.run[i];
+      const float high = co.high[i], low = co.low[i];
       const int j0 = 32 * jt + 16 * l.g;
       float w[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        w[e] = j0 + e <= i ? run.att_scale * exp_of(ri - co.run[j0 + e]) * a[e] : 0.f;
+        w[e] = j0 + e <= i ? run.att_scale * a[e] *
+                                 __builtin_amdgcn_exp2f((high - co.high[j0 + e]) +
+                                                        (low - co.low[j0 + e]))
+                           : 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const bs_parts<3> p = bs_split8<3>(w + 8 * half);
+        const bs_parts<3> p = sp.split<3>(w + 8 * half);
 #pragma unroll
         for (int x = 0; x < 3; ++x)
-          *(bs_bf16x8*)(la + x * 64 * 64 + place<64>(i, j0 + 8 * half)) = p.p[x];
+          *(bs_bf16x8*)((char*)la + (place<64>(i, j0 / 8) ^ 16 * half) + x * 128 * 64) = p.p[x];
       }
       if (GRAD && run.pairs) {
         a = zero16();
@@ -586,8 +668,9 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
 #pragma unroll
           for (int s = 0; s < kPairs; ++s) {
             uint4 y[W];
-            straight_v(lv, j, 16 * (kPairs * half + s) + 8 * l.g, y);
-            a = mma(parts_of<T>(y), parts_of<T>(px[s]), a);
+            straight_v(lv, W == 1 ? place<kPitch>(j, l.g) : j * kPitch + 8 * l.g,
+                       kPairs * half + s, y);
+            a = mma(parts_of<T>(sp, y), parts_of<T>(sp, px[s]), a);
           }
           if (half == 0) load_pairs(1);
         }
@@ -599,7 +682,7 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
         if (!(l.m & 1)) sums[wave][1][16 * l.g + l.m / 2] = column;
       }
     } else if (more) {
-      coefficients(plan, next, run.back, h, coef[at ^ 1]);
+      coefficients(g, coef[at ^ 1]);
     }
     __builtin_amdgcn_sched_barrier(0);        // phase by phase: registers for one at a time
     bs_f32x16 o[2] = {zero16(), zero16()};
@@ -613,13 +696,14 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
     if (live) {
       uint4 dx[2][2][W];
       if (GRAD && run.dot.p) {
-        const ChunkRows<T, VEC> rows(run.dot, c, h, run.dv, run.back);
+        const ChunkRows<T, VEC> rows(dh, c, run.dv, run.back);
 #pragma unroll
         for (int it = 0; it < 2; ++it)
 #pragma unroll
           for (int half = 0; half < 2; ++half)
             rows.raw(32 * it + l.m, col + 16 * l.g + 8 * half, dx[it][half]);
       }
+      const int qa = place<DC>(l.m, l.g);
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -627,17 +711,15 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
           float f[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[e] = s.s[i][8 * half + e];
-          const bs_parts<3> sp = bs_split8<3>(f);
+          const bs_parts<3> st = sp.split<3>(f);
 #pragma unroll
           for (int it = 0; it < 2; ++it) {
             bs_parts<PI> qp;
 #pragma unroll
             for (int p = 0; p < PI; ++p)
-              qp.p[p] = *(const bs_bf16x8*)(lq + p * 64 * DC +
-                                            place<DC>(32 * it + l.m, 32 * i + 16 * half + 8 * l.g));
-            o[it] = mma(sp, qp, o[it]);
+              qp.p[p] = piece_at(lq, (qa ^ 16 * (4 * i + 2 * half)) + (p * 64 + 32 * it) * 2 * DC);
+            o[it] = mma(st, qp, o[it]);
           }
-          __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
@@ -660,45 +742,68 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
     __syncthreads();                          // att
     if (live) {
       uint4 vf[4][W];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) turned_v<T>(lv, col, ks, l, vf[ks]);
+      turned_v<T>(lv, col, l, vf);
+      const int aa = place<64>(l.m, l.g);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        const bs_parts<PI> vp = parts_of<T>(vf[ks]);
+        const bs_parts<PI> vp = parts_of<T>(sp, vf[ks]);
 #pragma unroll
         for (int it = ks >> 1; it < 2; ++it) {
           bs_parts<3> ap;
 #pragma unroll
           for (int p = 0; p < 3; ++p)
-            ap.p[p] = *(const bs_bf16x8*)(la + p * 64 * 64 +
-                                          place<64>(32 * it + l.m, 16 * ks + 8 * l.g));
+            ap.p[p] = piece_at(la, (aa ^ 32 * ks) + (p * 64 + 32 * it) * 128);
           o[it] = mma(vp, ap, o[it]);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
-      s.template add<T, DC>(lk, vf, co, run.add_scale, l);
+      s.template add<T, DC>(lk, vf, co, run.add_scale, l, sp);
       const int oc = col + 16 * l.g;
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
         const int i = 32 * it + l.m;
-        if (i >= c.rows) continue;
-        const int64_t row = c.batch * plan.seq.tokens + c.token + (run.back ? c.rows - 1 - i : i);
-        const int64_t base = (row * plan.hv + h) * run.dv + oc;
-        auto put_out = [&](auto* p) {
+        // rows past the chunk's end lie past the buffer's
+        const int row = run.back ? c.rows - 1 - i : i;
+        auto put_out = [&](auto* out) {
+          using O = typename std::remove_pointer<decltype(out)>::type;
+          const int step = plan.hv * run.dv * (int)sizeof(O);
+          const uint64_t p = (uint64_t)(out + ((c.batch * plan.seq.tokens + c.token) * plan.hv + h) *
+                                                  run.dv);
+          const uint64_t base =
+              (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
+              (uint32_t)__builtin_amdgcn_readfirstlane((int)p);
+          const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)base, 0, (c.rows - 1) * step + run.dv * (int)sizeof(O), 0x00027000);
+          auto at = [&](int e) {
+            return row >= 0 && row < c.rows && oc + e < run.dv
+                       ? (uint32_t)(row * step) + (oc + e) * (uint32_t)sizeof(O)
+                       : 0xFFFFFF00u;
+          };
           if (run.vec_o) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              if (oc + e < run.dv)
-                bs_store4(p + e, bs_f32x4{o[it][e], o[it][e + 1], o[it][e + 2], o[it][e + 3]});
+            for (int e = 0; e < 16; e += 8) {
+              bs_u32x4 x[sizeof(O) / 2];
+              O t[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) t[j] = bs_from_f32<O>(o[it][e + j]);
+              __builtin_memcpy(x, t, sizeof(t));
+              const uint32_t to = at(e);
+#pragma unroll
+              for (int j = 0; j < (int)sizeof(O) / 2; ++j)
+                __builtin_amdgcn_raw_buffer_store_b128(x[j], rs, to + 16 * j, 0, 0);
+            }
           } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (oc + e < run.dv)
-                p[e] = bs_from_f32<typename std::remove_pointer<decltype(p)>::type>(o[it][e]);
+            for (int e = 0; e < 16; ++e) {
+              const O x = bs_from_f32<O>(o[it][e]);
+              if constexpr (sizeof(O) == 4)
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), rs, at(e), 0, 0);
+              else
+                __builtin_amdgcn_raw_buffer_store_b16(x.u, rs, at(e), 0, 0);
+            }
           }
         };
-        if (run.o_f32) put_out((float*)run.o + base);
-        else put_out((T*)run.o + base);
+        if (run.o_f32) put_out((float*)run.o);
+        else put_out((T*)run.o);
       }
       if (c.last && run.last.p) {
         float scale = 1.f;
@@ -730,6 +835,8 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
     if (!more) return;
     put();
     c = next;
+    more = chunks.next(plan.seq, next, empty);
+    if (more && wave == 3) g = decay_of(plan, next, run.back, h);
     __syncthreads();
   }
 }
@@ -918,7 +1025,7 @@ extern "C" int bs_decay_attention(const bs_delta_in* in, int32_t seqs, int32_t t
                            op(in->v, in->v_stride, 1), op(nullptr, in->v_stride, 1), in->dk,
                            in->dv);
   run.o = o;
-  run.vec_o = in->dv % 4 == 0 && (uintptr_t)o % (4 * bs_dtype_size(in->dtype)) == 0;
+  run.vec_o = in->dv % 8 == 0 && (uintptr_t)o % 16 == 0;
   run.first.p = const_cast<float*>(initial_state);
   run.last.p = final_state;
   if (plan.carry) {

@@ -179,7 +179,7 @@ extern "C" int bs_decay_attention_grad(const bs_delta_in* in, int32_t seqs, int3
   work_of(*in, plan, seqs, rows, dg != nullptr, workspace, &w);
   const int64_t states = (int64_t)seqs * in->hv * in->dk * in->dv;
   if (plan.seq.slots == 0 && dstate && states) decay_keep(grad_state, dstate, states, st);
-  const int group = in->hv / in->hk, size = bs_dtype_size(in->dtype);
+  const int group = in->hv / in->hk;
   auto op = [](const void* p, const int64_t* s, int rep) {
     return DecayOperand{p, {s[0], s[1], s[2]}, rep};
   };
@@ -197,7 +197,7 @@ extern "C" int bs_decay_attention_grad(const bs_delta_in* in, int32_t seqs, int3
     r[i].start.p = w.start;
   }
   r[0].o = dv, r[0].last.p = dstate;
-  r[0].vec_o = dvn % 4 == 0 && (uintptr_t)dv % (4 * size) == 0;
+  r[0].vec_o = dvn % 8 == 0 && (uintptr_t)dv % 16 == 0;
   r[1].o = group > 1 ? (void*)w.dk : dk, r[2].o = group > 1 ? (void*)w.dq : dq;
   r[1].dots = w.y, r[2].dots = w.x, r[2].pairs = dg != nullptr;
   r[2].first.p = const_cast<float*>(initial_state);
@@ -208,7 +208,7 @@ extern "C" int bs_decay_attention_grad(const bs_delta_in* in, int32_t seqs, int3
   }
   for (int i = 1; i < 3; ++i) {
     r[i].o_f32 = group > 1, r[i].rows = rows;
-    r[i].vec_o = dkn % 4 == 0 && (uintptr_t)r[i].o % (group > 1 ? 16 : 4 * size) == 0;
+    r[i].vec_o = dkn % 8 == 0 && (uintptr_t)r[i].o % 16 == 0;
     for (DecayState* s : {&r[i].first, &r[i].start, &r[i].last}) s->row = 1, s->col = dvn;
   }
   if (plan.carry) decay_carry(r[0], plan, in->dtype, w.carry, st);
