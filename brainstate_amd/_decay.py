@@ -5,8 +5,8 @@ import torch
 
 from . import _native as N
 from . import _trace
-from ._sequence import (_DELTA_IN, _DTYPES, _address, _floating, _heads, _recorded, _states,
-                        _tangent, _wants_grad)
+from ._sequence import (_DELTA_IN, _DTYPES, _address, _floating, _heads, _like, _once, _recorded,
+                        _states, _tangent, _wants_grad)
 
 
 def _operands(q, k, v, g, scale):
@@ -125,7 +125,7 @@ class _DecayAttention(torch.autograd.Function):
         return o, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, go, gstate):
         _recorded('decay_attention', go, gstate)
         *x, initial_state, seq_offsets, kept = ctx.saved_tensors
@@ -137,11 +137,10 @@ class _DecayAttention(torch.autograd.Function):
             seq_offsets, n = seq_offsets.contiguous(), seq_offsets.numel() - 1
         if initial_state is not None:
             initial_state = initial_state.contiguous()
-        go = torch.zeros(x[2].shape, dtype=x[2].dtype, device=dev) if go is None else \
-            go.contiguous()
+        go = _like(x[2]).zero_() if go is None else go.contiguous()
         gstate = None if gstate is None else gstate.contiguous()
         decays = ctx.needs_input_grad[3]
-        grads = [torch.empty(y.shape, dtype=y.dtype, device=dev) for y in x[:3 + decays]]
+        grads = [_like(y) for y in x[:3 + decays]]
         ds = torch.empty((n, hv, dk, dv), dtype=torch.float32, device=dev) \
             if ctx.needs_input_grad[4] else None
         nbytes = N.lib().bs_decay_attention_grad_workspace_size(

@@ -6,7 +6,7 @@ import struct
 import torch
 
 from . import _native as N
-from ._sequence import _DTYPES, _address, _floating, _recorded, _rows
+from ._sequence import _DTYPES, _address, _floating, _like, _once, _recorded, _rows
 
 _NORM_IN = struct.Struct('5P3qQ4i2I2f')      # bs_layer_norm_in
 
@@ -34,12 +34,15 @@ def _chance(p, seed, site, dev):
 
 
 def _dropout(x, drop, scale, seed, held, site):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if x.numel():
+    y, n = _like(x), x.numel()
+    if n:
         dim = x.shape[-1]
-        rows = _rows(x, dim)
-        N.call('bs_dropout', x.device, _address(rows), _DTYPES[x.dtype], rows.shape[0], dim,
-               rows.stride(0), seed, _address(held), site, drop, scale, _address(y))
+        rows, stride = (x, dim) if x.is_contiguous() else (None, 0)
+        if rows is None:
+            rows = _rows(x, dim)
+            stride = rows.stride(0)
+        N.call('bs_dropout', x.device, _address(rows), _DTYPES[x.dtype], n // dim, dim, stride, seed,
+               _address(held), site, drop, scale, _address(y))
     return y
 
 
@@ -53,7 +56,7 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, drop, scale, seed, held, site)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gy):
         _recorded('dropout', gy)
         drop, scale, seed, site = ctx.args
@@ -116,8 +119,8 @@ def _pack(x, residual, weight, bias, chance, site, eps):
 def _forward(x, residual, weight, bias, chance, site, eps, keep):
     """(stream or None, normed, statistics or None)."""
     hold, packed, rows, _ = _pack(x, residual, weight, bias, chance, site, eps)
-    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stream = torch.empty_like(normed) if residual is not None else None
+    normed = _like(x)
+    stream = _like(x) if residual is not None else None
     stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if keep else None
     N.call('bs_layer_norm', x.device, packed, _address(stream), _address(normed), _address(stats))
     return stream, normed, stats
@@ -137,7 +140,7 @@ class _LayerNorm(torch.autograd.Function):
         return stream, normed
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gs, gn):
         _recorded('layer_norm', gs, gn)
         x, residual, weight, bias, held, stats = ctx.saved_tensors
@@ -146,7 +149,7 @@ class _LayerNorm(torch.autograd.Function):
                                         eps)
         gs, gn = (None if t is None else t.contiguous() for t in (gs, gn))
         dev = x.device
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
+        grads = [_like(t) if need else None
                  for t, need in zip((x, residual, weight, bias), ctx.needs_input_grad)]
         if not drop and grads[0] is not None:      # one gradient for both
             grads[1] = None

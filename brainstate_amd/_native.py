@@ -269,14 +269,30 @@ def stream_handle(device=None):
     return ctypes.c_void_p(raw_stream(device))
 
 
+_entries = {}
+
+
+def _entry(name):
+    """(entry point, torch's current device, torch's current stream of one) for :func:`call`."""
+    import torch
+    torch.cuda.current_device()        # initialises torch's side
+    got = (getattr(lib(), name), getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device),
+           getattr(torch._C, '_cuda_getCurrentRawStream', None) or
+           (lambda i: torch.cuda.current_stream(i).cuda_stream))
+    _entries[name] = got
+    return got
+
+
 def call(name, device, *args):
     """Entry point ``name`` on the current stream of ``device``, which need not be the current
     device."""
-    import torch
-    f = getattr(lib(), name)
-    if device.index is None or device.index == torch.cuda.current_device():
-        rc = f(*args, raw_stream(device))
+    f, current, stream = _entries.get(name) or _entry(name)
+    index = device.index
+    if index is None or index == current():
+        rc = f(*args, stream(current() if index is None else index))
     else:
+        import torch
         with torch.cuda.device(device):
-            rc = f(*args, raw_stream(device))
-    check(rc, name)
+            rc = f(*args, stream(index))
+    if rc != BS_OK:
+        check(rc, name)

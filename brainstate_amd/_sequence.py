@@ -77,6 +77,21 @@ def _address(t):
         return N.ptr(t).value
 
 
+def _once(backward):
+    """``backward`` of a Function, itself without a derivative: what autograd has to be told only where
+    it records the backward pass."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
+def _like(t):
+    """An uninitialised tensor like ``t``, contiguous."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 # ------------------------------------------------------------------------- gated delta rule
 def _delta_operands(q, k, v, g, beta, scale):
     """Checked operands as (views, bytes of bs_delta_in, sizes)."""

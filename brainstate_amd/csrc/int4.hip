@@ -7,7 +7,7 @@
 // three exact bf16 parts (lane_types.h).  u - 8 has 4 bits and is exact in either type, so the
 // products are exact and the sums 32-bit; a group's sum is multiplied by its scale in 32 bits, when
 // it is whole, so no weight is ever rounded.  u - 8 goes through the instruction that makes a float
-// of a 4-bit integer, which gives sixteenths: scales are taken 16 times.
+// of a 4-bit integer, which gives sixteenths: sums are taken 16 times at the end.
 //
 // Few tokens (few_kernel): bound by the weights' bytes, and below a few MB by the latency of one
 // pass over k.  Many tokens (tile_kernel): bound by the matrix cores.
@@ -58,9 +58,14 @@ struct Form<bs_f16> {
 template <typename T>
 __device__ __forceinline__ uint4 weights(uint32_t u) {
   u ^= 0x88888888u;           // two's complement
+  uint32_t v = u >> 4;
+  asm("" : "+v"(v));          // else the bytes below are cut out of u, an instruction each
   float f[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = __builtin_amdgcn_cvt_off_f32_i4((int)(u >> 4 * i));
+  for (int i = 0; i < 4; ++i) {        // the instruction takes a byte of a register by itself
+    f[2 * i] = __builtin_amdgcn_cvt_off_f32_i4((int)(u >> 8 * i & 255));
+    f[2 * i + 1] = __builtin_amdgcn_cvt_off_f32_i4((int)(v >> 8 * i & 255));
+  }
   return make_uint4(Form<T>::pair(f[0], f[1]), Form<T>::pair(f[2], f[3]),
                     Form<T>::pair(f[4], f[5]), Form<T>::pair(f[6], f[7]));
 }
@@ -138,7 +143,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const T* x, int64_t
     for (int h = 0; h < H; ++h) {
       load_words<W>(wr, (k + G * h + G / 4 * g) / 2, bytes, whole, w[h]);
       const int at = k / G + h;
-      s[h] = whole || at < groups ? 16.f * sr[at] : 0.f;
+      s[h] = whole || at < groups ? sr[at] : 0.f;
     }
   };
   auto multiply = [&](int k, bool whole, uint32_t (*w)[W], const float* s) {
@@ -193,6 +198,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const T* x, int64_t
     float y = 0.f;
 #pragma unroll
     for (int v = 0; v < kFewWaves; ++v) y += p[v * MT * 256];
+    y *= 16.f;
     const int m = m0 + 16 * t + e;
     if (m >= o.m || n0 + c >= o.n) continue;
     if (o.bias) y += bs_load_any(o.bias, o.bias_dtype, n0 + c);
@@ -225,7 +231,7 @@ template <typename T, int TM, int TN, int WM, int WN, int G>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const uint16_t* x, int64_t ld,
                                                             int64_t plane, const uint8_t* w4,
                                                             const float* scale, int k_len, Out o,
-                                                            int tiles_m, int tiles_n, int whole) {
+                                                            int tiles_m, int tiles_n) {
   constexpr int PI = Form<T>::kParts, W = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN;
   constexpr int LA = BM * 256 / 1024 / W, H = kStep / G, S = G / 16;   // products of a group
   __shared__ __attribute__((aligned(16))) uint16_t sa0[PI][BM * kStep];
@@ -265,14 +271,25 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const uint16_t* x, i
   };
   struct Weights { uint32_t w[TN][H][S]; float s[TN][H]; } b;
   auto load = [&](int k) {
+    // of a whole step no lane has a test of its own: at a branch of the lanes every load in flight,
+    // the next tokens' too, would be waited for
+    if (k + kStep <= k_len) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+      for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        load_words<S>(gb[j], (k + G * h + G / 2 * g) / 2, bytes, whole, b.w[j][h]);
-        const int at = k / G + h;
-        b.s[j][h] = whole || at < groups ? 16.f * gs[j][at] : 0.f;
-      }
+        for (int h = 0; h < H; ++h) {
+          __builtin_memcpy(b.w[j][h], gb[j] + (k + G * h + G / 2 * g) / 2, 4 * S);
+          b.s[j][h] = gs[j][k / G + h];
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          load_words<S>(gb[j], (k + G * h + G / 2 * g) / 2, bytes, false, b.w[j][h]);
+          b.s[j][h] = k / G + h < groups ? gs[j][k / G + h] : 0.f;
+        }
+    }
   };
   bs_f32x16 acc[TM][TN];
 #pragma unroll
@@ -281,37 +298,47 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const uint16_t* x, i
     for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  // a step is 8 products deep, of 16 values each; weights are unpacked 4 products at a time, so that
+  // one wave's unpacking finds another wave's products to run beside
   auto multiply = [&](const uint16_t (*sa)[BM * kStep], int next) {
     Weights now = b;
     if (next < k_len) load(next);
+    bs_f32x16 c[TM][TN];
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      uint4 wf[TN][S];
+    for (int blk = 0; blk < 2; ++blk) {
+      uint4 wf[TN][4];
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int s = 0; s < S; ++s) wf[j][s] = weights<T>(now.w[j][h][s]);
+        for (int u = 0; u < 4; ++u)
+          wf[j][u] = weights<T>(now.w[j][(4 * blk + u) / S][(4 * blk + u) % S]);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int row = (wm * TM + i) * 32 + r;
-        bs_f32x16 c[TN];
+        uint4 a[4][PI];
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) c[j][e] = 0.f;
-#pragma unroll
-        for (int s = 0; s < S; ++s)
-#pragma unroll
-          for (int p = PI - 1; p >= 0; --p) {
-            const int piece = G / 8 * h + G / 16 * g + s;
-            const uint4 a = *(const uint4*)(sa[p] + row * kStep + 8 * (piece ^ (row & 15)));
-#pragma unroll
-            for (int j = 0; j < TN; ++j) c[j] = Form<T>::mma32(a, wf[j][s], c[j]);
+          for (int p = 0; p < PI; ++p) {
+            const int h = (4 * blk + u) / S, piece = G / 8 * h + G / 16 * g + (4 * blk + u) % S;
+            a[u][p] = *(const uint4*)(sa[p] + row * kStep + 8 * (piece ^ (row & 15)));
           }
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(now.s[j][h], c[j][e], acc[i][j][e]);
+          for (int j = 0; j < TN; ++j) {
+            const int h = (4 * blk + u) / S, at = (4 * blk + u) % S;
+            if (at == 0)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) c[i][j][e] = 0.f;
+#pragma unroll
+            for (int p = PI - 1; p >= 0; --p) c[i][j] = Form<T>::mma32(a[u][p], wf[j][u], c[i][j]);
+            if (at == S - 1)
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                acc[i][j][e] = fmaf(now.s[j][h], c[i][j][e], acc[i][j][e]);
+          }
+        if (S < 8) __builtin_amdgcn_sched_barrier(0);    // else every group's sum lives at once
       }
     }
   };
@@ -342,7 +369,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const uint16_t* x, i
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int m = m0 + (wm * TM + i) * 32 + 8 * (e >> 2) + 4 * g + (e & 3);
-        if (m < o.m) bs_store_any(o.y, o.y_dtype, (int64_t)m * o.n + n, acc[i][j][e] + bias);
+        if (m < o.m) bs_store_any(o.y, o.y_dtype, (int64_t)m * o.n + n, fmaf(16.f, acc[i][j][e], bias));
       }
   }
 }
@@ -425,7 +452,7 @@ void launch_tile(const uint16_t* x, int64_t ld, int64_t plane, const uint8_t* w4
   const int tm = (o.m + 32 * TM * WM - 1) / (32 * TM * WM);
   const int tn = (o.n + 32 * TN * WN - 1) / (32 * TN * WN);
   tile_kernel<T, TM, TN, WM, WN, G><<<(tm * tn + 7) / 8 * 8, 64 * WM * WN, 0, st>>>(
-      x, ld, plane, w4, scale, k, o, tm, tn, k % kStep == 0);
+      x, ld, plane, w4, scale, k, o, tm, tn);
 }
 
 template <typename T, int G>
@@ -435,7 +462,8 @@ void many(const uint16_t* x, int64_t ld, int64_t plane, const uint8_t* w4, const
     return (int64_t)((o.m + bm - 1) / bm) * ((o.n + bn - 1) / bn);
   };
   if (sizeof(T) == 2 && tiles(256, 128) >= bs_num_cus())
-    launch_tile<T, sizeof(T) == 2 ? 4 : 1, 2, 2, 2, G>(x, ld, plane, w4, scale, k, o, st);
+    launch_tile<T, sizeof(T) == 2 ? 2 : 1, 2, sizeof(T) == 2 ? 4 : 2, 2, G>(x, ld, plane, w4, scale,
+                                                                          k, o, st);
   else if (tiles(64, 128) >= bs_num_cus())
     launch_tile<T, 1, 2, 2, 2, G>(x, ld, plane, w4, scale, k, o, st);
   else
