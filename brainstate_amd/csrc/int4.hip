@@ -248,26 +248,31 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const uint16_t* x, i
   const int wm = wave / WN, wn = wave % WN, r = lane & 31, g = lane >> 5;
   const int bytes = (k_len + 1) / 2, groups = (k_len + G - 1) / G;
 
-  const uint16_t* ga[LA];
+  // places as a base of all lanes, which moves along k, and a lane's own 32 bits
+  const char* xb = (const char*)(x + (int64_t)m0 * ld);
+  uint32_t ga[LA];
 #pragma unroll
   for (int i = 0; i < LA; ++i) {
     const int row = 4 * (wave * LA + i) + (lane >> 4);
-    ga[i] = x + min(m0 + row, o.m - 1) * ld + 8 * ((lane & 15) ^ (row & 15));
+    ga[i] = (uint32_t)min(row, o.m - 1 - m0) * (uint32_t)(2 * ld) + 16 * ((lane & 15) ^ (row & 15));
   }
-  const uint8_t* gb[TN];
-  const float* gs[TN];
+  const uint8_t* wb = w4 + (int64_t)n0 * bytes;
+  const float* sb = scale + (int64_t)n0 * groups;
+  uint32_t gb[TN], gs[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
-    const int64_t n = min(n0 + (wn * TN + j) * 32 + r, o.n - 1);
-    gb[j] = w4 + n * bytes, gs[j] = scale + n * groups;
+    const int n = min((wn * TN + j) * 32 + r, o.n - 1 - n0);
+    gb[j] = (uint32_t)n * bytes, gs[j] = (uint32_t)n * groups;
   }
   auto stage = [&](int k, uint16_t (*sa)[BM * kStep]) {
 #pragma unroll
-    for (int p = 0; p < PI; ++p)
+    for (int p = 0; p < PI; ++p) {
+      const char* at = xb + (p * plane + k) * 2;
 #pragma unroll
       for (int i = 0; i < LA; ++i)
-        __builtin_amdgcn_global_load_lds((GlobalPtr)(ga[i] + p * plane + k),
+        __builtin_amdgcn_global_load_lds((GlobalPtr)(at + ga[i]),
                                          (LdsPtr)(sa[p] + (wave * LA + i) * 512), 16, 0, 0);
+    }
   };
   struct Weights { uint32_t w[TN][H][S]; float s[TN][H]; } b;
   auto load = [&](int k) {
@@ -278,16 +283,16 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const uint16_t* x, i
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          __builtin_memcpy(b.w[j][h], gb[j] + (k + G * h + G / 2 * g) / 2, 4 * S);
-          b.s[j][h] = gs[j][k / G + h];
+          __builtin_memcpy(b.w[j][h], wb + (k + G * h) / 2 + (gb[j] + G / 4 * g), 4 * S);
+          b.s[j][h] = sb[k / G + h + gs[j]];
         }
     } else {
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          load_words<S>(gb[j], (k + G * h + G / 2 * g) / 2, bytes, false, b.w[j][h]);
-          b.s[j][h] = k / G + h < groups ? gs[j][k / G + h] : 0.f;
+          load_words<S>(wb + gb[j], (k + G * h + G / 2 * g) / 2, bytes, false, b.w[j][h]);
+          b.s[j][h] = k / G + h < groups ? sb[gs[j] + k / G + h] : 0.f;
         }
     }
   };
@@ -298,47 +303,67 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const uint16_t* x, i
     for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  // a step is 8 products deep, of 16 values each; weights are unpacked 4 products at a time, so that
-  // one wave's unpacking finds another wave's products to run beside
+  // A step is 8 products deep, of 16 values each, in two halves: a half's weights are unpacked, and
+  // the next 32 tokens read, beside the products before them.
   auto multiply = [&](const uint16_t (*sa)[BM * kStep], int next) {
     Weights now = b;
     if (next < k_len) load(next);
     bs_f32x16 c[TM][TN];
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      uint4 wf[TN][4];
+    uint4 wf[TN][4], wn[TN][4], a[4][PI], an[4][PI];
+    auto unpack = [&](int half, uint4 (*to)[4]) {
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          wf[j][u] = weights<T>(now.w[j][(4 * blk + u) / S][(4 * blk + u) % S]);
+          to[j][u] = weights<T>(now.w[j][(4 * half + u) / S][(4 * half + u) % S]);
+    };
+    auto tokens = [&](int t, uint4 (*to)[PI]) {       // of half t / TM, rows t % TM
+      const int row = (wm * TM + t % TM) * 32 + r;
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int row = (wm * TM + i) * 32 + r;
-        uint4 a[4][PI];
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int p = 0; p < PI; ++p) {
+          const int at = 4 * (t / TM) + u, piece = G / 8 * (at / S) + G / 16 * g + at % S;
+          to[u][p] = *(const uint4*)(sa[p] + row * kStep + 8 * (piece ^ (row & 15)));
+        }
+    };
+    unpack(0, wf);
+    tokens(0, a);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int p = 0; p < PI; ++p) {
-            const int h = (4 * blk + u) / S, piece = G / 8 * h + G / 16 * g + (4 * blk + u) % S;
-            a[u][p] = *(const uint4*)(sa[p] + row * kStep + 8 * (piece ^ (row & 15)));
-          }
+    for (int t = 0; t < 2 * TM; ++t) {
+      const int i = t % TM, half = t / TM;
+      if (t + 1 < 2 * TM) tokens(t + 1, an);
+      if (t == 0) unpack(1, wn);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            const int h = (4 * blk + u) / S, at = (4 * blk + u) % S;
-            if (at == 0)
+        for (int j = 0; j < TN; ++j) {
+          const int h = (4 * half + u) / S, at = (4 * half + u) % S;
+          if (at == 0)
 #pragma unroll
-              for (int e = 0; e < 16; ++e) c[i][j][e] = 0.f;
+            for (int e = 0; e < 16; ++e) c[i][j][e] = 0.f;
 #pragma unroll
-            for (int p = PI - 1; p >= 0; --p) c[i][j] = Form<T>::mma32(a[u][p], wf[j][u], c[i][j]);
-            if (at == S - 1)
+          for (int p = PI - 1; p >= 0; --p) c[i][j] = Form<T>::mma32(a[u][p], wf[j][u], c[i][j]);
+          if (at == S - 1)
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                acc[i][j][e] = fmaf(now.s[j][h], c[i][j][e], acc[i][j][e]);
-          }
-        if (S < 8) __builtin_amdgcn_sched_barrier(0);    // else every group's sum lives at once
+            for (int e = 0; e < 16; ++e)
+              acc[i][j][e] = fmaf(now.s[j][h], c[i][j][e], acc[i][j][e]);
+        }
+      __builtin_amdgcn_sched_group_barrier(0x100, 4 * PI, 0);      // the next tokens first,
+#pragma unroll
+      for (int q = 0; q < 4 * TN * PI; ++q) {                      // then products with 16 others
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 16, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int p = 0; p < PI; ++p) a[u][p] = an[u][p];
+        if (t == TM - 1)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) wf[j][u] = wn[j][u];
       }
     }
   };
@@ -439,11 +464,12 @@ int check(int64_t m, int32_t k, int64_t n, int32_t group, const char* who) {
 }
 
 // Whether few_kernel takes the call.
-bool few(int64_t m, int64_t n) { return m <= 64; }
+bool few(int64_t m, int64_t n) { return m <= 16 || (m <= 64 && (n + 15) / 16 <= bs_num_cus()); }
 
 // Whether tile_kernel reads the tokens where they are.
 bool in_place(const void* x, int dtype, int k, int64_t stride) {
-  return dtype != BS_F32 && k % kStep == 0 && stride % 8 == 0 && (uintptr_t)x % 16 == 0;
+  return dtype != BS_F32 && k % kStep == 0 && stride % 8 == 0 && (uintptr_t)x % 16 == 0 &&
+         stride >= 0 && stride < 1 << 22;      // a tile's rows are addressed in 32 bits
 }
 
 template <typename T, int TM, int TN, int WM, int WN, int G>
@@ -461,11 +487,13 @@ void many(const uint16_t* x, int64_t ld, int64_t plane, const uint8_t* w4, const
   auto tiles = [&](int bm, int bn) {
     return (int64_t)((o.m + bm - 1) / bm) * ((o.n + bn - 1) / bn);
   };
-  if (sizeof(T) == 2 && tiles(256, 128) >= bs_num_cus())
-    launch_tile<T, sizeof(T) == 2 ? 2 : 1, 2, sizeof(T) == 2 ? 4 : 2, 2, G>(x, ld, plane, w4, scale,
-                                                                          k, o, st);
+  constexpr bool kLarge = sizeof(T) == 2 && G == kStep, kWide = sizeof(T) == 2 || G > 32;
+  if (kLarge && tiles(128, 256) >= bs_num_cus())
+    launch_tile<T, kLarge ? 4 : 2, 1, 1, kLarge ? 8 : 4, G>(x, ld, plane, w4, scale, k, o, st);
+  else if (kWide && tiles(64, 256) >= bs_num_cus())
+    launch_tile<T, 2, 1, 1, kWide ? 8 : 4, G>(x, ld, plane, w4, scale, k, o, st);
   else if (tiles(64, 128) >= bs_num_cus())
-    launch_tile<T, 1, 2, 2, 2, G>(x, ld, plane, w4, scale, k, o, st);
+    launch_tile<T, 2, 1, 1, 4, G>(x, ld, plane, w4, scale, k, o, st);
   else
     launch_tile<T, 1, 1, 2, 2, G>(x, ld, plane, w4, scale, k, o, st);
 }
