@@ -289,7 +289,11 @@ int grid_of(int64_t rows, const Shape& s, int threads) {   // threads: wanted on
   return (int)(need < most ? need : most);
 }
 
-constexpr int kThreads = 2048, kGradThreads = 512;   // a CU
+// Threads on a CU.  Forward and backward of 8,192 rows of 2,048 in bf16 take 153 us at 2,048 forward
+// ones (172 at 512, 157 at 1,024, 152 at 4,096, which takes 2,048 rows of 16,384 from 48 us to 55); the
+// gradients, whose workgroups each leave a row of sums, 226 us for 2,048 rows of 16,384 at 512 and
+// 1,024, 257 at 2,048.
+constexpr int kThreads = 2048, kGradThreads = 512;
 
 // f(lanes of a row or 0, runs a lane, largest workgroup, mode)
 template <typename F>
