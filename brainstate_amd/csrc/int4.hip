@@ -463,8 +463,14 @@ int check(int64_t m, int32_t k, int64_t n, int32_t group, const char* who) {
   return BS_OK;
 }
 
-// Whether few_kernel takes the call.
-bool few(int64_t m, int64_t n) { return m <= 16 || (m <= 64 && (n + 15) / 16 <= bs_num_cus()); }
+// Whether few_kernel takes the call: it unpacks each weight once, but a workgroup reads all tokens for
+// its 16 channels.  Against the best tiles, of 4,096 x 4,096 weights in groups of 128, tokens in bf16: 16
+// tokens 7.7 us (24), 32 tokens 12 (25), 64 tokens 22 (25), in 32 bits 43 (47).  Of 8,192 x 8,192, which
+// are two rounds of its workgroups: 32 tokens 40 us (52), 64 tokens 71 (52), in 32 bits 16 tokens 52 (84),
+// 32 tokens 104 (86).
+bool few(int dtype, int64_t m, int64_t n) {
+  return m <= (dtype == BS_F32 ? 16 : 32) || (m <= 64 && (n + 15) / 16 <= bs_num_cus());
+}
 
 // Whether tile_kernel reads the tokens where they are.
 bool in_place(const void* x, int dtype, int k, int64_t stride) {
@@ -484,15 +490,25 @@ void launch_tile(const uint16_t* x, int64_t ld, int64_t plane, const uint8_t* w4
 template <typename T, int G>
 void many(const uint16_t* x, int64_t ld, int64_t plane, const uint8_t* w4, const float* scale,
           int k, const Out& o, hipStream_t st) {
-  auto tiles = [&](int bm, int bn) {
-    return (int64_t)((o.m + bm - 1) / bm) * ((o.n + bn - 1) / bn);
+  // A launch takes its rounds of a workgroup a CU, and a round of tiles of 128 x 256, 64 x 256, 64 x 128
+  // and 64 x 64 about 75, 46, 34 and 25 us at 4,096 values in groups of 128 in bf16, and in that
+  // proportion for the others.  The largest tiles: 8,192 tokens x 4,096 channels 304 us (365, 379, 517
+  // with the others).  1,500 tokens: 72 (88, 79, 100); 700 tokens: 46 with the second (70, 48, 52); 512
+  // tokens: 35 with the third (69, 45, 36); 256 tokens: 26 with the last (67, 44, 34).  With the other
+  // groups' or 32-bit sums beside them the larger ones do not fit the registers.
+  auto rounds = [&](int bm, int bn) {
+    const int64_t tiles = (int64_t)((o.m + bm - 1) / bm) * ((o.n + bn - 1) / bn);
+    return (tiles + bs_num_cus() - 1) / bs_num_cus();
   };
   constexpr bool kLarge = sizeof(T) == 2 && G == kStep, kWide = sizeof(T) == 2 || G > 32;
-  if (kLarge && tiles(128, 256) >= bs_num_cus())
+  const int64_t large = 75 * rounds(128, 256), wide = 46 * rounds(64, 256),
+                mid = 34 * rounds(64, 128), small = 25 * rounds(64, 64);
+  const int64_t least = mid < small ? mid : small, wider = kWide && wide < least ? wide : least;
+  if (kLarge && large <= wider)
     launch_tile<T, kLarge ? 4 : 2, 1, 1, kLarge ? 8 : 4, G>(x, ld, plane, w4, scale, k, o, st);
-  else if (kWide && tiles(64, 256) >= bs_num_cus())
+  else if (kWide && wide <= least)
     launch_tile<T, 2, 1, 1, kWide ? 8 : 4, G>(x, ld, plane, w4, scale, k, o, st);
-  else if (tiles(64, 128) >= bs_num_cus())
+  else if (mid <= small)
     launch_tile<T, 2, 1, 1, 4, G>(x, ld, plane, w4, scale, k, o, st);
   else
     launch_tile<T, 1, 1, 2, 2, G>(x, ld, plane, w4, scale, k, o, st);
@@ -501,7 +517,7 @@ void many(const uint16_t* x, int64_t ld, int64_t plane, const uint8_t* w4, const
 template <typename T, int G>
 void run(const T* x, int64_t stride, int64_t m, const uint8_t* w4, const float* scale, int k,
          const Out& o, void* workspace, hipStream_t st) {
-  if (few(m, o.n)) {
+  if (few(o.y_dtype, m, o.n)) {
     const unsigned tn = (unsigned)((o.n + 15) / 16);
     if (m <= 16)
       few_kernel<T, 1, G><<<dim3(tn, 1), 64 * kFewWaves, 0, st>>>(x, stride, w4, scale, k, o);
@@ -554,7 +570,7 @@ extern "C" int bs_int4_quantize(const void* w, int32_t dtype, int64_t n, int32_t
 extern "C" size_t bs_int4_workspace_size(const void* x, int32_t dtype, int64_t stride, int64_t m,
                                          int32_t k, int32_t n) {
   if (m < 0 || k < 1 || k > 65536 || !bs_dtype_ok(dtype)) return 0;
-  if (few(m, n) || in_place(x, dtype, k, stride)) return 0;
+  if (few(dtype, m, n) || in_place(x, dtype, k, stride)) return 0;
   return (size_t)m * padded(k) * 2 * (dtype == BS_F32 ? 3 : 1);
 }
 
