@@ -6,12 +6,11 @@
 // by HBM) and is read once and written once whatever the number of tokens.  A workgroup keeps a
 // slice of 32 columns of one head's state in registers: 8 lanes x 4 columns side by side make
 // 128-byte pieces of a row, 32 rows a pass.  The slices of a state run on one XCD, so that pieces
-// which share a line of 128 bytes find it in one L2: 256 states of 16 heads of 100 x 100 take 107 us
+// which share a line of 128 bytes find it in one L2: 256 states of 16 heads of 100 x 100 took 107 us
 // (134 with slices dealt out one by one), 4 tokens of 64 states of 32 heads of 128 x 128 99 (111).
 //
-// 256 states of 32 heads of 128 x 128, one token: 251 us, 4.3 TB/s beside a large copy's 5.1; one
-// state: 5.2 us, the latency of a read, a sum over rows and a write.  With whole rows of 128 columns
-// to a workgroup the large call takes 281 us.
+// 256 states of 32 heads of 128 x 128, one token: 195 us, 5.5 TB/s of states beside a large copy's 5.1;
+// one state: 4.8 us, the latency of a read, a sum over rows and a write.
 #include "delta.h"
 
 namespace {
@@ -19,14 +18,26 @@ namespace {
 constexpr int kCols = 32;      // columns of the state a workgroup holds
 constexpr int kRows = 32;      // rows a pass covers
 
-__device__ __forceinline__ float4 load_cols(const float* p, int n, bool whole) {
-  if (whole) return *(const float4*)p;
+// How a row's columns are read and written: one by one, 4 at a time, or these past the caches.
+enum Columns { kSingle = 0, kFour = 1, kPast = 2 };
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float4 load_cols(const float* p, int n, int cols) {
+  if (cols == kPast) {
+    const f32x4 x = __builtin_nontemporal_load((const f32x4*)p);
+    return make_float4(x[0], x[1], x[2], x[3]);
+  }
+  if (cols == kFour) return *(const float4*)p;
   return make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f,
                      n > 3 ? p[3] : 0.f);
 }
 
-__device__ __forceinline__ void store_cols(float* p, int n, bool whole, const float4& r) {
-  if (whole) {
+__device__ __forceinline__ void store_cols(float* p, int n, int cols, const float4& r) {
+  if (cols == kPast) {
+    __builtin_nontemporal_store(f32x4{r.x, r.y, r.z, r.w}, (f32x4*)p);
+    return;
+  }
+  if (cols == kFour) {
     *(float4*)p = r;
     return;
   }
@@ -46,7 +57,7 @@ __device__ __forceinline__ float sum_rows(float x) {
 template <typename T, int NR>   // NR passes of 32 rows: dk <= 32 NR
 __global__ __launch_bounds__(256) void decay_step_kernel(bs_delta_in in, int tokens, float* state,
                                                          int64_t n_states, const int32_t* slots,
-                                                         T* o, int slices, int vec,
+                                                         T* o, int slices, int cols_of,
                                                          uint32_t heads) {
   __shared__ float4 part[2][4][8];
   // workgroups go round the 8 XCDs in turn; the slices of one state to the same one
@@ -67,12 +78,12 @@ __global__ __launch_bounds__(256) void decay_step_kernel(bs_delta_in in, int tok
     return;
   }
   float* sp = state + (at * in.hv + h) * (int64_t)in.dk * in.dv + c;
-  const bool whole = vec && n >= 4;
+  const int cols = n >= 4 ? cols_of : kSingle;
   float4 s[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const int r = row0 + i * kRows;
-    s[i] = r < in.dk && n > 0 ? load_cols(sp + (int64_t)r * in.dv, n, whole)
+    s[i] = r < in.dk && n > 0 ? load_cols(sp + (int64_t)r * in.dv, n, cols)
                               : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   for (int t = 0; t < tokens; ++t) {
@@ -111,7 +122,7 @@ __global__ __launch_bounds__(256) void decay_step_kernel(bs_delta_in in, int tok
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const int r = row0 + i * kRows;
-    if (r < in.dk && n > 0) store_cols(sp + (int64_t)r * in.dv, n, whole, s[i]);
+    if (r < in.dk && n > 0) store_cols(sp + (int64_t)r * in.dv, n, cols, s[i]);
   }
 }
 
@@ -121,13 +132,17 @@ void launch_step(const bs_delta_in& in, int batch, int tokens, float* state, int
   const int slices = (in.dv + kCols - 1) / kCols;
   const uint32_t heads = (uint32_t)batch * in.hv;
   const unsigned grid = (heads + 7) / 8 * 8 * slices;
-  const int vec = in.dv % 4 == 0 && (uintptr_t)state % 16 == 0;
+  // A state is read and written once a call, and many of them exceed the caches by far: past them 256
+  // states of 32 heads of 128 x 128 take 195 us (233 through them), of 16 heads of 112 x 112 94 (103).
+  // Rows that do not end on 64 bytes share pieces of that size, which the caches put together: 100 x 100
+  // takes 89 us (120 past them).
+  const int cols = in.dv % 4 || (uintptr_t)state % 16 ? kSingle : in.dv % 16 ? kFour : kPast;
   if (in.dk <= 64)
     decay_step_kernel<T, 2><<<grid, 256, 0, st>>>(in, tokens, state, n_states, slots, (T*)o,
-                                                  slices, vec, heads);
+                                                  slices, cols, heads);
   else
     decay_step_kernel<T, 4><<<grid, 256, 0, st>>>(in, tokens, state, n_states, slots, (T*)o,
-                                                  slices, vec, heads);
+                                                  slices, cols, heads);
 }
 
 }  // namespace

@@ -12,6 +12,10 @@
 // it is stored.  Workgroups stay for many rows: a lane's columns are the same in each, so the
 // weights are read once and their gradients are summed in registers, then over the workgroups in
 // their order (weight_sum_kernel): the same bits every time.
+//
+// 8,192 rows of 4,096 in bf16 with dropout of a tenth: forward 65.6 us (268 MB, 4.1 TB/s beside a large
+// copy's 5.1), gradients 89.5 (336 MB and the mask's words again, 3.8), weights' sums 4.9; dropout alone
+// 33.9 (134 MB, 4.0).
 #include "philox.h"
 #include "rows.h"
 
@@ -289,7 +293,7 @@ int grid_of(int64_t rows, const Shape& s, int threads) {   // threads: wanted on
   return (int)(need < most ? need : most);
 }
 
-// Threads on a CU.  Forward and backward of 8,192 rows of 2,048 in bf16 take 153 us at 2,048 forward
+// Threads on a CU.  Forward and backward of 8,192 rows of 4,096 in bf16 take 153 us at 2,048 forward
 // ones (172 at 512, 157 at 1,024, 152 at 4,096, which takes 2,048 rows of 16,384 from 48 us to 55); the
 // gradients, whose workgroups each leave a row of sums, 226 us for 2,048 rows of 16,384 at 512 and
 // 1,024, 257 at 2,048.
