@@ -9,7 +9,7 @@
 // which share a line of 128 bytes find it in one L2: 256 states of 16 heads of 100 x 100 took 107 us
 // (134 with slices dealt out one by one), 4 tokens of 64 states of 32 heads of 128 x 128 99 (111).
 //
-// 256 states of 32 heads of 128 x 128, one token: 195 us, 5.5 TB/s of states beside a large copy's 5.1;
+// 256 states of 32 heads of 128 x 128, one token: 195 to 202 us, 5.4 TB/s of states beside a large copy's 5.1;
 // one state: 4.8 us, the latency of a read, a sum over rows and a write.
 #include "delta.h"
 

@@ -103,6 +103,12 @@ def test_layer_norm_and_dropout_refusals(lib):
     assert lib.bs_dropout(None, F32, 0, 1, 1, 0, None, 0, 0, 1.0, None, None) == N.BS_OK
 
 
+def test_int4_channels_of_one_launch(lib):
+    # 16 channels to a workgroup of 512 threads: from 2^27 on a launch would have 2^32 threads
+    assert _refused(lib, lib.bs_int4_linear(AT, F32, 1, 1, 1, 1 << 27, 32, AT, AT, None, F32, AT, None, 0,
+                                            None), b'channels')
+
+
 def test_int4_refusals(lib):
     def linear(m=1, k=64, n=8, group=32, w4=AT, ws=AT, nbytes=1 << 40, dtype=BF16):
         return lib.bs_int4_linear(AT, dtype, k, m, k, n, group, w4, AT, None, F32, AT, ws, nbytes,
