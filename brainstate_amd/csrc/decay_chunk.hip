@@ -17,9 +17,9 @@
 // 46 us, scan_kernel 20, walk_kernel 111.  The walk is bound by what a wave issues: a chunk takes it
 // about 1,100 vector instructions, most of them splits of the state and its scaled values into parts,
 // 120 products and 110 reads of LDS, and with two waves a SIMD the vector units are busy 40 %, the matrix
-// cores 30 % and LDS 20 % of the time.  8 waves of 16 columns, four a SIMD, take the same 111 us, since each reads Q, K and att
-// again for half the columns; the three gradients' walks of 4 x 2,048 tokens, 16 heads, take 252 us this
-// way and 303 that way.
+// cores 30 % and LDS 20 % of the time.  8 waves of 16 columns, four a SIMD, take the same 111 us, since
+// each reads Q, K and att again for half the columns; the three gradients' walks of 4 x 2,048 tokens, 16
+// heads, take 252 us this way and 303 that way.
 //
 // Numbers: the state and all sums are 32-bit; products take 32-bit operands as three exact bf16
 // parts (lane_types.h).  Sums of log decays are 64-bit, since their differences are exponents.
