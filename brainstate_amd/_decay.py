@@ -5,8 +5,8 @@ import torch
 
 from . import _native as N
 from . import _trace
-from ._sequence import (_DELTA_IN, _DTYPES, _address, _floating, _heads, _like, _once, _recorded,
-                        _states, _tangent, _wants_grad)
+from ._sequence import (_DELTA_IN, _DTYPES, _address, _fits, _floating, _heads, _like, _once,
+                        _recorded, _states, _tangent, _wants_grad)
 
 
 def _operands(q, k, v, g, scale):
@@ -27,6 +27,8 @@ def _operands(q, k, v, g, scale):
         raise ValueError(f'head sizes {dk}, {dv} outside 1..128')
     if g.shape != vshape[:3] and g.shape != (hv,):
         raise ValueError(f'g must be {tuple(vshape[:3])} or [{hv}]: got {tuple(g.shape)}')
+    _fits(b, 'batch rows')
+    _fits(t, 'tokens')
     dev = q.device
     if not (dev == k.device == v.device == g.device):
         raise ValueError('q, k, v and g must be on one device')
@@ -94,8 +96,9 @@ def _forward(q, k, v, g, scale, initial_state, seq_offsets, keep):
         if seq_offsets.dtype != torch.int32 or seq_offsets.dim() != 1 or \
                 seq_offsets.numel() < 1 or seq_offsets.device != dev:
             raise ValueError(f'seq_offsets must be int32 [sequences + 1] on {dev}')
-        seq_offsets = seq_offsets.contiguous()
         n = seq_offsets.numel() - 1
+        _fits(n, 'sequences')
+        seq_offsets = seq_offsets.contiguous()
     if initial_state is not None:
         _states('initial_state', initial_state, n, hv, dk, dv, dev)
         initial_state = initial_state.contiguous()

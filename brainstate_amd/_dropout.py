@@ -64,8 +64,8 @@ class _Dropout(torch.autograd.Function):
 
 
 def dropout(x, p, seed, site=0):
-    """``x`` [.., dim] with each element dropped, to 0, with probability ``p`` in [0, 1) and the
-    others times 1 / (1 - p).
+    """``x`` [.., dim], dim below 2^31, with each element dropped, to 0, with probability ``p`` in
+    [0, 1) and the others times 1 / (1 - p).
 
     Element (row, column) of the rows [.., dim] is kept where word column % 4 of the Philox 4x32-10
     generator with counter (column // 4, site, row) and key ``seed`` is at least p 2^32: the same
@@ -75,8 +75,8 @@ def dropout(x, p, seed, site=0):
     model apart that share one.  What is dropped is 0 whatever it was.  Differentiable in ``x``, in
     reverse mode."""
     _floating('x', x)
-    if x.dim() < 1:
-        raise ValueError('x must have a dimension')
+    if x.dim() < 1 or x.shape[-1] >= 1 << 31:
+        raise ValueError(f'x [.., dim] with dim in 0..2^31 - 1: got {tuple(x.shape)}')
     args = _chance(p, seed, site, x.device)
     if _recorded('dropout', x):
         return _Dropout.apply(x, *args, site)

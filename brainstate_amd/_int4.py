@@ -4,7 +4,7 @@
 import torch
 
 from . import _native as N
-from ._sequence import _DTYPES, _address, _floating, _no_grad, _rows
+from ._sequence import _DTYPES, _address, _fits, _floating, _no_grad, _rows
 
 _GROUPS = (32, 64, 128)
 
@@ -51,6 +51,7 @@ def int4_linear(x, w4, w_scale, bias=None, group=128):
             w4.shape[1] != (k + 1) // 2 or w4.device != dev:
         raise ValueError(f'w4 must be uint8 [channels, {(k + 1) // 2}] on {dev}')
     n, groups = w4.shape[0], -(-k // group)
+    _fits(n, 'channels')
     if not isinstance(w_scale, torch.Tensor) or w_scale.dtype != torch.float32 or \
             w_scale.shape != (n, groups) or w_scale.device != dev:
         raise ValueError(f'w_scale must be float32 [{n}, {groups}] on {dev}')

@@ -179,7 +179,7 @@ SIGNATURES = {
     'bs_norm_gate_residual': (ctypes.c_int, [c_vp] * 4),
     'bs_norm_grad_workspace_size': (c_size, [ctypes.c_int64, c_i32]),
     'bs_norm_gate_residual_grad': (ctypes.c_int, [c_vp] * 10 + [c_size, c_vp]),
-    'bs_dropout': (ctypes.c_int, [c_vp, c_i32, ctypes.c_int64, c_i32, ctypes.c_int64,
+    'bs_dropout': (ctypes.c_int, [c_vp, c_i32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                   ctypes.c_uint64, c_vp, ctypes.c_uint32, ctypes.c_uint32, c_f32,
                                   c_vp, c_vp]),
     'bs_layer_norm': (ctypes.c_int, [c_vp] * 5),

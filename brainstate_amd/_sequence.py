@@ -31,6 +31,12 @@ def _floating(name, t, dtype=None):
     return number
 
 
+def _fits(n, what):
+    """Raises for a size past the entry points' 32-bit arguments, which ctypes would cut off."""
+    if n >= 1 << 31:
+        raise ValueError(f'{n} {what} exceed 2^31 - 1')
+
+
 def _wants_grad(*ts):
     if torch.is_grad_enabled():
         for t in ts:
@@ -112,6 +118,8 @@ def _delta_operands(q, k, v, g, beta, scale):
     if g.shape != vshape[:3] or beta.shape != vshape[:3]:
         raise ValueError(f'g and beta must be {tuple(vshape[:3])}: got {tuple(g.shape)}, '
                          f'{tuple(beta.shape)}')
+    _fits(b, 'batch rows')
+    _fits(t, 'tokens')
     dev = q.device
     if not (dev == k.device == v.device == g.device == beta.device):
         raise ValueError('q, k, v, g and beta must be on one device')
@@ -199,8 +207,9 @@ def _delta_forward(q, k, v, g, beta, scale, initial_state, seq_offsets, keep):
         if seq_offsets.dtype != torch.int32 or seq_offsets.dim() != 1 or \
                 seq_offsets.numel() < 1 or seq_offsets.device != dev:
             raise ValueError(f'seq_offsets must be int32 [sequences + 1] on {dev}')
-        seq_offsets = seq_offsets.contiguous()
         n = seq_offsets.numel() - 1
+        _fits(n, 'sequences')
+        seq_offsets = seq_offsets.contiguous()
     if initial_state is not None:
         _states('initial_state', initial_state, n, hv, dk, dv, dev)
         initial_state = initial_state.contiguous()
@@ -420,6 +429,7 @@ def _int8_product(x, x_scale, w8, w_scale, bias, out_dtype):
     if not isinstance(w8, torch.Tensor) or w8.dtype != torch.int8 or w8.dim() != 2 or w8.device != dev:
         raise ValueError(f'w8 must be int8 [channels, k] on {dev}')
     n, k = w8.shape
+    _fits(n, 'channels')
     if x.dim() < 1 or x.shape[-1] != k or not 1 <= k <= 65536:
         raise ValueError(f'tokens [.., {k}] with k in 1..65536 expected: got {tuple(x.shape)}')
     w8 = w8.contiguous()

@@ -387,16 +387,18 @@ extern "C" int bs_layer_norm_grad(const bs_layer_norm_in* in, const void* grad_s
   return BS_OK;
 }
 
-extern "C" int bs_dropout(const void* x, int32_t dtype, int64_t rows, int32_t dim, int64_t stride,
+extern "C" int bs_dropout(const void* x, int32_t dtype, int64_t rows, int64_t dim, int64_t stride,
                           uint64_t seed, const int64_t* seed_at, uint32_t site, uint32_t drop,
                           float scale, void* y, bs_stream_t stream) {
   BS_CHECK_ARG(bs_dtype_ok(dtype), "bs_dropout: dtype unknown");
-  BS_CHECK_ARG(rows >= 0 && dim >= 1, "bs_dropout: %lld rows of %d values", (long long)rows, dim);
+  BS_CHECK_ARG(rows >= 0 && dim >= 1 && dim <= INT32_MAX,
+               "bs_dropout: %lld rows of %lld values (1..2^31 - 1)", (long long)rows,
+               (long long)dim);
   if (rows == 0) return BS_OK;
   BS_CHECK_ARG(x && y, "bs_dropout: NULL pointer");
   hipStream_t st = bs_stream(stream);
-  const int64_t per = ((int64_t)dim + kVec - 1) / kVec, most = (1ll << 31) / per;
-  DropoutIn in = {x, y, stride, 0, seed, seed_at, 0, (uint32_t)per, dim, site, drop, scale};
+  const int64_t per = (dim + kVec - 1) / kVec, most = (1ll << 31) / per;
+  DropoutIn in = {x, y, stride, 0, seed, seed_at, 0, (uint32_t)per, (int)dim, site, drop, scale};
   // a launch has fewer than 2^32 threads: rows in pieces
   for (; in.row0 < rows; in.row0 += most) {
     const int64_t n = rows - in.row0 < most ? rows - in.row0 : most;

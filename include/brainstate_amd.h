@@ -656,8 +656,8 @@ BS_API int bs_norm_gate_residual_grad(const bs_norm_in* in, const void* grad_str
  * Philox 4x32-10 generator with counter (column / 4, site, row mod 2^32, row / 2^32) and key (seed
  * mod 2^32, seed / 2^32) is at least `drop` (p 2^32), and gives 0 elsewhere, whatever lies there.
  * The seed is *seed_at (device memory, read when the kernel runs) where that is given.  x has rows
- * `stride` elements apart, y [rows, dim] is of the same type.  The gradient is the same call. */
-BS_API int bs_dropout(const void* x, int32_t dtype, int64_t rows, int32_t dim, int64_t stride,
+ * of 1..2^31 - 1 values `stride` elements apart, y [rows, dim] is of the same type.  The gradient is the same call. */
+BS_API int bs_dropout(const void* x, int32_t dtype, int64_t rows, int64_t dim, int64_t stride,
                       uint64_t seed, const int64_t* seed_at, uint32_t site, uint32_t drop,
                       float scale, void* y, bs_stream_t stream);
 
