@@ -109,6 +109,14 @@ struct Splitter {
   }
 };
 
+// The same parts with a value's rest from that value alone.  Splitter's dot product takes its neighbour
+// times 0, which an infinity makes NaN: no matter where a product sums over both, but the values of a
+// key are rows of the state.
+struct Cutter {
+  template <int P>
+  __device__ __forceinline__ bs_parts<P> split(const float* x) const { return bs_split8<P>(x); }
+};
+
 // An operand's rows of one head; strides in bytes.
 struct HeadRows {
   const char* p;
@@ -174,8 +182,8 @@ __device__ __forceinline__ void floats(const uint4* x, float* f) {
   for (int j = 0; j < 8; ++j) f[j] = bs_to_f32(t[j]);
 }
 
-template <typename T>
-__device__ __forceinline__ bs_parts<kParts<T>> parts_of(const Splitter& sp, const uint4* x) {
+template <typename T, typename S>
+__device__ __forceinline__ bs_parts<kParts<T>> parts_of(const S& sp, const uint4* x) {
   if constexpr (kParts<T> == 1) {
     bs_parts<1> o;
     o.p[0] = __builtin_bit_cast(bs_bf16x8, x[0]);
@@ -183,7 +191,7 @@ __device__ __forceinline__ bs_parts<kParts<T>> parts_of(const Splitter& sp, cons
   } else {
     float f[8];
     floats<T>(x, f);
-    return sp.split<kParts<T>>(f);
+    return sp.template split<kParts<T>>(f);
   }
 }
 
@@ -199,7 +207,8 @@ struct Staged {
       r.raw(threadIdx.x / kPer + i * kRows, threadIdx.x % kPer * 8, x[i]);
   }
   // as bf16 parts, [part][64][D]
-  __device__ __forceinline__ void put(uint16_t* to, const Splitter& sp) const {
+  template <typename S>
+  __device__ __forceinline__ void put(uint16_t* to, const S& sp) const {
     const int at = place<D>(threadIdx.x / kPer, threadIdx.x % kPer);
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
@@ -470,7 +479,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void sum_kernel(D
   for (int at = 0; more; at ^= 1) {
     const Place l(true);
     __syncthreads();
-    k.put(lk, sp);
+    k.put(lk, Cutter());
     v.put_raw(lv);
     __syncthreads();
     more = ahead;
@@ -611,7 +620,7 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
   };
   auto put = [&]() {
     q.put(lq, sp);
-    k.put(lk, sp);
+    k.put(lk, Cutter());
     v.put_raw(lv);
   };
   DecayChunk c, next;
