@@ -574,6 +574,28 @@ __device__ __forceinline__ void straight_v(const T* v, int at, int step, uint4* 
   }
 }
 
+// Sets infinities and NaN among the values of a word to 0; whether there were any.
+template <typename T>
+__device__ __forceinline__ bool drop_values(uint32_t& w) {
+  constexpr uint32_t kExp = std::is_same<T, bs_f16>::value ? 0x7C00u : 0x7F80u;   // bits of an exponent
+  const bool high = (w & kExp << 16) == kExp << 16, low = (w & kExp) == kExp;
+  if constexpr (sizeof(T) == 4) {
+    w = high ? 0u : w;
+    return high;
+  } else {
+    w = high ? w & 0xFFFFu : w;
+    w = low ? w & 0xFFFF0000u : w;
+    return high | low;
+  }
+}
+
+// Value `col` of row j of V.
+template <typename T>
+__device__ __forceinline__ float value_at(const T* v, int j, int col) {
+  if constexpr (sizeof(T) == 4) return v[j * kPitch + col];
+  else return bs_to_f32(*(const T*)((const char*)v + place<kPitch>(j, col >> 3) + 2 * (col & 7)));
+}
+
 template <typename T, int RT, bool VEC, bool GRAD>
 __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(Runs runs,
                                                                               DecayPlan plan) {
@@ -760,6 +782,25 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
     if (live) {
       uint4 vf[4][W];
       turned_v<T>(lv, col, l, vf);
+      // A token takes nothing from a later one, but its 0 in att times an infinity or NaN is NaN.  One in
+      // a value column leaves every row of that column of the state so: a look at one row tells.  Such
+      // values are left out of the product here and taken one by one below.
+      const bool was = isfinite(s.s[0][0]);
+      s.template add<T, DC>(lk, vf, co, run.add_scale, l, sp);
+      uint32_t apart = 0;                      // bit m: column value_row(m) has such values
+      if (__ballot(was && !isfinite(s.s[0][0]))) {
+        bool any = false;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            any |= drop_values<T>(vf[ks][w].x) | drop_values<T>(vf[ks][w].y) |
+                   drop_values<T>(vf[ks][w].z) | drop_values<T>(vf[ks][w].w);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        const uint64_t hit = __ballot(any);
+        apart = (uint32_t)hit | (uint32_t)(hit >> 32);
+      }
       const int aa = place<64>(l.m, l.g);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
@@ -773,8 +814,24 @@ __global__ __launch_bounds__(kThreads, kParts<T> == 1 ? 2 : 1) void walk_kernel(
           o[it] = mma(vp, ap, o[it]);
         }
       }
-      s.template add<T, DC>(lk, vf, co, run.add_scale, l, sp);
       const int oc = col + 16 * l.g;
+      if (apart) {
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll 1
+          for (int j = 0; j <= 32 * it + l.m; ++j) {
+            const char* p = (const char*)la + place<64>(32 * it + l.m, j >> 3) + 2 * (j & 7);
+            float a = 0.f;
+#pragma unroll
+            for (int x = 2; x >= 0; --x) a += bs_to_f32(*(const bs_bf16*)(p + x * 128 * 64));
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (apart >> (8 * (e >> 2) + 4 * l.g + (e & 3)) & 1) {
+                const float x = value_at(lv, j, oc + e);
+                if (!isfinite(x)) o[it][e] = fmaf(a, x, o[it][e]);
+              }
+          }
+      }
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
         const int i = 32 * it + l.m;
