@@ -425,15 +425,23 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* w, int64_t strid
   const float most = __uint_as_float(top), a = most / 7.f;
   if (threadIdx.x % L == 0) scale[row * groups + group] = a;
   // 7 w is exact for 16-bit values, so quotients of exactly a half round to even there; both sides of
-  // the quotient are divided by 16 where 7 w could overflow
+  // the quotient are divided by 16 where 7 w could overflow.  In 32 bits it is off by 3 roundings, so one
+  // beside a half is formed again in 64: 7 w is exact there, and a quotient of 27 bits by 24 that is no
+  // half is 2^-28 away from one.  8,192 x 8,192: 124 us in 32 bits (123 without), 90 in bf16.
   const float up = most > 1e37f ? 7.f / 16.f : 7.f, den = most > 1e37f ? most / 16.f : most;
-  const bool ok = a > 0.f && a < INFINITY;     // a group of 0, or with NaN or infinity, is 0: its
-                                               // scale makes the result 0 or NaN
+  const bool ok = most > 0.f && most < INFINITY;   // a group of 0, or with NaN or infinity, is 0: its
+                                                   // scale makes the result 0 or NaN
+  auto nearest = [&](float x) {
+    const float q = up * x / den;
+    float r = rintf(q);
+    if constexpr (sizeof(T) == 4)
+      if (fabsf(fabsf(q - r) - 0.5f) < 1e-5f) r = (float)rint(7.0 * (double)x / (double)most);
+    return (int)r + 8;
+  };
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
     if (c + j >= k) continue;
-    const int lo = ok ? (int)rintf(up * f[j] / den) + 8 : 8;
-    const int hi = ok ? (int)rintf(up * f[j + 1] / den) + 8 : 8;
+    const int lo = ok ? nearest(f[j]) : 8, hi = ok ? nearest(f[j + 1]) : 8;
     w4[row * bytes + (c + j) / 2] = (uint8_t)(lo | hi << 4);
   }
 }
