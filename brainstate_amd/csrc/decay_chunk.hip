@@ -14,7 +14,7 @@
 // transposed operands (K^T, V^T) are read from LDS by its transposing reads.
 //
 // 8,192 tokens of 32 heads of 128 x 128 in bf16 (268 MB, 53 us at a large copy's 5.1 TB/s): sum_kernel
-// 46 us, scan_kernel 20, walk_kernel 111.  The walk is bound by what a wave issues: a chunk takes it
+// 46 us, scan_kernel 20, walk_kernel 112.  The walk is bound by what a wave issues: a chunk takes it
 // about 1,100 vector instructions, most of them splits of the state and its scaled values into parts,
 // 120 products and 110 reads of LDS, and with two waves a SIMD the vector units are busy 40 %, the matrix
 // cores 30 % and LDS 20 % of the time.  8 waves of 16 columns, four a SIMD, take the same 111 us, since
@@ -22,7 +22,8 @@
 // heads, take 252 us this way and 303 that way.
 //
 // Numbers: the state and all sums are 32-bit; products take 32-bit operands as three exact bf16
-// parts (lane_types.h).  Sums of log decays are 64-bit, since their differences are exponents.
+// parts (lane_types.h).  Sums of log decays are 64-bit, since their differences are exponents.  An
+// infinity or NaN reaches the outputs and states from its token on, as by the formula.
 #include "decay.h"
 #include "decay_slots.h"
 
@@ -957,9 +958,10 @@ DecayPlan decay_plan(const bs_delta_in& in, int seqs, int tokens, const int32_t*
   p.hv = in.hv, p.g = in.g, p.g_dtype = in.g_dtype;
   for (int i = 0; i < 3; ++i) p.g_stride[i] = in.g_stride[i];
   // As many segments as the card takes workgroups at a time: 8,192 tokens of 32 heads in bf16 take 165
-  // us with two workgroups a CU, 195 with one, 193 with three.  Of 2 chunks at least: a ragged batch of
-  // 5,003 tokens, 8 heads, takes 53 us so, 52 with 1, 59 with 4, 93 with 8, and a state a chunk is what
-  // the carry reads and writes.
+  // us with two workgroups a CU, 195 with one, 193 with three.  Of 2 chunks at least, since a state a
+  // segment is what the carry reads and writes: 16,384 tokens of one head of 128 in bf16 take 65 us so, 85
+  // with 1, 68 with 4; 2,048 tokens of 4 heads 39, 36 and 56; 700 tokens of 3 heads of 48 in 32 bits, where
+  // the latency of a chunk is most of it, 33, 24 and 54.
   const int64_t units = (int64_t)p.seq.slots * in.hv;
   const int64_t at_once = (in.dtype == BS_BF16 ? 2 : 1) * bs_num_cus();
   int64_t per = (units + at_once - 1) / at_once;

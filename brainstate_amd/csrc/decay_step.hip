@@ -6,8 +6,9 @@
 // by HBM) and is read once and written once whatever the number of tokens.  A workgroup keeps a
 // slice of 32 columns of one head's state in registers: 8 lanes x 4 columns side by side make
 // 128-byte pieces of a row, 32 rows a pass.  The slices of a state run on one XCD, so that pieces
-// which share a line of 128 bytes find it in one L2: 256 states of 16 heads of 100 x 100 took 107 us
-// (134 with slices dealt out one by one), 4 tokens of 64 states of 32 heads of 128 x 128 99 (111).
+// which share a line of 128 bytes find it in one L2: 256 states of 16 heads of 100 x 100 take 90 us, 4
+// tokens of 64 states of 32 heads of 128 x 128 78 (107 and 99 before launch_step chose how columns are
+// read, 134 and 111 then with slices dealt out one by one).
 //
 // 256 states of 32 heads of 128 x 128, one token: 195 to 202 us, 5.4 TB/s of states beside a large copy's 5.1;
 // one state: 4.8 us, the latency of a read, a sum over rows and a write.

@@ -12,8 +12,8 @@
 // Few tokens (few_kernel): bound by the weights' bytes, and below a few MB by the latency of one
 // pass over k: 4,096 x 4,096 with groups of 128 for one token in bf16 5.5 us, 8,192 x 8,192 13 us (2.7
 // TB/s).  Many tokens (tile_kernel): bound by the matrix cores, and by unpacking and LDS, which the
-// products of one tile wait for: 8,192 tokens x 4,096 x 4,096 in bf16 302 to 314 us, 875 to 910 TFLOP/s
-// beside a library product's 1,260 of weights that are whole; in 32 bits 810 to 840 us (library 1,820).
+// products of one tile wait for: 8,192 tokens x 4,096 x 4,096 in bf16 296 to 314 us, 875 to 930 TFLOP/s
+// beside a library product's 1,480 to 1,620 of weights that are whole; in 32 bits 810 to 840 us (library 1,820).
 #include "lane_types.h"
 
 #include <type_traits>
@@ -503,11 +503,15 @@ template <typename T, int G>
 void many(const uint16_t* x, int64_t ld, int64_t plane, const uint8_t* w4, const float* scale,
           int k, const Out& o, hipStream_t st) {
   // A launch takes its rounds of a workgroup a CU, and a round of tiles of 128 x 256, 64 x 256, 64 x 128
-  // and 64 x 64 about 75, 46, 34 and 25 us at 4,096 values in groups of 128 in bf16, and in that
-  // proportion for the others.  The largest tiles: 8,192 tokens x 4,096 channels 304 us (365, 379, 517
-  // with the others).  1,500 tokens: 72 (88, 79, 100); 700 tokens: 46 with the second (70, 48, 52); 512
-  // tokens: 35 with the third (69, 45, 36); 256 tokens: 26 with the last (67, 44, 34).  With the other
-  // groups' or 32-bit sums beside them the larger ones do not fit the registers.
+  // and 64 x 64 about 75, 46, 34 and 25 us at 4,096 values in groups of 128 in bf16.  Whole rounds, in
+  // which every CU has one: 85, 51, 37 and 30; in fp16 82, 49, 36, 30; groups of 64 -, 58, 41, 34; of 32
+  // -, 82, 58, 47; 32-bit tokens in groups of 128 -, 108, 75, 55; of 64 -, 112, 79, 58; of 32 -, -, 96,
+  // 69: in that proportion within an eighth.  Of 48 calls of 100 to 8,192 tokens x 4,096 channels the
+  // choice was the fastest tile but in three (1,500 and 2,500 tokens in groups of 64, 106 us for 88 and
+  // 158 for 139; 2,500 in groups of 128, 131 for 120).  The largest tiles: 8,192 tokens x 4,096 channels
+  // 304 us (365, 379, 517 with the others).  1,500 tokens: 72 (88, 79, 100); 700 tokens: 46 with the
+  // second (70, 48, 52); 512 tokens: 35 with the third (69, 45, 36); 256 tokens: 26 with the last (67, 44,
+  // 34).  With the other groups' or 32-bit sums beside them the larger ones do not fit the registers.
   auto rounds = [&](int bm, int bn) {
     const int64_t tiles = (int64_t)((o.m + bm - 1) / bm) * ((o.n + bn - 1) / bn);
     return (tiles + bs_num_cus() - 1) / bs_num_cus();

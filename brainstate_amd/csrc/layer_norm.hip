@@ -13,9 +13,9 @@
 // weights are read once and their gradients are summed in registers, then over the workgroups in
 // their order (weight_sum_kernel): the same bits every time.
 //
-// 8,192 rows of 4,096 in bf16 with dropout of a tenth: forward 61 to 70 us (268 MB, 4.1 TB/s beside a large
-// copy's 5.1), gradients 89.5 (336 MB and the mask's words again, 3.8), weights' sums 4.9; dropout alone
-// 29 (134 MB, 4.6).
+// 8,192 rows of 4,096 in bf16 with dropout of a tenth: forward 59 to 70 us (268 MB, 3.9 to 4.5 TB/s beside
+// a large copy's 5.1), gradients 91 (403 MB and the mask's words again, 4.4), weights' sums 4.1; dropout
+// alone 26 to 29 (134 MB, 4.6 to 5.1).  The larger figures are the tracer's, the smaller a run of calls'.
 #include "philox.h"
 #include "rows.h"
 
