@@ -6,7 +6,7 @@ import struct
 import torch
 
 from . import _native as N
-from ._sequence import _DTYPES, _address, _floating, _like, _once, _recorded, _rows
+from ._sequence import _DTYPES, _address, _fits, _floating, _like, _once, _recorded, _rows
 
 _NORM_IN = struct.Struct('5P3qQ4i2I2f')      # bs_layer_norm_in
 
@@ -75,8 +75,9 @@ def dropout(x, p, seed, site=0):
     model apart that share one.  What is dropped is 0 whatever it was.  Differentiable in ``x``, in
     reverse mode."""
     _floating('x', x)
-    if x.dim() < 1 or x.shape[-1] >= 1 << 31:
-        raise ValueError(f'x [.., dim] with dim in 0..2^31 - 1: got {tuple(x.shape)}')
+    if x.dim() < 1:
+        raise ValueError('x must have a dimension')
+    _fits(x.shape[-1], 'values of a row (dim)')
     args = _chance(p, seed, site, x.device)
     if _recorded('dropout', x):
         return _Dropout.apply(x, *args, site)
